@@ -54,6 +54,7 @@ typedef struct odie_grid_level {
 /* dtype codes */
 #define ODIE_F32 0
 #define ODIE_F16 1
+#define ODIE_BF16 2   /* the row operators (odie_linear_*, odie_sort_*, odie_rows_*, odie_embed_*) alone */
 
 /* Forward encode of n coordinates in [0,1]^2 (coords fp32 [n,2]).
  * Experts: coordinates [offsets[e], offsets[e+1]) read the table at params + e*expert_params
@@ -553,6 +554,89 @@ void odie_pin_contexts(void* handle);
 void odie_release_contexts(void* handle);
 /* Replaces odie_destroy (:330): waits for the stream, frees the handle's buffers. */
 void odie_destroy(void* handle);
+
+/* ---------------------------------------------------------------------------------------
+ * Mixtures of experts on rows: sorting rows by expert, sending them there and back with weights,
+ * linear layers dense or per expert, and lookups of a table by id.  No counterpart in the reference.
+ *
+ * dtype is ODIE_F32, ODIE_F16 or ODIE_BF16 for every tensor of a call unless stated; sums are fp32 and
+ * rounded once.  Rows are contiguous; a stride is the elements from row to row (at least the
+ * row's width).  No alignment is needed beyond the element's.  Workspaces are the caller's, so calls on
+ * different streams share nothing.  A call of no rows is fine; gradients of parameters are then 0.
+ * --------------------------------------------------------------------------------------- */
+
+/* Stable sort of n keys (int32 or int64: key_bytes 4 or 8) by bucket 0..buckets-1; a key outside them
+ * sorts after every bucket.  n < 2^31, buckets < 2^31 - 1.
+ *   order    int32 [n]            input position of each sorted place
+ *   sorted   int32 [n] or null    bucket of each sorted place (`buckets` for a key outside them)
+ *   slots    int32 [n] or null    sorted place of each input position, -1 for a key outside the buckets
+ *   offsets  int32 [buckets + 1] or null   first place of every bucket; the last entry is the count of
+ *                                 keys inside them
+ * workspace: odie_sort_workspace(n, buckets) bytes (0 for small n), 16-byte aligned. */
+int64_t odie_sort_workspace(int64_t n, int64_t buckets);
+int odie_sort(const void* keys, int key_bytes, int64_t n, int64_t buckets, int32_t* order, int32_t* sorted,
+              int32_t* slots, int32_t* offsets, void* workspace, int64_t workspace_bytes, uint64_t stream);
+
+/* Rows to their slots: n rows with `choices` entries each, entry f = i * choices + j of row i at
+ * slots[f] (odie_sort's over the entries' experts; -1: nowhere).  out [n * choices][width] receives
+ * out[slots[f]] = x[i], and 0 from offsets[experts] on. */
+int odie_rows_dispatch(const void* x, int64_t x_stride, const int32_t* slots, const int32_t* offsets, int64_t n,
+                       int choices, int experts, int64_t width, int dtype, void* out, uint64_t stream);
+
+/* Rows back from their slots: out[i] = sum over j of weights[f] * rows[slots[f]], out [n][width];
+ * weights fp32 [n * choices], or null: 1 (the gradient of odie_rows_dispatch). */
+int odie_rows_combine(const void* rows, int64_t rows_stride, const int32_t* slots, const float* weights, int64_t n,
+                      int choices, int64_t width, int dtype, void* out, uint64_t stream);
+
+/* Gradients of odie_rows_combine: drows[slots[f]] = weights[f] * upstream[i], 0 from offsets[experts] on
+ * ([n * choices][width], or null), and dweights[f] = <upstream[i], rows[slots[f]]> (fp32, 0 where
+ * slots[f] is -1; or null, and rows is then not read). */
+int odie_rows_combine_backward(const void* upstream, int64_t upstream_stride, const void* rows, int64_t rows_stride,
+                               const int32_t* slots, const float* weights, const int32_t* offsets, int64_t n,
+                               int choices, int experts, int64_t width, int dtype, void* drows, float* dweights,
+                               uint64_t stream);
+
+/* activation codes of the linear layer (gelu is the exact one, by erf) */
+#define ODIE_ACT_NONE 0
+#define ODIE_ACT_RELU 1
+#define ODIE_ACT_SIGMOID 2
+#define ODIE_ACT_SOFTPLUS 3
+#define ODIE_ACT_GELU 4
+#define ODIE_ACT_SILU 5
+
+/* out = act(x weight^T + bias) + residual.  weight [experts][outputs][inputs], bias [experts][outputs]
+ * or null, residual [rows][outputs] or null.  offsets: device int32 [experts + 1], nondecreasing,
+ * offsets[0] = 0, offsets[experts] <= rows; rows offsets[e]..offsets[e+1]-1 use expert e's matrix, rows
+ * from offsets[experts] on belong to none (out = residual, or 0).  offsets = NULL with experts = 1: one
+ * matrix for every row.  pre, if not null, receives the sums before the activation
+ * ([rows][outputs], unset in rows of no expert): what odie_linear_backward needs. */
+int odie_linear_forward(const void* x, int64_t x_stride, int64_t rows, const void* weight, const void* bias,
+                        const void* residual, int64_t residual_stride, const int32_t* offsets, int experts,
+                        int inputs, int outputs, int dtype, int activation, void* out, int64_t out_stride, void* pre,
+                        uint64_t stream);
+
+/* Gradients of odie_linear_forward: dx [rows][inputs] (0 in rows of no expert), dweight, dbias (shaped as
+ * weight and bias), each or null; the residual's gradient is upstream itself.  pre may be null
+ * with ODIE_ACT_NONE, x without dweight, weight without dx.  Deterministic.  workspace: 256-byte aligned,
+ * odie_linear_workspace bytes (grouped: offsets given; want_*: the output given). */
+int64_t odie_linear_workspace(int64_t rows, int experts, int grouped, int inputs, int outputs, int dtype,
+                              int activation, int want_dweight, int want_dbias);
+int odie_linear_backward(const void* upstream, int64_t upstream_stride, const void* x, int64_t x_stride,
+                         const void* pre, int64_t rows, const void* weight, const int32_t* offsets, int experts,
+                         int inputs, int outputs, int dtype, int activation, void* dx, void* dweight, void* dbias,
+                         void* workspace, int64_t workspace_bytes, uint64_t stream);
+
+/* out[i] = scale * table[ids[i]] (ids int32 or int64: id_bytes 4 or 8), 0 for an id outside
+ * [0, vocab); out [n][width]. */
+int odie_embed_forward(const void* table, int64_t table_stride, int64_t vocab, const void* ids, int id_bytes,
+                       int64_t n, float scale, int64_t width, int dtype, void* out, uint64_t stream);
+
+/* dtable [vocab][width] = scale * the sum of upstream over each row's ids, 0 for rows without one.
+ * Deterministic.  workspace: 256-byte aligned, odie_embed_workspace bytes. */
+int64_t odie_embed_workspace(int64_t n, int64_t vocab, int64_t width, int dtype);
+int odie_embed_backward(const void* upstream, int64_t upstream_stride, const void* ids, int id_bytes, int64_t n,
+                        int64_t vocab, float scale, int64_t width, int dtype, void* dtable, void* workspace,
+                        int64_t workspace_bytes, uint64_t stream);
 
 #ifdef __cplusplus
 }

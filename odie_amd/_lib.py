@@ -11,7 +11,7 @@ import re
 LIBRARY = Path(__file__).resolve().parent / 'libodie_amd.so'
 HEADER = Path(__file__).resolve().parent.parent / 'include' / 'odie_amd.h'
 
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 
 
 class GridLevel(C.Structure):
@@ -75,6 +75,18 @@ SIGNATURES = {
                                 _I),
     'odie_mean': ([_P, _I64, _P, _U64], _I),
     'odie_stratified_ids': ([_P, _I, _I, _I, _P, _U64], _I),
+    'odie_sort_workspace': ([_I64, _I64], _I64),
+    'odie_sort': ([_P, _I, _I64, _I64, _P, _P, _P, _P, _P, _I64, _U64], _I),
+    'odie_rows_dispatch': ([_P, _I64, _P, _P, _I64, _I, _I, _I64, _I, _P, _U64], _I),
+    'odie_rows_combine': ([_P, _I64, _P, _P, _I64, _I, _I64, _I, _P, _U64], _I),
+    'odie_rows_combine_backward': ([_P, _I64, _P, _I64, _P, _P, _P, _I64, _I, _I, _I64, _I, _P, _P, _U64], _I),
+    'odie_linear_forward': ([_P, _I64, _I64, _P, _P, _P, _I64, _P, _I, _I, _I, _I, _I, _P, _I64, _P, _U64], _I),
+    'odie_linear_workspace': ([_I64, _I, _I, _I, _I, _I, _I, _I, _I], _I64),
+    'odie_linear_backward': ([_P, _I64, _P, _I64, _P, _I64, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I64, _U64],
+                             _I),
+    'odie_embed_forward': ([_P, _I64, _I64, _P, _I, _I64, C.c_float, _I64, _I, _P, _U64], _I),
+    'odie_embed_workspace': ([_I64, _I64, _I64, _I], _I64),
+    'odie_embed_backward': ([_P, _I64, _P, _I, _I64, _I64, C.c_float, _I64, _I, _P, _P, _I64, _U64], _I),
     'odie_create': ([C.c_char_p], _P),
     'odie_step': ([_P, _U64, _I, _I], _I),
     'odie_configure': ([_P, C.c_char_p], _I),
@@ -147,6 +159,30 @@ def stream_of(tensor=None):
             raise ValueError('Expected a cuda device, but got: %s' % tensor.device)
         index = tensor.device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+def call(name, tensor, *arguments):
+    """Call entry point `name` with `arguments` and the current stream of the tensor's device, on that
+    device."""
+    import torch
+    index = tensor.device.index
+    function = getattr(library(), name)
+    if index == torch.cuda.current_device():
+        code = function(*arguments, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = function(*arguments, torch._C._cuda_getCurrentRawStream(index))
+    check(code)
+
+
+def scratch(name, tensor, *arguments):
+    """uint8 workspace on the tensor's device of the bytes entry point `name` answers for `arguments`; None
+    where it needs none."""
+    import torch
+    size = getattr(library(), name)(*arguments)
+    if size < 0:
+        check(-1)
+    return torch.empty(size, dtype=torch.uint8, device=tensor.device) if size else None
 
 
 def set_tuning(key, value):

@@ -1,0 +1,166 @@
+// The three element types of the row operators (fp32, fp16, bf16) and their 16-byte vectors.
+//
+// Values are widened to fp32 for every sum and rounded once, to nearest even, where they are
+// stored.  Rows may start at any element: 16-byte accesses go through memcpy, which compiles to the
+// wide global instructions whether or not the address is 16-byte aligned (unaligned access mode).
+#pragma once
+#include <cstdint>
+
+#include "common.h"
+#include "../../include/odie_amd.h"
+
+namespace odie {
+
+typedef uint32_t vec16 __attribute__((ext_vector_type(4)));   // 16 bytes of any element type
+
+template <class T> constexpr int kPerVec = 16 / static_cast<int>(sizeof(T));
+
+template <class T> __device__ inline vec16 load16(const T* p) {
+    vec16 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+
+template <class T> __device__ inline void store16(T* p, const vec16& v) { __builtin_memcpy(p, &v, 16); }
+
+// The first `count` elements at p (count >= 1), zeros after them.
+template <class T> __device__ inline vec16 load_some(const T* p, int count) {
+    if (count >= kPerVec<T>) return load16(p);
+    T e[kPerVec<T>] = {};
+#pragma unroll
+    for (int i = 0; i < kPerVec<T>; ++i)
+        if (i < count) e[i] = p[i];
+    vec16 v;
+    __builtin_memcpy(&v, e, 16);
+    return v;
+}
+
+template <class T> __device__ inline void store_some(T* p, const vec16& v, int count) {
+    if (count >= kPerVec<T>) {
+        store16(p, v);
+        return;
+    }
+    T e[kPerVec<T>];
+    __builtin_memcpy(e, &v, 16);
+#pragma unroll
+    for (int i = 0; i < kPerVec<T>; ++i)
+        if (i < count) p[i] = e[i];
+}
+
+template <class T> __device__ inline void widen(const vec16& v, float out[kPerVec<T>]) {
+    T e[kPerVec<T>];
+    __builtin_memcpy(e, &v, 16);
+#pragma unroll
+    for (int i = 0; i < kPerVec<T>; ++i) out[i] = static_cast<float>(e[i]);
+}
+
+template <class T> __device__ inline vec16 narrow(const float in[kPerVec<T>]) {
+    T e[kPerVec<T>];
+#pragma unroll
+    for (int i = 0; i < kPerVec<T>; ++i) e[i] = static_cast<T>(in[i]);
+    vec16 v;
+    __builtin_memcpy(&v, e, 16);
+    return v;
+}
+
+// Eight elements as fp32, the first `count` of them read (the others 0), and back.
+template <class T> __device__ inline void load8(const T* p, int count, float out[8]) {
+    if (count >= 8) {
+#pragma unroll
+        for (int h = 0; h < 8 / kPerVec<T>; ++h) widen<T>(load16(p + h * kPerVec<T>), out + h * kPerVec<T>);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out[i] = i < count ? static_cast<float>(p[i]) : 0.0f;
+    }
+}
+
+template <class T> __device__ inline void store8(T* p, int count, const float in[8]) {
+    if (count >= 8) {
+#pragma unroll
+        for (int h = 0; h < 8 / kPerVec<T>; ++h) store16(p + h * kPerVec<T>, narrow<T>(in + h * kPerVec<T>));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < count) p[i] = static_cast<T>(in[i]);
+    }
+}
+
+// A wave orders its own LDS accesses: lanes read what other lanes of the wave wrote.
+__device__ inline void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+inline bool known_dtype(int dtype) { return dtype == ODIE_F32 || dtype == ODIE_F16 || dtype == ODIE_BF16; }
+inline int64_t dtype_bytes(int dtype) { return dtype == ODIE_F32 ? 4 : 2; }
+
+// Calls f with a value of the element type `dtype` names (checked by the caller).
+template <class F> auto with_dtype(int dtype, F&& f) {
+    if (dtype == ODIE_F16) return f(_Float16{});
+    if (dtype == ODIE_BF16) return f(__bf16{});
+    return f(float{});
+}
+
+// Rows grouped by expert: expert e owns rows [offsets[e], offsets[e + 1]), the rows from
+// offsets[experts] on belong to none (they form group `experts`); a null offsets is one expert
+// that owns every row.  Groups are cut into pieces of `piece` rows.  Piece ids: group e's begin at
+//   s(e) = floor(offsets[e] / piece) + e,
+// which leaves each group room for its pieces, because s(e + 1) - s(e) >= ceil(rows of e / piece) and
+// >= 1; so a piece id finds its group by comparing s alone, with no table of counts, and ids left
+// over find no rows.  There are piece_ids() of them.
+struct Piece {
+    int group;
+    int first;       // piece number inside the group
+    int64_t begin;   // rows [begin, end) of the tensor; begin >= end: nothing to do
+    int64_t end;
+    int64_t group_begin;
+    int64_t group_end;
+};
+
+inline int64_t piece_ids(int64_t rows, int64_t piece, bool grouped, int experts, bool tail) {
+    return grouped ? rows / piece + experts + (tail ? 1 : 0) : (rows + piece - 1) / piece;
+}
+
+__device__ inline int64_t group_start(const int32_t* offsets, int group, int64_t rows) {
+    const int64_t at = offsets[group];
+    return at < 0 ? 0 : (at > rows ? rows : at);   // whatever offsets hold, no row outside the tensor
+}
+
+// floor(offsets[group] / piece) (offsets and, with them, rows are below 2^31).
+__device__ inline int64_t whole_pieces(const int32_t* offsets, int group, int64_t rows, int64_t piece) {
+    return static_cast<uint32_t>(group_start(offsets, group, rows)) / static_cast<uint32_t>(piece);
+}
+
+// The piece `id` of groups 0..groups-1 (groups = experts + 1 with the rows of no expert, else
+// experts).  All 64 lanes of the wave call it with the same id.
+__device__ inline Piece find_piece(const int32_t* offsets, int experts, int groups, int64_t rows, int64_t piece,
+                                   int64_t id) {
+    Piece p{};
+    if (!offsets) {
+        p.first = static_cast<int>(id);
+        p.group_end = rows;
+    } else {
+        const int lane = static_cast<int>(threadIdx.x % 64);
+        // the last group g with s(g) <= id: 64 probes a round, first spaced, then closer
+        int low = 0, span = groups;
+        while (span > 1) {
+            const int step = (span + 63) / 64;
+            const int g = low + lane * step;
+            const bool below = lane * step < span && whole_pieces(offsets, g, rows, piece) + g <= id;
+            const int count = __popcll(__ballot(below));    // s increases: the lanes below come first
+            const int found = count > 1 ? count : 1;
+            low += (found - 1) * step;                      // s(low) <= id always: lane 0 is one of them
+            span = span - (found - 1) * step < step ? span - (found - 1) * step : step;
+        }
+        p.group = __builtin_amdgcn_readfirstlane(low);
+        p.group_begin = group_start(offsets, p.group, rows);
+        p.group_end = p.group < experts ? group_start(offsets, p.group + 1, rows) : rows;
+        p.first = static_cast<int>(id - (whole_pieces(offsets, p.group, rows, piece) + p.group));
+    }
+    p.begin = p.group_begin + p.first * piece;
+    p.end = p.begin + piece < p.group_end ? p.begin + piece : p.group_end;
+    return p;
+}
+
+}  // namespace odie

@@ -1,0 +1,215 @@
+// Linear layers with bias, activation and residual fused into the product, dense or with one weight
+// matrix per expert over rows sorted by expert, and their gradients.
+//
+//   z = x w[e]^T + bias[e],  y = act(z) + residual            rows offsets[e] .. offsets[e + 1] - 1
+//   dz = dy act'(z),  dx = dz w[e],  dw[e] = dz^T x,  dbias[e] = sum dz,  dresidual = dy
+//
+// The forward is one launch.  The backward forms dz and its column sums in one pass over dy and z, then
+// dx and dw as products of dz; dw sums over rows, so the rows are cut into pieces whose fp32 sums are
+// joined in a fixed order: the result does not depend on timing.  Workspaces are the caller's.
+//
+// z is kept in the tensors' own type for the backward: its rounding moves act'(z) by less than half a
+// unit of that type, where the gradients themselves are rounded to it.
+#include "linear.h"
+
+namespace odie {
+namespace {
+
+constexpr int64_t kMaxRows = (int64_t{1} << 31) - 1;
+constexpr int kMaxWidth = 1 << 20;
+constexpr int kMaxExperts = 1 << 15;
+
+// Rows a bias piece sums: long enough that the partial sums stay small beside dz, short enough for a
+// few workgroups on every CU.
+int64_t slope_piece(int64_t rows) {
+    const int64_t piece = (rows / (4 * kCus) + 63) / 64 * 64;
+    return piece < 64 ? 64 : (piece > 1024 ? 1024 : piece);
+}
+
+// Rows a weight piece sums: about four workgroups a CU over all experts and tiles.
+int64_t weight_piece(int64_t rows, int experts, int outputs, int inputs) {
+    const int edge = outputs <= 64 || inputs <= 64 ? 64 : 128;
+    const int64_t tiles = static_cast<int64_t>((outputs + edge - 1) / edge) * ((inputs + edge - 1) / edge);
+    int64_t pieces = 4 * kCus / tiles - experts;
+    if (pieces < 1) pieces = experts > 1 ? 4 : 1;
+    int64_t piece = ((rows + pieces - 1) / pieces + 255) / 256 * 256;
+    return piece < 256 ? 256 : piece;
+}
+
+struct Plan {
+    int64_t dz_bytes, sums_bytes, partial_bytes;   // each a multiple of 256
+    int64_t slope_piece, slope_pieces, weight_piece, weight_pieces;
+};
+
+int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+Plan make_plan(int64_t rows, int experts, bool grouped, int outputs, int inputs, int dtype, int activation,
+               bool want_dweight, bool want_dbias) {
+    Plan p{};
+    p.slope_piece = slope_piece(rows);
+    p.slope_pieces = piece_ids(rows, p.slope_piece, grouped && want_dbias, experts, false);
+    p.weight_piece = weight_piece(rows, experts, outputs, inputs);
+    p.weight_pieces = piece_ids(rows, p.weight_piece, grouped, experts, false);
+    if (p.weight_pieces < 1) p.weight_pieces = 1;
+    p.dz_bytes = activation == kNone ? 0 : padded(rows * outputs * dtype_bytes(dtype));
+    p.sums_bytes = want_dbias ? padded(p.slope_pieces * outputs * 4) : 0;
+    p.partial_bytes = want_dweight && rows > p.weight_piece
+                          ? padded(p.weight_pieces * outputs * static_cast<int64_t>(inputs) * 4) : 0;
+    return p;
+}
+
+int check_sizes(const std::string& what, int64_t rows, int experts, bool grouped, int inputs, int outputs, int dtype,
+                int activation) {
+    if (!known_dtype(dtype)) return fail(what + ": dtype must be 0 (fp32), 1 (fp16) or 2 (bf16)");
+    if (activation < 0 || activation >= kActivations) return fail(what + ": activation must be within 0..5");
+    if (rows < 0 || rows > kMaxRows) return fail(what + ": rows must be within 0..2^31 - 1");
+    if (inputs < 1 || outputs < 1 || inputs > kMaxWidth || outputs > kMaxWidth)
+        return fail(what + ": inputs and outputs must be within 1..2^20");
+    if (experts < 1 || experts > kMaxExperts) return fail(what + ": experts must be within 1..32768");
+    if (!grouped && experts != 1) return fail(what + ": several experts need offsets");
+    return 0;
+}
+
+}  // namespace
+}  // namespace odie
+
+using namespace odie;
+
+ODIE_API int odie_linear_forward(const void* x, int64_t x_stride, int64_t rows, const void* weight, const void* bias,
+                                 const void* residual, int64_t residual_stride, const int32_t* offsets, int experts,
+                                 int inputs, int outputs, int dtype, int activation, void* out, int64_t out_stride,
+                                 void* pre, uint64_t stream) {
+    const char* what = "odie_linear_forward";
+    if (check_sizes(what, rows, experts, offsets != nullptr, inputs, outputs, dtype, activation)) return -1;
+    if (rows == 0) return 0;
+    if (!x || !weight || !out) return fail(std::string(what) + ": null pointer");
+    if (x_stride < inputs || out_stride < outputs || (residual && residual_stride < outputs))
+        return fail(std::string(what) + ": rows overlap (a stride below the row's width)");
+    RowsArgs a{};
+    a.a = x;
+    a.lda = x_stride;
+    a.b = weight;
+    a.bias = bias;
+    a.residual = residual;
+    a.ldr = residual_stride;
+    a.out = out;
+    a.ldo = out_stride;
+    a.pre = pre;
+    a.offsets = offsets;
+    a.rows = rows;
+    a.experts = experts;
+    a.depth = inputs;
+    a.columns = outputs;
+    a.activation = activation;
+    return with_dtype(dtype, [&](auto t) { return launch_rows<decltype(t)>(a, true, as_stream(stream)); });
+}
+
+ODIE_API int64_t odie_linear_workspace(int64_t rows, int experts, int grouped, int inputs, int outputs, int dtype,
+                                       int activation, int want_dweight, int want_dbias) {
+    if (check_sizes("odie_linear_workspace", rows, experts, grouped != 0, inputs, outputs, dtype, activation)) return -1;
+    const Plan p = make_plan(rows, experts, grouped != 0, outputs, inputs, dtype, activation, want_dweight != 0,
+                             want_dbias != 0);
+    return p.dz_bytes + p.sums_bytes + p.partial_bytes;
+}
+
+ODIE_API int odie_linear_backward(const void* upstream, int64_t upstream_stride, const void* x, int64_t x_stride,
+                                  const void* pre, int64_t rows, const void* weight, const int32_t* offsets,
+                                  int experts, int inputs, int outputs, int dtype, int activation, void* dx,
+                                  void* dweight, void* dbias, void* workspace, int64_t workspace_bytes,
+                                  uint64_t stream) {
+    const std::string what = "odie_linear_backward";
+    if (check_sizes(what, rows, experts, offsets != nullptr, inputs, outputs, dtype, activation)) return -1;
+    if (rows > 0 && (!upstream || (dweight && !x) || (dx && !weight) || (activation != kNone && !pre)))
+        return fail(what + ": null pointer");
+    if (rows > 0 && (upstream_stride < outputs || (dweight && x_stride < inputs)))
+        return fail(what + ": rows overlap (a stride below the row's width)");
+    const Plan p = make_plan(rows, experts, offsets != nullptr, outputs, inputs, dtype, activation, dweight != nullptr,
+                             dbias != nullptr);
+    const int64_t need = p.dz_bytes + p.sums_bytes + p.partial_bytes;
+    if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0))
+        return fail(what + ": needs a 256-byte aligned workspace of " + std::to_string(need) + " bytes");
+    hipStream_t s = as_stream(stream);
+    char* scratch = static_cast<char*>(workspace);
+    return with_dtype(dtype, [&](auto t) -> int {
+        using T = decltype(t);
+        const void* dz = upstream;
+        int64_t dz_stride = upstream_stride;
+        float* sums = p.sums_bytes ? reinterpret_cast<float*>(scratch + p.dz_bytes) : nullptr;
+        if ((activation != kNone || dbias) && rows > 0) {
+            SlopeArgs a{};
+            a.dy = upstream;
+            a.ldy = upstream_stride;
+            a.pre = pre;
+            a.dz = activation != kNone ? scratch : nullptr;
+            a.sums = sums;
+            a.offsets = dbias ? offsets : nullptr;   // the sums alone go by expert
+            a.rows = rows;
+            a.piece = p.slope_piece;
+            a.pieces = p.slope_pieces;
+            a.experts = experts;
+            a.columns = outputs;
+            a.activation = activation;
+            if (launch_slope<T>(a, s)) return -1;
+            if (activation != kNone) {
+                dz = scratch;
+                dz_stride = outputs;
+            }
+        }
+        if (dbias) {
+            FoldArgs a{};
+            a.partial = sums;
+            a.out = dbias;
+            a.offsets = offsets;
+            a.rows = rows;
+            a.piece = p.slope_piece;
+            a.size = outputs;
+            a.experts = experts;
+            a.single = true;
+            if (launch_fold<T>(a, s)) return -1;
+        }
+        if (dx && rows > 0) {
+            RowsArgs a{};
+            a.a = dz;
+            a.lda = dz_stride;
+            a.b = weight;
+            a.out = dx;
+            a.ldo = inputs;
+            a.offsets = offsets;
+            a.rows = rows;
+            a.experts = experts;
+            a.depth = outputs;
+            a.columns = inputs;
+            if (launch_rows<T>(a, false, s)) return -1;
+        }
+        if (dweight) {
+            WeightArgs a{};
+            a.dz = dz;
+            a.ldz = dz_stride;
+            a.x = x;
+            a.ldx = x_stride;
+            a.dw = dweight;
+            a.partial = reinterpret_cast<float*>(scratch + p.dz_bytes + p.sums_bytes);
+            a.offsets = offsets;
+            a.rows = rows;
+            a.piece = p.weight_piece;
+            a.pieces = p.weight_pieces;
+            a.experts = experts;
+            a.outputs = outputs;
+            a.inputs = inputs;
+            if (launch_weight<T>(a, s)) return -1;
+            if (p.partial_bytes) {
+                FoldArgs f{};
+                f.partial = a.partial;
+                f.out = dweight;
+                f.offsets = offsets;
+                f.rows = rows;
+                f.piece = p.weight_piece;
+                f.size = static_cast<int64_t>(outputs) * inputs;
+                f.experts = experts;
+                f.single = false;
+                if (launch_fold<T>(f, s)) return -1;
+            }
+        }
+        return 0;
+    });
+}

@@ -1,0 +1,36 @@
+"""What the row operators (linear, mixture, embedding) share: their element types and the checks of
+their tensors."""
+import torch
+
+from . import _lib
+
+DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+def check_rows(name, value, width=None, *, dtype=None, device=None, count=None):
+    """value as rows the kernels read: CUDA fp32, fp16 or bf16 [count, width], each row contiguous (a
+    tensor that is not is copied)."""
+    if not isinstance(value, torch.Tensor) or value.dtype not in DTYPES or value.ndim != 2 or not value.is_cuda:
+        raise ValueError('%s must be a CUDA fp32, fp16 or bf16 tensor of two dimensions' % name)
+    if dtype is not None and value.dtype != dtype:
+        raise ValueError('%s must have the dtype of the other tensors (%s)' % (name, dtype))
+    if device is not None and value.device != device:
+        raise ValueError('%s must be on the device of the other tensors (%s)' % (name, device))
+    if (width is not None and value.shape[1] != width) or (count is not None and value.shape[0] != count):
+        raise ValueError('%s must be [%s, %s]' % (name, 'N' if count is None else count,
+                                                  'width' if width is None else width))
+    if value.shape[1] == 0:
+        raise ValueError('%s must have at least one column' % name)
+    return row_major(value)
+
+
+def row_major(value):
+    """value, or its copy where a row is not contiguous or rows overlap."""
+    if value.stride(1) != 1 or value.stride(0) < value.shape[1]:
+        return value.contiguous()
+    return value
+
+
+def records(*tensors):
+    """Whether autograd will ask for a gradient of one of the tensors."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
