@@ -23,28 +23,72 @@ template <class T> __device__ inline vec16 load16(const T* p) {
 
 template <class T> __device__ inline void store16(T* p, const vec16& v) { __builtin_memcpy(p, &v, 16); }
 
-// The first `count` elements at p (count >= 1), zeros after them.
-template <class T> __device__ inline vec16 load_some(const T* p, int count) {
-    if (count >= kPerVec<T>) return load16(p);
-    T e[kPerVec<T>] = {};
+// The first `count` elements at p (0 <= count), zeros after them, element by element.
+template <class T> __device__ inline vec16 gather16(const T* p, int count) {
+    vec16 v{};
+    if constexpr (sizeof(T) == 4) {
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
 #pragma unroll
-    for (int i = 0; i < kPerVec<T>; ++i)
-        if (i < count) e[i] = p[i];
-    vec16 v;
-    __builtin_memcpy(&v, e, 16);
+        for (int i = 0; i < 4; ++i) v[i] = i < count ? q[i] : 0u;
+    } else {
+        const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t low = 2 * i < count ? q[2 * i] : 0u, high = 2 * i + 1 < count ? q[2 * i + 1] : 0u;
+            v[i] = low | high << 16;
+        }
+    }
     return v;
 }
 
-template <class T> __device__ inline void store_some(T* p, const vec16& v, int count) {
-    if (count >= kPerVec<T>) {
-        store16(p, v);
-        return;
-    }
-    T e[kPerVec<T>];
-    __builtin_memcpy(e, &v, 16);
+template <class T> __device__ inline void scatter16(T* p, const vec16& v, int count) {
+    if constexpr (sizeof(T) == 4) {
+        uint32_t* q = reinterpret_cast<uint32_t*>(p);
 #pragma unroll
-    for (int i = 0; i < kPerVec<T>; ++i)
-        if (i < count) p[i] = e[i];
+        for (int i = 0; i < 4; ++i)
+            if (i < count) q[i] = v[i];
+    } else {
+        uint16_t* q = reinterpret_cast<uint16_t*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (2 * i < count) q[2 * i] = static_cast<uint16_t>(v[i]);
+            if (2 * i + 1 < count) q[2 * i + 1] = static_cast<uint16_t>(v[i] >> 16);
+        }
+    }
+}
+
+template <class T> __device__ inline vec16 load_some(const T* p, int count) {
+    return count >= kPerVec<T> ? load16(p) : gather16(p, count);
+}
+
+template <class T> __device__ inline void store_some(T* p, const vec16& v, int count) {
+    if (count >= kPerVec<T>) store16(p, v);
+    else scatter16(p, v, count);
+}
+
+// v moved down by `bytes` (0..15), zeros above.
+__device__ inline vec16 shift_down(const vec16& v, int bytes) {
+    uint64_t low = static_cast<uint64_t>(v.y) << 32 | v.x, high = static_cast<uint64_t>(v.w) << 32 | v.z;
+    if (bytes >= 8) {
+        low = high;
+        high = 0;
+        bytes -= 8;
+    }
+    if (bytes > 0) {
+        low = low >> 8 * bytes | high << (64 - 8 * bytes);
+        high >>= 8 * bytes;
+    }
+    return vec16{static_cast<uint32_t>(low), static_cast<uint32_t>(low >> 32), static_cast<uint32_t>(high),
+                 static_cast<uint32_t>(high >> 32)};
+}
+
+// The first `count` elements at p (at least one) and zeros after them, where the `back` elements before p can be
+// read too: the last 16 bytes that end with them, moved down.
+template <class T> __device__ inline vec16 load_end(const T* p, int count, int64_t back) {
+    if (count >= kPerVec<T>) return load16(p);
+    const int missing = kPerVec<T> - count;
+    if (back < missing) return gather16(p, count);
+    return shift_down(load16(p - missing), missing * static_cast<int>(sizeof(T)));
 }
 
 template <class T> __device__ inline void widen(const vec16& v, float out[kPerVec<T>]) {
@@ -63,26 +107,31 @@ template <class T> __device__ inline vec16 narrow(const float in[kPerVec<T>]) {
     return v;
 }
 
-// Eight elements as fp32, the first `count` of them read (the others 0), and back.
-template <class T> __device__ inline void load8(const T* p, int count, float out[8]) {
-    if (count >= 8) {
+// Eight consecutive elements, of which `count` exist (those past them read as 0 and are not written).
+template <class T> struct Eight {
+    static constexpr int kWords = 8 / kPerVec<T>;
+    vec16 word[kWords];
+
+    __device__ void load(const T* p, int count) {
 #pragma unroll
-        for (int h = 0; h < 8 / kPerVec<T>; ++h) widen<T>(load16(p + h * kPerVec<T>), out + h * kPerVec<T>);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = i < count ? static_cast<float>(p[i]) : 0.0f;
+        for (int w = 0; w < kWords; ++w) word[w] = load_some(p + w * kPerVec<T>, count - w * kPerVec<T>);
     }
+    __device__ void get(float out[8]) const {
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) widen<T>(word[w], out + w * kPerVec<T>);
+    }
+};
+
+template <class T> __device__ inline void load8(const T* p, int count, float out[8]) {
+    Eight<T> e;
+    e.load(p, count);
+    e.get(out);
 }
 
 template <class T> __device__ inline void store8(T* p, int count, const float in[8]) {
-    if (count >= 8) {
 #pragma unroll
-        for (int h = 0; h < 8 / kPerVec<T>; ++h) store16(p + h * kPerVec<T>, narrow<T>(in + h * kPerVec<T>));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < count) p[i] = static_cast<T>(in[i]);
-    }
+    for (int w = 0; w < 8 / kPerVec<T>; ++w)
+        store_some(p + w * kPerVec<T>, narrow<T>(in + w * kPerVec<T>), count - w * kPerVec<T>);
 }
 
 // A wave orders its own LDS accesses: lanes read what other lanes of the wave wrote.

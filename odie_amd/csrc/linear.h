@@ -16,6 +16,8 @@
 // The epilogue passes each wave's accumulators through its own part of the LDS, so that bias,
 // activation, residual and the stores run on rows of 8 consecutive columns a lane.
 #pragma once
+#include <type_traits>
+
 #include "elements.h"
 
 namespace odie {
@@ -25,6 +27,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float accum16 __attribute__((ext_vector_type(16)));
 typedef int16_t i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
+typedef __attribute__((address_space(3))) void* lds_void;
 
 constexpr int kSlabBytes = 128;
 template <class T> constexpr int kSlab = kSlabBytes / static_cast<int>(sizeof(T));   // k values a slab
@@ -50,105 +53,38 @@ __device__ inline accum16 multiply(float, const vec16& b, const vec16& a, accum1
 // c ^ (r / 2 % 8), so that 16 consecutive rows of one chunk fall on all 64 banks.
 // LDS image, one row per k: rows of kRows elements; chunk c of row k lies at slot c ^ turn(k), so
 // that the rows one transposing read touches at once (k .. k + 3, 32 columns) fall on all 64 banks.
-template <class T, bool kByRow, int kRows, int kThreads> struct Operand {
+// Thread t fills the slots t, t + kThreads, ... of the image, in the order of their addresses.
+template <class T, bool kByRow, int kRows, int kThreads> struct Image {
     static constexpr int kBytes = kRows * kSlabBytes;
     static constexpr int kChunks = kRows * 8 / kThreads;       // 16-byte chunks a thread moves per slab
     static constexpr int kVec = kPerVec<T>;
-    static constexpr int kPerRow = kRows / kVec;                // chunks a row (one row per k)
-    static_assert(kChunks * kThreads == kRows * 8 && (kByRow || kThreads % kPerRow == 0), "whole chunks a thread");
+    static constexpr int kPerRow = kByRow ? 8 : kRows / kVec;   // chunks a row of the image
+    static constexpr int kStep = kThreads / kPerRow;            // rows between a thread's chunks
+    static_assert(kChunks * kThreads == kRows * 8 && kThreads % kPerRow == 0, "whole chunks a thread");
 
-    vec16 held[kChunks];
-    const T* at[kByRow ? kChunks : 1];
-    int64_t row_step;    // one row per k: elements between this thread's consecutive chunks
-    int64_t slab_step;   // elements from slab to slab
-    int lead;            // k of this thread's first chunk, relative to the slab
-    int columns;         // one row per k: columns of this thread's chunk inside the tensor
-
-    // One row per k: XOR on the chunk index of row k.
-    static __device__ int turn(int k) {
-        if constexpr (sizeof(T) == 4) return (k >> 2 & 1) << 3;
-        return kPerRow >= 16 ? (k & 3) << 2 : (k >> 1 & 1) << 2;
+    // XOR on the chunk number in row r of the image.
+    static __device__ int turn(int r) {
+        if constexpr (kByRow) return r >> 1 & 7;
+        if constexpr (sizeof(T) == 4) return (r >> 2 & 1) << 3;
+        return kPerRow >= 16 ? (r & 3) << 2 : (r >> 1 & 1) << 2;
     }
+    static_assert(kStep % 16 == 0 || (!kByRow && kStep % 8 == 0), "a thread's chunks turn alike");
 
-    // k consecutive: rows first .. first + kRows - 1 of base (those past last read row `last`, their
-    // products are not stored).  One row per k: columns first .. of base, `limit` of them in all.
-    __device__ void begin(const T* base, int64_t stride, int64_t first, int64_t limit) {
-        const int thread = static_cast<int>(threadIdx.x);
-        if constexpr (kByRow) {
-            lead = thread % 8 * kVec;
-            slab_step = kSlab<T>;
-#pragma unroll
-            for (int i = 0; i < kChunks; ++i) {
-                const int64_t row = first + thread / 8 + i * (kThreads / 8);
-                at[i] = base + (row < limit ? row : limit - 1) * stride + lead;
-            }
-        } else {
-            lead = thread / kPerRow;
-            const int64_t column = first + thread % kPerRow * kVec;
-            const int64_t left = limit - column;
-            columns = left >= kVec ? kVec : (left > 0 ? static_cast<int>(left) : 0);
-            at[0] = base + lead * stride + column;
-            row_step = kThreads / kPerRow * stride;
-            slab_step = kSlab<T> * stride;
-        }
-    }
+    static __device__ int row() { return static_cast<int>(threadIdx.x) / kPerRow; }    // of the first chunk
+    static __device__ int chunk() { return static_cast<int>(threadIdx.x) % kPerRow ^ turn(row()); }
 
-    // Starts the loads of the next slab, of which `left` values of k exist (the rest read as 0).
-    __device__ void load(int64_t left) {
-        if constexpr (kByRow) {
-            if (left >= kSlab<T>) {
-#pragma unroll
-                for (int i = 0; i < kChunks; ++i) held[i] = load16(at[i]);
-            } else {
-                const int count = static_cast<int>(left) - lead;
-#pragma unroll
-                for (int i = 0; i < kChunks; ++i) held[i] = count > 0 ? load_some(at[i], count) : vec16{};
-            }
-#pragma unroll
-            for (int i = 0; i < kChunks; ++i) at[i] += slab_step;
-        } else {
-            constexpr int kStride = kThreads / kPerRow;
-            if (left >= kSlab<T> && columns == kVec) {
-#pragma unroll
-                for (int i = 0; i < kChunks; ++i) held[i] = load16(at[0] + i * row_step);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kChunks; ++i) {
-                    const bool inside = lead + i * kStride < left && columns > 0;
-                    held[i] = inside ? load_some(at[0] + i * row_step, columns) : vec16{};
-                }
-            }
-            at[0] += slab_step;
-        }
-    }
-
-    __device__ void store(char* lds) const {
-        const int thread = static_cast<int>(threadIdx.x);
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-            int to;
-            if constexpr (kByRow) {
-                const int row = thread / 8 + i * (kThreads / 8);
-                to = row * kSlabBytes + ((thread % 8 ^ (row >> 1 & 7)) << 4);
-            } else {
-                const int k = lead + i * (kThreads / kPerRow);
-                to = k * (kPerRow * 16) + ((thread % kPerRow ^ turn(k)) << 4);
-            }
-            *reinterpret_cast<vec16*>(lds + to) = held[i];
-        }
-    }
-
-    // The 16 bytes of k that lane l holds of row base + l % 32: k chunk 2 * step + l / 32.
+    // The 16 bytes of k that lane l holds of own index base + l % 32: k chunk 2 * step + l / 32.
     static __device__ vec16 fragment(const char* lds, int base, int step, int lane) {
         if constexpr (kByRow) {
-            const int row = base + lane % 32;
-            return *reinterpret_cast<const vec16*>(lds + row * kSlabBytes + (((2 * step + lane / 32) ^ (row >> 1 & 7)) << 4));
+            const int r = base + lane % 32;
+            return *reinterpret_cast<const vec16*>(lds + r * kSlabBytes + ((2 * step + lane / 32 ^ turn(r)) << 4));
         } else if constexpr (sizeof(T) == 4) {
             const int column = base + lane % 32, k = 8 * step + 4 * (lane / 32);
             vec16 v;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                v[i] = *reinterpret_cast<const uint32_t*>(lds + (k + i) * (kPerRow * 16) + ((column >> 2 ^ turn(k + i)) << 4) + (column & 3) * 4);
+                v[i] = *reinterpret_cast<const uint32_t*>(lds + (k + i) * (kPerRow * 16) +
+                                                          ((column >> 2 ^ turn(k + i)) << 4) + (column & 3) * 4);
             return v;
         } else {
             // Each group of 16 lanes fetches 4 rows of k times 16 columns and gets back 4 values of k of
@@ -169,11 +105,139 @@ template <class T, bool kByRow, int kRows, int kThreads> struct Operand {
     }
 };
 
-// One workgroup's tile: kWaves waves in kBM / kWM x kBN / kWN.
-template <class T, bool kAByRow, bool kBByRow, int kBM, int kBN, int kWM, int kWN> struct Tile {
+constexpr uint32_t kNowhere = 0x80000000u;          // past every buffer: such a lane's bytes arrive as 0
+constexpr int kBufferLimit = 0x7fffffff;
+constexpr int kBufferWord3 = 0x00027000;
+
+// Global to LDS without registers, 16 bytes a lane, for rows that start on 16 bytes and hold whole
+// chunks.  Offsets of a tile's chunks from its first row stay below 2^31 (checked on the host).
+template <class T, bool kByRow, int kRows, int kThreads> struct Direct : Image<T, kByRow, kRows, kThreads> {
+    using I = Image<T, kByRow, kRows, kThreads>;
+    uint32_t offset[I::kChunks];
+    const char* base;    // uniform over the workgroup
+    int64_t slab;        // bytes from slab to slab
+    int lead;            // k of the first chunk, relative to the slab
+
+    // Own indices first .. of `limit` in all; k consecutive: rows past the last read the last (their products are
+    // not stored), else columns past the last read 0.
+    __device__ void begin(const T* data, int64_t stride, int64_t first, int64_t limit, int64_t) {
+        const uint32_t pitch = static_cast<uint32_t>(stride * sizeof(T));
+        if constexpr (kByRow) {
+            base = reinterpret_cast<const char*>(data + first * stride);
+            slab = kSlabBytes;
+            lead = I::chunk() * I::kVec;
+            const int last = limit - first < kRows ? static_cast<int>(limit - first) - 1 : kRows - 1;
+#pragma unroll
+            for (int i = 0; i < I::kChunks; ++i) {
+                const int r = I::row() + i * I::kStep;
+                offset[i] = static_cast<uint32_t>(r < last ? r : last) * pitch + I::chunk() * 16;
+            }
+        } else {
+            base = reinterpret_cast<const char*>(data + first);
+            slab = kSlab<T> * stride * static_cast<int64_t>(sizeof(T));
+            lead = I::row();
+            const bool inside = first + I::chunk() * I::kVec < limit;
+#pragma unroll
+            for (int i = 0; i < I::kChunks; ++i)
+                offset[i] = inside ? static_cast<uint32_t>(lead + i * I::kStep) * pitch + I::chunk() * 16 : kNowhere;
+        }
+    }
+
+    // Queues the next slab into lds; `left` values of k exist, the rest arrive as 0.
+    __device__ void load(int64_t left, char* lds) {
+        const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, kBufferLimit, kBufferWord3);
+        char* to = lds + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64) * 1024;
+        if (left >= kSlab<T>) {
+#pragma unroll
+            for (int i = 0; i < I::kChunks; ++i)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (lds_void)(to + i * kThreads * 16), 16, offset[i], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < I::kChunks; ++i) {
+                const bool inside = (kByRow ? lead : lead + i * I::kStep) < left;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (lds_void)(to + i * kThreads * 16), 16,
+                                                         inside ? offset[i] : kNowhere, 0, 0, 0);
+            }
+        }
+        base += slab;
+    }
+    __device__ void store(char*) const {}
+};
+
+// Through registers, for rows of any alignment and length.
+template <class T, bool kByRow, int kRows, int kThreads> struct Staged : Image<T, kByRow, kRows, kThreads> {
+    using I = Image<T, kByRow, kRows, kThreads>;
+    vec16 held[I::kChunks];
+    const T* at[kByRow ? I::kChunks : 1];
+    int64_t step;        // one row per k: elements between this thread's chunks
+    int64_t slab;        // elements from slab to slab
+    int64_t before;      // elements of the row before this thread's chunk
+    int lead;            // k of the first chunk, relative to the slab
+    int columns;         // one row per k: columns of this thread's chunk inside the tensor
+
+    __device__ void begin(const T* data, int64_t stride, int64_t first, int64_t limit, int64_t) {
+        if constexpr (kByRow) {
+            lead = I::chunk() * I::kVec;
+            slab = kSlab<T>;
+            before = lead;
+            columns = I::kVec;
+#pragma unroll
+            for (int i = 0; i < I::kChunks; ++i) {
+                const int64_t r = first + I::row() + i * I::kStep;
+                at[i] = data + (r < limit ? r : limit - 1) * stride + lead;
+            }
+        } else {
+            lead = I::row();
+            before = first + I::chunk() * I::kVec;
+            const int64_t left = limit - before;
+            columns = left >= I::kVec ? I::kVec : (left > 0 ? static_cast<int>(left) : 0);
+            at[0] = data + lead * stride + before;
+            step = I::kStep * stride;
+            slab = kSlab<T> * stride;
+        }
+    }
+
+    // Starts the loads of the next slab, of which `left` values of k exist (the rest read as 0).
+    __device__ void load(int64_t left, char*) {
+        if constexpr (kByRow) {
+            if (left >= kSlab<T>) {
+#pragma unroll
+                for (int i = 0; i < I::kChunks; ++i) held[i] = load16(at[i]);
+            } else {
+                const int count = static_cast<int>(left) - lead;
+#pragma unroll
+                for (int i = 0; i < I::kChunks; ++i) held[i] = count > 0 ? load_end(at[i], count, before) : vec16{};
+            }
+#pragma unroll
+            for (int i = 0; i < I::kChunks; ++i) at[i] += slab;
+            before += slab;
+        } else {
+            if (columns == I::kVec) {
+#pragma unroll
+                for (int i = 0; i < I::kChunks; ++i)
+                    held[i] = lead + i * I::kStep < left ? load16(at[0] + i * step) : vec16{};
+            } else {
+#pragma unroll
+                for (int i = 0; i < I::kChunks; ++i)
+                    held[i] = lead + i * I::kStep < left && columns > 0
+                                  ? load_end(at[0] + i * step, columns, before) : vec16{};
+            }
+            at[0] += slab;
+        }
+    }
+
+    __device__ void store(char* lds) const {
+#pragma unroll
+        for (int i = 0; i < I::kChunks; ++i)
+            *reinterpret_cast<vec16*>(lds + (threadIdx.x + i * kThreads) * 16) = held[i];
+    }
+};
+
+// One workgroup's tile: waves of kWM x kWN, kBM / kWM x kBN / kWN of them.
+template <class T, bool kAByRow, bool kBByRow, bool kDirect, int kBM, int kBN, int kWM, int kWN> struct Tile {
     static constexpr int kThreads = 64 * (kBM / kWM) * (kBN / kWN);
-    using A = Operand<T, kAByRow, kBM, kThreads>;
-    using B = Operand<T, kBByRow, kBN, kThreads>;
+    using A = std::conditional_t<kDirect, Direct<T, kAByRow, kBM, kThreads>, Staged<T, kAByRow, kBM, kThreads>>;
+    using B = std::conditional_t<kDirect, Direct<T, kBByRow, kBN, kThreads>, Staged<T, kBByRow, kBN, kThreads>>;
     static constexpr int kMs = kWM / 32, kNs = kWN / 32;
     static constexpr int kBuffer = A::kBytes + B::kBytes;
     static constexpr int kPitch = kWN + 4;                  // floats a row of the epilogue's region
@@ -182,60 +246,74 @@ template <class T, bool kAByRow, bool kBByRow, int kBM, int kBN, int kWM, int kW
 
     accum16 acc[kMs][kNs];
 
+    static __device__ int wave() { return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64)); }
+    static __device__ int wave_row() { return wave() % (kBM / kWM) * kWM; }
+    static __device__ int wave_column() { return wave() / (kBM / kWM) * kWN; }
+
     // Sums `depth` values of k.  a and b have begun.
     __device__ void sum(A& a, B& b, int64_t depth, char* lds) {
         const int lane = static_cast<int>(threadIdx.x % 64);
-        const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64));
-        const int wm = wave % (kBM / kWM) * kWM, wn = wave / (kBM / kWM) * kWN;
+        const int wm = wave_row(), wn = wave_column();
 #pragma unroll
         for (int i = 0; i < kMs; ++i)
 #pragma unroll
             for (int j = 0; j < kNs; ++j) acc[i][j] = accum16{};
-        a.load(depth);
-        b.load(depth);
+        a.load(depth, lds);
+        b.load(depth, lds + A::kBytes);
         a.store(lds);
         b.store(lds + A::kBytes);
-        __syncthreads();
-        int buffer = 0;
-        for (int64_t k = 0; k < depth; k += kSlab<T>) {
-            const char* now = lds + buffer * kBuffer;
-            const bool more = k + kSlab<T> < depth;
+        int now = 0;
+        for (int64_t left = depth; left > 0; left -= kSlab<T>) {
+            __syncthreads();   // this slab has arrived, and no wave reads the other buffer any more
+            char* const here = lds + now * kBuffer;
+            char* const next = lds + (now ^ 1) * kBuffer;
+            const bool more = left > kSlab<T>;
             if (more) {
-                a.load(depth - k - kSlab<T>);
-                b.load(depth - k - kSlab<T>);
+                a.load(left - kSlab<T>, next);
+                b.load(left - kSlab<T>, next + A::kBytes);
             }
 #pragma unroll
             for (int step = 0; step < kSlabBytes / 32; ++step) {
                 vec16 fa[kMs], fb[kNs];
 #pragma unroll
-                for (int i = 0; i < kMs; ++i) fa[i] = A::fragment(now, wm + 32 * i, step, lane);
+                for (int i = 0; i < kMs; ++i) fa[i] = A::fragment(here, wm + 32 * i, step, lane);
 #pragma unroll
-                for (int j = 0; j < kNs; ++j) fb[j] = B::fragment(now + A::kBytes, wn + 32 * j, step, lane);
+                for (int j = 0; j < kNs; ++j) fb[j] = B::fragment(here + A::kBytes, wn + 32 * j, step, lane);
 #pragma unroll
                 for (int i = 0; i < kMs; ++i)
 #pragma unroll
                     for (int j = 0; j < kNs; ++j) acc[i][j] = multiply(T{}, fb[j], fa[i], acc[i][j]);
             }
-            buffer ^= 1;
             if (more) {
-                a.store(lds + buffer * kBuffer);
-                b.store(lds + buffer * kBuffer + A::kBytes);
+                a.store(next);
+                b.store(next + A::kBytes);
             }
-            __syncthreads();
+            now ^= 1;
         }
+        __syncthreads();
     }
 
-    // Hands out the tile's values in rows: f(row, column, value[8]) with row and column relative to the tile.
-    template <class F> __device__ void rows(char* lds, F&& f) {
+    static constexpr int kLanes = kWN / 8;                   // lanes a row of the epilogue, 8 columns each
+    static constexpr int kHeight = 64 / kLanes;              // rows a pass
+    static constexpr int kPasses = 32 / kHeight;
+    static constexpr int kGroup = kPasses < 4 ? kPasses : 4; // passes handed out together
+
+    static __device__ int own_column() { return wave_column() + static_cast<int>(threadIdx.x % kLanes) * 8; }
+
+    // Hands out the tile's values: a lane's are the 8 columns from own_column() on of kGroup rows at a time, row,
+    // row + kHeight, ... (relative to the tile).
+    //   fetch(row) -> what use needs from memory for these rows, asked for a group ahead of
+    //   use(row, value[kGroup][8], fetched)
+    template <class Fetch, class Use> __device__ void rows(char* lds, Fetch&& fetch, Use&& use) {
         const int lane = static_cast<int>(threadIdx.x % 64);
-        const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64));
-        const int wm = wave % (kBM / kWM) * kWM, wn = wave / (kBM / kWM) * kWN;
-        float* region = reinterpret_cast<float*>(lds + wave * kRegion);
-        constexpr int kLanes = kWN / 8, kPass = 64 / kLanes;
+        float* region = reinterpret_cast<float*>(lds + wave() * kRegion);
+        const float* from = region + lane / kLanes * kPitch + lane % kLanes * 8;
+        // accumulator element v of lane l: row l % 32, column 8 (v / 4) + 4 (l / 32) + v % 4
+        float* to = region + lane % 32 * kPitch + lane / 32 * 4;
 #pragma unroll
         for (int i = 0; i < kMs; ++i) {
-            // accumulator element v of lane l: row l % 32, column 8 (v / 4) + 4 (l / 32) + v % 4
-            float* to = region + lane % 32 * kPitch + lane / 32 * 4;
+            const int row = wave_row() + 32 * i + lane / kLanes;
+            auto fetched = fetch(row);
 #pragma unroll
             for (int j = 0; j < kNs; ++j)
 #pragma unroll
@@ -243,13 +321,20 @@ template <class T, bool kAByRow, bool kBByRow, int kBM, int kBN, int kWM, int kW
                     *reinterpret_cast<float4*>(to + 32 * j + 8 * q) =
                         make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
             wave_fence();
+#pragma unroll 1
+            for (int pass = 0; pass < kPasses; pass += kGroup) {
+                auto ahead = fetched;
+                if (pass + kGroup < kPasses) ahead = fetch(row + (pass + kGroup) * kHeight);
+                float value[kGroup][8];
 #pragma unroll
-            for (int pass = 0; pass < 32 / kPass; ++pass) {
-                const int row = pass * kPass + lane / kLanes, column = lane % kLanes * 8;
-                const float* from = region + row * kPitch + column;
-                const float4 lo = *reinterpret_cast<const float4*>(from), hi = *reinterpret_cast<const float4*>(from + 4);
-                float value[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                f(wm + 32 * i + row, wn + column, value);
+                for (int u = 0; u < kGroup; ++u) {
+                    const float* p = from + (pass + u) * kHeight * kPitch;
+                    const float4 lo = *reinterpret_cast<const float4*>(p), hi = *reinterpret_cast<const float4*>(p + 4);
+                    value[u][0] = lo.x, value[u][1] = lo.y, value[u][2] = lo.z, value[u][3] = lo.w;
+                    value[u][4] = hi.x, value[u][5] = hi.y, value[u][6] = hi.z, value[u][7] = hi.w;
+                }
+                use(row + pass * kHeight, value, fetched);
+                fetched = ahead;
             }
             wave_fence();
         }
@@ -258,30 +343,78 @@ template <class T, bool kAByRow, bool kBByRow, int kBM, int kBN, int kWM, int kW
 
 enum Activation { kNone = 0, kRelu, kSigmoid, kSoftplus, kGelu, kSilu, kActivations };
 
-// exp of the negated absolute value never overflows; a NaN stays one.
-__device__ inline float activate(int activation, float z) {
-    switch (activation) {
-        case kRelu: return z < 0.0f ? 0.0f : z;
-        case kSigmoid: return 1.0f / (1.0f + expf(-z));
-        case kSoftplus: return (z > 0.0f ? z : 0.0f) + log1pf(expf(-fabsf(z)));
-        case kGelu: return 0.5f * z * erfcf(-0.70710678f * z);
-        case kSilu: return z / (1.0f + expf(-z));
-        default: return z;
-    }
+// Activations and their slopes in fp32.  A NaN stays one.
+// kExact, for fp32 tensors: the library's exp, log1p and erfc.  Otherwise, for values that are rounded to
+// 16 bits: the hardware's exp2, log2 and reciprocal (1 ulp each) and, for erfc, Abramowitz and Stegun,
+// Handbook of Mathematical Functions, 7.1.26 (off by at most 1.5e-7), which shares its exp(-z^2 / 2)
+// with the slope: on 65536 x 4096 the gelu's slope would otherwise be bound by its arithmetic, not by HBM.
+template <bool kExact> __device__ inline float exp_of(float x) {
+    if constexpr (kExact) return expf(x);
+    return __builtin_amdgcn_exp2f(x * 1.44269504f);
+}
+template <bool kExact> __device__ inline float inverse(float x) {
+    if constexpr (kExact) return 1.0f / x;
+    return __builtin_amdgcn_rcpf(x);
 }
 
-// Derivative at z.
-__device__ inline float slope(int activation, float z) {
+// The normal distribution at z, and exp(-z^2 / 2).
+template <bool kExact> __device__ inline float normal_below(float z, float& bell) {
+    bell = exp_of<kExact>(-0.5f * z * z);
+    if constexpr (kExact) return 0.5f * erfcf(-0.70710678f * z);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.70710678f * 0.3275911f, fabsf(z), 1.0f));
+    float p = fmaf(t, 1.061405429f, -1.453152027f);
+    p = fmaf(t, p, 1.421413741f);
+    p = fmaf(t, p, -0.284496736f);
+    p = fmaf(t, p, 0.254829592f);
+    const float above = 0.5f * t * p * bell;   // beyond |z|
+    return z < 0.0f ? above : 1.0f - above;
+}
+
+template <int kActivation, bool kExact> __device__ inline float activate(float z) {
+    if constexpr (kActivation == kRelu) return z < 0.0f ? 0.0f : z;
+    if constexpr (kActivation == kSigmoid) return inverse<kExact>(1.0f + exp_of<kExact>(-z));
+    if constexpr (kActivation == kSoftplus) {
+        const float e = exp_of<kExact>(-fabsf(z)), top = z > 0.0f ? z : 0.0f;
+        if constexpr (kExact) return top + log1pf(e);
+        const float log = e < 0.015625f ? e * fmaf(e, fmaf(e, 0.33333333f, -0.5f), 1.0f)
+                                        : 0.69314718f * __builtin_amdgcn_logf(1.0f + e);
+        return top + log;
+    }
+    if constexpr (kActivation == kGelu) {
+        float bell;
+        return z * normal_below<kExact>(z, bell);
+    }
+    if constexpr (kActivation == kSilu) return z * inverse<kExact>(1.0f + exp_of<kExact>(-z));
+    return z;
+}
+
+template <int kActivation, bool kExact> __device__ inline float slope(float z) {
+    if constexpr (kActivation == kRelu) return z > 0.0f ? 1.0f : 0.0f;
+    if constexpr (kActivation == kGelu) {
+        float bell;
+        const float below = normal_below<kExact>(z, bell);
+        return fmaf(z * 0.39894228f, bell, below);
+    }
+    if constexpr (kActivation == kSigmoid || kActivation == kSoftplus || kActivation == kSilu) {
+        // sigmoid(|z|) and sigmoid(-|z|), neither by a difference
+        const float e = exp_of<kExact>(-fabsf(z)), more = inverse<kExact>(1.0f + e), less = e * more;
+        if constexpr (kActivation == kSigmoid) return more * less;
+        const float s = z < 0.0f ? less : more;
+        if constexpr (kActivation == kSoftplus) return s;
+        return s * fmaf(z, z < 0.0f ? more : less, 1.0f);
+    }
+    return 1.0f;
+}
+
+// f<kActivation>() for the activation of this launch: one branch, the same for every lane.
+template <class F> __device__ inline void with_activation(int activation, F&& f) {
     switch (activation) {
-        case kRelu: return z > 0.0f ? 1.0f : 0.0f;
-        case kSigmoid: return 1.0f / ((1.0f + expf(-z)) * (1.0f + expf(z)));
-        case kSoftplus: return 1.0f / (1.0f + expf(-z));
-        case kGelu: return 0.5f * erfcf(-0.70710678f * z) + z * 0.39894228f * expf(-0.5f * z * z);
-        case kSilu: {
-            const float s = 1.0f / (1.0f + expf(-z));
-            return s * (1.0f + z / (1.0f + expf(z)));
-        }
-        default: return 1.0f;
+        case kRelu: return f(std::integral_constant<int, kRelu>{});
+        case kSigmoid: return f(std::integral_constant<int, kSigmoid>{});
+        case kSoftplus: return f(std::integral_constant<int, kSoftplus>{});
+        case kGelu: return f(std::integral_constant<int, kGelu>{});
+        case kSilu: return f(std::integral_constant<int, kSilu>{});
+        default: return f(std::integral_constant<int, kNone>{});
     }
 }
 
@@ -329,6 +462,13 @@ struct FoldArgs {             // out[e][i] = sum over e's pieces of partial[piec
     int experts;
     bool single;              // also the groups of one piece (and zeros for those of none)
 };
+
+// Edge of the weight gradient's tiles.
+inline int weight_edge(int outputs, int inputs) {
+    const int least = outputs < inputs ? outputs : inputs;
+    if (least <= 64) return 64;
+    return static_cast<int64_t>(outputs) * inputs >= int64_t{1} << 20 ? 256 : 128;
+}
 
 // Launches, per element type.
 template <class T> int launch_rows(const RowsArgs& a, bool forward, hipStream_t stream);

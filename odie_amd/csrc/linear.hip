@@ -19,18 +19,20 @@ constexpr int64_t kMaxRows = (int64_t{1} << 31) - 1;
 constexpr int kMaxWidth = 1 << 20;
 constexpr int kMaxExperts = 1 << 15;
 
-// Rows a bias piece sums: long enough that the partial sums stay small beside dz, short enough for a
-// few workgroups on every CU.
-int64_t slope_piece(int64_t rows) {
-    const int64_t piece = (rows / (4 * kCus) + 63) / 64 * 64;
-    return piece < 64 ? 64 : (piece > 1024 ? 1024 : piece);
+// Rows a piece of the slope pass takes (and a partial bias sums): about eight workgroups a CU, each of
+// them of at most 256 columns.
+int64_t slope_piece(int64_t rows, int outputs) {
+    const int64_t across = (outputs + 255) / 256;
+    const int64_t piece = (rows * across / (8 * kCus) + 63) / 64 * 64;
+    return piece < 64 ? 64 : piece;
 }
 
-// Rows a weight piece sums: about four workgroups a CU over all experts and tiles.
+// Rows a weight piece sums: workgroups for every CU over all experts and tiles (one a CU of the largest tiles).
 int64_t weight_piece(int64_t rows, int experts, int outputs, int inputs) {
-    const int edge = outputs <= 64 || inputs <= 64 ? 64 : 128;
+    const int edge = weight_edge(outputs, inputs);
     const int64_t tiles = static_cast<int64_t>((outputs + edge - 1) / edge) * ((inputs + edge - 1) / edge);
-    int64_t pieces = 4 * kCus / tiles - experts;
+    const int64_t wanted = (edge == 256 ? 1 : 4) * kCus;
+    int64_t pieces = wanted / tiles - (experts > 1 ? experts : 0);
     if (pieces < 1) pieces = experts > 1 ? 4 : 1;
     int64_t piece = ((rows + pieces - 1) / pieces + 255) / 256 * 256;
     return piece < 256 ? 256 : piece;
@@ -46,7 +48,7 @@ int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 Plan make_plan(int64_t rows, int experts, bool grouped, int outputs, int inputs, int dtype, int activation,
                bool want_dweight, bool want_dbias) {
     Plan p{};
-    p.slope_piece = slope_piece(rows);
+    p.slope_piece = slope_piece(rows, outputs);
     p.slope_pieces = piece_ids(rows, p.slope_piece, grouped && want_dbias, experts, false);
     p.weight_piece = weight_piece(rows, experts, outputs, inputs);
     p.weight_pieces = piece_ids(rows, p.weight_piece, grouped, experts, false);

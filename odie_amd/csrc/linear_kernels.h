@@ -5,22 +5,30 @@
 namespace odie {
 namespace {
 
-// Tiles: 128 x 128 with 64 x 64 a wave; 128 x 64 with 32 x 64 a wave for narrow outputs; 64 x 64 with 32 x 32 a
-// wave where there are too few tiles otherwise.
-template <class T, bool kAByRow, bool kBByRow> using Wide = Tile<T, kAByRow, kBByRow, 128, 128, 64, 64>;
-template <class T, bool kAByRow, bool kBByRow> using Narrow = Tile<T, kAByRow, kBByRow, 128, 64, 32, 64>;
-template <class T, bool kAByRow, bool kBByRow> using Small = Tile<T, kAByRow, kBByRow, 64, 64, 32, 32>;
+constexpr uint32_t kBand = 4;
 
-template <class T, bool kForward, int kBM, int kBN, int kWM, int kWN>
+struct TileAt {
+    uint32_t row, column;
+};
+
+// Tiles in bands of kBand rows, down each band's columns first: tiles that run at the same time on an XCD
+// form a block of about kBand by 8, and read the fewest rows of both operands through its L2.
+__device__ inline TileAt tile_at(uint32_t id, uint32_t down, uint32_t across) {
+    const uint32_t band = id / (kBand * across), inside = id - band * kBand * across;
+    const uint32_t high = down - band * kBand < kBand ? down - band * kBand : kBand;
+    return TileAt{band * kBand + inside % high, inside / high};
+}
+
+template <class T, bool kForward, bool kDirect, int kBM, int kBN, int kWM, int kWN>
 __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(RowsArgs a, uint32_t blocks) {
-    using Work = Tile<T, true, kForward, kBM, kBN, kWM, kWN>;
+    using Work = Tile<T, true, kForward, kDirect, kBM, kBN, kWM, kWN>;
     __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
     const uint32_t id = xcd_major(blockIdx.x, gridDim.x);
     if (id >= blocks) return;
-    const uint32_t across = (a.columns + kBN - 1) / kBN;
-    const Piece p = find_piece(a.offsets, a.experts, a.experts + 1, a.rows, kBM, id / across);
+    const TileAt t = tile_at(id, static_cast<uint32_t>(a.tiles), (a.columns + kBN - 1) / kBN);
+    const Piece p = find_piece(a.offsets, a.experts, a.experts + 1, a.rows, kBM, t.row);
     if (p.begin >= p.end) return;
-    const int column0 = static_cast<int>(id % across) * kBN;
+    const int column0 = static_cast<int>(t.column) * kBN;
     const T* residual = static_cast<const T*>(a.residual);
     T* out = static_cast<T*>(a.out);
     if (p.group >= a.experts) {   // rows of no expert
@@ -38,67 +46,99 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(Ro
     const T* b = static_cast<const T*>(a.b) + p.group * matrix;
     typename Work::A opa;
     typename Work::B opb;
-    opa.begin(static_cast<const T*>(a.a), a.lda, p.begin, p.end);
-    opb.begin(b, kForward ? a.depth : a.columns, column0, a.columns);
+    opa.begin(static_cast<const T*>(a.a), a.lda, p.begin, p.end, a.depth);
+    opb.begin(b, kForward ? a.depth : a.columns, column0, a.columns, a.depth);
     Work work;
     work.sum(opa, opb, a.depth, lds);
     const T* bias = a.bias ? static_cast<const T*>(a.bias) + static_cast<int64_t>(p.group) * a.columns : nullptr;
     T* pre = static_cast<T*>(a.pre);
-    work.rows(lds, [&](int r, int c, float value[8]) {
-        const int64_t row = p.begin + r;
-        const int column = column0 + c, count = a.columns - column;
-        if (row >= p.end || count <= 0) return;
-        float more[8];
-        if (bias) {
-            load8(bias + column, count, more);
+    constexpr int kGroup = Work::kGroup, kHeight = Work::kHeight;
+    struct Fetched {
+        Eight<T> row[kGroup];
+    };
+    const int column = column0 + Work::own_column(), count = a.columns - column;   // the lane's through every row
+    float shift[8] = {};
+    if (bias && count > 0) load8(bias + column, count, shift);
+    work.rows(
+        lds,
+        [&](int r) {
+            Fetched f{};
+            if (residual && count > 0)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) value[i] += more[i];
-        }
-        if (pre) store8(pre + row * a.columns + column, count, value);
-        if (a.activation != kNone) {
+                for (int u = 0; u < kGroup; ++u) {
+                    const int64_t row = p.begin + r + u * kHeight;
+                    if (row < p.end) f.row[u].load(residual + row * a.ldr + column, count);
+                }
+            return f;
+        },
+        [&](int r, float value[kGroup][8], const Fetched& f) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) value[i] = activate(a.activation, value[i]);
-        }
-        if (residual) {
-            load8(residual + row * a.ldr + column, count, more);
+            for (int u = 0; u < kGroup; ++u)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) value[i] += more[i];
-        }
-        store8(out + row * a.ldo + column, count, value);
-    });
+                for (int i = 0; i < 8; ++i) value[u][i] += shift[i];
+            if (pre && count > 0)
+#pragma unroll
+                for (int u = 0; u < kGroup; ++u) {
+                    const int64_t row = p.begin + r + u * kHeight;
+                    if (row < p.end) store8(pre + row * a.columns + column, count, value[u]);
+                }
+            with_activation(a.activation, [&](auto activation) {
+#pragma unroll
+                for (int u = 0; u < kGroup; ++u)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) value[u][i] = activate<activation, sizeof(T) == 4>(value[u][i]);
+            });
+#pragma unroll
+            for (int u = 0; u < kGroup; ++u) {
+                const int64_t row = p.begin + r + u * kHeight;
+                if (row >= p.end || count <= 0) continue;
+                if (residual) {
+                    float more[8];
+                    f.row[u].get(more);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) value[u][i] += more[i];
+                }
+                store8(out + row * a.ldo + column, count, value[u]);
+            }
+        });
 }
 
-template <class T, int kBM, int kBN, int kWM, int kWN>
+template <class T, bool kDirect, int kBM, int kBN, int kWM, int kWN>
 __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void weight_kernel(WeightArgs a, uint32_t blocks) {
-    using Work = Tile<T, false, false, kBM, kBN, kWM, kWN>;
+    using Work = Tile<T, false, false, kDirect, kBM, kBN, kWM, kWN>;
     __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
     const uint32_t id = xcd_major(blockIdx.x, gridDim.x);
     if (id >= blocks) return;
-    const uint32_t across = (a.inputs + kBN - 1) / kBN, tiles = (a.outputs + kBM - 1) / kBM * across;
-    const uint32_t piece = id / tiles, tile = id % tiles;
+    const uint32_t across = (a.inputs + kBN - 1) / kBN, down = (a.outputs + kBM - 1) / kBM;
+    const uint32_t piece = id / (down * across);
+    const TileAt t = tile_at(id % (down * across), down, across);
     const Piece p = find_piece(a.offsets, a.experts, a.experts, a.rows, a.piece, piece);
     if (p.first > 0 && p.begin >= p.end) return;
-    const int row0 = static_cast<int>(tile / across) * kBM, column0 = static_cast<int>(tile % across) * kBN;
+    const int row0 = static_cast<int>(t.row) * kBM, column0 = static_cast<int>(t.column) * kBN;
     Work work;
     const int64_t depth = p.end > p.begin ? p.end - p.begin : 0;
     typename Work::A opa;
     typename Work::B opb;
-    opa.begin(static_cast<const T*>(a.dz) + p.begin * a.ldz, a.ldz, row0, a.outputs);
-    opb.begin(static_cast<const T*>(a.x) + p.begin * a.ldx, a.ldx, column0, a.inputs);
+    opa.begin(static_cast<const T*>(a.dz) + p.begin * a.ldz, a.ldz, row0, a.outputs, depth);
+    opb.begin(static_cast<const T*>(a.x) + p.begin * a.ldx, a.ldx, column0, a.inputs, depth);
     work.sum(opa, opb, depth, lds);   // no rows: zeros
     const int64_t matrix = static_cast<int64_t>(a.outputs) * a.inputs;
     const bool whole = p.group_end - p.group_begin <= a.piece;
     T* dw = static_cast<T*>(a.dw) + p.group * matrix;
     float* partial = whole ? nullptr : a.partial + piece * matrix;
-    work.rows(lds, [&](int r, int c, float value[8]) {
-        const int row = row0 + r, column = column0 + c, count = a.inputs - column;
-        if (row >= a.outputs || count <= 0) return;
-        const int64_t at = static_cast<int64_t>(row) * a.inputs + column;
-        if (whole)
-            store8(dw + at, count, value);
-        else
-            store8(partial + at, count, value);
-    });
+    const int column = column0 + Work::own_column(), count = a.inputs - column;
+    work.rows(
+        lds, [](int) { return 0; },
+        [&](int r, float value[Work::kGroup][8], int) {
+#pragma unroll
+            for (int u = 0; u < Work::kGroup; ++u) {
+                const int row = row0 + r + u * Work::kHeight;
+                if (row >= a.outputs || count <= 0) continue;
+                const int64_t at = static_cast<int64_t>(row) * a.inputs + column;
+                if (whole) store8(dw + at, count, value[u]);
+                else store8(partial + at, count, value[u]);
+            }
+        });
 }
 
 constexpr int kSlopeBlock = 256;
@@ -115,19 +155,31 @@ template <class T> __global__ __launch_bounds__(kSlopeBlock) void slope_kernel(S
         const T* dy = static_cast<const T*>(a.dy);
         const T* pre = static_cast<const T*>(a.pre);
         T* dz = static_cast<T*>(a.dz);
-        for (int64_t row = p.begin + static_cast<int>(threadIdx.x) / lanes; row < p.end; row += height) {
-            float d[8];
-            load8(dy + row * a.ldy + column, count, d);
-            if (dz) {
-                float z[8];
-                load8(pre + row * a.columns + column, count, z);
+        const int64_t start = p.begin + static_cast<int>(threadIdx.x) / lanes;
+        constexpr int kAhead = 4;   // rows whose loads are in flight together
+        with_activation(dz ? a.activation : kNone, [&](auto activation) {
+            for (int64_t row = start; row < p.end; row += kAhead * height) {
+                float d[kAhead][8], z[kAhead][8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] *= slope(a.activation, z[i]);
-                store8(dz + row * a.columns + column, count, d);
+                for (int u = 0; u < kAhead; ++u) {
+                    const int64_t r = row + u * height < p.end ? row + u * height : row;
+                    load8(dy + r * a.ldy + column, count, d[u]);
+                    if (activation != kNone) load8(pre + r * a.columns + column, count, z[u]);
+                }
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int64_t r = row + u * height;
+                    if (r >= p.end) break;
+                    if (activation != kNone) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) d[u][i] *= slope<activation, sizeof(T) == 4>(z[u][i]);
+                        store8(dz + r * a.columns + column, count, d[u]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum[i] += d[u][i];
+                }
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] += d[i];
-        }
+        });
     }
     if (!a.sums) return;
 #pragma unroll
@@ -142,45 +194,76 @@ template <class T> __global__ __launch_bounds__(kSlopeBlock) void slope_kernel(S
     }
 }
 
-template <class T> __global__ __launch_bounds__(256) void fold_kernel(FoldArgs a) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (i >= a.size) return;
+// A workgroup takes 256 / kGroups elements; its groups take every kGroups-th piece, added up at the end in order.
+template <class T, int kGroups> __global__ __launch_bounds__(256) void fold_kernel(FoldArgs a) {
+    constexpr int kLanes = 256 / kGroups;
+    __shared__ float total[kGroups > 1 ? 256 : 1];
+    const int lane = static_cast<int>(threadIdx.x) % kLanes, group = static_cast<int>(threadIdx.x) / kLanes;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kLanes + lane;
     const int e = static_cast<int>(blockIdx.y);
     const int64_t begin = a.offsets ? group_start(a.offsets, e, a.rows) : 0;
     const int64_t end = a.offsets ? group_start(a.offsets, e + 1, a.rows) : a.rows;
     const int64_t first = a.offsets ? whole_pieces(a.offsets, e, a.rows, a.piece) + e : 0;
     const int64_t pieces = end > begin ? (end - begin + a.piece - 1) / a.piece : 0;
     if (pieces <= 1 && !a.single) return;
-    const float* from = a.partial + first * a.size + i;
     float sum = 0.0f;
-    for (int64_t p = 0; p < pieces; ++p) sum += from[p * a.size];
-    static_cast<T*>(a.out)[e * a.size + i] = static_cast<T>(sum);
+    if (i < a.size) {
+        const float* from = a.partial + first * a.size + i;
+#pragma unroll 4
+        for (int64_t p = group; p < pieces; p += kGroups) sum += from[p * a.size];
+    }
+    if constexpr (kGroups > 1) {
+        total[threadIdx.x] = sum;
+        __syncthreads();
+        if (group > 0) return;
+        for (int g = 1; g < kGroups; ++g) sum += total[g * kLanes + lane];
+    }
+    if (i < a.size) static_cast<T*>(a.out)[e * a.size + i] = static_cast<T>(sum);
 }
 
 uint32_t whole_xcds(int64_t blocks) { return static_cast<uint32_t>((blocks + kXcds - 1) / kXcds * kXcds); }
 
-template <class T, bool kForward, int kBM, int kBN, int kWM, int kWN> int launch_rows_as(RowsArgs a, hipStream_t stream) {
+template <class T, bool kForward, bool kDirect, int kBM, int kBN, int kWM, int kWN> int launch_rows_as(RowsArgs a, hipStream_t stream) {
     const int64_t across = (a.columns + kBN - 1) / kBN;
     a.tiles = piece_ids(a.rows, kBM, a.offsets != nullptr, a.experts, true);
     const int64_t blocks = a.tiles * across;
     if (blocks >= int64_t{1} << 31) return fail("linear: too many tiles for one launch");
-    rows_kernel<T, kForward, kBM, kBN, kWM, kWN>
+    rows_kernel<T, kForward, kDirect, kBM, kBN, kWM, kWN>
         <<<whole_xcds(blocks), 64 * (kBM / kWM) * (kBN / kWN), 0, stream>>>(a, static_cast<uint32_t>(blocks));
     return check_launch("linear");
 }
 
-template <class T, bool kForward> int launch_rows_of(const RowsArgs& a, hipStream_t stream) {
-    const int64_t wide = (a.rows + 127) / 128 * ((a.columns + 127) / 128);
-    if (a.columns <= 64 && a.rows >= 128 * kCus) return launch_rows_as<T, kForward, 128, 64, 32, 64>(a, stream);
-    if (a.columns > 64 && wide >= kCus) return launch_rows_as<T, kForward, 128, 128, 64, 64>(a, stream);
-    return launch_rows_as<T, kForward, 64, 64, 32, 32>(a, stream);
+// Whether rows of `width` elements can go to LDS directly, 16 bytes a lane.
+template <class T> bool direct(const void* data, int64_t stride, int64_t width) {
+    const int64_t pitch = stride * static_cast<int64_t>(sizeof(T));
+    return reinterpret_cast<uintptr_t>(data) % 16 == 0 && pitch % 16 == 0 && width % kPerVec<T> == 0 &&
+           pitch < (int64_t{1} << 22);   // 256 rows of a tile within 2^30 bytes
 }
 
-template <class T, int kBM, int kBN, int kWM, int kWN> int launch_weight_as(const WeightArgs& a, hipStream_t stream) {
+// Tiles by the work there is (us of one bf16 product, 65536 x 1024 x 4096 and 65536 x 256 x 512):
+//   256 x 256, 64 x 128 a wave   620, 33   where every CU gets one and a group's rows fill them (the path
+//                                          through registers has no room for it)
+//   128 x 128, 64 x 64 a wave    777, 30   two a CU
+//   128 x 64, 32 x 64 a wave     narrow outputs: no columns wasted
+//   64 x 64, 32 x 32 a wave      what is left: too few tiles otherwise
+template <class T, bool kForward, bool kDirect> int launch_rows_of(const RowsArgs& a, hipStream_t stream) {
+    const int64_t each = a.rows / a.experts;   // rows of a group, on average
+    const int64_t large = (a.rows + 255) / 256 * ((a.columns + 255) / 256);
+    const int64_t wide = (a.rows + 127) / 128 * ((a.columns + 127) / 128);
+    if constexpr (kDirect)
+        if (a.columns > 128 && large >= kCus && each >= 1024)
+            return launch_rows_as<T, kForward, true, 256, 256, 64, 128>(a, stream);
+    if (a.columns <= 64 && a.rows >= 128 * kCus) return launch_rows_as<T, kForward, kDirect, 128, 64, 32, 64>(a, stream);
+    if (a.columns > 64 && wide >= kCus && each >= 128)
+        return launch_rows_as<T, kForward, kDirect, 128, 128, 64, 64>(a, stream);
+    return launch_rows_as<T, kForward, kDirect, 64, 64, 32, 32>(a, stream);
+}
+
+template <class T, bool kDirect, int kBM, int kBN, int kWM, int kWN> int launch_weight_as(const WeightArgs& a, hipStream_t stream) {
     const int64_t tiles = static_cast<int64_t>((a.outputs + kBM - 1) / kBM) * ((a.inputs + kBN - 1) / kBN);
     const int64_t blocks = a.pieces * tiles;
     if (blocks >= int64_t{1} << 31) return fail("linear: too many tiles for one launch");
-    weight_kernel<T, kBM, kBN, kWM, kWN>
+    weight_kernel<T, kDirect, kBM, kBN, kWM, kWN>
         <<<whole_xcds(blocks), 64 * (kBM / kWM) * (kBN / kWN), 0, stream>>>(a, static_cast<uint32_t>(blocks));
     return check_launch("linear weight gradient");
 }
@@ -188,12 +271,25 @@ template <class T, int kBM, int kBN, int kWM, int kWN> int launch_weight_as(cons
 }  // namespace
 
 template <class T> int launch_rows(const RowsArgs& a, bool forward, hipStream_t stream) {
-    return forward ? launch_rows_of<T, true>(a, stream) : launch_rows_of<T, false>(a, stream);
+    const bool straight = direct<T>(a.a, a.lda, a.depth) && direct<T>(a.b, forward ? a.depth : a.columns, a.depth) &&
+                          a.columns % (forward ? 1 : kPerVec<T>) == 0;
+    if (forward) return straight ? launch_rows_of<T, true, true>(a, stream) : launch_rows_of<T, true, false>(a, stream);
+    return straight ? launch_rows_of<T, false, true>(a, stream) : launch_rows_of<T, false, false>(a, stream);
+}
+
+template <class T, bool kDirect> int launch_weight_of(const WeightArgs& a, hipStream_t stream) {
+    switch (weight_edge(a.outputs, a.inputs)) {
+        case 256:
+            if constexpr (kDirect) return launch_weight_as<T, true, 256, 256, 64, 128>(a, stream);
+            [[fallthrough]];
+        case 128: return launch_weight_as<T, kDirect, 128, 128, 64, 64>(a, stream);
+        default: return launch_weight_as<T, kDirect, 64, 64, 32, 32>(a, stream);
+    }
 }
 
 template <class T> int launch_weight(const WeightArgs& a, hipStream_t stream) {
-    if (a.outputs <= 64 || a.inputs <= 64) return launch_weight_as<T, 64, 64, 32, 32>(a, stream);
-    return launch_weight_as<T, 128, 128, 64, 64>(a, stream);
+    const bool straight = direct<T>(a.dz, a.ldz, a.outputs) && direct<T>(a.x, a.ldx, a.inputs);
+    return straight ? launch_weight_of<T, true>(a, stream) : launch_weight_of<T, false>(a, stream);
 }
 
 template <class T> int launch_slope(const SlopeArgs& a, hipStream_t stream) {
@@ -208,9 +304,13 @@ template <class T> int launch_slope(const SlopeArgs& a, hipStream_t stream) {
 }
 
 template <class T> int launch_fold(const FoldArgs& a, hipStream_t stream) {
-    if ((a.size + 255) / 256 >= int64_t{1} << 31) return fail("linear: too many sums for one launch");
-    const dim3 grid(static_cast<uint32_t>((a.size + 255) / 256), static_cast<uint32_t>(a.experts));
-    fold_kernel<T><<<grid, 256, 0, stream>>>(a);
+    // many pieces of few elements (a bias): several groups share them
+    const bool tall = a.rows / a.piece >= 8 * static_cast<int64_t>(a.experts);
+    const int64_t lanes = tall ? 16 : 256, blocks = (a.size + lanes - 1) / lanes;
+    if (blocks >= int64_t{1} << 31) return fail("linear: too many sums for one launch");
+    const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(a.experts));
+    if (tall) fold_kernel<T, 16><<<grid, 256, 0, stream>>>(a);
+    else fold_kernel<T, 1><<<grid, 256, 0, stream>>>(a);
     return check_launch("linear fold");
 }
 
