@@ -584,7 +584,8 @@ int odie_rows_dispatch(const void* x, int64_t x_stride, const int32_t* slots, co
                        int choices, int experts, int64_t width, int dtype, void* out, uint64_t stream);
 
 /* Rows back from their slots: out[i] = sum over j of weights[f] * rows[slots[f]], out [n][width];
- * weights fp32 [n * choices], or null: 1 (the gradient of odie_rows_dispatch). */
+ * slots: odie_sort's, -1 for an entry that adds nothing; weights fp32 [n * choices], or null: 1 (the
+ * gradient of odie_rows_dispatch). */
 int odie_rows_combine(const void* rows, int64_t rows_stride, const int32_t* slots, const float* weights, int64_t n,
                       int choices, int64_t width, int dtype, void* out, uint64_t stream);
 

@@ -66,6 +66,30 @@ template <class T> __device__ inline void store_some(T* p, const vec16& v, int c
     else scatter16(p, v, count);
 }
 
+// A row of `width` elements as ceil(width / kPerVec) chunks of 16 bytes.  The last chunk ends with the row:
+// where the width is no multiple it begins inside the chunk before it, and writes the same values there
+// again.  Only a row shorter than a chunk goes element by element.
+template <class T> __device__ inline int chunk_column(int chunk, int width) {
+    const int column = chunk * kPerVec<T>, last = width - kPerVec<T>;
+    return column < last || last < 0 ? column : last;
+}
+
+// Elements of the chunk that the chunk before it holds as well.
+template <class T> __device__ inline int chunk_overlap(int chunk, int width) {
+    return chunk * kPerVec<T> - chunk_column<T>(chunk, width);
+}
+
+template <class T> __device__ inline vec16 load_chunk(const T* row, int chunk, int width) {
+    const T* p = row + chunk_column<T>(chunk, width);
+    return width >= kPerVec<T> ? load16(p) : gather16(p, width);
+}
+
+template <class T> __device__ inline void store_chunk(T* row, int chunk, int width, const vec16& v) {
+    T* p = row + chunk_column<T>(chunk, width);
+    if (width >= kPerVec<T>) store16(p, v);
+    else scatter16(p, v, width);
+}
+
 // v moved down by `bytes` (0..15), zeros above.
 __device__ inline vec16 shift_down(const vec16& v, int bytes) {
     uint64_t low = static_cast<uint64_t>(v.y) << 32 | v.x, high = static_cast<uint64_t>(v.w) << 32 | v.z;
@@ -98,10 +122,17 @@ template <class T> __device__ inline void widen(const vec16& v, float out[kPerVe
     for (int i = 0; i < kPerVec<T>; ++i) out[i] = static_cast<float>(e[i]);
 }
 
+// Rounds fp32 values.  They are materialised first: folded into the conversion, a product or sum is rounded
+// once instead of twice, and the compiler does so for some places of a vector and not for others, so that
+// an element's value would depend on where in a chunk it lies.
 template <class T> __device__ inline vec16 narrow(const float in[kPerVec<T>]) {
     T e[kPerVec<T>];
 #pragma unroll
-    for (int i = 0; i < kPerVec<T>; ++i) e[i] = static_cast<T>(in[i]);
+    for (int i = 0; i < kPerVec<T>; ++i) {
+        float value = in[i];
+        asm("" : "+v"(value));
+        e[i] = static_cast<T>(value);
+    }
     vec16 v;
     __builtin_memcpy(&v, e, 16);
     return v;

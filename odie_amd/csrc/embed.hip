@@ -34,27 +34,36 @@ template <class T> __global__ __launch_bounds__(kEmbedBlock) void lookup_kernel(
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.block_rows;
     const int64_t left = a.n - row0;
     const uint32_t items = (left < a.block_rows ? static_cast<uint32_t>(left) : a.block_rows) * a.chunks;
-    for (uint32_t t = threadIdx.x; t < items; t += kEmbedBlock) {
-        const uint32_t r = divide(t, a.by_chunks);
-        const int column = static_cast<int>(t - r * a.chunks) * kPerVec<T>, count = a.width - column;
-        const int64_t i = row0 + r;
-        const int64_t id = a.id_bytes == 8 ? static_cast<const int64_t*>(a.ids)[i] : static_cast<const int32_t*>(a.ids)[i];
-        vec16 v{};
-        if (id >= 0 && id < a.vocab) {
+    constexpr int kAhead = 4;   // chunks a thread has in flight
+    for (uint32_t t = threadIdx.x; t < items; t += kAhead * kEmbedBlock) {
+        vec16 v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const uint32_t item = t + u * kEmbedBlock < items ? t + u * kEmbedBlock : t;
+            const uint32_t r = divide(item, a.by_chunks);
+            const int64_t i = row0 + r;
+            const int64_t id = a.id_bytes == 8 ? static_cast<const int64_t*>(a.ids)[i] : static_cast<const int32_t*>(a.ids)[i];
+            v[u] = vec16{};
+            if (id >= 0 && id < a.vocab)
+                v[u] = load_chunk(static_cast<const T*>(a.table) + id * a.stride, static_cast<int>(item - r * a.chunks), a.width);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const uint32_t item = t + u * kEmbedBlock;
+            if (item >= items) break;
+            const uint32_t r = divide(item, a.by_chunks);
             float f[kPerVec<T>];
-            widen<T>(load_some(static_cast<const T*>(a.table) + id * a.stride + column, count), f);
+            widen<T>(v[u], f);
 #pragma unroll
             for (int e = 0; e < kPerVec<T>; ++e) f[e] *= a.scale;
-            v = narrow<T>(f);
+            store_chunk(static_cast<T*>(a.out) + (row0 + r) * a.width, static_cast<int>(item - r * a.chunks), a.width, narrow<T>(f));
         }
-        store_some(static_cast<T*>(a.out) + i * a.width + column, v, count);
     }
 }
 
 struct RunArgs {
     const void* up;           // [n][width], stride
-    const int32_t* order;     // sorted place -> input position
-    const int32_t* sorted;    // sorted place -> row; `vocab` for an id outside the table
+    const int2* sorted;       // sorted place -> (input position, row; `vocab` for an id outside the table)
     void* out;                // [vocab][width]
     float* head;              // [runs][columns]: fp32 sums, columns padded to whole chunks
     float* tail;
@@ -76,8 +85,7 @@ template <class T> __device__ inline void write_row(const RunArgs& a, int64_t ro
     float f[kPerVec<T>];
 #pragma unroll
     for (int e = 0; e < kPerVec<T>; ++e) f[e] = sum[e] * a.scale;
-    const int column = chunk * kPerVec<T>;
-    store_some(static_cast<T*>(a.out) + row * a.width + column, narrow<T>(f), a.width - column);
+    store_chunk(static_cast<T*>(a.out) + row * a.width, chunk, a.width, narrow<T>(f));
 }
 
 template <class T> __device__ inline void keep(float* to, const RunArgs& a, int64_t run, int chunk, const float* sum) {
@@ -93,13 +101,12 @@ template <class T> __global__ __launch_bounds__(kEmbedBlock) void runs_kernel(Ru
     const int chunk = static_cast<int>(group % a.blocks) * a.lanes + static_cast<int>(threadIdx.x) % a.lanes;
     if (run >= a.runs || chunk >= a.chunks) return;
     const int64_t begin = run * a.run, end = begin + a.run < a.n ? begin + a.run : a.n;
-    const T* up = static_cast<const T*>(a.up) + chunk * kPerVec<T>;
-    const int count = a.width - chunk * kPerVec<T>;
-    const int32_t before = begin > 0 ? a.sorted[begin - 1] : -1;
-    const int32_t after = end < a.n ? a.sorted[end] : -1;
+    const T* up = static_cast<const T*>(a.up);
+    const int32_t before = begin > 0 ? a.sorted[begin - 1].y : -1;
+    const int32_t after = end < a.n ? a.sorted[end].y : -1;
     constexpr int kAhead = 8;
     float sum[kPerVec<T>] = {};
-    int32_t row = a.sorted[begin];
+    int32_t row = a.sorted[begin].y;
     bool first = true;   // the row began at or before this run's first place
     for (int64_t p = begin; p < end; p += kAhead) {
         int32_t rows[kAhead];
@@ -107,8 +114,9 @@ template <class T> __global__ __launch_bounds__(kEmbedBlock) void runs_kernel(Ru
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const int64_t q = p + u < end ? p + u : end - 1;
-            rows[u] = a.sorted[q];
-            v[u] = load_some(up + a.order[q] * a.stride, count);
+            const int2 at = a.sorted[q];
+            rows[u] = at.y;
+            v[u] = load_chunk(up + static_cast<int64_t>(at.x) * a.stride, chunk, a.width);
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
@@ -132,46 +140,74 @@ template <class T> __global__ __launch_bounds__(kEmbedBlock) void runs_kernel(Ru
     else write_row<T>(a, row, chunk, sum);
 }
 
-// One wave looks at 64 runs, then joins those that go on one after the other: its lanes take 64 / lanes
-// of the heads at once, which are added pairwise at the end.
+constexpr int kNear = 16;   // runs a group of lanes follows by itself
+
+// Each group of lanes takes one run, and where its last row goes on adds the heads of up to kNear runs after
+// it.  Rows that reach further are left to the whole workgroup, one after the other: its groups take every
+// so many heads each and their sums are added in order.
 template <class T> __global__ __launch_bounds__(kEmbedBlock) void join_kernel(RunArgs a) {
-    const int lane = static_cast<int>(threadIdx.x % 64);
-    const int64_t wave = static_cast<int64_t>(blockIdx.x) * (kEmbedBlock / 64) + threadIdx.x / 64;
-    const int64_t own = wave / a.blocks * 64 + lane;
-    const int block = static_cast<int>(wave % a.blocks);
-    bool goes_on = false;
-    if (own < a.runs - 1) {
-        const int64_t begin = own * a.run, end = begin + a.run;   // not the last run: whole
-        const int32_t row = a.sorted[end - 1];
-        goes_on = row < a.vocab && a.sorted[end] == row && (begin == 0 || a.sorted[begin - 1] != row);
+    __shared__ float part[kEmbedBlock * kPerVec<T>];
+    __shared__ int far[kEmbedBlock / 4];
+    __shared__ int count;
+    const int groups = kEmbedBlock / a.lanes, group = static_cast<int>(threadIdx.x) / a.lanes;
+    const int lane = static_cast<int>(threadIdx.x) % a.lanes;
+    const int64_t run0 = blockIdx.x / a.blocks * static_cast<int64_t>(groups);
+    const int chunk = static_cast<int>(blockIdx.x % a.blocks) * a.lanes + lane;
+    const int64_t pitch = static_cast<int64_t>(a.chunks) * kPerVec<T>;
+    const float* head = a.head + static_cast<int64_t>(chunk) * kPerVec<T>;
+    const float* tail = a.tail + static_cast<int64_t>(chunk) * kPerVec<T>;
+    const bool own = chunk < a.chunks;
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    const int64_t run = run0 + group;
+    if (run < a.runs - 1) {
+        const int64_t begin = run * a.run, end = begin + a.run;   // not the last run: whole
+        const int32_t row = a.sorted[end].y;
+        if (row < a.vocab && a.sorted[end - 1].y == row && (begin == 0 || a.sorted[begin - 1].y != row)) {
+            const int64_t past = end + static_cast<int64_t>(kNear) * a.run;
+            if (past < a.n && a.sorted[past].y == row) {
+                if (lane == 0) far[atomicAdd(&count, 1)] = group;
+            } else if (own) {
+                float sum[kPerVec<T>];
+#pragma unroll
+                for (int e = 0; e < kPerVec<T>; ++e) sum[e] = tail[run * pitch + e];
+                for (int64_t r = run + 1; r < a.runs && a.sorted[r * a.run].y == row; ++r)
+#pragma unroll
+                    for (int e = 0; e < kPerVec<T>; ++e) sum[e] += head[r * pitch + e];
+                write_row<T>(a, row, chunk, sum);
+            }
+        }
     }
-    for (uint64_t todo = __ballot(goes_on); todo; todo &= todo - 1) {
-        const int64_t run = wave / a.blocks * 64 + __ffsll(static_cast<unsigned long long>(todo)) - 1;
-        const int64_t from = (run + 1) * a.run;
-        const int32_t row = a.sorted[from];
-        int64_t low = from, high = a.n;   // the first place past the row
+    __syncthreads();
+    const int rows = count;
+    for (int k = 0; k < rows; ++k) {   // their order does not matter: each is another row
+        const int64_t from = run0 + far[k] + 1;
+        const int32_t row = a.sorted[from * a.run].y;
+        int64_t low = from * a.run, high = a.n;   // the first place past the row
         while (low < high) {
             const int64_t mid = (low + high) / 2;
-            if (a.sorted[mid] <= row) low = mid + 1; else high = mid;
+            if (a.sorted[mid].y <= row) low = mid + 1; else high = mid;
         }
-        const int64_t last = (low - 1) / a.run;   // heads of runs run + 1 .. last
-        const int chunk = block * a.lanes + lane % a.lanes;
+        const int64_t last = (low - 1) / a.run;
         float sum[kPerVec<T>] = {};
-        if (chunk < a.chunks) {
-            const int part = lane / a.lanes, parts = 64 / a.lanes;
-            const int64_t pitch = static_cast<int64_t>(a.chunks) * kPerVec<T>;
-            const float* head = a.head + static_cast<int64_t>(chunk) * kPerVec<T>;
-            for (int64_t r = run + 1 + part; r <= last; r += parts)
+        if (own)
+#pragma unroll 2
+            for (int64_t r = from + group; r <= last; r += groups)
 #pragma unroll
                 for (int e = 0; e < kPerVec<T>; ++e) sum[e] += head[r * pitch + e];
-            if (part == 0)
 #pragma unroll
-                for (int e = 0; e < kPerVec<T>; ++e) sum[e] += a.tail[run * pitch + static_cast<int64_t>(chunk) * kPerVec<T> + e];
+        for (int e = 0; e < kPerVec<T>; ++e) part[e * kEmbedBlock + threadIdx.x] = sum[e];
+        __syncthreads();
+        if (group == 0 && own) {
+#pragma unroll
+            for (int e = 0; e < kPerVec<T>; ++e) {
+                float s = tail[(from - 1) * pitch + e];
+                for (int g = 0; g < groups; ++g) s += part[e * kEmbedBlock + g * a.lanes + lane];
+                sum[e] = s;
+            }
+            write_row<T>(a, row, chunk, sum);
         }
-        for (int m = a.lanes; m < 64; m *= 2)
-#pragma unroll
-            for (int e = 0; e < kPerVec<T>; ++e) sum[e] += __shfl_xor(sum[e], m);
-        if (chunk < a.chunks && lane < a.lanes) write_row<T>(a, row, chunk, sum);
+        __syncthreads();
     }
 }
 
@@ -210,7 +246,7 @@ int run_length(int64_t n, int chunks) {
 }
 
 struct EmbedPlan {
-    int64_t order, sorted, heads, sort;   // bytes
+    int64_t sorted, heads, sort;   // bytes
     int run, chunks;
     int64_t runs;
 };
@@ -220,8 +256,7 @@ EmbedPlan embed_plan(int64_t n, int64_t vocab, int64_t width, int dtype) {
     p.chunks = chunks_of(width, dtype);
     p.run = run_length(n, p.chunks);
     p.runs = (n + p.run - 1) / p.run;
-    p.order = padded(4 * n);
-    p.sorted = padded(4 * n);
+    p.sorted = padded(8 * n);
     p.heads = padded(p.runs * p.chunks * (16 / dtype_bytes(dtype)) * 4);
     p.sort = padded(sort_workspace(n, vocab));
     return p;
@@ -267,7 +302,7 @@ ODIE_API int odie_embed_forward(const void* table, int64_t table_stride, int64_t
 ODIE_API int64_t odie_embed_workspace(int64_t n, int64_t vocab, int64_t width, int dtype) {
     if (check_embed("odie_embed_workspace", n, vocab, width, 4, dtype)) return -1;
     const EmbedPlan p = embed_plan(n, vocab, width, dtype);
-    return p.order + p.sorted + 2 * p.heads + p.sort;
+    return p.sorted + 2 * p.heads + p.sort;
 }
 
 ODIE_API int odie_embed_backward(const void* upstream, int64_t upstream_stride, const void* ids, int id_bytes,
@@ -278,7 +313,7 @@ ODIE_API int odie_embed_backward(const void* upstream, int64_t upstream_stride, 
     if (!dtable || (n > 0 && (!upstream || !ids))) return fail(what + ": null pointer");
     if (n > 0 && upstream_stride < width) return fail(what + ": rows overlap (a stride below the row's width)");
     const EmbedPlan p = embed_plan(n, vocab, width, dtype);
-    const int64_t need = p.order + p.sorted + 2 * p.heads + p.sort;
+    const int64_t need = p.sorted + 2 * p.heads + p.sort;
     if (n > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0))
         return fail(what + ": needs a 256-byte aligned workspace of " + std::to_string(need) + " bytes");
     hipStream_t s = as_stream(stream);
@@ -289,15 +324,13 @@ ODIE_API int odie_embed_backward(const void* upstream, int64_t upstream_stride, 
     if (n == 0) return 0;
     char* scratch = static_cast<char*>(workspace);
     RunArgs a{};
-    int32_t* order = reinterpret_cast<int32_t*>(scratch);
-    int32_t* sorted = reinterpret_cast<int32_t*>(scratch + p.order);
-    a.head = reinterpret_cast<float*>(scratch + p.order + p.sorted);
-    a.tail = reinterpret_cast<float*>(scratch + p.order + p.sorted + p.heads);
-    if (launch_sort(SortKeys{ids, id_bytes, n, vocab}, SortOut{order, sorted, nullptr, nullptr},
-                    scratch + p.order + p.sorted + 2 * p.heads, s))
+    int2* sorted = reinterpret_cast<int2*>(scratch);
+    a.head = reinterpret_cast<float*>(scratch + p.sorted);
+    a.tail = reinterpret_cast<float*>(scratch + p.sorted + p.heads);
+    if (launch_sort(SortKeys{ids, id_bytes, n, vocab}, SortOut{nullptr, sorted, nullptr, nullptr, nullptr},
+                    scratch + p.sorted + 2 * p.heads, s))
         return -1;
     a.up = upstream;
-    a.order = order;
     a.sorted = sorted;
     a.out = dtable;
     a.n = n;
@@ -310,13 +343,13 @@ ODIE_API int odie_embed_backward(const void* upstream, int64_t upstream_stride, 
     a.chunks = p.chunks;
     a.lanes = run_lanes(p.chunks);
     a.blocks = (p.chunks + a.lanes - 1) / a.lanes;
-    const int64_t threads = p.runs * a.blocks * a.lanes, waves = (p.runs + 63) / 64 * a.blocks;
+    const int64_t threads = p.runs * a.blocks * a.lanes, joins = (p.runs + kEmbedBlock / a.lanes - 1) / (kEmbedBlock / a.lanes) * a.blocks;
     if (threads / kEmbedBlock >= int64_t{1} << 31) return fail(what + ": too many runs for one launch");
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         runs_kernel<T><<<static_cast<uint32_t>((threads + kEmbedBlock - 1) / kEmbedBlock), kEmbedBlock, 0, s>>>(a);
         if (p.runs > 1)
-            join_kernel<T><<<static_cast<uint32_t>((waves + kEmbedBlock / 64 - 1) / (kEmbedBlock / 64)), kEmbedBlock, 0, s>>>(a);
+            join_kernel<T><<<static_cast<uint32_t>(joins), kEmbedBlock, 0, s>>>(a);
     });
     return check_launch("embed gradient");
 }

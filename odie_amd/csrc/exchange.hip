@@ -9,6 +9,8 @@
 // The gradient of dispatch is combine without weights.  Each of them reads and writes every row once and
 // is bound by HBM, so the walk is over input rows: x and dy are read once however many choices there are,
 // and the scattered side moves whole rows.  Sums are fp32 in the order of the choices, rounded once.
+#include <type_traits>
+
 #include "elements.h"
 #include "tiles.h"
 
@@ -18,8 +20,8 @@ namespace {
 constexpr int kMoveBlock = 256;
 
 struct MoveArgs {
-    const void* x;            // dispatch: [n]; combine: [n choices]; both [.][width], stride ldx
-    const void* rows;         // the gradient of combine: the sorted rows, stride ldr
+    const void* x;            // dispatch: x; combine: the sorted rows; gradient of combine: dy; stride ldx
+    const void* rows;         // gradient of combine: the sorted rows, stride ldr
     const int32_t* slots;     // [n choices]
     const float* weights;     // [n choices], or null: 1
     const int32_t* offsets;   // [experts + 1]
@@ -29,7 +31,8 @@ struct MoveArgs {
     Divisor by_chunks;
     uint32_t block_rows;      // input rows a workgroup takes
     int choices, experts, width, chunks;
-    int lanes;                // gradient of combine: lanes a row
+    int lanes;                // dispatch and the gradient of combine: lanes a row
+    bool by_xcd;
 };
 
 // Zeros in the slots that no expert owns, shared out over the workgroups.
@@ -41,95 +44,143 @@ template <class T> __device__ inline void clear_rest(const MoveArgs& a) {
     const int64_t begin = held + each * blockIdx.x, end = begin + each < entries ? begin + each : entries;
     for (int64_t s = begin; s < end; ++s) {
         T* to = static_cast<T*>(a.out) + s * a.width;
-        for (int c = threadIdx.x; c < a.chunks; c += kMoveBlock)
-            store_some(to + c * kPerVec<T>, vec16{}, a.width - c * kPerVec<T>);
+        for (int c = threadIdx.x; c < a.chunks; c += kMoveBlock) store_chunk(to, c, a.width, vec16{});
     }
 }
 
-template <class T> __global__ __launch_bounds__(kMoveBlock) void dispatch_kernel(MoveArgs a) {
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.block_rows;
-    const int64_t left = a.n - row0;
-    const uint32_t items = (left < a.block_rows ? static_cast<uint32_t>(left) : a.block_rows) * a.chunks;
-    const int64_t entries = a.n * a.choices;
-    for (uint32_t t = threadIdx.x; t < items; t += kMoveBlock) {
-        const uint32_t r = divide(t, a.by_chunks);
-        const int column = static_cast<int>(t - r * a.chunks) * kPerVec<T>, count = a.width - column;
-        const int64_t i = row0 + r;
-        const vec16 v = load_some(static_cast<const T*>(a.x) + i * a.ldx + column, count);
-        for (int j = 0; j < a.choices; ++j) {
-            const int64_t slot = a.slots[i * a.choices + j];
-            if (slot >= 0 && slot < entries) store_some(static_cast<T*>(a.out) + slot * a.width + column, v, count);
+// The slot of entry first + j of row i; -1 where there is none.
+template <int kChoices> __device__ inline int64_t slot_of(const MoveArgs& a, int64_t i, int choices, int j) {
+    if (!kChoices && j >= choices) return -1;
+    const int64_t slot = a.slots[i * choices + j];
+    return slot < a.n * choices ? slot : -1;
+}
+
+// The input row of this thread's group of `lanes` lanes (lanes divides 64), n or more for none.  Where rows do
+// not fill their 64-byte blocks, workgroups that follow each other in rows run on one XCD: the rows that they
+// send to an expert lie side by side, and the lines that two of them share meet in that XCD's L2 (300007 x 4
+// rows of 272 bytes sent: 124 -> 92 us).  Whole blocks go faster spread over the XCDs (256 bytes: 81 -> 74 us).
+__device__ inline int64_t lane_row(const MoveArgs& a) {
+    const uint32_t block = a.by_xcd ? xcd_major(blockIdx.x, gridDim.x) : blockIdx.x;
+    return static_cast<int64_t>(block) * (kMoveBlock / a.lanes) + static_cast<int>(threadIdx.x) / a.lanes;
+}
+
+// kChoices entries of a row are handled together (0: any number of choices, in twos).
+template <class T, int kChoices> __global__ __launch_bounds__(kMoveBlock) void dispatch_kernel(MoveArgs a) {
+    constexpr int kStep = kChoices ? kChoices : 2;
+    const int choices = kChoices ? kChoices : a.choices;
+    const int lane = static_cast<int>(threadIdx.x) % a.lanes;
+    const int64_t i = lane_row(a);
+    if (i < a.n)
+        for (int first = 0; first < choices; first += kStep) {
+            int64_t slot[kStep];
+#pragma unroll
+            for (int j = 0; j < kStep; ++j) slot[j] = slot_of<kChoices>(a, i, choices, first + j);
+            for (int c = lane; c < a.chunks; c += a.lanes) {
+                const vec16 v = load_chunk(static_cast<const T*>(a.x) + i * a.ldx, c, a.width);
+#pragma unroll
+                for (int j = 0; j < kStep; ++j)
+                    if (slot[j] >= 0) store_chunk(static_cast<T*>(a.out) + slot[j] * a.width, c, a.width, v);
+            }
         }
-    }
     clear_rest<T>(a);
 }
 
-template <class T> __global__ __launch_bounds__(kMoveBlock) void combine_kernel(MoveArgs a) {
+template <class T, int kChoices> __global__ __launch_bounds__(kMoveBlock) void combine_kernel(MoveArgs a) {
+    constexpr int kStep = kChoices ? kChoices : 2;
+    const int choices = kChoices ? kChoices : a.choices;
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.block_rows;
     const int64_t left = a.n - row0;
     const uint32_t items = (left < a.block_rows ? static_cast<uint32_t>(left) : a.block_rows) * a.chunks;
-    const int64_t entries = a.n * a.choices;
     for (uint32_t t = threadIdx.x; t < items; t += kMoveBlock) {
         const uint32_t r = divide(t, a.by_chunks);
-        const int column = static_cast<int>(t - r * a.chunks) * kPerVec<T>, count = a.width - column;
+        const int chunk = static_cast<int>(t - r * a.chunks);
         const int64_t i = row0 + r;
         float sum[kPerVec<T>] = {};
-        for (int j = 0; j < a.choices; ++j) {
-            const int64_t slot = a.slots[i * a.choices + j];
-            if (slot < 0 || slot >= entries) continue;
-            float v[kPerVec<T>];
-            widen<T>(load_some(static_cast<const T*>(a.x) + slot * a.ldx + column, count), v);
-            const float w = a.weights ? a.weights[i * a.choices + j] : 1.0f;
+        for (int first = 0; first < choices; first += kStep) {
+            vec16 v[kStep];
+            float w[kStep];
 #pragma unroll
-            for (int e = 0; e < kPerVec<T>; ++e) sum[e] += w * v[e];
+            for (int j = 0; j < kStep; ++j) {
+                const int64_t slot = slot_of<kChoices>(a, i, choices, first + j);
+                w[j] = slot >= 0 ? (a.weights ? a.weights[i * choices + first + j] : 1.0f) : 0.0f;
+                v[j] = slot >= 0 ? load_chunk(static_cast<const T*>(a.x) + slot * a.ldx, chunk, a.width) : vec16{};
+            }
+#pragma unroll
+            for (int j = 0; j < kStep; ++j) {
+                float f[kPerVec<T>];
+                widen<T>(v[j], f);
+#pragma unroll
+                for (int e = 0; e < kPerVec<T>; ++e) sum[e] += w[j] * f[e];
+            }
         }
-        store_some(static_cast<T*>(a.out) + i * a.width + column, narrow<T>(sum), count);
+        store_chunk(static_cast<T*>(a.out) + i * a.width, chunk, a.width, narrow<T>(sum));
     }
 }
 
-// A group of `lanes` lanes takes an input row; lanes divides 64.
-template <class T> __global__ __launch_bounds__(kMoveBlock) void combine_backward_kernel(MoveArgs a) {
+template <class T, int kChoices> __global__ __launch_bounds__(kMoveBlock) void combine_backward_kernel(MoveArgs a) {
+    constexpr int kStep = kChoices ? kChoices : 2;
+    const int choices = kChoices ? kChoices : a.choices;
     const int lane = static_cast<int>(threadIdx.x) % a.lanes;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kMoveBlock / a.lanes) + static_cast<int>(threadIdx.x) / a.lanes;
-    const int64_t entries = a.n * a.choices;
+    const int64_t i = lane_row(a);
     if (i < a.n) {
         const T* up = static_cast<const T*>(a.x) + i * a.ldx;
-        for (int j = 0; j < a.choices; ++j) {
-            const int64_t f = i * a.choices + j, slot = a.slots[f];
-            const bool held = slot >= 0 && slot < entries;
-            const float w = a.weights ? a.weights[f] : 1.0f;
-            float dot = 0.0f;
-            if (held)
-                for (int c = lane; c < a.chunks; c += a.lanes) {
-                    const int column = c * kPerVec<T>, count = a.width - column;
-                    float d[kPerVec<T>], v[kPerVec<T>];
-                    widen<T>(load_some(up + column, count), d);
-                    if (a.dweights) {
-                        widen<T>(load_some(static_cast<const T*>(a.rows) + slot * a.ldr + column, count), v);
+        for (int first = 0; first < choices; first += kStep) {
+            int64_t slot[kStep];
+            float w[kStep], dot[kStep] = {};
 #pragma unroll
-                        for (int e = 0; e < kPerVec<T>; ++e) dot += d[e] * v[e];
-                    }
-                    if (a.out) {
+            for (int j = 0; j < kStep; ++j) {
+                slot[j] = slot_of<kChoices>(a, i, choices, first + j);
+                w[j] = slot[j] >= 0 && a.weights ? a.weights[i * choices + first + j] : 1.0f;
+            }
+            for (int c = lane; c < a.chunks; c += a.lanes) {
+                const vec16 u = load_chunk(up, c, a.width);
+                vec16 v[kStep];
 #pragma unroll
-                        for (int e = 0; e < kPerVec<T>; ++e) d[e] *= w;
-                        store_some(static_cast<T*>(a.out) + slot * a.width + column, narrow<T>(d), count);
+                for (int j = 0; j < kStep; ++j)
+                    v[j] = a.dweights && slot[j] >= 0
+                               ? load_chunk(static_cast<const T*>(a.rows) + slot[j] * a.ldr, c, a.width) : vec16{};
+                const int again = chunk_overlap<T>(c, a.width);   // elements that the chunk before holds too
+                float d[kPerVec<T>];
+                widen<T>(u, d);
+#pragma unroll
+                for (int j = 0; j < kStep; ++j) {
+                    float f[kPerVec<T>], g[kPerVec<T>];
+                    widen<T>(v[j], f);
+#pragma unroll
+                    for (int e = 0; e < kPerVec<T>; ++e) {
+                        if (e >= again) dot[j] += d[e] * f[e];
+                        g[e] = d[e] * w[j];
                     }
+                    if (a.out && slot[j] >= 0)
+                        store_chunk(static_cast<T*>(a.out) + slot[j] * a.width, c, a.width, narrow<T>(g));
                 }
+            }
             if (a.dweights) {
-                for (int m = a.lanes / 2; m > 0; m /= 2) dot += __shfl_xor(dot, m);
-                if (lane == 0) a.dweights[f] = dot;
+#pragma unroll
+                for (int j = 0; j < kStep; ++j) {
+                    for (int m = a.lanes / 2; m > 0; m /= 2) dot[j] += __shfl_xor(dot[j], m);
+                    if (lane == 0 && (kChoices || first + j < choices))
+                        a.dweights[i * choices + first + j] = slot[j] >= 0 ? dot[j] : 0.0f;   // not NaN times 0
+                }
             }
         }
     }
     if (a.out) clear_rest<T>(a);
 }
 
-// Lanes for a row of `chunks` 16-byte pieces: the most (up to 64) that keep four of five busy.
+// f with the number of choices as a constant where it is 1, 2 or 4, else 0.
+template <class F> void with_choices(int choices, F&& f) {
+    if (choices == 1) f(std::integral_constant<int, 1>{});
+    else if (choices == 2) f(std::integral_constant<int, 2>{});
+    else if (choices == 4) f(std::integral_constant<int, 4>{});
+    else f(std::integral_constant<int, 0>{});
+}
+
+// Lanes for a row of `chunks` 16-byte pieces: a whole row at once where 64 lanes can.
 int row_lanes(int chunks) {
-    int best = 4;
-    for (int lanes = 8; lanes <= 64; lanes *= 2)
-        if (5 * chunks >= 4 * ((chunks + lanes - 1) / lanes * lanes)) best = lanes;
-    return best;
+    int lanes = 1;
+    while (lanes < 64 && lanes < chunks) lanes *= 2;
+    return lanes;
 }
 
 int check_move(const std::string& what, int64_t n, int choices, int experts, int64_t width, int dtype) {
@@ -153,7 +204,13 @@ MoveArgs move_args(int64_t n, int choices, int experts, int64_t width, int dtype
     // about 1024 pieces of 16 bytes a workgroup
     a.block_rows = a.chunks >= 1024 ? 1u : static_cast<uint32_t>(1024 / a.chunks);
     a.lanes = row_lanes(a.chunks);
+    a.by_xcd = width * dtype_bytes(dtype) % 64 != 0;
     return a;
+}
+
+uint32_t row_blocks(const MoveArgs& a) {
+    const int64_t height = kMoveBlock / a.lanes, blocks = (a.n + height - 1) / height;
+    return static_cast<uint32_t>((blocks + kXcds - 1) / kXcds * kXcds);
 }
 
 uint32_t move_blocks(const MoveArgs& a) { return static_cast<uint32_t>((a.n + a.block_rows - 1) / a.block_rows); }
@@ -177,7 +234,11 @@ ODIE_API int odie_rows_dispatch(const void* x, int64_t x_stride, const int32_t* 
     a.slots = slots;
     a.offsets = offsets;
     a.out = out;
-    with_dtype(dtype, [&](auto t) { dispatch_kernel<decltype(t)><<<move_blocks(a), kMoveBlock, 0, as_stream(stream)>>>(a); });
+    with_dtype(dtype, [&](auto t) {
+        with_choices(choices, [&](auto k) {
+            dispatch_kernel<decltype(t), k><<<row_blocks(a), kMoveBlock, 0, as_stream(stream)>>>(a);
+        });
+    });
     return check_launch("rows dispatch");
 }
 
@@ -194,7 +255,11 @@ ODIE_API int odie_rows_combine(const void* rows, int64_t rows_stride, const int3
     a.slots = slots;
     a.weights = weights;
     a.out = out;
-    with_dtype(dtype, [&](auto t) { combine_kernel<decltype(t)><<<move_blocks(a), kMoveBlock, 0, as_stream(stream)>>>(a); });
+    with_dtype(dtype, [&](auto t) {
+        with_choices(choices, [&](auto k) {
+            combine_kernel<decltype(t), k><<<move_blocks(a), kMoveBlock, 0, as_stream(stream)>>>(a);
+        });
+    });
     return check_launch("rows combine");
 }
 
@@ -218,10 +283,11 @@ ODIE_API int odie_rows_combine_backward(const void* upstream, int64_t upstream_s
     a.offsets = offsets;
     a.out = drows;
     a.dweights = dweights;
-    const int height = kMoveBlock / a.lanes;
     with_dtype(dtype, [&](auto t) {
-        combine_backward_kernel<decltype(t)>
-            <<<static_cast<uint32_t>((n + height - 1) / height), kMoveBlock, 0, as_stream(stream)>>>(a);
+        with_choices(choices, [&](auto k) {
+            combine_backward_kernel<decltype(t), k>
+                <<<row_blocks(a), kMoveBlock, 0, as_stream(stream)>>>(a);
+        });
     });
     return check_launch("rows combine gradient");
 }

@@ -12,7 +12,8 @@ struct SortKeys {
 };
 
 struct SortOut {
-    int32_t* order;     // [n] input position of each sorted place
+    int32_t* order;     // [n] input position of each sorted place, or null
+    int2* pairs;        // [n] (input position, bucket) of each sorted place, or null
     int32_t* sorted;    // [n] bucket of each sorted place, or null
     int32_t* slots;     // [n] sorted place of each input position, -1 where its key is no bucket, or null
     int32_t* offsets;   // [buckets + 1] first place of each bucket, then that of the keys without one, or null

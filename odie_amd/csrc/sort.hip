@@ -130,7 +130,8 @@ __global__ __launch_bounds__(kSmallBlock) void small_sort_kernel(SmallArgs a) {
     }
     for (int i = threadIdx.x; i < n; i += kSmallBlock) {
         const int f = from[now][i];
-        a.out.order[i] = f;
+        if (a.out.order) a.out.order[i] = f;
+        if (a.out.pairs) a.out.pairs[i] = make_int2(f, static_cast<int>(key[now][i]));
         if (a.out.sorted) a.out.sorted[i] = static_cast<int32_t>(key[now][i]);
         if (a.out.slots) a.out.slots[f] = key[now][i] < buckets ? i : -1;
     }
@@ -148,9 +149,8 @@ __global__ __launch_bounds__(kSmallBlock) void small_sort_kernel(SmallArgs a) {
 struct PassArgs {
     const void* raw;          // the caller's keys (first pass)
     int raw_bytes;
-    const uint32_t* key;      // later passes: the keys and their input positions so far
-    const uint32_t* from;
-    uint32_t* key_out;        // null on the last pass
+    const uint2* pairs;       // later passes: (input position, key) so far
+    uint2* pairs_out;         // earlier passes
     uint32_t* table;          // [digits][parts]
     uint32_t* totals;         // [digits]
     SortOut out;              // last pass
@@ -158,13 +158,12 @@ struct PassArgs {
     int64_t part;             // keys a workgroup (a multiple of kSortBlock)
     uint32_t parts;
     uint32_t buckets;
-    uint32_t* from_out;
     int shift, bits, digits;
     bool last, only;          // only: the sole pass, digits are buckets
 };
 
 __device__ inline uint32_t pass_key(const PassArgs& a, int64_t i) {
-    return a.raw ? read_key(a.raw, a.raw_bytes, i, a.buckets) : a.key[i];
+    return a.raw ? read_key(a.raw, a.raw_bytes, i, a.buckets) : a.pairs[i].y;
 }
 
 __global__ __launch_bounds__(kSortBlock) void count_kernel(PassArgs a) {
@@ -193,28 +192,30 @@ __global__ __launch_bounds__(256) void scan_kernel(PassArgs a) {
 }
 
 __global__ __launch_bounds__(kSortBlock) void scatter_kernel(PassArgs a) {
-    __shared__ uint32_t start[kDigits];
-    __shared__ uint32_t at[kSortWaves][kDigits];
+    extern __shared__ uint32_t lds[];              // as much as the digits need: more workgroups a CU
     __shared__ uint32_t wave_sums[kSortWaves];
+    uint32_t* const start = lds;                   // first place of each digit
+    uint32_t* const next = lds + a.digits;         // [wave][digit]: the next key's
     const int lane = static_cast<int>(threadIdx.x % 64), wave = static_cast<int>(threadIdx.x / 64);
+    uint32_t* const own_next = next + wave * a.digits;
     for (int d = threadIdx.x; d < a.digits; d += kSortBlock) {
         start[d] = a.totals[d];
 #pragma unroll
-        for (int w = 0; w < kSortWaves; ++w) at[w][d] = 0;
+        for (int w = 0; w < kSortWaves; ++w) next[w * a.digits + d] = 0;
     }
     __syncthreads();
     block_scan<kSortBlock>(start, a.digits, wave_sums);
     const uint32_t mask = (1u << a.bits) - 1;
     const int64_t share = a.part / kSortWaves;
     const int64_t begin = blockIdx.x * a.part + wave * share, end = begin + share < a.n ? begin + share : a.n;
-    for (int64_t i = begin + lane; i < end; i += 64) atomicAdd(&at[wave][pass_key(a, i) >> a.shift & mask], 1u);
+    for (int64_t i = begin + lane; i < end; i += 64) atomicAdd(&own_next[pass_key(a, i) >> a.shift & mask], 1u);
     __syncthreads();
     for (int d = threadIdx.x; d < a.digits; d += kSortBlock) {
         uint32_t place = start[d] + a.table[static_cast<int64_t>(d) * a.parts + blockIdx.x];
 #pragma unroll
         for (int w = 0; w < kSortWaves; ++w) {
-            const uint32_t own = at[w][d];
-            at[w][d] = place;
+            const uint32_t own = next[w * a.digits + d];
+            next[w * a.digits + d] = place;
             place += own;
         }
     }
@@ -224,23 +225,27 @@ __global__ __launch_bounds__(kSortBlock) void scatter_kernel(PassArgs a) {
     for (int64_t base = begin; base < end; base += 64) {
         const int64_t i = base + lane;
         const bool valid = i < end;
-        const uint32_t k = valid ? pass_key(a, i) : 0u;
-        const uint32_t f = valid ? (a.raw ? static_cast<uint32_t>(i) : a.from[i]) : 0u;
+        uint2 pair = make_uint2(static_cast<uint32_t>(i), 0u);
+        if (valid) {
+            if (a.raw) pair.y = pass_key(a, i);
+            else pair = a.pairs[i];
+        }
+        const uint32_t k = pair.y, f = pair.x;
         const uint32_t digit = k >> a.shift & mask;
         const uint64_t same = same_digit(digit, a.bits, __ballot(valid));
-        const uint32_t place = valid ? at[wave][digit] : 0u;
+        const uint32_t place = valid ? own_next[digit] : 0u;
         const int rank = lanes_below(same, lane);
         wave_fence();
-        if (valid && rank == 0) at[wave][digit] = place + __popcll(same);
+        if (valid && rank == 0) own_next[digit] = place + __popcll(same);
         wave_fence();
         if (!valid) continue;
         const uint32_t to = place + rank;
         if (!a.last) {
-            a.key_out[to] = k;
-            a.from_out[to] = f;
+            a.pairs_out[to] = pair;
             continue;
         }
-        a.out.order[to] = static_cast<int32_t>(f);
+        if (a.out.order) a.out.order[to] = static_cast<int32_t>(f);
+        if (a.out.pairs) a.out.pairs[to] = make_int2(static_cast<int>(f), static_cast<int>(k));
         if (a.out.sorted) a.out.sorted[to] = static_cast<int32_t>(k);
         if (a.out.slots) a.out.slots[f] = k < a.buckets ? static_cast<int32_t>(to) : -1;
     }
@@ -264,9 +269,10 @@ int key_bits(int64_t buckets) {   // of the numbers 0..buckets
     return bits;
 }
 
+// Keys a workgroup: enough for two workgroups a CU where there are, at least one round of every wave.
 int64_t sort_part(int64_t n) {
-    int64_t part = 4096;
-    while (part * kMaxParts < n) part *= 2;
+    int64_t part = kSortBlock;
+    while ((part < 4096 && part * 2 * kCus < n) || part * kMaxParts < n) part *= 2;
     return part;
 }
 
@@ -282,8 +288,8 @@ int check_sort(const char* what, const SortKeys& k) {
     return 0;
 }
 
-// 32-bit words: the table and totals of a pass, two (key, position) pairs of arrays for several passes
-// (the second keeps the sorted keys for the offsets).
+// 32-bit words: the table and totals of a pass, two arrays of (position, key) for several passes
+// (one of them keeps the sorted keys for the offsets).
 int64_t sort_workspace(int64_t n, int64_t buckets) {
     if (n <= kSmall) return 0;
     const int bits = key_bits(buckets), passes = (bits + kDigitBits - 1) / kDigitBits;
@@ -310,23 +316,22 @@ int launch_sort(const SortKeys& k, const SortOut& out, void* workspace, hipStrea
     uint32_t* words = static_cast<uint32_t*>(workspace);
     a.table = words;
     a.totals = a.table + padded(digits * a.parts);
-    uint32_t* pair[2] = {a.totals + padded(digits), a.totals + padded(digits) + 2 * padded(k.n)};
+    uint2* pairs[2] = {reinterpret_cast<uint2*>(a.totals + padded(digits)),
+                       reinterpret_cast<uint2*>(a.totals + padded(digits)) + padded(k.n)};
     for (int pass = 0; pass < passes; ++pass) {
         a.raw = pass == 0 ? k.keys : nullptr;
         a.raw_bytes = k.bytes;
-        a.key = pair[(pass + 1) % 2];
-        a.from = a.key + padded(k.n);
+        a.pairs = pairs[(pass + 1) % 2];
         a.last = pass == passes - 1;
-        a.key_out = pair[pass % 2];
-        a.from_out = a.key_out + padded(k.n);
+        a.pairs_out = pairs[pass % 2];
         a.shift = pass * width;
         a.bits = bits - a.shift < width ? bits - a.shift : width;
         a.digits = static_cast<int>(passes == 1 ? digits : int64_t{1} << a.bits);
         if (a.last && passes > 1 && out.offsets && !out.sorted)   // the offsets read the sorted buckets
-            a.out.sorted = reinterpret_cast<int32_t*>(a.key_out);
+            a.out.sorted = reinterpret_cast<int32_t*>(a.pairs_out);
         count_kernel<<<a.parts, kSortBlock, 0, stream>>>(a);
         scan_kernel<<<a.digits, 256, 0, stream>>>(a);
-        scatter_kernel<<<a.parts, kSortBlock, 0, stream>>>(a);
+        scatter_kernel<<<a.parts, kSortBlock, (1 + kSortWaves) * a.digits * sizeof(uint32_t), stream>>>(a);
         if (check_launch("sort")) return -1;
     }
     if (passes > 1 && out.offsets) {
@@ -355,5 +360,5 @@ ODIE_API int odie_sort(const void* keys, int key_bytes, int64_t n, int64_t bucke
     const int64_t need = sort_workspace(n, buckets);
     if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
         return fail("odie_sort: needs a 16-byte aligned workspace of " + std::to_string(need) + " bytes");
-    return launch_sort(k, SortOut{order, sorted, slots, offsets}, workspace, as_stream(stream));
+    return launch_sort(k, SortOut{order, nullptr, sorted, slots, offsets}, workspace, as_stream(stream));
 }
