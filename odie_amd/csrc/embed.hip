@@ -140,7 +140,8 @@ template <class T> __global__ __launch_bounds__(kEmbedBlock) void runs_kernel(Ru
     else write_row<T>(a, row, chunk, sum);
 }
 
-constexpr int kNear = 16;   // runs a group of lanes follows by itself
+constexpr int kNear = 16;    // runs a group of lanes follows by itself,
+constexpr int kAtOnce = 4;   // so many heads in flight
 
 // Each group of lanes takes one run, and where its last row goes on adds the heads of up to kNear runs after
 // it.  Rows that reach further are left to the whole workgroup, one after the other: its groups take every
@@ -171,9 +172,22 @@ template <class T> __global__ __launch_bounds__(kEmbedBlock) void join_kernel(Ru
                 float sum[kPerVec<T>];
 #pragma unroll
                 for (int e = 0; e < kPerVec<T>; ++e) sum[e] = tail[run * pitch + e];
-                for (int64_t r = run + 1; r < a.runs && a.sorted[r * a.run].y == row; ++r)
+                for (int64_t r = run + 1; r < a.runs; r += kAtOnce) {
+                    float h[kAtOnce][kPerVec<T>];
+                    bool goes_on[kAtOnce];
 #pragma unroll
-                    for (int e = 0; e < kPerVec<T>; ++e) sum[e] += head[r * pitch + e];
+                    for (int u = 0; u < kAtOnce; ++u) {   // heads of runs that the row does not reach are not added
+                        const int64_t q = r + u < a.runs ? r + u : a.runs - 1;
+                        goes_on[u] = r + u < a.runs && a.sorted[q * a.run].y == row;
+#pragma unroll
+                        for (int e = 0; e < kPerVec<T>; ++e) h[u][e] = head[q * pitch + e];
+                    }
+#pragma unroll
+                    for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                        for (int e = 0; e < kPerVec<T>; ++e) sum[e] += goes_on[u] ? h[u][e] : 0.0f;
+                    if (!goes_on[kAtOnce - 1]) break;
+                }
                 write_row<T>(a, row, chunk, sum);
             }
         }

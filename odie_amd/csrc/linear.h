@@ -48,6 +48,23 @@ __device__ inline accum16 multiply(float, const vec16& b, const vec16& a, accum1
     return c;
 }
 
+// The same for 16 x 16 tiles: lane l holds row l % 16, k quarter l / 16.
+typedef float accum4 __attribute__((ext_vector_type(4)));
+__device__ inline accum4 multiply16(_Float16, const vec16& b, const vec16& a, accum4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, b), __builtin_bit_cast(f16x8, a), c, 0, 0, 0);
+}
+__device__ inline accum4 multiply16(__bf16, const vec16& b, const vec16& a, accum4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), c, 0, 0, 0);
+}
+__device__ inline accum4 multiply16(float, const vec16& b, const vec16& a, accum4 c) {
+    float fb[4], fa[4];
+    __builtin_memcpy(fb, &b, 16);
+    __builtin_memcpy(fa, &a, 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[i], fa[i], c, 0, 0, 0);
+    return c;
+}
+
 // One operand of a tile: kRows of its own index times one slab of k, kThreads threads.
 // LDS image, k consecutive: kRows rows of 128 bytes; the 16-byte chunk c of row r lies at slot
 // c ^ (r / 2 % 8), so that 16 consecutive rows of one chunk fall on all 64 banks.
@@ -161,13 +178,14 @@ template <class T, bool kByRow, int kRows, int kThreads> struct Direct : Image<T
         }
         base += slab;
     }
-    __device__ void store(char*) const {}
 };
 
 // Through registers, for rows of any alignment and length.
 template <class T, bool kByRow, int kRows, int kThreads> struct Staged : Image<T, kByRow, kRows, kThreads> {
     using I = Image<T, kByRow, kRows, kThreads>;
-    vec16 held[I::kChunks];
+    struct Held {
+        vec16 chunk[I::kChunks];
+    };
     const T* at[kByRow ? I::kChunks : 1];
     int64_t step;        // one row per k: elements between this thread's chunks
     int64_t slab;        // elements from slab to slab
@@ -198,15 +216,15 @@ template <class T, bool kByRow, int kRows, int kThreads> struct Staged : Image<T
     }
 
     // Starts the loads of the next slab, of which `left` values of k exist (the rest read as 0).
-    __device__ void load(int64_t left, char*) {
+    __device__ void load(int64_t left, Held& held) {
         if constexpr (kByRow) {
             if (left >= kSlab<T>) {
 #pragma unroll
-                for (int i = 0; i < I::kChunks; ++i) held[i] = load16(at[i]);
+                for (int i = 0; i < I::kChunks; ++i) held.chunk[i] = load16(at[i]);
             } else {
                 const int count = static_cast<int>(left) - lead;
 #pragma unroll
-                for (int i = 0; i < I::kChunks; ++i) held[i] = count > 0 ? load_end(at[i], count, before) : vec16{};
+                for (int i = 0; i < I::kChunks; ++i) held.chunk[i] = count > 0 ? load_end(at[i], count, before) : vec16{};
             }
 #pragma unroll
             for (int i = 0; i < I::kChunks; ++i) at[i] += slab;
@@ -215,26 +233,27 @@ template <class T, bool kByRow, int kRows, int kThreads> struct Staged : Image<T
             if (columns == I::kVec) {
 #pragma unroll
                 for (int i = 0; i < I::kChunks; ++i)
-                    held[i] = lead + i * I::kStep < left ? load16(at[0] + i * step) : vec16{};
+                    held.chunk[i] = lead + i * I::kStep < left ? load16(at[0] + i * step) : vec16{};
             } else {
 #pragma unroll
                 for (int i = 0; i < I::kChunks; ++i)
-                    held[i] = lead + i * I::kStep < left && columns > 0
+                    held.chunk[i] = lead + i * I::kStep < left && columns > 0
                                   ? load_end(at[0] + i * step, columns, before) : vec16{};
             }
             at[0] += slab;
         }
     }
 
-    __device__ void store(char* lds) const {
+    static __device__ void store(const Held& held, char* lds) {
 #pragma unroll
         for (int i = 0; i < I::kChunks; ++i)
-            *reinterpret_cast<vec16*>(lds + (threadIdx.x + i * kThreads) * 16) = held[i];
+            *reinterpret_cast<vec16*>(lds + (threadIdx.x + i * kThreads) * 16) = held.chunk[i];
     }
 };
 
 // One workgroup's tile: waves of kWM x kWN, kBM / kWM x kBN / kWN of them.
-template <class T, bool kAByRow, bool kBByRow, bool kDirect, int kBM, int kBN, int kWM, int kWN> struct Tile {
+template <class T, bool kAByRow, bool kBByRow, bool kDirect, int kBM, int kBN, int kWM, int kWN, int kWantedStages = 2>
+struct Tile {
     static constexpr int kThreads = 64 * (kBM / kWM) * (kBN / kWN);
     using A = std::conditional_t<kDirect, Direct<T, kAByRow, kBM, kThreads>, Staged<T, kAByRow, kBM, kThreads>>;
     using B = std::conditional_t<kDirect, Direct<T, kBByRow, kBN, kThreads>, Staged<T, kBByRow, kBN, kThreads>>;
@@ -242,7 +261,8 @@ template <class T, bool kAByRow, bool kBByRow, bool kDirect, int kBM, int kBN, i
     static constexpr int kBuffer = A::kBytes + B::kBytes;
     static constexpr int kPitch = kWN + 4;                  // floats a row of the epilogue's region
     static constexpr int kRegion = 32 * kPitch * 4;
-    static constexpr int kLds = 2 * kBuffer > kThreads / 64 * kRegion ? 2 * kBuffer : kThreads / 64 * kRegion;
+    static constexpr int kStages = kDirect ? kWantedStages : 2;   // slabs in LDS: one read, the others under way
+    static constexpr int kLds = kStages * kBuffer > kThreads / 64 * kRegion ? kStages * kBuffer : kThreads / 64 * kRegion;
 
     accum16 acc[kMs][kNs];
 
@@ -250,45 +270,96 @@ template <class T, bool kAByRow, bool kBByRow, bool kDirect, int kBM, int kBN, i
     static __device__ int wave_row() { return wave() % (kBM / kWM) * kWM; }
     static __device__ int wave_column() { return wave() / (kBM / kWM) * kWN; }
 
-    // Sums `depth` values of k.  a and b have begun.
-    __device__ void sum(A& a, B& b, int64_t depth, char* lds) {
-        const int lane = static_cast<int>(threadIdx.x % 64);
-        const int wm = wave_row(), wn = wave_column();
+    __device__ void clear() {
 #pragma unroll
         for (int i = 0; i < kMs; ++i)
 #pragma unroll
             for (int j = 0; j < kNs; ++j) acc[i][j] = accum16{};
-        a.load(depth, lds);
-        b.load(depth, lds + A::kBytes);
-        a.store(lds);
-        b.store(lds + A::kBytes);
-        int now = 0;
-        for (int64_t left = depth; left > 0; left -= kSlab<T>) {
-            __syncthreads();   // this slab has arrived, and no wave reads the other buffer any more
-            char* const here = lds + now * kBuffer;
-            char* const next = lds + (now ^ 1) * kBuffer;
-            const bool more = left > kSlab<T>;
-            if (more) {
-                a.load(left - kSlab<T>, next);
-                b.load(left - kSlab<T>, next + A::kBytes);
+    }
+
+    __device__ void add_slab(const char* here) {
+        const int lane = static_cast<int>(threadIdx.x % 64);
+        const int wm = wave_row(), wn = wave_column();
+#pragma unroll
+        for (int step = 0; step < kSlabBytes / 32; ++step) {
+            vec16 fa[kMs], fb[kNs];
+#pragma unroll
+            for (int i = 0; i < kMs; ++i) fa[i] = A::fragment(here, wm + 32 * i, step, lane);
+#pragma unroll
+            for (int j = 0; j < kNs; ++j) fb[j] = B::fragment(here + A::kBytes, wn + 32 * j, step, lane);
+#pragma unroll
+            for (int i = 0; i < kMs; ++i)
+#pragma unroll
+                for (int j = 0; j < kNs; ++j) acc[i][j] = multiply(T{}, fb[j], fa[i], acc[i][j]);
+        }
+    }
+
+    // Sums `depth` values of k.  a and b have begun.
+    __device__ void sum(A& a, B& b, int64_t depth, char* lds) {
+        clear();
+        if constexpr (kStages > 2) {
+            // Each wave waits for its own loads of the slab (the kAhead - 1 later slabs stay under way) and for its
+            // reads of the one before; past the barrier all of it is there, and the buffer read last is
+            // free.  Slabs past the end are queued as well, as zeros, so that the count of loads is constant.
+            constexpr int kAhead = kStages - 1, kPending = (kAhead - 1) * (A::kChunks + B::kChunks);
+            static_assert(kPending < 64, "the wait's count has 6 bits");
+            int64_t left = depth;   // of the next slab to queue
+#pragma unroll
+            for (int s = 0; s < kAhead; ++s, left -= kSlab<T>) {
+                a.load(left, lds + s * kBuffer);
+                b.load(left, lds + s * kBuffer + A::kBytes);
             }
-#pragma unroll
-            for (int step = 0; step < kSlabBytes / 32; ++step) {
-                vec16 fa[kMs], fb[kNs];
-#pragma unroll
-                for (int i = 0; i < kMs; ++i) fa[i] = A::fragment(here, wm + 32 * i, step, lane);
-#pragma unroll
-                for (int j = 0; j < kNs; ++j) fb[j] = B::fragment(here + A::kBytes, wn + 32 * j, step, lane);
-#pragma unroll
-                for (int i = 0; i < kMs; ++i)
-#pragma unroll
-                    for (int j = 0; j < kNs; ++j) acc[i][j] = multiply(T{}, fb[j], fa[i], acc[i][j]);
+            int now = 0;
+            for (int64_t done = 0; done < depth; done += kSlab<T>, left -= kSlab<T>) {
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kPending) : "memory");
+                const int then = now == 0 ? kStages - 1 : now - 1;
+                a.load(left, lds + then * kBuffer);
+                b.load(left, lds + then * kBuffer + A::kBytes);
+                add_slab(lds + now * kBuffer);
+                now = now + 1 == kStages ? 0 : now + 1;
             }
-            if (more) {
-                a.store(next);
-                b.store(next + A::kBytes);
+        } else if constexpr (kDirect) {
+            a.load(depth, lds);
+            b.load(depth, lds + A::kBytes);
+            int now = 0;
+            for (int64_t left = depth; left > 0; left -= kSlab<T>) {
+                __syncthreads();   // this slab has arrived, and no wave reads the other buffer any more
+                char* const next = lds + (now ^ 1) * kBuffer;
+                if (left > kSlab<T>) {
+                    a.load(left - kSlab<T>, next);
+                    b.load(left - kSlab<T>, next + A::kBytes);
+                }
+                add_slab(lds + now * kBuffer);
+                now ^= 1;
             }
-            now ^= 1;
+        } else {
+            // kAhead slabs under way in registers, two in LDS
+            constexpr int kAhead = kBM * kBN <= 64 * 64 ? 3 : (kBM * kBN < 128 * 128 ? 2 : 1);
+            typename A::Held ha[kAhead];
+            typename B::Held hb[kAhead];
+            int64_t left = depth;   // of the next slab to load
+#pragma unroll
+            for (int s = 0; s < kAhead; ++s, left -= kSlab<T>) {
+                a.load(left, ha[s]);
+                b.load(left, hb[s]);
+            }
+            int now = 0;
+            for (int64_t done = 0; done < depth;) {
+#pragma unroll
+                for (int s = 0; s < kAhead; ++s) {
+                    if (done >= depth) break;
+                    char* const here = lds + now * kBuffer;
+                    A::store(ha[s], here);
+                    B::store(hb[s], here + A::kBytes);
+                    __syncthreads();   // the slab is there; and no wave reads the buffer of the slab before last
+                    a.load(left, ha[s]);
+                    b.load(left, hb[s]);
+                    left -= kSlab<T>;
+                    add_slab(here);
+                    done += kSlab<T>;
+                    now ^= 1;
+                }
+            }
         }
         __syncthreads();
     }
@@ -440,6 +511,7 @@ struct WeightArgs {           // dw[e] = dz^T x over each expert's rows
     int64_t rows, ldz, ldx;
     int64_t piece;            // rows a workgroup sums
     int64_t pieces;           // piece ids
+    int edge;                 // of the tiles: 256, 128 or 64
     int experts, outputs, inputs;
 };
 
@@ -462,13 +534,6 @@ struct FoldArgs {             // out[e][i] = sum over e's pieces of partial[piec
     int experts;
     bool single;              // also the groups of one piece (and zeros for those of none)
 };
-
-// Edge of the weight gradient's tiles.
-inline int weight_edge(int outputs, int inputs) {
-    const int least = outputs < inputs ? outputs : inputs;
-    if (least <= 64) return 64;
-    return static_cast<int64_t>(outputs) * inputs >= int64_t{1} << 20 ? 256 : 128;
-}
 
 // Launches, per element type.
 template <class T> int launch_rows(const RowsArgs& a, bool forward, hipStream_t stream);

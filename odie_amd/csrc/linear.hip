@@ -27,20 +27,43 @@ int64_t slope_piece(int64_t rows, int outputs) {
     return piece < 64 ? 64 : piece;
 }
 
-// Rows a weight piece sums: workgroups for every CU over all experts and tiles (one a CU of the largest tiles).
-int64_t weight_piece(int64_t rows, int experts, int outputs, int inputs) {
-    const int edge = weight_edge(outputs, inputs);
-    const int64_t tiles = static_cast<int64_t>((outputs + edge - 1) / edge) * ((inputs + edge - 1) / edge);
-    const int64_t wanted = (edge == 256 ? 1 : 4) * kCus;
-    int64_t pieces = wanted / tiles - (experts > 1 ? experts : 0);
-    if (pieces < 1) pieces = experts > 1 ? 4 : 1;
-    int64_t piece = ((rows + pieces - 1) / pieces + 255) / 256 * 256;
-    return piece < 256 ? 256 : piece;
+// Tiles of the weight gradient and the rows a workgroup sums.  Every CU is to have a workgroup (four of the
+// smallest tiles, two of the middle ones), from several pieces of the rows where there are too few tiles;
+// but partial sums, written and read again, are to stay below twice what the operands hold.  The
+// largest tiles that manage it are taken (a 1024 x 1024 gradient over 4096 bf16 rows: 61 us as 16 tiles of
+// 256 x 256 and 16 pieces, 29 us as 64 of 128 x 128 and 4 pieces).
+struct WeightPlan {
+    int edge;
+    int64_t piece;
+};
+
+WeightPlan weight_plan(int64_t rows, int experts, int outputs, int inputs, int dtype) {
+    const int least = outputs < inputs ? outputs : inputs;
+    const int64_t matrix = static_cast<int64_t>(outputs) * inputs;
+    const int64_t most = rows * (static_cast<int64_t>(outputs) + inputs) * dtype_bytes(dtype) / (4 * matrix);
+    auto tiles_of = [&](int64_t edge) { return ((outputs + edge - 1) / edge) * ((inputs + edge - 1) / edge); };
+    auto whole = [](int64_t piece) { return piece < 256 ? 256 : (piece + 255) / 256 * 256; };
+    if (experts > 1) {
+        // Groups of up to twice the average stay whole where there are workgroups enough.
+        const int edge = least > 64 ? 128 : 64;   // 256 gains nothing where groups differ in length
+        const int64_t wanted = 4 * kCus / tiles_of(edge), pieces = wanted < most ? wanted : most;
+        if (pieces <= 2 * experts) return WeightPlan{edge, whole(2 * (rows / experts))};
+        return WeightPlan{edge, whole(rows / (pieces - experts / 2))};
+    }
+    for (int edge = 256;; edge /= 2) {
+        if (edge > 64 && least <= edge / 2) continue;
+        const int64_t tiles = tiles_of(edge);
+        int64_t pieces = 256 / edge * kCus / tiles;
+        if (pieces > most) pieces = most;
+        if (edge > 64 && tiles * pieces < kCus) continue;
+        return WeightPlan{edge, whole(pieces > 1 ? (rows + pieces - 1) / pieces : rows)};
+    }
 }
 
 struct Plan {
     int64_t dz_bytes, sums_bytes, partial_bytes;   // each a multiple of 256
     int64_t slope_piece, slope_pieces, weight_piece, weight_pieces;
+    int weight_edge;
 };
 
 int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -50,7 +73,9 @@ Plan make_plan(int64_t rows, int experts, bool grouped, int outputs, int inputs,
     Plan p{};
     p.slope_piece = slope_piece(rows, outputs);
     p.slope_pieces = piece_ids(rows, p.slope_piece, grouped && want_dbias, experts, false);
-    p.weight_piece = weight_piece(rows, experts, outputs, inputs);
+    const WeightPlan weight = weight_plan(rows, experts, outputs, inputs, dtype);
+    p.weight_piece = weight.piece;
+    p.weight_edge = weight.edge;
     p.weight_pieces = piece_ids(rows, p.weight_piece, grouped, experts, false);
     if (p.weight_pieces < 1) p.weight_pieces = 1;
     p.dz_bytes = activation == kNone ? 0 : padded(rows * outputs * dtype_bytes(dtype));
@@ -195,6 +220,7 @@ ODIE_API int odie_linear_backward(const void* upstream, int64_t upstream_stride,
             a.rows = rows;
             a.piece = p.weight_piece;
             a.pieces = p.weight_pieces;
+            a.edge = p.weight_edge;
             a.experts = experts;
             a.outputs = outputs;
             a.inputs = inputs;

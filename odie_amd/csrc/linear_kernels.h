@@ -19,9 +19,9 @@ __device__ inline TileAt tile_at(uint32_t id, uint32_t down, uint32_t across) {
     return TileAt{band * kBand + inside % high, inside / high};
 }
 
-template <class T, bool kForward, bool kDirect, int kBM, int kBN, int kWM, int kWN>
+template <class T, bool kForward, bool kDirect, int kBM, int kBN, int kWM, int kWN, int kStages>
 __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(RowsArgs a, uint32_t blocks) {
-    using Work = Tile<T, true, kForward, kDirect, kBM, kBN, kWM, kWN>;
+    using Work = Tile<T, true, kForward, kDirect, kBM, kBN, kWM, kWN, kStages>;
     __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
     const uint32_t id = xcd_major(blockIdx.x, gridDim.x);
     if (id >= blocks) return;
@@ -103,15 +103,100 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(Ro
         });
 }
 
+constexpr int kFewWaves = 8;
+
+// Few rows a group: the weights are read once, straight into registers in the layout of the products, and
+// everything else is small beside them.  A wave takes 16 columns of the output, 16 kRowTiles rows and one of
+// kSplit shares of the depth, of which it has several hundred bytes of every weight row under way; the
+// shares' sums are added in order through LDS.
+template <class T, int kRowTiles, int kSplit> __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(RowsArgs a) {
+    constexpr int kColumns = 16 * kFewWaves / kSplit;   // of a workgroup
+    __shared__ accum4 part[kFewWaves][kRowTiles][64];
+    constexpr int kStep = 4 * kPerVec<T>;          // k values a wave takes at a time
+    constexpr int kAhead = kRowTiles == 1 ? 8 : 4; // steps in flight
+    const uint32_t across = (a.columns + kColumns - 1) / kColumns;
+    const Piece p = find_piece(a.offsets, a.experts, a.experts + 1, a.rows, 16 * kRowTiles, blockIdx.x / across);
+    if (p.begin >= p.end) return;
+    const int column0 = static_cast<int>(blockIdx.x % across) * kColumns;
+    const T* residual = static_cast<const T*>(a.residual);
+    T* out = static_cast<T*>(a.out);
+    const int lane = static_cast<int>(threadIdx.x % 64);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64));
+    const bool owned = p.group < a.experts;        // else rows of no expert
+    if (owned && column0 + wave / kSplit * 16 < a.columns) {
+        const int own = lane % 16, quarter = lane / 16 * kPerVec<T>;
+        int column = column0 + wave / kSplit * 16 + own;
+        column = column < a.columns ? column : a.columns - 1;   // those past the last are not stored
+        const T* w = static_cast<const T*>(a.b) + (static_cast<int64_t>(p.group) * a.columns + column) * a.depth;
+        const T* x[kRowTiles];
+#pragma unroll
+        for (int t = 0; t < kRowTiles; ++t) {
+            const int64_t row = p.begin + 16 * t + own;
+            x[t] = static_cast<const T*>(a.a) + (row < p.end ? row : p.end - 1) * a.lda;
+        }
+        accum4 acc[kRowTiles] = {};
+        const int share = ((a.depth + kStep - 1) / kStep + kSplit - 1) / kSplit * kStep;
+        const int first = wave % kSplit * share, last = first + share < a.depth ? first + share : a.depth;
+        for (int k0 = first; k0 < last; k0 += kAhead * kStep) {
+            vec16 fw[kAhead], fx[kAhead][kRowTiles];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int k = k0 + u * kStep + quarter, count = last - k;
+                if (k0 + u * kStep + kStep <= last) {
+                    fw[u] = load16(w + k);
+#pragma unroll
+                    for (int t = 0; t < kRowTiles; ++t) fx[u][t] = load16(x[t] + k);
+                } else {
+                    fw[u] = count > 0 ? load_end(w + k, count, k) : vec16{};
+#pragma unroll
+                    for (int t = 0; t < kRowTiles; ++t) fx[u][t] = count > 0 ? load_end(x[t] + k, count, k) : vec16{};
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+                for (int t = 0; t < kRowTiles; ++t) acc[t] = multiply16(T{}, fw[u], fx[u][t], acc[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < kRowTiles; ++t) part[wave][t][lane] = acc[t];
+    }
+    __syncthreads();
+    const T* bias = a.bias && owned ? static_cast<const T*>(a.bias) + static_cast<int64_t>(p.group) * a.columns : nullptr;
+    T* pre = static_cast<T*>(a.pre);
+    for (int i = threadIdx.x; i < 16 * kRowTiles * kColumns; i += 64 * kFewWaves) {
+        const int r = i / kColumns, c = i % 16, tile = i % kColumns / 16, column = column0 + i % kColumns;
+        const int64_t row = p.begin + r;
+        if (row >= p.end || column >= a.columns) continue;
+        float value = 0.0f;
+        if (owned) {
+            // accumulator element v of lane l: row l % 16, column 4 (l / 16) + v
+#pragma unroll
+            for (int s = 0; s < kSplit; ++s) value += part[tile * kSplit + s][r / 16][c / 4 * 16 + r % 16][c % 4];
+            if (bias) value += static_cast<float>(bias[column]);
+            if (pre) pre[row * a.columns + column] = static_cast<T>(value);
+            with_activation(a.activation, [&](auto activation) { value = activate<activation, sizeof(T) == 4>(value); });
+        }
+        if (residual) value += static_cast<float>(residual[row * a.ldr + column]);
+        out[row * a.ldo + column] = static_cast<T>(value);
+    }
+}
+
 template <class T, bool kDirect, int kBM, int kBN, int kWM, int kWN>
 __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void weight_kernel(WeightArgs a, uint32_t blocks) {
-    using Work = Tile<T, false, false, kDirect, kBM, kBN, kWM, kWN>;
+    using Work = Tile<T, false, false, kDirect, kBM, kBN, kWM, kWN, kBM == 64 ? 4 : 2>;
     __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
-    const uint32_t id = xcd_major(blockIdx.x, gridDim.x);
+    const uint32_t across = (a.inputs + kBN - 1) / kBN, down = (a.outputs + kBM - 1) / kBM, tiles = down * across;
+    // A piece's tiles share its rows in one XCD's L2.  Several experts' pieces differ in length, and an XCD could be
+    // left with the long ones: where there are tiles enough each piece is spread over the XCDs instead, eighths of
+    // its tiles together (bf16, 131072 x 1024 x 1024 over 64 experts: 604 -> 561 us, 262144 x 512 x 2048 over 8: 1180 ->
+    // 921; but 131072 x 256 x 512 over 64, 8 tiles a piece: 104 -> 148).
+    const bool spread = a.offsets && tiles >= 64 && tiles % kXcds == 0;
+    const uint32_t id = spread ? blockIdx.x : xcd_major(blockIdx.x, gridDim.x);
     if (id >= blocks) return;
-    const uint32_t across = (a.inputs + kBN - 1) / kBN, down = (a.outputs + kBM - 1) / kBM;
-    const uint32_t piece = id / (down * across);
-    const TileAt t = tile_at(id % (down * across), down, across);
+    const uint32_t piece = id / tiles;
+    uint32_t tile = id % tiles;
+    if (spread) tile = tile % kXcds * (tiles / kXcds) + tile / kXcds;
+    const TileAt t = tile_at(tile, down, across);
     const Piece p = find_piece(a.offsets, a.experts, a.experts, a.rows, a.piece, piece);
     if (p.first > 0 && p.begin >= p.end) return;
     const int row0 = static_cast<int>(t.row) * kBM, column0 = static_cast<int>(t.column) * kBN;
@@ -223,14 +308,31 @@ template <class T, int kGroups> __global__ __launch_bounds__(256) void fold_kern
 
 uint32_t whole_xcds(int64_t blocks) { return static_cast<uint32_t>((blocks + kXcds - 1) / kXcds * kXcds); }
 
-template <class T, bool kForward, bool kDirect, int kBM, int kBN, int kWM, int kWN> int launch_rows_as(RowsArgs a, hipStream_t stream) {
+template <class T, bool kForward, bool kDirect, int kBM, int kBN, int kWM, int kWN, int kStages = 2>
+int launch_rows_as(RowsArgs a, hipStream_t stream) {
     const int64_t across = (a.columns + kBN - 1) / kBN;
     a.tiles = piece_ids(a.rows, kBM, a.offsets != nullptr, a.experts, true);
     const int64_t blocks = a.tiles * across;
     if (blocks >= int64_t{1} << 31) return fail("linear: too many tiles for one launch");
-    rows_kernel<T, kForward, kDirect, kBM, kBN, kWM, kWN>
+    rows_kernel<T, kForward, kDirect, kBM, kBN, kWM, kWN, kStages>
         <<<whole_xcds(blocks), 64 * (kBM / kWM) * (kBN / kWN), 0, stream>>>(a, static_cast<uint32_t>(blocks));
     return check_launch("linear");
+}
+
+template <class T, int kRowTiles, int kSplit> int launch_few_rows_as(const RowsArgs& a, hipStream_t stream) {
+    const int64_t across = (a.columns + 16 * kFewWaves / kSplit - 1) / (16 * kFewWaves / kSplit);
+    const int64_t blocks = piece_ids(a.rows, 16 * kRowTiles, a.offsets != nullptr, a.experts, true) * across;
+    if (blocks >= int64_t{1} << 31) return fail("linear: too many tiles for one launch");
+    few_rows_kernel<T, kRowTiles, kSplit><<<static_cast<uint32_t>(blocks), 64 * kFewWaves, 0, stream>>>(a);
+    return check_launch("linear");
+}
+
+// The depth is split over all eight waves where a share is still long or there are too few workgroups otherwise.
+template <class T, int kRowTiles> int launch_few_rows(const RowsArgs& a, hipStream_t stream) {
+    const int64_t steps = a.depth / (4 * kPerVec<T>);
+    const int64_t busy = a.rows < a.experts ? a.rows : a.experts;
+    if (steps >= 64 || busy * a.columns < 64 * kCus) return launch_few_rows_as<T, kRowTiles, 8>(a, stream);
+    return launch_few_rows_as<T, kRowTiles, 2>(a, stream);
 }
 
 // Whether rows of `width` elements can go to LDS directly, 16 bytes a lane.
@@ -241,22 +343,23 @@ template <class T> bool direct(const void* data, int64_t stride, int64_t width) 
 }
 
 // Tiles by the work there is (us of one bf16 product, 65536 x 1024 x 4096 and 65536 x 256 x 512):
-//   256 x 256, 64 x 128 a wave   620, 33   where every CU gets one and a group's rows fill them (the path
-//                                          through registers has no room for it)
+//   256 x 256, 64 x 128 a wave   620, 33   where every CU gets one, a group's rows fill them and the depth outlasts
+//                                          their start and end (the path through registers has no room)
 //   128 x 128, 64 x 64 a wave    777, 30   two a CU
 //   128 x 64, 32 x 64 a wave     narrow outputs: no columns wasted
-//   64 x 64, 32 x 32 a wave      what is left: too few tiles otherwise
+//   64 x 64, 32 x 32 a wave      what is left: too few tiles otherwise; straight to LDS with three slabs under way
+//                                (seven are no faster: 512 x 2048 x 2048 14.4 us with three, 15.5 with seven)
 template <class T, bool kForward, bool kDirect> int launch_rows_of(const RowsArgs& a, hipStream_t stream) {
     const int64_t each = a.rows / a.experts;   // rows of a group, on average
     const int64_t large = (a.rows + 255) / 256 * ((a.columns + 255) / 256);
     const int64_t wide = (a.rows + 127) / 128 * ((a.columns + 127) / 128);
     if constexpr (kDirect)
-        if (a.columns > 128 && large >= kCus && each >= 1024)
+        if (a.columns > 128 && large >= kCus && each >= 1024 && a.depth >= 512)
             return launch_rows_as<T, kForward, true, 256, 256, 64, 128>(a, stream);
     if (a.columns <= 64 && a.rows >= 128 * kCus) return launch_rows_as<T, kForward, kDirect, 128, 64, 32, 64>(a, stream);
     if (a.columns > 64 && wide >= kCus && each >= 128)
         return launch_rows_as<T, kForward, kDirect, 128, 128, 64, 64>(a, stream);
-    return launch_rows_as<T, kForward, kDirect, 64, 64, 32, 32>(a, stream);
+    return launch_rows_as<T, kForward, kDirect, 64, 64, 32, 32, kDirect ? 4 : 2>(a, stream);
 }
 
 template <class T, bool kDirect, int kBM, int kBN, int kWM, int kWN> int launch_weight_as(const WeightArgs& a, hipStream_t stream) {
@@ -273,12 +376,19 @@ template <class T, bool kDirect, int kBM, int kBN, int kWM, int kWN> int launch_
 template <class T> int launch_rows(const RowsArgs& a, bool forward, hipStream_t stream) {
     const bool straight = direct<T>(a.a, a.lda, a.depth) && direct<T>(a.b, forward ? a.depth : a.columns, a.depth) &&
                           a.columns % (forward ? 1 : kPerVec<T>) == 0;
+    if (forward) {
+        // groups of varying sizes: room for twice the average
+        const int64_t each = (a.rows + a.experts - 1) / a.experts * (a.experts > 1 ? 2 : 1);
+        if (each <= 16) return launch_few_rows<T, 1>(a, stream);
+        if (each <= 32) return launch_few_rows<T, 2>(a, stream);
+        if (each <= 64) return launch_few_rows<T, 4>(a, stream);
+    }
     if (forward) return straight ? launch_rows_of<T, true, true>(a, stream) : launch_rows_of<T, true, false>(a, stream);
     return straight ? launch_rows_of<T, false, true>(a, stream) : launch_rows_of<T, false, false>(a, stream);
 }
 
 template <class T, bool kDirect> int launch_weight_of(const WeightArgs& a, hipStream_t stream) {
-    switch (weight_edge(a.outputs, a.inputs)) {
+    switch (a.edge) {
         case 256:
             if constexpr (kDirect) return launch_weight_as<T, true, 256, 256, 64, 128>(a, stream);
             [[fallthrough]];
