@@ -180,88 +180,129 @@ template <class T, bool kByRow, int kRows, int kThreads> struct Direct : Image<T
     }
 };
 
-// Through registers, for rows of any alignment and length.
+// Through registers, for rows of any alignment.  Every load is issued without a condition, from an address moved
+// back into the tensor where it would leave it (a branch around loads makes the compiler wait for those in
+// flight); what was moved is put right on the way to LDS.  Needs 16 bytes of k (k consecutive) or of columns (one row
+// per k) at least, and one k.
 template <class T, bool kByRow, int kRows, int kThreads> struct Staged : Image<T, kByRow, kRows, kThreads> {
     using I = Image<T, kByRow, kRows, kThreads>;
     struct Held {
         vec16 chunk[I::kChunks];
     };
-    const T* at[kByRow ? I::kChunks : 1];
-    int64_t step;        // one row per k: elements between this thread's chunks
-    int64_t slab;        // elements from slab to slab
-    int64_t before;      // elements of the row before this thread's chunk
+    const T* at[kByRow ? I::kChunks : 1];   // k consecutive: the rows' begins; else this thread's column in row 0
+    int64_t stride, next;                   // next: k of the slab to load
+    int64_t depth;
     int lead;            // k of the first chunk, relative to the slab
-    int columns;         // one row per k: columns of this thread's chunk inside the tensor
+    int back;            // one row per k: columns that the chunk was moved back by
 
-    __device__ void begin(const T* data, int64_t stride, int64_t first, int64_t limit, int64_t) {
+    __device__ void begin(const T* data, int64_t pitch, int64_t first, int64_t limit, int64_t ks) {
+        stride = pitch;
+        depth = ks;
+        next = 0;
+        back = 0;
         if constexpr (kByRow) {
             lead = I::chunk() * I::kVec;
-            slab = kSlab<T>;
-            before = lead;
-            columns = I::kVec;
 #pragma unroll
             for (int i = 0; i < I::kChunks; ++i) {
                 const int64_t r = first + I::row() + i * I::kStep;
-                at[i] = data + (r < limit ? r : limit - 1) * stride + lead;
+                at[i] = data + (r < limit ? r : limit - 1) * stride;
             }
         } else {
             lead = I::row();
-            before = first + I::chunk() * I::kVec;
-            const int64_t left = limit - before;
-            columns = left >= I::kVec ? I::kVec : (left > 0 ? static_cast<int>(left) : 0);
-            at[0] = data + lead * stride + before;
-            step = I::kStep * stride;
-            slab = kSlab<T> * stride;
+            const int64_t column = first + I::chunk() * I::kVec, last = limit - I::kVec;
+            at[0] = data + (column < last ? column : last);
+            if (column > last) back = column - last < I::kVec ? static_cast<int>(column - last) : 0;
         }
     }
 
-    // Starts the loads of the next slab, of which `left` values of k exist (the rest read as 0).
-    __device__ void load(int64_t left, Held& held) {
+    __device__ void load(Held& held) {
         if constexpr (kByRow) {
-            if (left >= kSlab<T>) {
+            const int64_t k = next + lead < depth - I::kVec ? next + lead : depth - I::kVec;
 #pragma unroll
-                for (int i = 0; i < I::kChunks; ++i) held.chunk[i] = load16(at[i]);
-            } else {
-                const int count = static_cast<int>(left) - lead;
-#pragma unroll
-                for (int i = 0; i < I::kChunks; ++i) held.chunk[i] = count > 0 ? load_end(at[i], count, before) : vec16{};
-            }
-#pragma unroll
-            for (int i = 0; i < I::kChunks; ++i) at[i] += slab;
-            before += slab;
+            for (int i = 0; i < I::kChunks; ++i) held.chunk[i] = load16(at[i] + k);
         } else {
-            if (columns == I::kVec) {
 #pragma unroll
-                for (int i = 0; i < I::kChunks; ++i)
-                    held.chunk[i] = lead + i * I::kStep < left ? load16(at[0] + i * step) : vec16{};
-            } else {
-#pragma unroll
-                for (int i = 0; i < I::kChunks; ++i)
-                    held.chunk[i] = lead + i * I::kStep < left && columns > 0
-                                  ? load_end(at[0] + i * step, columns, before) : vec16{};
+            for (int i = 0; i < I::kChunks; ++i) {
+                const int64_t k = next + lead + i * I::kStep;
+                held.chunk[i] = load16(at[0] + (k < depth ? k : depth - 1) * stride);
             }
-            at[0] += slab;
         }
+        next += kSlab<T>;
     }
 
-    static __device__ void store(const Held& held, char* lds) {
+    // `left` values of k of this slab exist; the rest become 0.
+    __device__ void store(const Held& held, char* lds, int64_t left) const {
+        const int count = left < kSlab<T> ? static_cast<int>(left) - lead : kSlab<T>;   // of k, from the first chunk on
+#pragma unroll
+        for (int i = 0; i < I::kChunks; ++i) {
+            vec16 v = held.chunk[i];
+            if constexpr (kByRow) {
+                if (count < I::kVec) v = count > 0 ? shift_down(v, (I::kVec - count) * static_cast<int>(sizeof(T))) : vec16{};
+            } else {
+                if (i * I::kStep >= count) v = vec16{};
+                if (back > 0) v = shift_down(v, back * static_cast<int>(sizeof(T)));
+            }
+            *reinterpret_cast<vec16*>(lds + (threadIdx.x + i * kThreads) * 16) = v;
+        }
+    }
+};
+
+// The same element by element, for tensors without 16 bytes a row.
+template <class T, bool kByRow, int kRows, int kThreads> struct Gathered : Image<T, kByRow, kRows, kThreads> {
+    using I = Image<T, kByRow, kRows, kThreads>;
+    struct Held {
+        vec16 chunk[I::kChunks];
+    };
+    const T* data;
+    int64_t stride, next, first, limit, depth;
+
+    __device__ void begin(const T* base, int64_t pitch, int64_t begin, int64_t end, int64_t ks) {
+        data = base;
+        stride = pitch;
+        next = 0;
+        first = begin;
+        limit = end;
+        depth = ks;
+    }
+
+    __device__ void load(Held& held) {
+#pragma unroll
+        for (int i = 0; i < I::kChunks; ++i) {
+            const int r = I::row() + i * I::kStep, c = I::chunk() * I::kVec;
+            const int64_t own = first + (kByRow ? r : c), k = next + (kByRow ? c : r);
+            const int64_t left = kByRow ? depth - k : limit - own;
+            const bool inside = own < limit && k < depth;
+            held.chunk[i] = inside ? gather16(data + (kByRow ? own * stride + k : k * stride + own),
+                                              left < I::kVec ? static_cast<int>(left) : I::kVec) : vec16{};
+        }
+        next += kSlab<T>;
+    }
+
+    __device__ void store(const Held& held, char* lds, int64_t) const {
 #pragma unroll
         for (int i = 0; i < I::kChunks; ++i)
             *reinterpret_cast<vec16*>(lds + (threadIdx.x + i * kThreads) * 16) = held.chunk[i];
     }
 };
 
+// How operands reach LDS.
+enum Way { kDirect, kStaged, kGathered };
+
 // One workgroup's tile: waves of kWM x kWN, kBM / kWM x kBN / kWN of them.
-template <class T, bool kAByRow, bool kBByRow, bool kDirect, int kBM, int kBN, int kWM, int kWN, int kWantedStages = 2>
+template <class T, bool kAByRow, bool kBByRow, Way kWay, int kBM, int kBN, int kWM, int kWN, int kWantedStages = 2>
 struct Tile {
     static constexpr int kThreads = 64 * (kBM / kWM) * (kBN / kWN);
-    using A = std::conditional_t<kDirect, Direct<T, kAByRow, kBM, kThreads>, Staged<T, kAByRow, kBM, kThreads>>;
-    using B = std::conditional_t<kDirect, Direct<T, kBByRow, kBN, kThreads>, Staged<T, kBByRow, kBN, kThreads>>;
+    template <bool kByRow, int kRows>
+    using Loader = std::conditional_t<kWay == kDirect, Direct<T, kByRow, kRows, kThreads>,
+                                      std::conditional_t<kWay == kStaged, Staged<T, kByRow, kRows, kThreads>,
+                                                         Gathered<T, kByRow, kRows, kThreads>>>;
+    using A = Loader<kAByRow, kBM>;
+    using B = Loader<kBByRow, kBN>;
     static constexpr int kMs = kWM / 32, kNs = kWN / 32;
     static constexpr int kBuffer = A::kBytes + B::kBytes;
     static constexpr int kPitch = kWN + 4;                  // floats a row of the epilogue's region
     static constexpr int kRegion = 32 * kPitch * 4;
-    static constexpr int kStages = kDirect ? kWantedStages : 2;   // slabs in LDS: one read, the others under way
+    static constexpr int kStages = kWay == kDirect ? kWantedStages : 2;   // slabs in LDS: one read, the others under way
     static constexpr int kLds = kStages * kBuffer > kThreads / 64 * kRegion ? kStages * kBuffer : kThreads / 64 * kRegion;
 
     accum16 acc[kMs][kNs];
@@ -294,9 +335,10 @@ struct Tile {
         }
     }
 
-    // Sums `depth` values of k.  a and b have begun.
+    // Sums `depth` values of k, the same for the whole workgroup.  a and b have begun.
     __device__ void sum(A& a, B& b, int64_t depth, char* lds) {
         clear();
+        if (depth <= 0) return;
         if constexpr (kStages > 2) {
             // Each wave waits for its own loads of the slab (the kAhead - 1 later slabs stay under way) and for its
             // reads of the one before; past the barrier all of it is there, and the buffer read last is
@@ -318,7 +360,7 @@ struct Tile {
                 add_slab(lds + now * kBuffer);
                 now = now + 1 == kStages ? 0 : now + 1;
             }
-        } else if constexpr (kDirect) {
+        } else if constexpr (kWay == kDirect) {
             a.load(depth, lds);
             b.load(depth, lds + A::kBytes);
             int now = 0;
@@ -334,29 +376,27 @@ struct Tile {
             }
         } else {
             // kAhead slabs under way in registers, two in LDS
-            constexpr int kAhead = kBM * kBN <= 64 * 64 ? 3 : (kBM * kBN < 128 * 128 ? 2 : 1);
+            constexpr int kAhead = kWay == kGathered ? 1 : (kBM * kBN <= 64 * 64 ? 3 : 2);
             typename A::Held ha[kAhead];
             typename B::Held hb[kAhead];
-            int64_t left = depth;   // of the next slab to load
 #pragma unroll
-            for (int s = 0; s < kAhead; ++s, left -= kSlab<T>) {
-                a.load(left, ha[s]);
-                b.load(left, hb[s]);
+            for (int s = 0; s < kAhead; ++s) {
+                a.load(ha[s]);
+                b.load(hb[s]);
             }
             int now = 0;
-            for (int64_t done = 0; done < depth;) {
+            for (int64_t left = depth; left > 0;) {
 #pragma unroll
                 for (int s = 0; s < kAhead; ++s) {
-                    if (done >= depth) break;
+                    if (left <= 0) break;
                     char* const here = lds + now * kBuffer;
-                    A::store(ha[s], here);
-                    B::store(hb[s], here + A::kBytes);
+                    a.store(ha[s], here, left);
+                    b.store(hb[s], here + A::kBytes, left);
                     __syncthreads();   // the slab is there; and no wave reads the buffer of the slab before last
-                    a.load(left, ha[s]);
-                    b.load(left, hb[s]);
-                    left -= kSlab<T>;
+                    a.load(ha[s]);
+                    b.load(hb[s]);
                     add_slab(here);
-                    done += kSlab<T>;
+                    left -= kSlab<T>;
                     now ^= 1;
                 }
             }

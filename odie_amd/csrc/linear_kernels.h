@@ -19,9 +19,9 @@ __device__ inline TileAt tile_at(uint32_t id, uint32_t down, uint32_t across) {
     return TileAt{band * kBand + inside % high, inside / high};
 }
 
-template <class T, bool kForward, bool kDirect, int kBM, int kBN, int kWM, int kWN, int kStages>
+template <class T, bool kForward, Way kWay, int kBM, int kBN, int kWM, int kWN, int kStages>
 __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(RowsArgs a, uint32_t blocks) {
-    using Work = Tile<T, true, kForward, kDirect, kBM, kBN, kWM, kWN, kStages>;
+    using Work = Tile<T, true, kForward, kWay, kBM, kBN, kWM, kWN, kStages>;
     __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
     const uint32_t id = xcd_major(blockIdx.x, gridDim.x);
     if (id >= blocks) return;
@@ -181,9 +181,9 @@ template <class T, int kRowTiles, int kSplit> __global__ __launch_bounds__(64 * 
     }
 }
 
-template <class T, bool kDirect, int kBM, int kBN, int kWM, int kWN>
+template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN>
 __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void weight_kernel(WeightArgs a, uint32_t blocks) {
-    using Work = Tile<T, false, false, kDirect, kBM, kBN, kWM, kWN, kBM == 64 ? 4 : 2>;
+    using Work = Tile<T, false, false, kWay, kBM, kBN, kWM, kWN, kBM == 64 ? 4 : 2>;
     __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
     const uint32_t across = (a.inputs + kBN - 1) / kBN, down = (a.outputs + kBM - 1) / kBM, tiles = down * across;
     // A piece's tiles share its rows in one XCD's L2.  Several experts' pieces differ in length, and an XCD could be
@@ -284,37 +284,40 @@ template <class T, int kGroups> __global__ __launch_bounds__(256) void fold_kern
     constexpr int kLanes = 256 / kGroups;
     __shared__ float total[kGroups > 1 ? 256 : 1];
     const int lane = static_cast<int>(threadIdx.x) % kLanes, group = static_cast<int>(threadIdx.x) / kLanes;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kLanes + lane;
     const int e = static_cast<int>(blockIdx.y);
     const int64_t begin = a.offsets ? group_start(a.offsets, e, a.rows) : 0;
     const int64_t end = a.offsets ? group_start(a.offsets, e + 1, a.rows) : a.rows;
     const int64_t first = a.offsets ? whole_pieces(a.offsets, e, a.rows, a.piece) + e : 0;
     const int64_t pieces = end > begin ? (end - begin + a.piece - 1) / a.piece : 0;
     if (pieces <= 1 && !a.single) return;
-    float sum = 0.0f;
-    if (i < a.size) {
-        const float* from = a.partial + first * a.size + i;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * kLanes; base < a.size; base += static_cast<int64_t>(gridDim.x) * kLanes) {
+        const int64_t i = base + lane;
+        float sum = 0.0f;
+        if (i < a.size) {
+            const float* from = a.partial + first * a.size + i;
 #pragma unroll 4
-        for (int64_t p = group; p < pieces; p += kGroups) sum += from[p * a.size];
+            for (int64_t p = group; p < pieces; p += kGroups) sum += from[p * a.size];
+        }
+        if constexpr (kGroups > 1) {
+            total[threadIdx.x] = sum;
+            __syncthreads();
+            if (group == 0)
+                for (int g = 1; g < kGroups; ++g) sum += total[g * kLanes + lane];
+            __syncthreads();
+        }
+        if (group == 0 && i < a.size) static_cast<T*>(a.out)[e * a.size + i] = static_cast<T>(sum);
     }
-    if constexpr (kGroups > 1) {
-        total[threadIdx.x] = sum;
-        __syncthreads();
-        if (group > 0) return;
-        for (int g = 1; g < kGroups; ++g) sum += total[g * kLanes + lane];
-    }
-    if (i < a.size) static_cast<T*>(a.out)[e * a.size + i] = static_cast<T>(sum);
 }
 
 uint32_t whole_xcds(int64_t blocks) { return static_cast<uint32_t>((blocks + kXcds - 1) / kXcds * kXcds); }
 
-template <class T, bool kForward, bool kDirect, int kBM, int kBN, int kWM, int kWN, int kStages = 2>
+template <class T, bool kForward, Way kWay, int kBM, int kBN, int kWM, int kWN, int kStages = 2>
 int launch_rows_as(RowsArgs a, hipStream_t stream) {
     const int64_t across = (a.columns + kBN - 1) / kBN;
     a.tiles = piece_ids(a.rows, kBM, a.offsets != nullptr, a.experts, true);
     const int64_t blocks = a.tiles * across;
     if (blocks >= int64_t{1} << 31) return fail("linear: too many tiles for one launch");
-    rows_kernel<T, kForward, kDirect, kBM, kBN, kWM, kWN, kStages>
+    rows_kernel<T, kForward, kWay, kBM, kBN, kWM, kWN, kStages>
         <<<whole_xcds(blocks), 64 * (kBM / kWM) * (kBN / kWN), 0, stream>>>(a, static_cast<uint32_t>(blocks));
     return check_launch("linear");
 }
@@ -335,38 +338,56 @@ template <class T, int kRowTiles> int launch_few_rows(const RowsArgs& a, hipStre
     return launch_few_rows_as<T, kRowTiles, 2>(a, stream);
 }
 
-// Whether rows of `width` elements can go to LDS directly, 16 bytes a lane.
-template <class T> bool direct(const void* data, int64_t stride, int64_t width) {
+// The way to LDS of rows of `width` elements: directly where each row starts on 16 bytes and is a multiple of them.
+template <class T> Way way_of(const void* data, int64_t stride, int64_t width) {
     const int64_t pitch = stride * static_cast<int64_t>(sizeof(T));
+    if (width < kPerVec<T>) return kGathered;
     return reinterpret_cast<uintptr_t>(data) % 16 == 0 && pitch % 16 == 0 && width % kPerVec<T> == 0 &&
-           pitch < (int64_t{1} << 22);   // 256 rows of a tile within 2^30 bytes
+                   pitch < (int64_t{1} << 22)   // 256 rows of a tile within 2^30 bytes
+               ? kDirect : kStaged;
 }
 
-// Tiles by the work there is (us of one bf16 product, 65536 x 1024 x 4096 and 65536 x 256 x 512):
-//   256 x 256, 64 x 128 a wave   620, 33   where every CU gets one, a group's rows fill them and the depth outlasts
-//                                          their start and end (the path through registers has no room)
-//   128 x 128, 64 x 64 a wave    777, 30   two a CU
+inline Way slower(Way a, Way b) { return a > b ? a : b; }
+
+// Whether `tiles` keep three quarters of the CUs busy to the end.
+inline bool even(int64_t tiles) { return tiles >= kCus && 4 * tiles >= 3 * ((tiles + kCus - 1) / kCus * kCus); }
+
+// Tiles by the work there is (us of one bf16 product, 65536 x 1024 x 4096; and with its epilogue, 131072 x 256 x 512
+// over 64 experts):
+//   256 x 256, 64 x 128 a wave   620, 112  where they go round and a group's rows fill them (the path through
+//                                          registers has no room)
+//   128 x 128, 64 x 64 a wave    777, 130  two a CU, where they go round
 //   128 x 64, 32 x 64 a wave     narrow outputs: no columns wasted
-//   64 x 64, 32 x 32 a wave      what is left: too few tiles otherwise; straight to LDS with three slabs under way
-//                                (seven are no faster: 512 x 2048 x 2048 14.4 us with three, 15.5 with seven)
-template <class T, bool kForward, bool kDirect> int launch_rows_of(const RowsArgs& a, hipStream_t stream) {
+//   64 x 64, 32 x 32 a wave      what is left; straight to LDS with three slabs under way (seven are no
+//                                faster: 512 x 2048 x 2048 14.4 us with three, 15.5 with seven)
+// Tiles that leave CUs idle in their last round are passed over where the products bound them: the largest, and fp32's
+// (4096 x 1023 x 1025: 288 tiles of 128 x 128 155 us, 1105 of 64 x 64 119 us; in bf16 31 and 37).
+template <class T, bool kForward, Way kWay> int launch_rows_of(const RowsArgs& a, hipStream_t stream) {
     const int64_t each = a.rows / a.experts;   // rows of a group, on average
     const int64_t large = (a.rows + 255) / 256 * ((a.columns + 255) / 256);
     const int64_t wide = (a.rows + 127) / 128 * ((a.columns + 127) / 128);
-    if constexpr (kDirect)
-        if (a.columns > 128 && large >= kCus && each >= 1024 && a.depth >= 512)
-            return launch_rows_as<T, kForward, true, 256, 256, 64, 128>(a, stream);
-    if (a.columns <= 64 && a.rows >= 128 * kCus) return launch_rows_as<T, kForward, kDirect, 128, 64, 32, 64>(a, stream);
-    if (a.columns > 64 && wide >= kCus && each >= 128)
-        return launch_rows_as<T, kForward, kDirect, 128, 128, 64, 64>(a, stream);
-    return launch_rows_as<T, kForward, kDirect, 64, 64, 32, 32, kDirect ? 4 : 2>(a, stream);
+    if constexpr (kWay == kDirect)
+        if (a.columns > 128 && even(large) && each >= 1024)
+            return launch_rows_as<T, kForward, kWay, 256, 256, 64, 128>(a, stream);
+    if constexpr (kWay != kGathered) {
+        if (a.columns <= 64 && a.rows >= 128 * kCus) return launch_rows_as<T, kForward, kWay, 128, 64, 32, 64>(a, stream);
+        if (a.columns > 64 && (sizeof(T) == 4 ? even(wide) : wide >= kCus) && each >= 128)
+            return launch_rows_as<T, kForward, kWay, 128, 128, 64, 64>(a, stream);
+    }
+    return launch_rows_as<T, kForward, kWay, 64, 64, 32, 32, kWay == kDirect ? 4 : 2>(a, stream);
 }
 
-template <class T, bool kDirect, int kBM, int kBN, int kWM, int kWN> int launch_weight_as(const WeightArgs& a, hipStream_t stream) {
+template <class T, bool kForward> int launch_rows_by(Way way, const RowsArgs& a, hipStream_t stream) {
+    if (way == kDirect) return launch_rows_of<T, kForward, kDirect>(a, stream);
+    if (way == kStaged) return launch_rows_of<T, kForward, kStaged>(a, stream);
+    return launch_rows_of<T, kForward, kGathered>(a, stream);
+}
+
+template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> int launch_weight_as(const WeightArgs& a, hipStream_t stream) {
     const int64_t tiles = static_cast<int64_t>((a.outputs + kBM - 1) / kBM) * ((a.inputs + kBN - 1) / kBN);
     const int64_t blocks = a.pieces * tiles;
     if (blocks >= int64_t{1} << 31) return fail("linear: too many tiles for one launch");
-    weight_kernel<T, kDirect, kBM, kBN, kWM, kWN>
+    weight_kernel<T, kWay, kBM, kBN, kWM, kWN>
         <<<whole_xcds(blocks), 64 * (kBM / kWM) * (kBN / kWN), 0, stream>>>(a, static_cast<uint32_t>(blocks));
     return check_launch("linear weight gradient");
 }
@@ -374,32 +395,30 @@ template <class T, bool kDirect, int kBM, int kBN, int kWM, int kWN> int launch_
 }  // namespace
 
 template <class T> int launch_rows(const RowsArgs& a, bool forward, hipStream_t stream) {
-    const bool straight = direct<T>(a.a, a.lda, a.depth) && direct<T>(a.b, forward ? a.depth : a.columns, a.depth) &&
-                          a.columns % (forward ? 1 : kPerVec<T>) == 0;
     if (forward) {
         // groups of varying sizes: room for twice the average
         const int64_t each = (a.rows + a.experts - 1) / a.experts * (a.experts > 1 ? 2 : 1);
         if (each <= 16) return launch_few_rows<T, 1>(a, stream);
         if (each <= 32) return launch_few_rows<T, 2>(a, stream);
         if (each <= 64) return launch_few_rows<T, 4>(a, stream);
+        return launch_rows_by<T, true>(slower(way_of<T>(a.a, a.lda, a.depth), way_of<T>(a.b, a.depth, a.depth)), a, stream);
     }
-    if (forward) return straight ? launch_rows_of<T, true, true>(a, stream) : launch_rows_of<T, true, false>(a, stream);
-    return straight ? launch_rows_of<T, false, true>(a, stream) : launch_rows_of<T, false, false>(a, stream);
+    return launch_rows_by<T, false>(slower(way_of<T>(a.a, a.lda, a.depth), way_of<T>(a.b, a.columns, a.columns)), a, stream);
 }
 
-template <class T, bool kDirect> int launch_weight_of(const WeightArgs& a, hipStream_t stream) {
-    switch (a.edge) {
-        case 256:
-            if constexpr (kDirect) return launch_weight_as<T, true, 256, 256, 64, 128>(a, stream);
-            [[fallthrough]];
-        case 128: return launch_weight_as<T, kDirect, 128, 128, 64, 64>(a, stream);
-        default: return launch_weight_as<T, kDirect, 64, 64, 32, 32>(a, stream);
-    }
+template <class T, Way kWay> int launch_weight_of(const WeightArgs& a, hipStream_t stream) {
+    if constexpr (kWay == kDirect)
+        if (a.edge == 256) return launch_weight_as<T, kWay, 256, 256, 64, 128>(a, stream);
+    if constexpr (kWay != kGathered)
+        if (a.edge >= 128) return launch_weight_as<T, kWay, 128, 128, 64, 64>(a, stream);
+    return launch_weight_as<T, kWay, 64, 64, 32, 32>(a, stream);
 }
 
 template <class T> int launch_weight(const WeightArgs& a, hipStream_t stream) {
-    const bool straight = direct<T>(a.dz, a.ldz, a.outputs) && direct<T>(a.x, a.ldx, a.inputs);
-    return straight ? launch_weight_of<T, true>(a, stream) : launch_weight_of<T, false>(a, stream);
+    const Way way = slower(way_of<T>(a.dz, a.ldz, a.outputs), way_of<T>(a.x, a.ldx, a.inputs));
+    if (way == kDirect) return launch_weight_of<T, kDirect>(a, stream);
+    if (way == kStaged) return launch_weight_of<T, kStaged>(a, stream);
+    return launch_weight_of<T, kGathered>(a, stream);
 }
 
 template <class T> int launch_slope(const SlopeArgs& a, hipStream_t stream) {
@@ -416,8 +435,10 @@ template <class T> int launch_slope(const SlopeArgs& a, hipStream_t stream) {
 template <class T> int launch_fold(const FoldArgs& a, hipStream_t stream) {
     // many pieces of few elements (a bias): several groups share them
     const bool tall = a.rows / a.piece >= 8 * static_cast<int64_t>(a.experts);
-    const int64_t lanes = tall ? 16 : 256, blocks = (a.size + lanes - 1) / lanes;
-    if (blocks >= int64_t{1} << 31) return fail("linear: too many sums for one launch");
+    const int64_t lanes = tall ? 16 : 256;
+    // most experts' groups are whole and have nothing to add: few workgroups each
+    const int64_t most = a.experts > 1 ? 16 * kCus / a.experts + 8 : 16 * kCus;
+    const int64_t blocks = (a.size + lanes - 1) / lanes < most ? (a.size + lanes - 1) / lanes : most;
     const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(a.experts));
     if (tall) fold_kernel<T, 16><<<grid, 256, 0, stream>>>(a);
     else fold_kernel<T, 1><<<grid, 256, 0, stream>>>(a);
