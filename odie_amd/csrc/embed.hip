@@ -278,6 +278,7 @@ EmbedPlan embed_plan(int64_t n, int64_t vocab, int64_t width, int dtype) {
 
 int check_embed(const std::string& what, int64_t n, int64_t vocab, int64_t width, int id_bytes, int dtype) {
     if (!known_dtype(dtype)) return fail(what + ": dtype must be 0 (fp32), 1 (fp16) or 2 (bf16)");
+    if (vocab < 1 || vocab >= (int64_t{1} << 31) - 1) return fail(what + ": vocab must be within 1..2^31 - 2");
     if (check_sort(what.c_str(), SortKeys{nullptr, id_bytes, n, vocab})) return -1;
     if (width < 1 || width > 1 << 20) return fail(what + ": width must be within 1..2^20");
     return 0;

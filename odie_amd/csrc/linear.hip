@@ -23,8 +23,8 @@ constexpr int kMaxExperts = 1 << 15;
 // them of at most 256 columns.
 int64_t slope_piece(int64_t rows, int outputs) {
     const int64_t across = (outputs + 255) / 256;
-    const int64_t piece = (rows * across / (8 * kCus) + 63) / 64 * 64;
-    return piece < 64 ? 64 : piece;
+    const int64_t piece = (rows * across / (8 * kCus) + 63) / 64 * 64, most = int64_t{1} << 30;
+    return piece < 64 ? 64 : (piece < most ? piece : most);
 }
 
 // Tiles of the weight gradient and the rows a workgroup sums.  Every CU is to have a workgroup (four of the
