@@ -5,6 +5,7 @@
 // wide global instructions whether or not the address is 16-byte aligned (unaligned access mode).
 #pragma once
 #include <cstdint>
+#include <type_traits>
 
 #include "common.h"
 #include "../../include/odie_amd.h"
@@ -12,6 +13,8 @@
 namespace odie {
 
 typedef uint32_t vec16 __attribute__((ext_vector_type(4)));   // 16 bytes of any element type
+
+constexpr int64_t kStreamBytes = int64_t{32} << 20;   // the L2s' 4 MB on each of 8 XCDs
 
 template <class T> constexpr int kPerVec = 16 / static_cast<int>(sizeof(T));
 
@@ -21,7 +24,14 @@ template <class T> __device__ inline vec16 load16(const T* p) {
     return v;
 }
 
-template <class T> __device__ inline void store16(T* p, const vec16& v) { __builtin_memcpy(p, &v, 16); }
+// kStream: past the caches' retention, for outputs too large for the L2s to hold until they are read
+// (kStreamBytes): 4M looked-up rows of 64 bytes 92 -> 44 us.  A constant, because the compiler makes one store of the two
+// sides of a branch.
+typedef uint32_t vec16_any __attribute__((ext_vector_type(4), aligned(2)));
+template <bool kStream = false, class T> __device__ inline void store16(T* p, const vec16& v) {
+    if constexpr (kStream) __builtin_nontemporal_store(v, reinterpret_cast<vec16_any*>(p));
+    else __builtin_memcpy(p, &v, 16);
+}
 
 // The first `count` elements at p (0 <= count), zeros after them, element by element.
 template <class T> __device__ inline vec16 gather16(const T* p, int count) {
@@ -84,9 +94,9 @@ template <class T> __device__ inline vec16 load_chunk(const T* row, int chunk, i
     return width >= kPerVec<T> ? load16(p) : gather16(p, width);
 }
 
-template <class T> __device__ inline void store_chunk(T* row, int chunk, int width, const vec16& v) {
+template <bool kStream = false, class T> __device__ inline void store_chunk(T* row, int chunk, int width, const vec16& v) {
     T* p = row + chunk_column<T>(chunk, width);
-    if (width >= kPerVec<T>) store16(p, v);
+    if (width >= kPerVec<T>) store16<kStream>(p, v);
     else scatter16(p, v, width);
 }
 
@@ -174,6 +184,12 @@ __device__ inline void wave_fence() {
 
 inline bool known_dtype(int dtype) { return dtype == ODIE_F32 || dtype == ODIE_F16 || dtype == ODIE_BF16; }
 inline int64_t dtype_bytes(int dtype) { return dtype == ODIE_F32 ? 4 : 2; }
+
+// Calls f with a constant of the flag's value.
+template <class F> void with_flag(bool flag, F&& f) {
+    if (flag) f(std::true_type{});
+    else f(std::false_type{});
+}
 
 // Calls f with a value of the element type `dtype` names (checked by the caller).
 template <class F> auto with_dtype(int dtype, F&& f) {

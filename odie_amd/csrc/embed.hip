@@ -30,7 +30,7 @@ struct LookupArgs {
     int id_bytes, width, chunks;
 };
 
-template <class T> __global__ __launch_bounds__(kEmbedBlock) void lookup_kernel(LookupArgs a) {
+template <class T, bool kStream> __global__ __launch_bounds__(kEmbedBlock) void lookup_kernel(LookupArgs a) {
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.block_rows;
     const int64_t left = a.n - row0;
     const uint32_t items = (left < a.block_rows ? static_cast<uint32_t>(left) : a.block_rows) * a.chunks;
@@ -56,7 +56,8 @@ template <class T> __global__ __launch_bounds__(kEmbedBlock) void lookup_kernel(
             widen<T>(v[u], f);
 #pragma unroll
             for (int e = 0; e < kPerVec<T>; ++e) f[e] *= a.scale;
-            store_chunk(static_cast<T*>(a.out) + (row0 + r) * a.width, static_cast<int>(item - r * a.chunks), a.width, narrow<T>(f));
+            store_chunk<kStream>(static_cast<T*>(a.out) + (row0 + r) * a.width, static_cast<int>(item - r * a.chunks), a.width,
+                                 narrow<T>(f));
         }
     }
 }
@@ -310,7 +311,11 @@ ODIE_API int odie_embed_forward(const void* table, int64_t table_stride, int64_t
     a.by_chunks = make_divisor(static_cast<uint32_t>(a.chunks));
     a.block_rows = a.chunks >= 1024 ? 1u : static_cast<uint32_t>(1024 / a.chunks);
     const uint32_t blocks = static_cast<uint32_t>((n + a.block_rows - 1) / a.block_rows);
-    with_dtype(dtype, [&](auto t) { lookup_kernel<decltype(t)><<<blocks, kEmbedBlock, 0, as_stream(stream)>>>(a); });
+    with_dtype(dtype, [&](auto t) {
+        with_flag(n * width * dtype_bytes(dtype) >= kStreamBytes, [&](auto far) {
+            lookup_kernel<decltype(t), far><<<blocks, kEmbedBlock, 0, as_stream(stream)>>>(a);
+        });
+    });
     return check_launch("embed");
 }
 

@@ -65,7 +65,7 @@ __device__ inline int64_t lane_row(const MoveArgs& a) {
 }
 
 // kChoices entries of a row are handled together (0: any number of choices, in twos).
-template <class T, int kChoices> __global__ __launch_bounds__(kMoveBlock) void dispatch_kernel(MoveArgs a) {
+template <class T, int kChoices, bool kStream> __global__ __launch_bounds__(kMoveBlock) void dispatch_kernel(MoveArgs a) {
     constexpr int kStep = kChoices ? kChoices : 2;
     const int choices = kChoices ? kChoices : a.choices;
     const int lane = static_cast<int>(threadIdx.x) % a.lanes;
@@ -79,13 +79,13 @@ template <class T, int kChoices> __global__ __launch_bounds__(kMoveBlock) void d
                 const vec16 v = load_chunk(static_cast<const T*>(a.x) + i * a.ldx, c, a.width);
 #pragma unroll
                 for (int j = 0; j < kStep; ++j)
-                    if (slot[j] >= 0) store_chunk(static_cast<T*>(a.out) + slot[j] * a.width, c, a.width, v);
+                    if (slot[j] >= 0) store_chunk<kStream>(static_cast<T*>(a.out) + slot[j] * a.width, c, a.width, v);
             }
         }
     clear_rest<T>(a);
 }
 
-template <class T, int kChoices> __global__ __launch_bounds__(kMoveBlock) void combine_kernel(MoveArgs a) {
+template <class T, int kChoices, bool kStream> __global__ __launch_bounds__(kMoveBlock) void combine_kernel(MoveArgs a) {
     constexpr int kStep = kChoices ? kChoices : 2;
     const int choices = kChoices ? kChoices : a.choices;
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.block_rows;
@@ -113,11 +113,11 @@ template <class T, int kChoices> __global__ __launch_bounds__(kMoveBlock) void c
                 for (int e = 0; e < kPerVec<T>; ++e) sum[e] += w[j] * f[e];
             }
         }
-        store_chunk(static_cast<T*>(a.out) + i * a.width, chunk, a.width, narrow<T>(sum));
+        store_chunk<kStream>(static_cast<T*>(a.out) + i * a.width, chunk, a.width, narrow<T>(sum));
     }
 }
 
-template <class T, int kChoices> __global__ __launch_bounds__(kMoveBlock) void combine_backward_kernel(MoveArgs a) {
+template <class T, int kChoices, bool kStream> __global__ __launch_bounds__(kMoveBlock) void combine_backward_kernel(MoveArgs a) {
     constexpr int kStep = kChoices ? kChoices : 2;
     const int choices = kChoices ? kChoices : a.choices;
     const int lane = static_cast<int>(threadIdx.x) % a.lanes;
@@ -152,7 +152,7 @@ template <class T, int kChoices> __global__ __launch_bounds__(kMoveBlock) void c
                         g[e] = d[e] * w[j];
                     }
                     if (a.out && slot[j] >= 0)
-                        store_chunk(static_cast<T*>(a.out) + slot[j] * a.width, c, a.width, narrow<T>(g));
+                        store_chunk<kStream>(static_cast<T*>(a.out) + slot[j] * a.width, c, a.width, narrow<T>(g));
                 }
             }
             if (a.dweights) {
@@ -168,12 +168,20 @@ template <class T, int kChoices> __global__ __launch_bounds__(kMoveBlock) void c
     if (a.out) clear_rest<T>(a);
 }
 
-// f with the number of choices as a constant where it is 1, 2 or 4, else 0.
-template <class F> void with_choices(int choices, F&& f) {
-    if (choices == 1) f(std::integral_constant<int, 1>{});
-    else if (choices == 2) f(std::integral_constant<int, 2>{});
-    else if (choices == 4) f(std::integral_constant<int, 4>{});
-    else f(std::integral_constant<int, 0>{});
+// f with the number of choices as a constant where it is 1, 2 or 4, else 0, and whether to stream.
+template <class F> void with_choices(int choices, bool stream, F&& f) {
+    with_flag(stream, [&](auto far) {
+        if (choices == 1) f(std::integral_constant<int, 1>{}, far);
+        else if (choices == 2) f(std::integral_constant<int, 2>{}, far);
+        else if (choices == 4) f(std::integral_constant<int, 4>{}, far);
+        else f(std::integral_constant<int, 0>{}, far);
+    });
+}
+
+// Whether rows scattered over the sorted ones are streamed: those that share lines have to meet in the L2 (131 bf16
+// columns: 102 us through it, 144 past it; 256 columns 145 and 117).
+bool stream_scattered(const MoveArgs& a, int dtype) {
+    return !a.by_xcd && a.n * a.choices * a.width * dtype_bytes(dtype) >= kStreamBytes;
 }
 
 // Lanes for a row of `chunks` 16-byte pieces: a whole row at once where 64 lanes can.
@@ -235,8 +243,8 @@ ODIE_API int odie_rows_dispatch(const void* x, int64_t x_stride, const int32_t* 
     a.offsets = offsets;
     a.out = out;
     with_dtype(dtype, [&](auto t) {
-        with_choices(choices, [&](auto k) {
-            dispatch_kernel<decltype(t), k><<<row_blocks(a), kMoveBlock, 0, as_stream(stream)>>>(a);
+        with_choices(choices, stream_scattered(a, dtype), [&](auto k, auto far) {
+            dispatch_kernel<decltype(t), k, far><<<row_blocks(a), kMoveBlock, 0, as_stream(stream)>>>(a);
         });
     });
     return check_launch("rows dispatch");
@@ -256,8 +264,8 @@ ODIE_API int odie_rows_combine(const void* rows, int64_t rows_stride, const int3
     a.weights = weights;
     a.out = out;
     with_dtype(dtype, [&](auto t) {
-        with_choices(choices, [&](auto k) {
-            combine_kernel<decltype(t), k><<<move_blocks(a), kMoveBlock, 0, as_stream(stream)>>>(a);
+        with_choices(choices, n * width * dtype_bytes(dtype) >= kStreamBytes, [&](auto k, auto far) {
+            combine_kernel<decltype(t), k, far><<<move_blocks(a), kMoveBlock, 0, as_stream(stream)>>>(a);
         });
     });
     return check_launch("rows combine");
@@ -284,8 +292,8 @@ ODIE_API int odie_rows_combine_backward(const void* upstream, int64_t upstream_s
     a.out = drows;
     a.dweights = dweights;
     with_dtype(dtype, [&](auto t) {
-        with_choices(choices, [&](auto k) {
-            combine_backward_kernel<decltype(t), k>
+        with_choices(choices, drows && stream_scattered(a, dtype), [&](auto k, auto far) {
+            combine_backward_kernel<decltype(t), k, far>
                 <<<row_blocks(a), kMoveBlock, 0, as_stream(stream)>>>(a);
         });
     });

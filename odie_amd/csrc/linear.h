@@ -123,8 +123,24 @@ template <class T, bool kByRow, int kRows, int kThreads> struct Image {
 };
 
 constexpr uint32_t kNowhere = 0x80000000u;          // past every buffer: such a lane's bytes arrive as 0
-constexpr int kBufferLimit = 0x7fffffff;
-constexpr int kBufferWord3 = 0x00027000;
+constexpr uint32_t kBufferLimit = 0x7fffffff;
+constexpr uint32_t kBufferWord3 = 0x00027000;
+
+// Queues 16 bytes a lane from buffer + offset to LDS address `to` + 16 * lane (`to` and buffer uniform over the
+// wave).  Written out, with no register result, because of the builtin's transposing LDS reads the compiler waits for
+// every such load in flight, the next slab's too.  So it knows of none of them: arrived() has to come before the
+// bytes are read.
+__device__ inline void queue16(uint32_t to, uint32_t offset, const vec16& buffer) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer)
+                 : "memory", "m0");
+}
+
+// Waits until this wave's queued loads but the last kPending have arrived and its LDS reads are done, then for the
+// other waves of the workgroup.
+template <int kPending> __device__ inline void arrived() {
+    static_assert(kPending < 64, "the wait's count has 6 bits");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kPending) : "memory");
+}
 
 // Global to LDS without registers, 16 bytes a lane, for rows that start on 16 bytes and hold whole
 // chunks.  Offsets of a tile's chunks from its first row stay below 2^31 (checked on the host).
@@ -162,18 +178,21 @@ template <class T, bool kByRow, int kRows, int kThreads> struct Direct : Image<T
 
     // Queues the next slab into lds; `left` values of k exist, the rest arrive as 0.
     __device__ void load(int64_t left, char* lds) {
-        const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, kBufferLimit, kBufferWord3);
-        char* to = lds + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64) * 1024;
+        const uint64_t address = reinterpret_cast<uint64_t>(base);
+        vec16 buffer{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address))),
+                           static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32))),
+                           kBufferLimit, kBufferWord3};
+        asm volatile("s_nop 4" : "+s"(buffer));   // wait states between its writing and the loads
+        const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void)(lds))) +
+                            __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64) * 1024;
         if (left >= kSlab<T>) {
 #pragma unroll
-            for (int i = 0; i < I::kChunks; ++i)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (lds_void)(to + i * kThreads * 16), 16, offset[i], 0, 0, 0);
+            for (int i = 0; i < I::kChunks; ++i) queue16(to + i * kThreads * 16, offset[i], buffer);
         } else {
 #pragma unroll
             for (int i = 0; i < I::kChunks; ++i) {
                 const bool inside = (kByRow ? lead : lead + i * I::kStep) < left;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (lds_void)(to + i * kThreads * 16), 16,
-                                                         inside ? offset[i] : kNowhere, 0, 0, 0);
+                queue16(to + i * kThreads * 16, inside ? offset[i] : kNowhere, buffer);
             }
         }
         base += slab;
@@ -318,6 +337,7 @@ struct Tile {
             for (int j = 0; j < kNs; ++j) acc[i][j] = accum16{};
     }
 
+    // (Reading a step's fragments while the step before is multiplied gains nothing: two waves a SIMD do that already.)
     __device__ void add_slab(const char* here) {
         const int lane = static_cast<int>(threadIdx.x % 64);
         const int wm = wave_row(), wn = wave_column();
@@ -344,7 +364,6 @@ struct Tile {
             // reads of the one before; past the barrier all of it is there, and the buffer read last is
             // free.  Slabs past the end are queued as well, as zeros, so that the count of loads is constant.
             constexpr int kAhead = kStages - 1, kPending = (kAhead - 1) * (A::kChunks + B::kChunks);
-            static_assert(kPending < 64, "the wait's count has 6 bits");
             int64_t left = depth;   // of the next slab to queue
 #pragma unroll
             for (int s = 0; s < kAhead; ++s, left -= kSlab<T>) {
@@ -353,19 +372,20 @@ struct Tile {
             }
             int now = 0;
             for (int64_t done = 0; done < depth; done += kSlab<T>, left -= kSlab<T>) {
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kPending) : "memory");
+                arrived<kPending>();
                 const int then = now == 0 ? kStages - 1 : now - 1;
                 a.load(left, lds + then * kBuffer);
                 b.load(left, lds + then * kBuffer + A::kBytes);
                 add_slab(lds + now * kBuffer);
                 now = now + 1 == kStages ? 0 : now + 1;
             }
+            arrived<0>();   // the zeros too, before the LDS is used otherwise
         } else if constexpr (kWay == kDirect) {
             a.load(depth, lds);
             b.load(depth, lds + A::kBytes);
             int now = 0;
             for (int64_t left = depth; left > 0; left -= kSlab<T>) {
-                __syncthreads();   // this slab has arrived, and no wave reads the other buffer any more
+                arrived<0>();   // this slab; and no wave reads the other buffer any more
                 char* const next = lds + (now ^ 1) * kBuffer;
                 if (left > kSlab<T>) {
                     a.load(left - kSlab<T>, next);

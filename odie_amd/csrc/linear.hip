@@ -55,8 +55,9 @@ WeightPlan weight_plan(int64_t rows, int experts, int outputs, int inputs, int d
         const int64_t tiles = tiles_of(edge);
         int64_t pieces = 256 / edge * kCus / tiles;
         if (pieces > most) pieces = most;
+        if (pieces < 1) pieces = 1;
         if (edge > 64 && tiles * pieces < kCus) continue;
-        return WeightPlan{edge, whole(pieces > 1 ? (rows + pieces - 1) / pieces : rows)};
+        return WeightPlan{edge, whole((rows + pieces - 1) / pieces)};
     }
 }
 
