@@ -71,8 +71,8 @@ template <class T> __device__ inline vec16 load_some(const T* p, int count) {
     return count >= kPerVec<T> ? load16(p) : gather16(p, count);
 }
 
-template <class T> __device__ inline void store_some(T* p, const vec16& v, int count) {
-    if (count >= kPerVec<T>) store16(p, v);
+template <bool kStream = false, class T> __device__ inline void store_some(T* p, const vec16& v, int count) {
+    if (count >= kPerVec<T>) store16<kStream>(p, v);
     else scatter16(p, v, count);
 }
 
@@ -169,10 +169,10 @@ template <class T> __device__ inline void load8(const T* p, int count, float out
     e.get(out);
 }
 
-template <class T> __device__ inline void store8(T* p, int count, const float in[8]) {
+template <bool kStream = false, class T> __device__ inline void store8(T* p, int count, const float in[8]) {
 #pragma unroll
     for (int w = 0; w < 8 / kPerVec<T>; ++w)
-        store_some(p + w * kPerVec<T>, narrow<T>(in + w * kPerVec<T>), count - w * kPerVec<T>);
+        store_some<kStream>(p + w * kPerVec<T>, narrow<T>(in + w * kPerVec<T>), count - w * kPerVec<T>);
 }
 
 // A wave orders its own LDS accesses: lanes read what other lanes of the wave wrote.

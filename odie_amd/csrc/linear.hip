@@ -27,8 +27,8 @@ int64_t slope_piece(int64_t rows, int outputs) {
     return piece < 64 ? 64 : (piece < most ? piece : most);
 }
 
-// Tiles of the weight gradient and the rows a workgroup sums.  Every CU is to have a workgroup (four of the
-// smallest tiles, two of the middle ones), from several pieces of the rows where there are too few tiles;
+// Tiles of the weight gradient and the rows a workgroup sums.  Three CUs of four at least are to have a workgroup (four
+// of the smallest tiles, two of the middle ones), from several pieces of the rows where there are too few tiles;
 // but partial sums, written and read again, are to stay below twice what the operands hold.  The
 // largest tiles that manage it are taken (a 1024 x 1024 gradient over 4096 bf16 rows: 61 us as 16 tiles of
 // 256 x 256 and 16 pieces, 29 us as 64 of 128 x 128 and 4 pieces).
@@ -56,7 +56,7 @@ WeightPlan weight_plan(int64_t rows, int experts, int outputs, int inputs, int d
         int64_t pieces = 256 / edge * kCus / tiles;
         if (pieces > most) pieces = most;
         if (pieces < 1) pieces = 1;
-        if (edge > 64 && tiles * pieces < kCus) continue;
+        if (edge > 64 && 4 * tiles * pieces < 3 * kCus) continue;
         return WeightPlan{edge, whole((rows + pieces - 1) / pieces)};
     }
 }

@@ -53,6 +53,7 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(Ro
     const T* bias = a.bias ? static_cast<const T*>(a.bias) + static_cast<int64_t>(p.group) * a.columns : nullptr;
     T* pre = static_cast<T*>(a.pre);
     constexpr int kGroup = Work::kGroup, kHeight = Work::kHeight;
+    constexpr bool kStream = kBM == 256;   // taken for outputs near the L2s' size and larger alone (17 MB at least)
     struct Fetched {
         Eight<T> row[kGroup];
     };
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(Ro
 #pragma unroll
                 for (int u = 0; u < kGroup; ++u) {
                     const int64_t row = p.begin + r + u * kHeight;
-                    if (row < p.end) store8(pre + row * a.columns + column, count, value[u]);
+                    if (row < p.end) store8<kStream>(pre + row * a.columns + column, count, value[u]);
                 }
             with_activation(a.activation, [&](auto activation) {
 #pragma unroll
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(Ro
 #pragma unroll
                     for (int i = 0; i < 8; ++i) value[u][i] += more[i];
                 }
-                store8(out + row * a.ldo + column, count, value[u]);
+                store8<kStream>(out + row * a.ldo + column, count, value[u]);
             }
         });
 }
@@ -229,7 +230,7 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void weight_kernel(
 constexpr int kSlopeBlock = 256;
 
 // A workgroup takes one piece of rows and `lanes` groups of 8 columns; 256 / lanes rows at a time.
-template <class T> __global__ __launch_bounds__(kSlopeBlock) void slope_kernel(SlopeArgs a, int lanes, uint32_t across) {
+template <class T, bool kStream> __global__ __launch_bounds__(kSlopeBlock) void slope_kernel(SlopeArgs a, int lanes, uint32_t across) {
     __shared__ float total[kSlopeBlock * 8];
     const Piece p = find_piece(a.offsets, a.experts, a.experts, a.rows, a.piece, blockIdx.x / across);
     if (p.begin >= p.end) return;
@@ -258,7 +259,7 @@ template <class T> __global__ __launch_bounds__(kSlopeBlock) void slope_kernel(S
                     if (activation != kNone) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) d[u][i] *= slope<activation, sizeof(T) == 4>(z[u][i]);
-                        store8(dz + r * a.columns + column, count, d[u]);
+                        store8<kStream>(dz + r * a.columns + column, count, d[u]);
                     }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) sum[i] += d[u][i];
@@ -428,7 +429,9 @@ template <class T> int launch_slope(const SlopeArgs& a, hipStream_t stream) {
     const int64_t across = (groups + lanes - 1) / lanes, blocks = a.pieces * across;
     if (blocks >= int64_t{1} << 31) return fail("linear: too many workgroups for one launch");
     if (blocks == 0) return 0;
-    slope_kernel<T><<<static_cast<uint32_t>(blocks), kSlopeBlock, 0, stream>>>(a, lanes, static_cast<uint32_t>(across));
+    with_flag(a.rows * a.columns * static_cast<int64_t>(sizeof(T)) >= kStreamBytes, [&](auto far) {
+        slope_kernel<T, far><<<static_cast<uint32_t>(blocks), kSlopeBlock, 0, stream>>>(a, lanes, static_cast<uint32_t>(across));
+    });
     return check_launch("linear activation gradient");
 }
 

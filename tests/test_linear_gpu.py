@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 # one value; odd sizes below and above every tile edge; an empty batch; wide and narrow tiles in earnest
 SHAPES = [(1, 1, 1), (2, 32, 64), (3, 33, 65), (63, 64, 63), (64, 128, 64), (65, 130, 129), (200, 257, 100),
           (129, 8, 300), (16, 1000, 24), (7, 2049, 130), (1000, 520, 264)]
-LARGE = [(32773, 24, 40), (4099, 40, 1000), (2500, 136, 2056)]
+LARGE = [(32773, 24, 40), (4099, 40, 1000), (2500, 136, 2056), (65436, 264, 520), (65436, 265, 517)]
 
 
 def _normal(generator, dtype, *shape, scale=1.0):
