@@ -9,6 +9,9 @@
 // The gradient of dispatch is combine without weights.  Each of them reads and writes every row once and
 // is bound by HBM, so the walk is over input rows: x and dy are read once however many choices there are,
 // and the scattered side moves whole rows.  Sums are fp32 in the order of the choices, rounded once.
+// 65536 rows x 2 choices of 256 fp16: dispatch and combine 17 us each (5.8 TB/s, the caches helping), gradients 29.
+// 300007 x 4 of 131 bf16, which share lines: 104, 99 and 198 us (3.6 to 4.0 TB/s).  (By slot instead of by row:
+// dispatch 114 -> 116 and the gradients 302 -> 339 at the time.)
 #include <type_traits>
 
 #include "elements.h"
