@@ -165,17 +165,42 @@ struct PassArgs {
     bool last, only;          // only: the sole pass, digits are buckets
 };
 
-__device__ inline uint32_t pass_key(const PassArgs& a, int64_t i) {
-    return a.raw ? read_key(a.raw, a.raw_bytes, i, a.buckets) : a.pairs[i].y;
+constexpr int kHeld = 8;   // keys a lane loads together: 4M in two passes 118 -> 91 us against one at a time
+
+// (input position, key) of places i, i + 64, ... below end, which is past i's wave; places from end on repeat the last.
+__device__ inline void load_pairs(const PassArgs& a, int64_t i, int64_t end, uint2 pair[kHeld]) {
+    auto at = [&](int u) { return i + u * 64 < end ? i + u * 64 : end - 1; };
+    if (!a.raw) {
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) pair[u] = a.pairs[at(u)];
+    } else if (a.raw_bytes == 8) {
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) pair[u] = make_uint2(static_cast<uint32_t>(at(u)), read_key(a.raw, 8, at(u), a.buckets));
+    } else {
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) pair[u] = make_uint2(static_cast<uint32_t>(at(u)), read_key(a.raw, 4, at(u), a.buckets));
+    }
+}
+
+// Counts the digits of the wave's places begin..end - 1 in LDS.
+__device__ inline void count_digits(const PassArgs& a, int64_t begin, int64_t end, int lane, uint32_t* count) {
+    const uint32_t mask = (1u << a.bits) - 1;
+    for (int64_t base = begin; base < end; base += 64 * kHeld) {
+        uint2 pair[kHeld];
+        load_pairs(a, base + lane, end, pair);
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u)
+            if (base + u * 64 + lane < end) atomicAdd(&count[pair[u].y >> a.shift & mask], 1u);
+    }
 }
 
 __global__ __launch_bounds__(kSortBlock) void count_kernel(PassArgs a) {
     __shared__ uint32_t count[kDigits];
     for (int d = threadIdx.x; d < a.digits; d += kSortBlock) count[d] = 0;
     __syncthreads();
-    const uint32_t mask = (1u << a.bits) - 1;
-    const int64_t begin = blockIdx.x * a.part, end = begin + a.part < a.n ? begin + a.part : a.n;
-    for (int64_t i = begin + threadIdx.x; i < end; i += kSortBlock) atomicAdd(&count[pass_key(a, i) >> a.shift & mask], 1u);
+    const int64_t share = a.part / kSortWaves, begin = blockIdx.x * a.part + threadIdx.x / 64 * share;
+    const int64_t end = begin + share < a.n ? begin + share : a.n;
+    count_digits(a, begin, end, static_cast<int>(threadIdx.x % 64), count);
     __syncthreads();
     for (int d = threadIdx.x; d < a.digits; d += kSortBlock) a.table[static_cast<int64_t>(d) * a.parts + blockIdx.x] = count[d];
 }
@@ -211,7 +236,7 @@ __global__ __launch_bounds__(kSortBlock) void scatter_kernel(PassArgs a) {
     const uint32_t mask = (1u << a.bits) - 1;
     const int64_t share = a.part / kSortWaves;
     const int64_t begin = blockIdx.x * a.part + wave * share, end = begin + share < a.n ? begin + share : a.n;
-    for (int64_t i = begin + lane; i < end; i += 64) atomicAdd(&own_next[pass_key(a, i) >> a.shift & mask], 1u);
+    count_digits(a, begin, end, lane, own_next);
     __syncthreads();
     for (int d = threadIdx.x; d < a.digits; d += kSortBlock) {
         uint32_t place = start[d] + a.table[static_cast<int64_t>(d) * a.parts + blockIdx.x];
@@ -225,32 +250,32 @@ __global__ __launch_bounds__(kSortBlock) void scatter_kernel(PassArgs a) {
     if (a.only && a.out.offsets && blockIdx.x == 0)
         for (int d = threadIdx.x; d < a.digits; d += kSortBlock) a.out.offsets[d] = static_cast<int32_t>(start[d]);
     __syncthreads();
-    for (int64_t base = begin; base < end; base += 64) {
-        const int64_t i = base + lane;
-        const bool valid = i < end;
-        uint2 pair = make_uint2(static_cast<uint32_t>(i), 0u);
-        if (valid) {
-            if (a.raw) pair.y = pass_key(a, i);
-            else pair = a.pairs[i];
+    for (int64_t base = begin; base < end; base += 64 * kHeld) {
+        uint2 pair[kHeld];
+        load_pairs(a, base + lane, end, pair);
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) {
+            if (base + u * 64 >= end) break;
+            const bool valid = base + u * 64 + lane < end;
+            const uint32_t k = pair[u].y, f = pair[u].x;
+            const uint32_t digit = k >> a.shift & mask;
+            const uint64_t same = same_digit(digit, a.bits, __ballot(valid));
+            const uint32_t place = valid ? own_next[digit] : 0u;
+            const int rank = lanes_below(same, lane);
+            wave_fence();
+            if (valid && rank == 0) own_next[digit] = place + __popcll(same);
+            wave_fence();
+            if (!valid) continue;
+            const uint32_t to = place + rank;
+            if (!a.last) {
+                a.pairs_out[to] = pair[u];
+                continue;
+            }
+            if (a.out.order) a.out.order[to] = static_cast<int32_t>(f);
+            if (a.out.pairs) a.out.pairs[to] = make_int2(static_cast<int>(f), static_cast<int>(k));
+            if (a.out.sorted) a.out.sorted[to] = static_cast<int32_t>(k);
+            if (a.out.slots) a.out.slots[f] = k < a.buckets ? static_cast<int32_t>(to) : -1;
         }
-        const uint32_t k = pair.y, f = pair.x;
-        const uint32_t digit = k >> a.shift & mask;
-        const uint64_t same = same_digit(digit, a.bits, __ballot(valid));
-        const uint32_t place = valid ? own_next[digit] : 0u;
-        const int rank = lanes_below(same, lane);
-        wave_fence();
-        if (valid && rank == 0) own_next[digit] = place + __popcll(same);
-        wave_fence();
-        if (!valid) continue;
-        const uint32_t to = place + rank;
-        if (!a.last) {
-            a.pairs_out[to] = pair;
-            continue;
-        }
-        if (a.out.order) a.out.order[to] = static_cast<int32_t>(f);
-        if (a.out.pairs) a.out.pairs[to] = make_int2(static_cast<int>(f), static_cast<int>(k));
-        if (a.out.sorted) a.out.sorted[to] = static_cast<int32_t>(k);
-        if (a.out.slots) a.out.slots[f] = k < a.buckets ? static_cast<int32_t>(to) : -1;
     }
 }
 
