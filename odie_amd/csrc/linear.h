@@ -586,6 +586,13 @@ struct SlopeArgs {            // dz = dy act'(pre), and the column sums of dz
     int experts, columns, activation;
 };
 
+// Lanes across the columns, 8 each, of the slope pass' workgroups.
+inline int slope_lanes(int columns) {
+    int lanes = 1;
+    while (lanes < 32 && 8 * lanes < columns) lanes *= 2;
+    return lanes;
+}
+
 struct FoldArgs {             // out[e][i] = sum over e's pieces of partial[piece][i]
     const float* partial;
     void* out;

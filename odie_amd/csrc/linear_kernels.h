@@ -434,9 +434,7 @@ template <class T> int launch_weight(const WeightArgs& a, hipStream_t stream) {
 }
 
 template <class T> int launch_slope(const SlopeArgs& a, hipStream_t stream) {
-    const int groups = (a.columns + 7) / 8;
-    int lanes = 1;
-    while (lanes < 32 && lanes < groups) lanes *= 2;
+    const int groups = (a.columns + 7) / 8, lanes = slope_lanes(a.columns);
     const int64_t across = (groups + lanes - 1) / lanes, blocks = a.pieces * across;
     if (blocks >= int64_t{1} << 31) return fail("linear: too many workgroups for one launch");
     if (blocks == 0) return 0;
