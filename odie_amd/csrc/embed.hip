@@ -10,7 +10,7 @@
 //          written at once, one that crosses into the next leaves a partial sum (`tail` in the run
 //          where it begins, `head` in every later run it reaches)
 //   join   for every run whose last row goes on, adds the later runs' heads to its tail
-// 4M ids of 16384 rows, 32 bf16 columns: lookup 88 us (3.4 TB/s), gradient 250: the sort 120 (scattered stores of 8
+// 4M ids of 16384 rows, 32 bf16 columns: lookup 88 us (3.4 TB/s), gradient 223: the sort 91 (scattered stores of 8
 // bytes), runs 95 (rows of 64 bytes in the ids' order, 2.8 TB/s), join 35 (one row a run or less: its latency).
 // 300007 ids on few of 65032 rows, 97 fp32 columns: 28, and sort 33, runs 38, join 21 (the longest row's chain).
 #include "elements.h"
