@@ -22,8 +22,8 @@ __device__ inline TileAt tile_at(uint32_t id, uint32_t down, uint32_t across) {
 // One tile of act(a b^T + bias) + residual (forward) or of a b (the input's gradient).  65536 rows, 1024 -> 4096,
 // bf16: 550 GFLOP; the bare product 540 to 615 us (900 to 1020 TFLOP/s), bound by the feeding of the matrix
 // instructions.  With bias, gelu, the sums kept and a residual 800 to 980 us (the least over and over, the most in a
-// training step): 1.75 GB more, which come in bursts as
-// the workgroups, one a CU, reach their ends together (about 120 us), and the gelu's arithmetic (about 80).
+// training step): 1.1 GB more, which come in bursts as the workgroups, one a CU, reach their ends together (120 us
+// at least), and the gelu's arithmetic (about 80).
 template <class T, bool kForward, Way kWay, int kBM, int kBN, int kWM, int kWN, int kStages>
 __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(RowsArgs a, uint32_t blocks) {
     using Work = Tile<T, true, kForward, kWay, kBM, kBN, kWM, kWN, kStages>;
