@@ -182,6 +182,17 @@ __device__ inline void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// Workgroups of `threads` threads that one launch takes, in whole rounds of the XCDs.  Past 2^32 threads the runtime
+// launches fewer workgroups than it was asked for, without an error.
+inline int64_t most_blocks(int threads) { return ((int64_t{1} << 32) - 1) / threads / kXcds * kXcds; }
+
+// Calls f(first, count) for as many launches as `blocks` workgroups need: one, up to billions of rows.
+template <class F> void in_launches(int64_t blocks, int threads, F&& f) {
+    const int64_t most = most_blocks(threads);
+    for (int64_t first = 0; first < blocks; first += most)
+        f(static_cast<uint32_t>(first), static_cast<uint32_t>(blocks - first < most ? blocks - first : most));
+}
+
 inline bool known_dtype(int dtype) { return dtype == ODIE_F32 || dtype == ODIE_F16 || dtype == ODIE_BF16; }
 inline int64_t dtype_bytes(int dtype) { return dtype == ODIE_F32 ? 4 : 2; }
 

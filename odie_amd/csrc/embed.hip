@@ -313,10 +313,11 @@ ODIE_API int odie_embed_forward(const void* table, int64_t table_stride, int64_t
     a.chunks = chunks_of(width, dtype);
     a.by_chunks = make_divisor(static_cast<uint32_t>(a.chunks));
     a.block_rows = a.chunks >= 1024 ? 1u : static_cast<uint32_t>(1024 / a.chunks);
-    const uint32_t blocks = static_cast<uint32_t>((n + a.block_rows - 1) / a.block_rows);
+    const int64_t blocks = (n + a.block_rows - 1) / a.block_rows;
+    if (blocks > most_blocks(kEmbedBlock)) return fail(what + ": too many rows for one launch");
     with_dtype(dtype, [&](auto t) {
         with_flag(n * width * dtype_bytes(dtype) >= kStreamBytes, [&](auto far) {
-            lookup_kernel<decltype(t), far><<<blocks, kEmbedBlock, 0, as_stream(stream)>>>(a);
+            lookup_kernel<decltype(t), far><<<static_cast<uint32_t>(blocks), kEmbedBlock, 0, as_stream(stream)>>>(a);
         });
     });
     return check_launch("embed");
@@ -339,6 +340,11 @@ ODIE_API int odie_embed_backward(const void* upstream, int64_t upstream_stride, 
     const int64_t need = p.sorted + 2 * p.heads + p.sort;
     if (n > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0))
         return fail(what + ": needs a 256-byte aligned workspace of " + std::to_string(need) + " bytes");
+    const int lanes = run_lanes(p.chunks), across = (p.chunks + lanes - 1) / lanes;
+    const int64_t walks = (p.runs * across * lanes + kEmbedBlock - 1) / kEmbedBlock;
+    const int64_t joins = (p.runs + kEmbedBlock / lanes - 1) / (kEmbedBlock / lanes) * across;
+    if (walks > most_blocks(kEmbedBlock) || joins > most_blocks(kEmbedBlock))
+        return fail(what + ": too many runs for one launch");
     hipStream_t s = as_stream(stream);
     const int64_t bytes = vocab * width * dtype_bytes(dtype);
     const int64_t fill = (bytes + kEmbedBlock * 16 - 1) / (kEmbedBlock * 16);
@@ -364,13 +370,11 @@ ODIE_API int odie_embed_backward(const void* upstream, int64_t upstream_stride, 
     a.scale = scale;
     a.width = static_cast<int>(width);
     a.chunks = p.chunks;
-    a.lanes = run_lanes(p.chunks);
-    a.blocks = (p.chunks + a.lanes - 1) / a.lanes;
-    const int64_t threads = p.runs * a.blocks * a.lanes, joins = (p.runs + kEmbedBlock / a.lanes - 1) / (kEmbedBlock / a.lanes) * a.blocks;
-    if (threads / kEmbedBlock >= int64_t{1} << 31) return fail(what + ": too many runs for one launch");
+    a.lanes = lanes;
+    a.blocks = across;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        runs_kernel<T><<<static_cast<uint32_t>((threads + kEmbedBlock - 1) / kEmbedBlock), kEmbedBlock, 0, s>>>(a);
+        runs_kernel<T><<<static_cast<uint32_t>(walks), kEmbedBlock, 0, s>>>(a);
         if (p.runs > 1)
             join_kernel<T><<<static_cast<uint32_t>(joins), kEmbedBlock, 0, s>>>(a);
     });

@@ -34,12 +34,14 @@ struct MoveArgs {
     Divisor by_chunks;
     uint32_t block_rows;      // input rows a workgroup takes
     int choices, experts, width, chunks;
-    int lanes;                // dispatch and the gradient of combine: lanes a row
+    int lanes;                // dispatch and the gradient of combine: lanes a row,
+    uint32_t first;           // and the first workgroup of this launch
     bool by_xcd;
 };
 
-// Zeros in the slots that no expert owns, shared out over the workgroups.
+// Zeros in the slots that no expert owns, shared out over the workgroups of the first launch.
 template <class T> __device__ inline void clear_rest(const MoveArgs& a) {
+    if (a.first > 0) return;
     const int64_t entries = a.n * a.choices;
     const int64_t held = group_start(a.offsets, a.experts, entries), rest = entries - held;
     if (rest == 0) return;
@@ -63,7 +65,7 @@ template <int kChoices> __device__ inline int64_t slot_of(const MoveArgs& a, int
 // send to an expert lie side by side, and the lines that two of them share meet in that XCD's L2 (300007 x 4
 // rows of 272 bytes sent: 124 -> 92 us).  Whole blocks go faster spread over the XCDs (256 bytes: 81 -> 74 us).
 __device__ inline int64_t lane_row(const MoveArgs& a) {
-    const uint32_t block = a.by_xcd ? xcd_major(blockIdx.x, gridDim.x) : blockIdx.x;
+    const uint32_t block = a.first + (a.by_xcd ? xcd_major(blockIdx.x, gridDim.x) : blockIdx.x);
     return static_cast<int64_t>(block) * (kMoveBlock / a.lanes) + static_cast<int>(threadIdx.x) / a.lanes;
 }
 
@@ -219,12 +221,12 @@ MoveArgs move_args(int64_t n, int choices, int experts, int64_t width, int dtype
     return a;
 }
 
-uint32_t row_blocks(const MoveArgs& a) {
+int64_t row_blocks(const MoveArgs& a) {
     const int64_t height = kMoveBlock / a.lanes, blocks = (a.n + height - 1) / height;
-    return static_cast<uint32_t>((blocks + kXcds - 1) / kXcds * kXcds);
+    return (blocks + kXcds - 1) / kXcds * kXcds;
 }
 
-uint32_t move_blocks(const MoveArgs& a) { return static_cast<uint32_t>((a.n + a.block_rows - 1) / a.block_rows); }
+int64_t move_blocks(const MoveArgs& a) { return (a.n + a.block_rows - 1) / a.block_rows; }
 
 }  // namespace
 }  // namespace odie
@@ -247,7 +249,10 @@ ODIE_API int odie_rows_dispatch(const void* x, int64_t x_stride, const int32_t* 
     a.out = out;
     with_dtype(dtype, [&](auto t) {
         with_choices(choices, stream_scattered(a, dtype), [&](auto k, auto far) {
-            dispatch_kernel<decltype(t), k, far><<<row_blocks(a), kMoveBlock, 0, as_stream(stream)>>>(a);
+            in_launches(row_blocks(a), kMoveBlock, [&](uint32_t first, uint32_t count) {
+                a.first = first;
+                dispatch_kernel<decltype(t), k, far><<<count, kMoveBlock, 0, as_stream(stream)>>>(a);
+            });
         });
     });
     return check_launch("rows dispatch");
@@ -261,6 +266,8 @@ ODIE_API int odie_rows_combine(const void* rows, int64_t rows_stride, const int3
     if (!rows || !slots || !out) return fail(what + ": null pointer");
     if (rows_stride < width) return fail(what + ": rows overlap (a stride below the row's width)");
     MoveArgs a = move_args(n, choices, 1, width, dtype);
+    const int64_t blocks = move_blocks(a);
+    if (blocks > most_blocks(kMoveBlock)) return fail(what + ": too many rows for one launch");
     a.x = rows;
     a.ldx = rows_stride;
     a.slots = slots;
@@ -268,7 +275,7 @@ ODIE_API int odie_rows_combine(const void* rows, int64_t rows_stride, const int3
     a.out = out;
     with_dtype(dtype, [&](auto t) {
         with_choices(choices, n * width * dtype_bytes(dtype) >= kStreamBytes, [&](auto k, auto far) {
-            combine_kernel<decltype(t), k, far><<<move_blocks(a), kMoveBlock, 0, as_stream(stream)>>>(a);
+            combine_kernel<decltype(t), k, far><<<static_cast<uint32_t>(blocks), kMoveBlock, 0, as_stream(stream)>>>(a);
         });
     });
     return check_launch("rows combine");
@@ -296,8 +303,10 @@ ODIE_API int odie_rows_combine_backward(const void* upstream, int64_t upstream_s
     a.dweights = dweights;
     with_dtype(dtype, [&](auto t) {
         with_choices(choices, drows && stream_scattered(a, dtype), [&](auto k, auto far) {
-            combine_backward_kernel<decltype(t), k, far>
-                <<<row_blocks(a), kMoveBlock, 0, as_stream(stream)>>>(a);
+            in_launches(row_blocks(a), kMoveBlock, [&](uint32_t first, uint32_t count) {
+                a.first = first;
+                combine_backward_kernel<decltype(t), k, far><<<count, kMoveBlock, 0, as_stream(stream)>>>(a);
+            });
         });
     });
     return check_launch("rows combine gradient");

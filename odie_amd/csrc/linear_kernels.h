@@ -25,10 +25,10 @@ __device__ inline TileAt tile_at(uint32_t id, uint32_t down, uint32_t across) {
 // training step): 1.1 GB more, which come in bursts as the workgroups, one a CU, reach their ends together (120 us
 // at least), and the gelu's arithmetic (about 80).
 template <class T, bool kForward, Way kWay, int kBM, int kBN, int kWM, int kWN, int kStages>
-__global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(RowsArgs a, uint32_t blocks) {
+__global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(RowsArgs a, uint32_t first, uint32_t blocks) {
     using Work = Tile<T, true, kForward, kWay, kBM, kBN, kWM, kWN, kStages>;
     __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
-    const uint32_t id = xcd_major(blockIdx.x, gridDim.x);
+    const uint32_t id = first + xcd_major(blockIdx.x, gridDim.x);
     if (id >= blocks) return;
     const TileAt t = tile_at(id, static_cast<uint32_t>(a.tiles), (a.columns + kBN - 1) / kBN);
     const Piece p = find_piece(a.offsets, a.experts, a.experts + 1, a.rows, kBM, t.row);
@@ -330,15 +330,18 @@ int launch_rows_as(RowsArgs a, hipStream_t stream) {
     a.tiles = piece_ids(a.rows, kBM, a.offsets != nullptr, a.experts, true);
     const int64_t blocks = a.tiles * across;
     if (blocks >= int64_t{1} << 31) return fail("linear: too many tiles for one launch");
-    rows_kernel<T, kForward, kWay, kBM, kBN, kWM, kWN, kStages>
-        <<<whole_xcds(blocks), 64 * (kBM / kWM) * (kBN / kWN), 0, stream>>>(a, static_cast<uint32_t>(blocks));
+    constexpr int kThreads = 64 * (kBM / kWM) * (kBN / kWN);
+    in_launches(blocks, kThreads, [&](uint32_t first, uint32_t count) {
+        rows_kernel<T, kForward, kWay, kBM, kBN, kWM, kWN, kStages>
+            <<<whole_xcds(count), kThreads, 0, stream>>>(a, first, static_cast<uint32_t>(blocks));
+    });
     return check_launch("linear");
 }
 
 template <class T, int kRowTiles, int kSplit> int launch_few_rows_as(const RowsArgs& a, hipStream_t stream) {
     const int64_t across = (a.columns + 16 * kFewWaves / kSplit - 1) / (16 * kFewWaves / kSplit);
     const int64_t blocks = piece_ids(a.rows, 16 * kRowTiles, a.offsets != nullptr, a.experts, true) * across;
-    if (blocks >= int64_t{1} << 31) return fail("linear: too many tiles for one launch");
+    if (blocks > most_blocks(64 * kFewWaves)) return fail("linear: too many tiles for one launch");
     few_rows_kernel<T, kRowTiles, kSplit><<<static_cast<uint32_t>(blocks), 64 * kFewWaves, 0, stream>>>(a);
     return check_launch("linear");
 }
@@ -399,7 +402,7 @@ template <class T, bool kForward> int launch_rows_by(Way way, const RowsArgs& a,
 template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> int launch_weight_as(const WeightArgs& a, hipStream_t stream) {
     const int64_t tiles = static_cast<int64_t>((a.outputs + kBM - 1) / kBM) * ((a.inputs + kBN - 1) / kBN);
     const int64_t blocks = a.pieces * tiles;
-    if (blocks >= int64_t{1} << 31) return fail("linear: too many tiles for one launch");
+    if (blocks > most_blocks(64 * (kBM / kWM) * (kBN / kWN))) return fail("linear: too many tiles for one launch");
     weight_kernel<T, kWay, kBM, kBN, kWM, kWN>
         <<<whole_xcds(blocks), 64 * (kBM / kWM) * (kBN / kWN), 0, stream>>>(a, static_cast<uint32_t>(blocks));
     return check_launch("linear weight gradient");
@@ -437,7 +440,7 @@ template <class T> int launch_weight(const WeightArgs& a, hipStream_t stream) {
 template <class T> int launch_slope(const SlopeArgs& a, hipStream_t stream) {
     const int groups = (a.columns + 7) / 8, lanes = slope_lanes(a.columns);
     const int64_t across = (groups + lanes - 1) / lanes, blocks = a.pieces * across;
-    if (blocks >= int64_t{1} << 31) return fail("linear: too many workgroups for one launch");
+    if (blocks > most_blocks(kSlopeBlock)) return fail("linear: too many workgroups for one launch");
     if (blocks == 0) return 0;
     with_flag(a.rows * a.columns * static_cast<int64_t>(sizeof(T)) >= kStreamBytes, [&](auto far) {
         slope_kernel<T, far><<<static_cast<uint32_t>(blocks), kSlopeBlock, 0, stream>>>(a, lanes, static_cast<uint32_t>(across));
