@@ -519,12 +519,15 @@ template <int kActivation, bool kExact> __device__ inline float activate(float z
     return z;
 }
 
+// The limits at infinity: a sum past fp16's range is kept as an infinite one.  gelu's and silu's slopes multiply z by a
+// factor that is 0 in fp32 well before |z| = 128, and take z no further than that (a NaN stays in the other factor).
 template <int kActivation, bool kExact> __device__ inline float slope(float z) {
     if constexpr (kActivation == kRelu) return z > 0.0f ? 1.0f : 0.0f;
+    const float near = __builtin_amdgcn_fmed3f(z, -128.0f, 128.0f);
     if constexpr (kActivation == kGelu) {
         float bell;
         const float below = normal_below<kExact>(z, bell);
-        return fmaf(z * 0.39894228f, bell, below);
+        return fmaf(near * 0.39894228f, bell, below);
     }
     if constexpr (kActivation == kSigmoid || kActivation == kSoftplus || kActivation == kSilu) {
         // sigmoid(|z|) and sigmoid(-|z|), neither by a difference
@@ -532,7 +535,7 @@ template <int kActivation, bool kExact> __device__ inline float slope(float z) {
         if constexpr (kActivation == kSigmoid) return more * less;
         const float s = z < 0.0f ? less : more;
         if constexpr (kActivation == kSoftplus) return s;
-        return s * fmaf(z, z < 0.0f ? more : less, 1.0f);
+        return s * fmaf(near, z < 0.0f ? more : less, 1.0f);
     }
     return 1.0f;
 }
