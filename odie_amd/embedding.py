@@ -4,7 +4,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .rows import DTYPES, check_rows, records, row_major
+from .rows import DTYPES, check_rows, pitch, records, row_major
 
 
 def embed(table, ids, scale=1.0):
@@ -24,7 +24,7 @@ def embed(table, ids, scale=1.0):
 
 def _forward(table, ids, scale):
     out = torch.empty((*ids.shape, table.shape[1]), dtype=table.dtype, device=table.device)
-    _lib.call('odie_embed_forward', table, table.data_ptr(), table.stride(0), table.shape[0], ids.data_ptr(),
+    _lib.call('odie_embed_forward', table, table.data_ptr(), pitch(table), table.shape[0], ids.data_ptr(),
               ids.element_size(), ids.numel(), scale, table.shape[1], DTYPES[table.dtype], out.data_ptr())
     return out
 
@@ -45,7 +45,7 @@ class _Embed(torch.autograd.Function):
         dtype = DTYPES[ctx.dtype]
         dtable = torch.empty((vocab, width), dtype=ctx.dtype, device=ids.device)
         scratch = _lib.scratch('odie_embed_workspace', ids, ids.numel(), vocab, width, dtype)
-        _lib.call('odie_embed_backward', ids, rows.data_ptr(), rows.stride(0), ids.data_ptr(), ids.element_size(),
+        _lib.call('odie_embed_backward', ids, rows.data_ptr(), pitch(rows), ids.data_ptr(), ids.element_size(),
                   ids.numel(), vocab, ctx.scale, width, dtype, dtable.data_ptr(), _lib.ptr(scratch),
                   0 if scratch is None else scratch.numel())
         return dtable, None, None

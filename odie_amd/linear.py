@@ -9,7 +9,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .rows import DTYPES, check_rows, records, row_major
+from .rows import DTYPES, check_rows, pitch, records, row_major
 
 ACTIVATIONS = ('none', 'relu', 'sigmoid', 'softplus', 'gelu', 'silu')   # their ODIE_ACT_ codes in order
 _CODES = {name: code for code, name in enumerate(ACTIVATIONS)}
@@ -52,8 +52,8 @@ def linear(x, weight, bias=None, *, activation='none', residual=None, offsets=No
 def _forward(x, weight, bias, residual, offsets, activation, pre):
     n, outputs = x.shape[0], weight.shape[-2]
     out = torch.empty((n, outputs), dtype=x.dtype, device=x.device)
-    _lib.call('odie_linear_forward', x, x.data_ptr(), x.stride(0), n, weight.data_ptr(), _lib.ptr(bias),
-              _lib.ptr(residual), 0 if residual is None else residual.stride(0), _lib.ptr(offsets),
+    _lib.call('odie_linear_forward', x, x.data_ptr(), pitch(x), n, weight.data_ptr(), _lib.ptr(bias),
+              _lib.ptr(residual), 0 if residual is None else pitch(residual), _lib.ptr(offsets),
               1 if offsets is None else weight.shape[0], x.shape[1], outputs, DTYPES[x.dtype], activation,
               out.data_ptr(), outputs, _lib.ptr(pre))
     return out
@@ -88,7 +88,7 @@ class _Linear(torch.autograd.Function):
             dbias = torch.empty(weight.shape[:-1], dtype=x.dtype, device=x.device) if want_bias else None
             scratch = _lib.scratch('odie_linear_workspace', x, n, experts, int(offsets is not None), inputs, outputs,
                                    dtype, ctx.activation, int(want_weight), int(want_bias))
-            _lib.call('odie_linear_backward', x, rows.data_ptr(), rows.stride(0), x.data_ptr(), x.stride(0),
+            _lib.call('odie_linear_backward', x, rows.data_ptr(), pitch(rows), x.data_ptr(), pitch(x),
                       _lib.ptr(pre), n, weight.data_ptr(), _lib.ptr(offsets), experts, inputs, outputs, dtype,
                       ctx.activation, _lib.ptr(dx), _lib.ptr(dweight), _lib.ptr(dbias), _lib.ptr(scratch),
                       0 if scratch is None else scratch.numel())

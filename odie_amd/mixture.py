@@ -18,7 +18,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .embedding import embed
 from .linear import ACTIVATIONS, linear
-from .rows import DTYPES, check_rows, records, row_major
+from .rows import DTYPES, check_rows, pitch, records, row_major
 
 
 class ExpertOrder:
@@ -74,7 +74,7 @@ def combine(rows, order, weights=None):
 def _dispatch(x, order):
     n, choices = order.slots.shape
     out = torch.empty((n * choices, x.shape[1]), dtype=x.dtype, device=x.device)
-    _lib.call('odie_rows_dispatch', x, x.data_ptr(), x.stride(0), order.slots.data_ptr(), order.offsets.data_ptr(),
+    _lib.call('odie_rows_dispatch', x, x.data_ptr(), pitch(x), order.slots.data_ptr(), order.offsets.data_ptr(),
               n, choices, order.experts, x.shape[1], DTYPES[x.dtype], out.data_ptr())
     return out
 
@@ -82,7 +82,7 @@ def _dispatch(x, order):
 def _combine(rows, order, weights):
     n, choices = order.slots.shape
     out = torch.empty((n, rows.shape[1]), dtype=rows.dtype, device=rows.device)
-    _lib.call('odie_rows_combine', rows, rows.data_ptr(), rows.stride(0), order.slots.data_ptr(), _lib.ptr(weights),
+    _lib.call('odie_rows_combine', rows, rows.data_ptr(), pitch(rows), order.slots.data_ptr(), _lib.ptr(weights),
               n, choices, rows.shape[1], DTYPES[rows.dtype], out.data_ptr())
     return out
 
@@ -120,8 +120,8 @@ class _Combine(torch.autograd.Function):
             drows = torch.empty((n * choices, width), dtype=upstream.dtype, device=upstream.device)
         if want_weights:
             dweights = torch.empty((n, choices), dtype=torch.float32, device=upstream.device)
-        _lib.call('odie_rows_combine_backward', upstream, upstream.data_ptr(), upstream.stride(0), _lib.ptr(rows),
-                  0 if rows is None else rows.stride(0), order.slots.data_ptr(), _lib.ptr(weights),
+        _lib.call('odie_rows_combine_backward', upstream, upstream.data_ptr(), pitch(upstream), _lib.ptr(rows),
+                  0 if rows is None else pitch(rows), order.slots.data_ptr(), _lib.ptr(weights),
                   order.offsets.data_ptr(), n, choices, order.experts, width, DTYPES[upstream.dtype], _lib.ptr(drows),
                   _lib.ptr(dweights))
         return drows, dweights, None

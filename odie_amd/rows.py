@@ -26,9 +26,16 @@ def check_rows(name, value, width=None, *, dtype=None, device=None, count=None):
 
 def row_major(value):
     """value, or its copy where a row is not contiguous or rows overlap."""
-    if value.stride(1) != 1 or value.stride(0) < value.shape[1]:
+    n, width = value.shape
+    if (width > 1 and value.stride(1) != 1) or (n > 1 and value.stride(0) < width):
         return value.contiguous()
     return value
+
+
+def pitch(rows):
+    """Elements from row to row of what row_major returned.  The stride of a single row means nothing and may be any
+    number, also after contiguous()."""
+    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
 
 
 def records(*tensors):
