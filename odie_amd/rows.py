@@ -1,6 +1,7 @@
 """What the row operators (linear, mixture, embedding) share: their element types and the checks of
 their tensors."""
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -39,5 +40,9 @@ def pitch(rows):
 
 
 def records(*tensors):
-    """Whether autograd will ask for a gradient of one of the tensors."""
+    """Whether autograd has to see the call: it will ask for a gradient of one of the tensors, or one of them carries a
+    tangent (forward mode, also without gradients), which autograd refuses for these operators."""
+    if forward_ad._current_level >= 0:      # a level is open; asking each tensor costs more
+        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
