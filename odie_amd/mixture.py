@@ -68,7 +68,7 @@ def combine(rows, order, weights=None):
         if weights.shape != order.slots.shape or not weights.is_floating_point() or weights.device != rows.device:
             raise ValueError('weights must be a floating-point tensor of the shape and device of order.slots')
         weights = weights.float().contiguous()
-    return _Combine.apply(rows, weights, order) if records(rows, weights) else _combine(rows, order, weights)
+    return _Combine.apply(rows, weights, order) if records(rows, weights) else _combine(rows, order.slots, weights)
 
 
 def _dispatch(x, order):
@@ -79,10 +79,10 @@ def _dispatch(x, order):
     return out
 
 
-def _combine(rows, order, weights):
-    n, choices = order.slots.shape
+def _combine(rows, slots, weights):
+    n, choices = slots.shape
     out = torch.empty((n, rows.shape[1]), dtype=rows.dtype, device=rows.device)
-    _lib.call('odie_rows_combine', rows, rows.data_ptr(), pitch(rows), order.slots.data_ptr(), _lib.ptr(weights),
+    _lib.call('odie_rows_combine', rows, rows.data_ptr(), pitch(rows), slots.data_ptr(), _lib.ptr(weights),
               n, choices, rows.shape[1], DTYPES[rows.dtype], out.data_ptr())
     return out
 
@@ -90,30 +90,30 @@ def _combine(rows, order, weights):
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, order):
-        ctx.order = order
+        ctx.save_for_backward(order.slots)
         return _dispatch(x, order)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream):
-        return _combine(row_major(upstream), ctx.order, None), None
+        return _combine(row_major(upstream), ctx.saved_tensors[0], None), None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, order):
-        ctx.order = order
-        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, weights)
-        return _combine(rows, order, weights)
+        want_rows, want_weights = ctx.needs_input_grad[:2]
+        ctx.experts = order.experts
+        ctx.save_for_backward(rows if want_weights else None, weights, order.slots, order.offsets if want_rows else None)
+        return _combine(rows, order.slots, weights)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream):
-        rows, weights = ctx.saved_tensors
-        order = ctx.order
+        rows, weights, slots, offsets = ctx.saved_tensors
         want_rows, want_weights = ctx.needs_input_grad[:2]
         upstream = row_major(upstream)
-        n, choices = order.slots.shape
+        n, choices = slots.shape
         width = upstream.shape[1]
         drows = dweights = None
         if want_rows:
@@ -121,8 +121,8 @@ class _Combine(torch.autograd.Function):
         if want_weights:
             dweights = torch.empty((n, choices), dtype=torch.float32, device=upstream.device)
         _lib.call('odie_rows_combine_backward', upstream, upstream.data_ptr(), pitch(upstream), _lib.ptr(rows),
-                  0 if rows is None else pitch(rows), order.slots.data_ptr(), _lib.ptr(weights),
-                  order.offsets.data_ptr(), n, choices, order.experts, width, DTYPES[upstream.dtype], _lib.ptr(drows),
+                  0 if rows is None else pitch(rows), slots.data_ptr(), _lib.ptr(weights),
+                  _lib.ptr(offsets), n, choices, ctx.experts, width, DTYPES[upstream.dtype], _lib.ptr(drows),
                   _lib.ptr(dweights))
         return drows, dweights, None
 
