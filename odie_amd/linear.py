@@ -64,12 +64,15 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, offsets, activation):
         weight = weight.contiguous()
         bias = None if bias is None else bias.contiguous()
+        want_x, want_weight, want_bias = ctx.needs_input_grad[:3]
+        computed = want_x or want_weight or want_bias       # the residual's gradient is the upstream itself
         # the sums before the activation, from which the backward takes its slope
-        keep = activation and any(ctx.needs_input_grad[:3])
+        keep = activation and computed
         pre = torch.empty((x.shape[0], weight.shape[-2]), dtype=x.dtype, device=x.device) if keep else None
         out = _forward(x, weight, bias, residual, offsets, activation, pre)
-        ctx.save_for_backward(x, weight, pre, offsets)
-        ctx.activation = activation
+        # what the wanted gradients read
+        ctx.save_for_backward(x if want_weight else None, weight if want_x else None, pre, offsets if computed else None)
+        ctx.activation, ctx.inputs, ctx.weights = activation, x.shape[1], weight.shape
         return out
 
     @staticmethod
@@ -80,16 +83,16 @@ class _Linear(torch.autograd.Function):
         dx = dweight = dbias = None
         if want_x or want_weight or want_bias:
             rows = row_major(upstream)
-            n, inputs = x.shape
-            outputs, experts = weight.shape[-2], 1 if offsets is None else weight.shape[0]
-            dtype = DTYPES[x.dtype]
-            dx = torch.empty((n, inputs), dtype=x.dtype, device=x.device) if want_x else None
-            dweight = torch.empty_like(weight) if want_weight else None
-            dbias = torch.empty(weight.shape[:-1], dtype=x.dtype, device=x.device) if want_bias else None
-            scratch = _lib.scratch('odie_linear_workspace', x, n, experts, int(offsets is not None), inputs, outputs,
+            n, inputs = rows.shape[0], ctx.inputs
+            outputs, experts = rows.shape[1], 1 if offsets is None else ctx.weights[0]
+            dtype = DTYPES[rows.dtype]
+            dx = rows.new_empty((n, inputs)) if want_x else None
+            dweight = rows.new_empty(ctx.weights) if want_weight else None
+            dbias = rows.new_empty(ctx.weights[:-1]) if want_bias else None
+            scratch = _lib.scratch('odie_linear_workspace', rows, n, experts, int(offsets is not None), inputs, outputs,
                                    dtype, ctx.activation, int(want_weight), int(want_bias))
-            _lib.call('odie_linear_backward', x, rows.data_ptr(), pitch(rows), x.data_ptr(), pitch(x),
-                      _lib.ptr(pre), n, weight.data_ptr(), _lib.ptr(offsets), experts, inputs, outputs, dtype,
+            _lib.call('odie_linear_backward', rows, rows.data_ptr(), pitch(rows), _lib.ptr(x), 0 if x is None else pitch(x),
+                      _lib.ptr(pre), n, _lib.ptr(weight), _lib.ptr(offsets), experts, inputs, outputs, dtype,
                       ctx.activation, _lib.ptr(dx), _lib.ptr(dweight), _lib.ptr(dbias), _lib.ptr(scratch),
                       0 if scratch is None else scratch.numel())
         return dx, dweight, dbias, upstream if want_residual else None, None, None

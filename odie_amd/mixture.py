@@ -104,7 +104,9 @@ class _Combine(torch.autograd.Function):
     def forward(ctx, rows, weights, order):
         want_rows, want_weights = ctx.needs_input_grad[:2]
         ctx.experts = order.experts
-        ctx.save_for_backward(rows if want_weights else None, weights, order.slots, order.offsets if want_rows else None)
+        # what the wanted gradients read
+        ctx.save_for_backward(rows if want_weights else None, weights if want_rows else None, order.slots,
+                              order.offsets if want_rows else None)
         return _combine(rows, order.slots, weights)
 
     @staticmethod
