@@ -239,6 +239,18 @@ __device__ inline int64_t whole_pieces(const int32_t* offsets, int group, int64_
     return static_cast<uint32_t>(group_start(offsets, group, rows)) / static_cast<uint32_t>(piece);
 }
 
+// Partial sums of groups that are longer than a piece, and of those alone: piece `first` of a group that begins at row
+// `begin` has slot floor(2 begin / piece) + first.  A group of more than a piece has at most twice its length in
+// pieces, rounded down, so that the next group's slots begin past its own, and partial_slots(rows) are enough
+// however many groups there are.
+inline int64_t partial_slots(int64_t rows, int64_t piece, bool grouped) {
+    return grouped ? 2 * rows / piece : (rows + piece - 1) / piece;
+}
+
+__device__ inline int64_t partial_slot(int64_t begin, int64_t piece, int first) {
+    return static_cast<uint32_t>(2 * begin) / static_cast<uint32_t>(piece) + static_cast<int64_t>(first);
+}
+
 // The piece `id` of groups 0..groups-1 (groups = experts + 1 with the rows of no expert, else
 // experts).  All 64 lanes of the wave call it with the same id.
 __device__ inline Piece find_piece(const int32_t* offsets, int experts, int groups, int64_t rows, int64_t piece,

@@ -569,7 +569,7 @@ struct WeightArgs {           // dw[e] = dz^T x over each expert's rows
     const void* dz;           // [rows][outputs], stride ldz
     const void* x;            // [rows][inputs], stride ldx
     void* dw;                 // [experts][outputs][inputs]
-    float* partial;           // [piece ids][outputs][inputs] sums of groups cut into several pieces
+    float* partial;           // [partial slots][outputs][inputs] sums of groups cut into several pieces
     const int32_t* offsets;
     int64_t rows, ldz, ldx;
     int64_t piece;            // rows a workgroup sums
@@ -596,13 +596,14 @@ inline int slope_lanes(int columns) {
     return lanes;
 }
 
-struct FoldArgs {             // out[e][i] = sum over e's pieces of partial[piece][i]
+struct FoldArgs {             // out[e][i] = sum over e's pieces of partial[place of the piece][i]
     const float* partial;
     void* out;
     const int32_t* offsets;
     int64_t rows, piece, size;
     int experts;
-    bool single;              // also the groups of one piece (and zeros for those of none)
+    bool single;              // partial sums of every piece by its id, whole groups' too (zeros for groups of none);
+                              // else by partial_slot, and whole groups are left alone
 };
 
 // Launches, per element type.

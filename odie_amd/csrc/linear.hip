@@ -30,7 +30,8 @@ int64_t slope_piece(int64_t rows, int outputs) {
 
 // Tiles of the weight gradient and the rows a workgroup sums.  Three CUs of four at least are to have a workgroup (four
 // of the smallest tiles, two of the middle ones), from several pieces of the rows where there are too few tiles;
-// but partial sums, written and read again, are to stay below twice what the operands hold.  The
+// but partial sums, written and read again, are to stay below twice what the operands hold, with several experts
+// too (131072 bf16 rows over 1024 experts of 1024 x 1024: pieces of 1024 rows and 1.1 GB of sums).  The
 // largest tiles that manage it are taken (a 1024 x 1024 gradient over 4096 bf16 rows: 61 us as 16 tiles of
 // 256 x 256 and 16 pieces, 29 us as 64 of 128 x 128 and 4 pieces).
 struct WeightPlan {
@@ -48,8 +49,9 @@ WeightPlan weight_plan(int64_t rows, int experts, int outputs, int inputs, int d
         // Groups of up to twice the average stay whole where there are workgroups enough.
         const int edge = least > 64 ? 128 : 64;   // 256 gains nothing where groups differ in length
         const int64_t wanted = 4 * kCus / tiles_of(edge), pieces = wanted < most ? wanted : most;
-        if (pieces <= 2 * experts) return WeightPlan{edge, whole(2 * (rows / experts))};
-        return WeightPlan{edge, whole(rows / (pieces - experts / 2))};
+        const int64_t twice = 2 * (rows / experts), least_piece = most > 0 ? (rows + most - 1) / most : rows;
+        if (pieces <= 2 * experts) return WeightPlan{edge, whole(twice > least_piece ? twice : least_piece)};
+        return WeightPlan{edge, whole((rows + pieces - experts / 2 - 1) / (pieces - experts / 2))};
     }
     for (int edge = 256;; edge /= 2) {
         if (edge > 64 && least <= edge / 2) continue;
@@ -83,7 +85,7 @@ Plan make_plan(int64_t rows, int experts, bool grouped, int outputs, int inputs,
     p.dz_bytes = activation == kNone ? 0 : padded(rows * outputs * dtype_bytes(dtype));
     p.sums_bytes = want_dbias ? padded(p.slope_pieces * outputs * 4) : 0;
     p.partial_bytes = want_dweight && rows > p.weight_piece
-                          ? padded(p.weight_pieces * outputs * static_cast<int64_t>(inputs) * 4) : 0;
+                          ? padded(partial_slots(rows, p.weight_piece, grouped) * outputs * static_cast<int64_t>(inputs) * 4) : 0;
     return p;
 }
 

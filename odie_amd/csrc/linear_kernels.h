@@ -221,7 +221,7 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void weight_kernel(
     const int64_t matrix = static_cast<int64_t>(a.outputs) * a.inputs;
     const bool whole = p.group_end - p.group_begin <= a.piece;
     T* dw = static_cast<T*>(a.dw) + p.group * matrix;
-    float* partial = whole ? nullptr : a.partial + piece * matrix;
+    float* partial = whole ? nullptr : a.partial + partial_slot(p.group_begin, a.piece, p.first) * matrix;
     const int column = column0 + Work::own_column(), count = a.inputs - column;
     work.rows(
         lds, [](int) { return 0; },
@@ -300,7 +300,8 @@ template <class T, int kGroups> __global__ __launch_bounds__(256) void fold_kern
     const int e = static_cast<int>(blockIdx.y);
     const int64_t begin = a.offsets ? group_start(a.offsets, e, a.rows) : 0;
     const int64_t end = a.offsets ? group_start(a.offsets, e + 1, a.rows) : a.rows;
-    const int64_t first = a.offsets ? whole_pieces(a.offsets, e, a.rows, a.piece) + e : 0;
+    const int64_t first = a.single ? (a.offsets ? whole_pieces(a.offsets, e, a.rows, a.piece) + e : 0)
+                                   : partial_slot(begin, a.piece, 0);
     const int64_t pieces = end > begin ? (end - begin + a.piece - 1) / a.piece : 0;
     if (pieces <= 1 && !a.single) return;
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * kLanes; base < a.size; base += static_cast<int64_t>(gridDim.x) * kLanes) {
