@@ -33,14 +33,15 @@ def linear(x, weight, bias=None, *, activation='none', residual=None, offsets=No
         raise ValueError('weight must be %s of x\'s dtype and device' %
                          ('[outputs, inputs]' if offsets is None else '[experts, outputs, inputs]'))
     outputs, experts = weight.shape[-2], 1 if offsets is None else weight.shape[0]
-    if bias is not None and (bias.shape != weight.shape[:-1] or bias.dtype != x.dtype or bias.device != x.device):
+    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.shape != weight.shape[:-1]
+                             or bias.dtype != x.dtype or bias.device != x.device):
         raise ValueError('bias must be %s of x\'s dtype and device' %
                          ('[outputs]' if offsets is None else '[experts, outputs]'))
     if residual is not None:
         residual = check_rows('residual', residual, outputs, dtype=x.dtype, device=x.device, count=n)
     if offsets is not None:
-        if (offsets.dtype != torch.int32 or offsets.ndim != 1 or offsets.numel() != experts + 1
-                or offsets.device != x.device):
+        if (not isinstance(offsets, torch.Tensor) or offsets.dtype != torch.int32 or offsets.ndim != 1
+                or offsets.numel() != experts + 1 or offsets.device != x.device):
             raise ValueError('offsets must be a CUDA int32 tensor of experts + 1 entries')
         offsets = offsets.contiguous()
     if records(x, weight, bias, residual):
@@ -71,7 +72,8 @@ class _Linear(torch.autograd.Function):
         pre = torch.empty((x.shape[0], weight.shape[-2]), dtype=x.dtype, device=x.device) if keep else None
         out = _forward(x, weight, bias, residual, offsets, activation, pre)
         # what the wanted gradients read
-        ctx.save_for_backward(x if want_weight else None, weight if want_x else None, pre, offsets if computed else None)
+        ctx.save_for_backward(x if want_weight else None, weight if want_x else None, pre,
+                              offsets if computed else None)
         ctx.activation, ctx.inputs, ctx.weights = activation, x.shape[1], weight.shape
         return out
 
@@ -91,8 +93,8 @@ class _Linear(torch.autograd.Function):
             dbias = rows.new_empty(ctx.weights[:-1]) if want_bias else None
             scratch = _lib.scratch('odie_linear_workspace', rows, n, experts, int(offsets is not None), inputs, outputs,
                                    dtype, ctx.activation, int(want_weight), int(want_bias))
-            _lib.call('odie_linear_backward', rows, rows.data_ptr(), pitch(rows), _lib.ptr(x), 0 if x is None else pitch(x),
-                      _lib.ptr(pre), n, _lib.ptr(weight), _lib.ptr(offsets), experts, inputs, outputs, dtype,
+            _lib.call('odie_linear_backward', rows, rows.data_ptr(), pitch(rows), _lib.ptr(x),
+                      0 if x is None else pitch(x), _lib.ptr(pre), n, _lib.ptr(weight), _lib.ptr(offsets), experts, inputs, outputs, dtype,
                       ctx.activation, _lib.ptr(dx), _lib.ptr(dweight), _lib.ptr(dbias), _lib.ptr(scratch),
                       0 if scratch is None else scratch.numel())
         return dx, dweight, dbias, upstream if want_residual else None, None, None

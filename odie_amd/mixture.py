@@ -10,6 +10,7 @@ number of experts with a weight each: a blend over the borders of neighbouring t
   y     = combine(rows, order, weights)            y[i] = sum_j weights[i, j] rows[slots[i, j]]
 """
 import math
+import numbers
 
 import torch
 from torch import nn
@@ -39,8 +40,9 @@ def expert_order(expert, experts):
         raise ValueError('expert must be a CUDA int32 or int64 tensor, [N] or [N, choices]')
     if expert.ndim == 2 and expert.shape[1] == 0:
         raise ValueError('expert must have at least one choice a row')
-    if experts < 1:
-        raise ValueError('experts must be at least 1')
+    if not isinstance(experts, numbers.Integral) or experts < 1:
+        raise ValueError('experts must be a whole number, at least 1')
+    experts = int(experts)
     expert = expert.contiguous()
     n, device = expert.numel(), expert.device
     scratch = _lib.scratch('odie_sort_workspace', expert, n, experts)
@@ -65,7 +67,8 @@ def combine(rows, order, weights=None):
     n, choices = order.slots.shape
     rows = check_rows('rows', rows, count=n * choices, device=order.slots.device)
     if weights is not None:
-        if weights.shape != order.slots.shape or not weights.is_floating_point() or weights.device != rows.device:
+        if (not isinstance(weights, torch.Tensor) or weights.shape != order.slots.shape
+                or not weights.is_floating_point() or weights.device != rows.device):
             raise ValueError('weights must be a floating-point tensor of the shape and device of order.slots')
         weights = weights.float().contiguous()
     return _Combine.apply(rows, weights, order) if records(rows, weights) else _combine(rows, order.slots, weights)
