@@ -560,8 +560,8 @@ void odie_destroy(void* handle);
  * linear layers dense or per expert, and lookups of a table by id.  No counterpart in the reference.
  *
  * dtype is ODIE_F32, ODIE_F16 or ODIE_BF16 for every tensor of a call unless stated; sums are fp32 and
- * rounded once.  Rows are contiguous; a stride is the elements from row to row (at least the
- * row's width).  No alignment is needed beyond the element's.  Workspaces are the caller's, so calls on
+ * outputs rounded once (odie_linear_backward states what else is rounded).  Rows are contiguous; a stride is the
+ * elements from row to row (at least the row's width, also of a single row).  A width is at most 2^20.  No alignment is needed beyond the element's.  Workspaces are the caller's, so calls on
  * different streams share nothing.  A call of no rows is fine; gradients of parameters are then 0.
  * --------------------------------------------------------------------------------------- */
 
@@ -610,7 +610,8 @@ int odie_rows_combine_backward(const void* upstream, int64_t upstream_stride, co
  * offsets[0] = 0, offsets[experts] <= rows; rows offsets[e]..offsets[e+1]-1 use expert e's matrix, rows
  * from offsets[experts] on belong to none (out = residual, or 0).  offsets = NULL with experts = 1: one
  * matrix for every row.  pre, if not null, receives the sums before the activation
- * ([rows][outputs], unset in rows of no expert): what odie_linear_backward needs. */
+ * ([rows][outputs], rounded to dtype, an infinity where that does not hold them; unset in rows of no expert): what
+ * odie_linear_backward needs.  At most 32768 experts. */
 int odie_linear_forward(const void* x, int64_t x_stride, int64_t rows, const void* weight, const void* bias,
                         const void* residual, int64_t residual_stride, const int32_t* offsets, int experts,
                         int inputs, int outputs, int dtype, int activation, void* out, int64_t out_stride, void* pre,
@@ -618,7 +619,9 @@ int odie_linear_forward(const void* x, int64_t x_stride, int64_t rows, const voi
 
 /* Gradients of odie_linear_forward: dx [rows][inputs] (0 in rows of no expert), dweight, dbias (shaped as
  * weight and bias), each or null; the residual's gradient is upstream itself.  pre may be null
- * with ODIE_ACT_NONE, x without dweight, weight without dx.  Deterministic.  workspace: 256-byte aligned,
+ * with ODIE_ACT_NONE, x without dweight, weight without dx.  Deterministic.  The slope is that of pre, at infinity its
+ * limit; its product with upstream is rounded to dtype for dx and dweight (with ODIE_ACT_NONE there is neither), and
+ * summed as it is for dbias.  workspace: 256-byte aligned,
  * odie_linear_workspace bytes (grouped: offsets given; want_*: the output given). */
 int64_t odie_linear_workspace(int64_t rows, int experts, int grouped, int inputs, int outputs, int dtype,
                               int activation, int want_dweight, int want_dbias);

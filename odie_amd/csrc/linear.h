@@ -8,8 +8,9 @@
 //   weight    dw[n][k] = sum_m  dz[m][n] x[m][k]     both one row per m
 //
 // A workgroup owns a kBM x kBN tile of C and walks k in slabs of 128 bytes (64 16-bit or 32 fp32
-// values).  Per slab both operands pass through LDS in their memory orientation: global loads of the
-// next slab are in flight while the current one is multiplied, two LDS buffers, one barrier a slab.
+// values).  Per slab both operands pass through LDS in their memory orientation, with one barrier a slab and later
+// slabs under way while one is multiplied: straight to LDS one in a second buffer, in 64 x 64 tiles three in four
+// buffers; through registers two in registers (64 x 64 tiles three, element by element one) and two buffers.
 // A 16-bit operand stored one row per k is turned by ds_read_b64_tr_b16 as it is read.  Products are
 // v_mfma_f32_32x32x16 (16-bit) or v_mfma_f32_32x32x2 (fp32), accumulated in fp32.
 //

@@ -240,7 +240,9 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void weight_kernel(
 constexpr int kSlopeBlock = 256;
 
 // dz = dy act'(pre), rounded to the tensors' type as every operand of a 16-bit product is, and its column sums,
-// which take dz before that rounding.  A workgroup takes one piece of rows and `lanes` groups of 8 columns;
+// which take dz before that rounding (its slope is that of the kept sums).  The rounding is most of what the gradients
+// are off by beside their own: 65536 x 1024 -> 4096 bf16, gelu, dx and dw relative to 64 bits 0.0024; the result's own
+// rounding alone 0.0017, with the kept sums' 0.00175, with dz's 0.00235.  A workgroup takes one piece of rows and `lanes` groups of 8 columns;
 // 256 / lanes rows at a time.  Bound by HBM: 65536 x 4096 bf16 gelu 322 us, 1.6 GB at 5.0 TB/s.
 template <class T, bool kStream> __global__ __launch_bounds__(kSlopeBlock) void slope_kernel(SlopeArgs a, int lanes, uint32_t across) {
     __shared__ float total[kSlopeBlock * 8];
@@ -347,7 +349,10 @@ template <class T, int kRowTiles, int kSplit> int launch_few_rows_as(const RowsA
     return check_launch("linear");
 }
 
-// The depth is split over all eight waves where a share is still long or there are too few workgroups otherwise.
+// The depth is split over all eight waves where a share is still long or there are too few workgroups otherwise.  us
+// with eight shares and with two: one bf16 row, 2048 -> 2048 4.6 and 11.1, 512 -> 4096 3.6 and 4.7, 512 -> 16384 6.4
+// and 5.0; 16 fp16 rows over 64 experts of 512 -> 1024 12.5 and 8.3.  Long shares with workgroups enough lose a little:
+// 2048 -> 16384 15.2 and 12.5, 4096 -> 16384 22.1 and 21.8.
 template <class T, int kRowTiles> int launch_few_rows(const RowsArgs& a, hipStream_t stream) {
     const int64_t steps = a.depth / (4 * kPerVec<T>);
     const int64_t busy = a.rows < a.experts ? a.rows : a.experts;
@@ -374,7 +379,8 @@ inline bool even(int64_t tiles) { return tiles >= kCus && 4 * tiles >= 3 * ((til
 //   256 x 256, 64 x 128 a wave   620, 112  where they go round and a group's rows fill them (the path through
 //                                          registers has no room)
 //   128 x 128, 64 x 64 a wave    777, 130  two a CU, where they go round
-//   128 x 64, 32 x 64 a wave     narrow outputs: no columns wasted
+//   128 x 64, 32 x 64 a wave     narrow outputs: no columns wasted (64 -> 64 fp16: 262144 rows 14.8 us, as 64 x 64
+//                                25.3; 32768 rows 4.9 and 5.1; 16384 rows 4.5 and 4.2)
 //   64 x 64, 32 x 32 a wave      what is left; straight to LDS with three slabs under way (seven are no
 //                                faster: 512 x 2048 x 2048 14.4 us with three, 15.5 with seven)
 // Tiles that leave CUs idle in their last round are passed over where the products bound them: the largest, and fp32's
@@ -413,7 +419,10 @@ template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> int launch_weig
 
 template <class T> int launch_rows(const RowsArgs& a, bool forward, hipStream_t stream) {
     if (forward) {
-        // groups of varying sizes: room for twice the average
+        // Groups of varying sizes: room for twice the average.  us of 16, 32, 64 rows a piece, and of tiles: 2048 -> 2048
+        // bf16, 16, 32, 64 rows 6.1, 7.8, 11.7 and 14.5 to 14.7 (128 rows 11.9 and 14.8); fp32, 64 rows 26 and 50.  Over 64
+        // fp16 experts of 512 -> 1024, 16 and 64 rows in all 8.9, 13.1 and 13.1, 17.5; groups of several rows read
+        // their weights for each piece, and tiles would be faster: 512 rows 21.9 and 18.9, 2048 rows 39.5 and 23.9.
         const int64_t each = (a.rows + a.experts - 1) / a.experts * (a.experts > 1 ? 2 : 1);
         if (each <= 16) return launch_few_rows<T, 1>(a, stream);
         if (each <= 32) return launch_few_rows<T, 2>(a, stream);
@@ -450,7 +459,9 @@ template <class T> int launch_slope(const SlopeArgs& a, hipStream_t stream) {
 }
 
 template <class T> int launch_fold(const FoldArgs& a, hipStream_t stream) {
-    // many pieces of few elements (a bias): several groups share them
+    // many pieces of few elements (a bias): several groups share them (us, shared and not: a bias over 2^20 x 64 fp16
+    // 36 and 158 with its slope pass, over 131072 x 512 and 64 experts 27 and 26; a weight gradient of 64 x 64 over
+    // 65536 rows 10 and 25, of 1024 x 1024 over 4096, four pieces, 41 and 25)
     const bool tall = a.rows / a.piece >= 8 * static_cast<int64_t>(a.experts);
     const int64_t lanes = tall ? 16 : 256;
     // most experts' groups are whole and have nothing to add: few workgroups each
