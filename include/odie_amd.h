@@ -562,7 +562,8 @@ void odie_destroy(void* handle);
  * dtype is ODIE_F32, ODIE_F16 or ODIE_BF16 for every tensor of a call unless stated; sums are fp32 and
  * outputs rounded once (odie_linear_backward states what else is rounded).  Rows are contiguous; a stride is the
  * elements from row to row (at least the row's width, also of a single row).  A width is at most 2^20.  No alignment is needed beyond the element's.  Workspaces are the caller's, so calls on
- * different streams share nothing.  A call of no rows is fine; gradients of parameters are then 0.
+ * different streams share nothing.  A call of no rows is fine; gradients of parameters are then 0.  A lookup or a
+ * return that writes more than about 137 GB (2^32 threads in one launch) is refused.
  * --------------------------------------------------------------------------------------- */
 
 /* Stable sort of n keys (int32 or int64: key_bytes 4 or 8) by bucket 0..buckets-1; a key outside them

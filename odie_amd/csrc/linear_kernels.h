@@ -111,8 +111,8 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(Ro
 
 constexpr int kFewWaves = 8;
 
-// Few rows a group: the weights are read once, straight into registers in the layout of the products, and
-// everything else is small beside them.  A wave takes 16 columns of the output, 16 kRowTiles rows and one of
+// Few rows a group: the weights are read once for every 16 kRowTiles rows, straight into registers in the layout of the
+// products, and everything else is small beside them.  A wave takes 16 columns of the output, 16 kRowTiles rows and one of
 // kSplit shares of the depth, of which it has several hundred bytes of every weight row under way; the
 // shares' sums are added in order through LDS.  Bound by the latency of one chain of loads: one bf16 row through
 // 2048 x 2048 (8.4 MB) 4.9 us; 16 rows over 64 fp16 experts of 512 -> 1024 (17 MB of
