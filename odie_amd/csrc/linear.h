@@ -308,22 +308,12 @@ template <class T, bool kByRow, int kRows, int kThreads> struct Gathered : Image
 // How operands reach LDS.
 enum Way { kDirect, kStaged, kGathered };
 
-// One workgroup's tile: waves of kWM x kWN, kBM / kWM x kBN / kWN of them.
-template <class T, bool kAByRow, bool kBByRow, Way kWay, int kBM, int kBN, int kWM, int kWN, int kWantedStages = 2>
-struct Tile {
+// The sums of one workgroup's tile: waves of kWM x kWN, kBM / kWM x kBN / kWN of them.
+template <int kBM, int kBN, int kWM, int kWN> struct Sums {
     static constexpr int kThreads = 64 * (kBM / kWM) * (kBN / kWN);
-    template <bool kByRow, int kRows>
-    using Loader = std::conditional_t<kWay == kDirect, Direct<T, kByRow, kRows, kThreads>,
-                                      std::conditional_t<kWay == kStaged, Staged<T, kByRow, kRows, kThreads>,
-                                                         Gathered<T, kByRow, kRows, kThreads>>>;
-    using A = Loader<kAByRow, kBM>;
-    using B = Loader<kBByRow, kBN>;
     static constexpr int kMs = kWM / 32, kNs = kWN / 32;
-    static constexpr int kBuffer = A::kBytes + B::kBytes;
     static constexpr int kPitch = kWN + 4;                  // floats a row of the epilogue's region
     static constexpr int kRegion = 32 * kPitch * 4;
-    static constexpr int kStages = kWay == kDirect ? kWantedStages : 2;   // slabs in LDS: one read, the others under way
-    static constexpr int kLds = kStages * kBuffer > kThreads / 64 * kRegion ? kStages * kBuffer : kThreads / 64 * kRegion;
 
     accum16 acc[kMs][kNs];
 
@@ -337,11 +327,77 @@ struct Tile {
 #pragma unroll
             for (int j = 0; j < kNs; ++j) acc[i][j] = accum16{};
     }
+    static constexpr int kLanes = kWN / 8;                   // lanes a row of the epilogue, 8 columns each
+    static constexpr int kHeight = 64 / kLanes;              // rows a pass
+    static constexpr int kPasses = 32 / kHeight;
+    static constexpr int kGroup = kPasses < 4 ? kPasses : 4; // passes handed out together
+
+    static __device__ int own_column() { return wave_column() + static_cast<int>(threadIdx.x % kLanes) * 8; }
+
+    // Hands out the tile's values: a lane's are the 8 columns from own_column() on of kGroup rows at a time, row,
+    // row + kHeight, ... (relative to the tile).
+    //   fetch(row) -> what use needs from memory for these rows, asked for a group ahead of
+    //   use(row, value[kGroup][8], fetched)
+    template <class Fetch, class Use> __device__ void rows(char* lds, Fetch&& fetch, Use&& use) {
+        const int lane = static_cast<int>(threadIdx.x % 64);
+        float* region = reinterpret_cast<float*>(lds + wave() * kRegion);
+        const float* from = region + lane / kLanes * kPitch + lane % kLanes * 8;
+        // accumulator element v of lane l: row l % 32, column 8 (v / 4) + 4 (l / 32) + v % 4
+        float* to = region + lane % 32 * kPitch + lane / 32 * 4;
+#pragma unroll
+        for (int i = 0; i < kMs; ++i) {
+            const int row = wave_row() + 32 * i + lane / kLanes;
+            auto fetched = fetch(row);
+#pragma unroll
+            for (int j = 0; j < kNs; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<float4*>(to + 32 * j + 8 * q) =
+                        make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+            wave_fence();
+#pragma unroll 1
+            for (int pass = 0; pass < kPasses; pass += kGroup) {
+                auto ahead = fetched;
+                if (pass + kGroup < kPasses) ahead = fetch(row + (pass + kGroup) * kHeight);
+                float value[kGroup][8];
+#pragma unroll
+                for (int u = 0; u < kGroup; ++u) {
+                    const float* p = from + (pass + u) * kHeight * kPitch;
+                    const float4 lo = *reinterpret_cast<const float4*>(p), hi = *reinterpret_cast<const float4*>(p + 4);
+                    value[u][0] = lo.x, value[u][1] = lo.y, value[u][2] = lo.z, value[u][3] = lo.w;
+                    value[u][4] = hi.x, value[u][5] = hi.y, value[u][6] = hi.z, value[u][7] = hi.w;
+                }
+                use(row + pass * kHeight, value, fetched);
+                fetched = ahead;
+            }
+            wave_fence();
+        }
+    }
+};
+
+// One workgroup's tile of a product.
+template <class T, bool kAByRow, bool kBByRow, Way kWay, int kBM, int kBN, int kWM, int kWN, int kWantedStages = 2>
+struct Tile : Sums<kBM, kBN, kWM, kWN> {
+    using Base = Sums<kBM, kBN, kWM, kWN>;
+    using Base::acc;
+    using Base::kMs;
+    using Base::kNs;
+    using Base::kRegion;
+    using Base::kThreads;
+    template <bool kByRow, int kRows>
+    using Loader = std::conditional_t<kWay == kDirect, Direct<T, kByRow, kRows, kThreads>,
+                                      std::conditional_t<kWay == kStaged, Staged<T, kByRow, kRows, kThreads>,
+                                                         Gathered<T, kByRow, kRows, kThreads>>>;
+    using A = Loader<kAByRow, kBM>;
+    using B = Loader<kBByRow, kBN>;
+    static constexpr int kBuffer = A::kBytes + B::kBytes;
+    static constexpr int kStages = kWay == kDirect ? kWantedStages : 2;   // slabs in LDS: one read, the others under way
+    static constexpr int kLds = kStages * kBuffer > kThreads / 64 * kRegion ? kStages * kBuffer : kThreads / 64 * kRegion;
 
     // (Reading a step's fragments while the step before is multiplied gains nothing: two waves a SIMD do that already.)
     __device__ void add_slab(const char* here) {
         const int lane = static_cast<int>(threadIdx.x % 64);
-        const int wm = wave_row(), wn = wave_column();
+        const int wm = Base::wave_row(), wn = Base::wave_column();
 #pragma unroll
         for (int step = 0; step < kSlabBytes / 32; ++step) {
             vec16 fa[kMs], fb[kNs];
@@ -358,7 +414,7 @@ struct Tile {
 
     // Sums `depth` values of k, the same for the whole workgroup.  a and b have begun.
     __device__ void sum(A& a, B& b, int64_t depth, char* lds) {
-        clear();
+        Base::clear();
         if (depth <= 0) return;
         if constexpr (kStages > 2) {
             // Each wave waits for its own loads of the slab (the kAhead - 1 later slabs stay under way) and for its
@@ -423,53 +479,6 @@ struct Tile {
             }
         }
         __syncthreads();
-    }
-
-    static constexpr int kLanes = kWN / 8;                   // lanes a row of the epilogue, 8 columns each
-    static constexpr int kHeight = 64 / kLanes;              // rows a pass
-    static constexpr int kPasses = 32 / kHeight;
-    static constexpr int kGroup = kPasses < 4 ? kPasses : 4; // passes handed out together
-
-    static __device__ int own_column() { return wave_column() + static_cast<int>(threadIdx.x % kLanes) * 8; }
-
-    // Hands out the tile's values: a lane's are the 8 columns from own_column() on of kGroup rows at a time, row,
-    // row + kHeight, ... (relative to the tile).
-    //   fetch(row) -> what use needs from memory for these rows, asked for a group ahead of
-    //   use(row, value[kGroup][8], fetched)
-    template <class Fetch, class Use> __device__ void rows(char* lds, Fetch&& fetch, Use&& use) {
-        const int lane = static_cast<int>(threadIdx.x % 64);
-        float* region = reinterpret_cast<float*>(lds + wave() * kRegion);
-        const float* from = region + lane / kLanes * kPitch + lane % kLanes * 8;
-        // accumulator element v of lane l: row l % 32, column 8 (v / 4) + 4 (l / 32) + v % 4
-        float* to = region + lane % 32 * kPitch + lane / 32 * 4;
-#pragma unroll
-        for (int i = 0; i < kMs; ++i) {
-            const int row = wave_row() + 32 * i + lane / kLanes;
-            auto fetched = fetch(row);
-#pragma unroll
-            for (int j = 0; j < kNs; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<float4*>(to + 32 * j + 8 * q) =
-                        make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-            wave_fence();
-#pragma unroll 1
-            for (int pass = 0; pass < kPasses; pass += kGroup) {
-                auto ahead = fetched;
-                if (pass + kGroup < kPasses) ahead = fetch(row + (pass + kGroup) * kHeight);
-                float value[kGroup][8];
-#pragma unroll
-                for (int u = 0; u < kGroup; ++u) {
-                    const float* p = from + (pass + u) * kHeight * kPitch;
-                    const float4 lo = *reinterpret_cast<const float4*>(p), hi = *reinterpret_cast<const float4*>(p + 4);
-                    value[u][0] = lo.x, value[u][1] = lo.y, value[u][2] = lo.z, value[u][3] = lo.w;
-                    value[u][4] = hi.x, value[u][5] = hi.y, value[u][6] = hi.z, value[u][7] = hi.w;
-                }
-                use(row + pass * kHeight, value, fetched);
-                fetched = ahead;
-            }
-            wave_fence();
-        }
     }
 };
 

@@ -1,23 +1,9 @@
 // The kernels of linear.hip, instantiated by linear_f16.hip, linear_bf16.hip and linear_f32.hip.
 #pragma once
-#include "linear.h"
+#include "linear_epilogue.h"
 
 namespace odie {
 namespace {
-
-constexpr uint32_t kBand = 4;
-
-struct TileAt {
-    uint32_t row, column;
-};
-
-// Tiles in bands of kBand rows, down each band's columns first: tiles that run at the same time on an XCD
-// form a block of about kBand by 8, and read the fewest rows of both operands through its L2.
-__device__ inline TileAt tile_at(uint32_t id, uint32_t down, uint32_t across) {
-    const uint32_t band = id / (kBand * across), inside = id - band * kBand * across;
-    const uint32_t high = down - band * kBand < kBand ? down - band * kBand : kBand;
-    return TileAt{band * kBand + inside % high, inside / high};
-}
 
 // One tile of act(a b^T + bias) + residual (forward) or of a b (the input's gradient).  65536 rows, 1024 -> 4096,
 // bf16: 550 GFLOP; the bare product 540 to 615 us (900 to 1020 TFLOP/s), bound by the feeding of the matrix
@@ -34,19 +20,7 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(Ro
     const Piece p = find_piece(a.offsets, a.experts, a.experts + 1, a.rows, kBM, t.row);
     if (p.begin >= p.end) return;
     const int column0 = static_cast<int>(t.column) * kBN;
-    const T* residual = static_cast<const T*>(a.residual);
-    T* out = static_cast<T*>(a.out);
-    if (p.group >= a.experts) {   // rows of no expert
-        for (int i = threadIdx.x; i < kBM * (kBN / 8); i += Work::kThreads) {
-            const int64_t row = p.begin + i / (kBN / 8);
-            const int column = column0 + i % (kBN / 8) * 8;
-            if (row >= p.end || column >= a.columns) continue;
-            float value[8] = {};
-            if (residual) load8(residual + row * a.ldr + column, a.columns - column, value);
-            store8(out + row * a.ldo + column, a.columns - column, value);
-        }
-        return;
-    }
+    if (p.group >= a.experts) return rows_of_none<T, kBM, kBN, Work::kThreads>(a, p, column0);
     const int64_t matrix = static_cast<int64_t>(a.columns) * a.depth;
     const T* b = static_cast<const T*>(a.b) + p.group * matrix;
     typename Work::A opa;
@@ -55,61 +29,8 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void rows_kernel(Ro
     opb.begin(b, kForward ? a.depth : a.columns, column0, a.columns, a.depth);
     Work work;
     work.sum(opa, opb, a.depth, lds);
-    const T* bias = a.bias ? static_cast<const T*>(a.bias) + static_cast<int64_t>(p.group) * a.columns : nullptr;
-    T* pre = static_cast<T*>(a.pre);
-    constexpr int kGroup = Work::kGroup, kHeight = Work::kHeight;
-    constexpr bool kStream = kBM == 256;   // taken for outputs near the L2s' size and larger alone (17 MB at least)
-    struct Fetched {
-        Eight<T> row[kGroup];
-    };
-    const int column = column0 + Work::own_column(), count = a.columns - column;   // the lane's through every row
-    float shift[8] = {};
-    if (bias && count > 0) load8(bias + column, count, shift);
-    work.rows(
-        lds,
-        [&](int r) {
-            Fetched f{};
-            if (residual && count > 0)
-#pragma unroll
-                for (int u = 0; u < kGroup; ++u) {
-                    const int64_t row = p.begin + r + u * kHeight;
-                    if (row < p.end) f.row[u].load(residual + row * a.ldr + column, count);
-                }
-            return f;
-        },
-        [&](int r, float value[kGroup][8], const Fetched& f) {
-#pragma unroll
-            for (int u = 0; u < kGroup; ++u)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) value[u][i] += shift[i];
-            if (pre && count > 0)
-#pragma unroll
-                for (int u = 0; u < kGroup; ++u) {
-                    const int64_t row = p.begin + r + u * kHeight;
-                    if (row < p.end) store8<kStream>(pre + row * a.columns + column, count, value[u]);
-                }
-            with_activation(a.activation, [&](auto activation) {
-#pragma unroll
-                for (int u = 0; u < kGroup; ++u)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) value[u][i] = activate<activation, sizeof(T) == 4>(value[u][i]);
-            });
-#pragma unroll
-            for (int u = 0; u < kGroup; ++u) {
-                const int64_t row = p.begin + r + u * kHeight;
-                if (row >= p.end || count <= 0) continue;
-                if (residual) {
-                    float more[8];
-                    f.row[u].get(more);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) value[u][i] += more[i];
-                }
-                store8<kStream>(out + row * a.ldo + column, count, value[u]);
-            }
-        });
+    finish_tile<T, kBM == 256>(work, a, p, column0, lds);   // 256: taken for outputs near the L2s' size and larger alone (17 MB at least)
 }
-
-constexpr int kFewWaves = 8;
 
 // Few rows a group: the weights are read once for every 16 kRowTiles rows, straight into registers in the layout of the
 // products, and everything else is small beside them.  A wave takes 16 columns of the output, 16 kRowTiles rows and one of
@@ -126,8 +47,6 @@ template <class T, int kRowTiles, int kSplit> __global__ __launch_bounds__(64 * 
     const Piece p = find_piece(a.offsets, a.experts, a.experts + 1, a.rows, 16 * kRowTiles, blockIdx.x / across);
     if (p.begin >= p.end) return;
     const int column0 = static_cast<int>(blockIdx.x % across) * kColumns;
-    const T* residual = static_cast<const T*>(a.residual);
-    T* out = static_cast<T*>(a.out);
     const int lane = static_cast<int>(threadIdx.x % 64);
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64));
     const bool owned = p.group < a.experts;        // else rows of no expert
@@ -169,24 +88,7 @@ template <class T, int kRowTiles, int kSplit> __global__ __launch_bounds__(64 * 
         for (int t = 0; t < kRowTiles; ++t) part[wave][t][lane] = acc[t];
     }
     __syncthreads();
-    const T* bias = a.bias && owned ? static_cast<const T*>(a.bias) + static_cast<int64_t>(p.group) * a.columns : nullptr;
-    T* pre = static_cast<T*>(a.pre);
-    for (int i = threadIdx.x; i < 16 * kRowTiles * kColumns; i += 64 * kFewWaves) {
-        const int r = i / kColumns, c = i % 16, tile = i % kColumns / 16, column = column0 + i % kColumns;
-        const int64_t row = p.begin + r;
-        if (row >= p.end || column >= a.columns) continue;
-        float value = 0.0f;
-        if (owned) {
-            // accumulator element v of lane l: row l % 16, column 4 (l / 16) + v
-#pragma unroll
-            for (int s = 0; s < kSplit; ++s) value += part[tile * kSplit + s][r / 16][c / 4 * 16 + r % 16][c % 4];
-            if (bias) value += static_cast<float>(bias[column]);
-            if (pre) pre[row * a.columns + column] = static_cast<T>(value);
-            with_activation(a.activation, [&](auto activation) { value = activate<activation, sizeof(T) == 4>(value); });
-        }
-        if (residual) value += static_cast<float>(residual[row * a.ldr + column]);
-        out[row * a.ldo + column] = static_cast<T>(value);
-    }
+    finish_few<T, kRowTiles, kSplit>(part, a, p, column0, owned);
 }
 
 // One tile of one piece of rows: dw[e] = dz^T x where the piece is all of the expert's rows, else a partial sum
@@ -325,8 +227,6 @@ template <class T, int kGroups> __global__ __launch_bounds__(256) void fold_kern
     }
 }
 
-uint32_t whole_xcds(int64_t blocks) { return static_cast<uint32_t>((blocks + kXcds - 1) / kXcds * kXcds); }
-
 template <class T, bool kForward, Way kWay, int kBM, int kBN, int kWM, int kWN, int kStages = 2>
 int launch_rows_as(RowsArgs a, hipStream_t stream) {
     const int64_t across = (a.columns + kBN - 1) / kBN;
@@ -359,20 +259,6 @@ template <class T, int kRowTiles> int launch_few_rows(const RowsArgs& a, hipStre
     if (steps >= 64 || busy * a.columns < 64 * kCus) return launch_few_rows_as<T, kRowTiles, 8>(a, stream);
     return launch_few_rows_as<T, kRowTiles, 2>(a, stream);
 }
-
-// The way to LDS of rows of `width` elements: directly where each row starts on 16 bytes and is a multiple of them.
-template <class T> Way way_of(const void* data, int64_t stride, int64_t width) {
-    const int64_t pitch = stride * static_cast<int64_t>(sizeof(T));
-    if (width < kPerVec<T>) return kGathered;
-    return reinterpret_cast<uintptr_t>(data) % 16 == 0 && pitch % 16 == 0 && width % kPerVec<T> == 0 &&
-                   pitch < (int64_t{1} << 22)   // 256 rows of a tile within 2^30 bytes
-               ? kDirect : kStaged;
-}
-
-inline Way slower(Way a, Way b) { return a > b ? a : b; }
-
-// Whether `tiles` keep three quarters of the CUs busy to the end.
-inline bool even(int64_t tiles) { return tiles >= kCus && 4 * tiles >= 3 * ((tiles + kCus - 1) / kCus * kCus); }
 
 // Tiles by the work there is (us of one bf16 product, 65536 x 1024 x 4096; and with its epilogue, 131072 x 256 x 512
 // over 64 experts):
