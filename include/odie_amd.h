@@ -643,6 +643,84 @@ int odie_embed_backward(const void* upstream, int64_t upstream_stride, const voi
                         int64_t vocab, float scale, int64_t width, int dtype, void* dtable, void* workspace,
                         int64_t workspace_bytes, uint64_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * A learned router over experts or classes.  logits [n][width] of dtype ODIE_F32, ODIE_F16 or ODIE_BF16 in contiguous
+ * rows of any stride from the width on; a logit of -inf is masked (no share, never chosen), NaN and +inf make their
+ * row's softmax NaN.  Everything else of floating type is fp32, and so are sums; gradients are of the logits' type, written whole in
+ * contiguous rows, each value rounded once.  Deterministic.  Workspaces are the caller's.  Calls of no rows are fine.
+ * No counterpart in the reference.
+ * --------------------------------------------------------------------------------------- */
+
+/* The `choices` largest logits of each row, the lowest index first among equal ones (a NaN is the largest): expert int32
+ * [n][choices], -1 where the row has fewer above -inf, and weights [n][choices], their softmax over the chosen
+ * (normalize = 1) or over all experts (0), 0 with -1.  stats fp32 [n][2] or null: what the backward needs with
+ * normalize = 0.  At most 32768 experts and 64 choices, n * choices < 2^31. */
+int odie_choose_forward(const void* logits, int64_t stride, int64_t n, int experts, int choices, int normalize, int dtype,
+                        int32_t* expert, float* weights, float* stats, uint64_t stream);
+
+/* Gradient of odie_choose_forward's weights: dlogits [n][experts] from upstream [n][choices].  logits and stats: null for
+ * normalised weights, else the forward's. */
+int odie_choose_backward(const float* upstream, const int32_t* expert, const float* weights, const void* logits,
+                         int64_t stride, const float* stats, int64_t n, int experts, int choices, int dtype, void* dlogits,
+                         uint64_t stream);
+
+/* loss = experts / (M R) * sum over rows and experts of counts[e] p[i][e]: counts int32 [experts] are the entries of
+ * expert [n][choices] that name each expert, M their number (entries outside 0..experts-1 are none), R the rows with an
+ * entry, p the softmax of their logits (0 where all are masked).  Other rows' logits are not used; without entries the
+ * loss is 0.  stats fp32 [n][3] or null: for the backward.  norm: one value, experts / (M R).
+ * At most 32768 experts, n * choices < 2^31.  workspace: odie_balance_workspace bytes, 8-byte aligned. */
+int64_t odie_balance_workspace(int64_t n, int choices, int experts);
+int odie_balance_forward(const void* logits, int64_t stride, const int32_t* expert, int64_t n, int choices, int experts,
+                         int dtype, float* loss, int32_t* counts, float* stats, float* norm, void* workspace,
+                         int64_t workspace_bytes, uint64_t stream);
+
+/* Gradient of the loss: dlogits [n][experts] from upstream (one value on the device) and what the forward wrote. */
+int odie_balance_backward(const float* upstream, const void* logits, int64_t stride, const int32_t* counts,
+                          const float* stats, const float* norm, int64_t n, int experts, int dtype, void* dlogits,
+                          uint64_t stream);
+
+/* loss [n] = sum over j of q_j (log q_j - log p[ids_j]): p = softmax(logits / temperature), ids [n][top] (int32 or int64:
+ * id_bytes 4 or 8), q = softmax over the row's valid entries of teacher / temperature (teacher [n][top], of
+ * teacher_dtype).  An id outside 0..classes-1 or a teacher's -inf is no entry; without any the loss is 0.  A
+ * row whose logits are all masked has p = 0.  stats fp32 [n][4] or null: for the backward.  At most 2^24 classes and 1024
+ * entries a row.  workspace: odie_distill_workspace bytes (0 for many rows), 8-byte aligned. */
+int64_t odie_distill_workspace(int64_t n, int classes, int dtype);
+int odie_distill_forward(const void* logits, int64_t stride, const void* ids, int id_bytes, const void* teacher,
+                         int teacher_dtype, int64_t n, int classes, int top, float temperature, int dtype, float* loss,
+                         float* stats, void* workspace, int64_t workspace_bytes, uint64_t stream);
+
+/* Gradient of the losses: dlogits [n][classes] = upstream[i] / temperature (p - Q), Q[e] the sum of q_j over the entries
+ * of class e; 0 in rows without entries. */
+int odie_distill_backward(const float* upstream, const void* logits, int64_t stride, const void* ids, int id_bytes,
+                          const void* teacher, int teacher_dtype, const float* stats, int64_t n, int classes, int top,
+                          float temperature, int dtype, void* dlogits, uint64_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Microscaled 4-bit floating point: values +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} (sign, two bits of exponent, one of fraction)
+ * in blocks of 32 along a row that share a scale 2^(s - 127) (s = 255: the block is NaN).
+ *   codes   [rows][16 * blocks], blocks = ceil(width / 32): two values a byte, the first in the low half; 0 past the width
+ *   scales  [rows][blocks rounded up to a multiple of 4]; 0 past the last block
+ * codes are 16-byte and scales 4-byte aligned.  No counterpart in the reference.
+ * --------------------------------------------------------------------------------------- */
+
+/* Rows x of dtype to codes and scales: a block's scale is the power of two of its largest magnitude over 4 (within
+ * 2^-127..2^127), each value over it is rounded to the nearest, ties to the even code, and clamped at 6.  A block of
+ * zeros has s = 0; one that holds a NaN or an infinity becomes NaN. */
+int odie_mx_quantize(const void* x, int64_t x_stride, int64_t rows, int64_t width, int dtype, uint8_t* codes, uint8_t* scales,
+                     uint64_t stream);
+
+/* The values as dtype, rounded to nearest even where it does not hold them. */
+int odie_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t width, int dtype, void* out,
+                       int64_t out_stride, uint64_t stream);
+
+/* odie_linear_forward with a weight in codes and scales ([experts][outputs] rows of `inputs` values), whose values are
+ * taken in dtype (rounded where it does not hold them).  x_scales null: x [rows][inputs] of dtype, stride x_stride.  Else x
+ * is codes as well (x_stride unused), and products are exact.  bias, residual, out and pre are of dtype. */
+int odie_mx_linear_forward(const void* x, const uint8_t* x_scales, int64_t x_stride, int64_t rows, const uint8_t* codes,
+                           const uint8_t* scales, const void* bias, const void* residual, int64_t residual_stride,
+                           const int32_t* offsets, int experts, int inputs, int outputs, int dtype, int activation, void* out,
+                           int64_t out_stride, void* pre, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

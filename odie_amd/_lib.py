@@ -87,6 +87,18 @@ SIGNATURES = {
     'odie_embed_forward': ([_P, _I64, _I64, _P, _I, _I64, C.c_float, _I64, _I, _P, _U64], _I),
     'odie_embed_workspace': ([_I64, _I64, _I64, _I], _I64),
     'odie_embed_backward': ([_P, _I64, _P, _I, _I64, _I64, C.c_float, _I64, _I, _P, _P, _I64, _U64], _I),
+    'odie_choose_forward': ([_P, _I64, _I64, _I, _I, _I, _I, _P, _P, _P, _U64], _I),
+    'odie_choose_backward': ([_P, _P, _P, _P, _I64, _P, _I64, _I, _I, _I, _P, _U64], _I),
+    'odie_balance_workspace': ([_I64, _I, _I], _I64),
+    'odie_balance_forward': ([_P, _I64, _P, _I64, _I, _I, _I, _P, _P, _P, _P, _P, _I64, _U64], _I),
+    'odie_balance_backward': ([_P, _P, _I64, _P, _P, _P, _I64, _I, _I, _P, _U64], _I),
+    'odie_distill_workspace': ([_I64, _I, _I], _I64),
+    'odie_distill_forward': ([_P, _I64, _P, _I, _P, _I, _I64, _I, _I, C.c_float, _I, _P, _P, _P, _I64, _U64], _I),
+    'odie_distill_backward': ([_P, _P, _I64, _P, _I, _P, _I, _P, _I64, _I, _I, C.c_float, _I, _P, _U64], _I),
+    'odie_mx_quantize': ([_P, _I64, _I64, _I64, _I, _P, _P, _U64], _I),
+    'odie_mx_dequantize': ([_P, _P, _I64, _I64, _I, _P, _I64, _U64], _I),
+    'odie_mx_linear_forward': ([_P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _P, _I, _I, _I, _I, _I, _P, _I64, _P, _U64],
+                               _I),
     'odie_create': ([C.c_char_p], _P),
     'odie_step': ([_P, _U64, _I, _I], _I),
     'odie_configure': ([_P, C.c_char_p], _I),

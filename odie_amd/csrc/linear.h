@@ -184,8 +184,8 @@ template <class T, bool kByRow, int kRows, int kThreads> struct Direct : Image<T
                            static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32))),
                            kBufferLimit, kBufferWord3};
         asm volatile("s_nop 4" : "+s"(buffer));   // wait states between its writing and the loads
-        const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void)(lds))) +
-                            __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / 64) * 1024;
+        const uint32_t to = __builtin_amdgcn_readfirstlane(
+            static_cast<int>(reinterpret_cast<uintptr_t>((lds_void)(lds))) + static_cast<int>(threadIdx.x) / 64 * 1024);
         if (left >= kSlab<T>) {
 #pragma unroll
             for (int i = 0; i < I::kChunks; ++i) queue16(to + i * kThreads * 16, offset[i], buffer);

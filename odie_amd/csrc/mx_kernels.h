@@ -1,0 +1,469 @@
+// Products with a microscaled 4-bit weight, instantiated by mx_f16.hip, mx_bf16.hip and mx_f32.hip; the tiles' sums,
+// their epilogue and the way of rows to LDS are linear.h's.
+//
+//   y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n],  w[n][k] = code(n, k) 2^(s(n, k / 32) - 127)
+//
+// Rows of 4 bits too: v_mfma_scale_f32_32x32x64_f8f6f4 takes both operands' codes and their scales as they are stored;
+// products are exact.  Rows of T: the weight stays in 4 bits up to the registers, where it becomes T for
+// v_mfma_f32_32x32x16 (fp32: 32x32x2), each value once for all 32-row tiles of a wave.
+//
+// Which k a lane holds at a step is free as long as both operands agree.  Here a lane of half h = lane / 32 takes whole
+// blocks: its 16 bytes of codes belong to one scale, and the scales of its next four blocks are the bytes
+// of one word.
+#pragma once
+#include "linear_epilogue.h"
+#include "mx.h"
+
+namespace odie {
+
+struct MxRowsArgs {
+    RowsArgs rows;               // a: rows of T, or their codes; b: the weight's codes
+    const uint8_t* a_scales;     // null: rows of T
+    const uint8_t* b_scales;
+    int64_t code_pitch, scale_pitch;   // bytes a row of codes and of scales
+};
+
+template <class T> int launch_mx(const MxRowsArgs& a, hipStream_t stream);
+
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kMxSlab = 256;          // values of k in a 128-byte row of codes: 8 blocks
+constexpr int kMxSlabScales = 8;
+
+__device__ inline i32x8 mx_operand(const vec16& v) {
+    return i32x8{static_cast<int>(v[0]), static_cast<int>(v[1]), static_cast<int>(v[2]), static_cast<int>(v[3]), 0, 0, 0, 0};
+}
+
+// acc[n][m] += the 64 values of k of two blocks, one a lane half; kByte of the scale words is theirs.  4: 4-bit operands.
+template <int kByte> __device__ inline accum16 multiply_mx(const vec16& b, const vec16& a, uint32_t sb, uint32_t sa, accum16 c) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(b), mx_operand(a), c, 4, 4, kByte, static_cast<int>(sb), kByte, static_cast<int>(sa));
+}
+// The same for 16 x 16 tiles and 128 values, a block a lane quarter.
+__device__ inline accum4 multiply16_mx(const vec16& b, const vec16& a, uint32_t sb, uint32_t sa, accum4 c) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(b), mx_operand(a), c, 4, 4, 0, static_cast<int>(sb), 0, static_cast<int>(sa));
+}
+
+// Queues 4 bytes a lane from buffer + offset to LDS address `to` + 4 * lane, as queue16 does 16.
+__device__ inline void queue4(uint32_t to, uint32_t offset, const vec16& buffer) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer)
+                 : "memory", "m0");
+}
+
+// An operand's scales on their way to LDS, two words a row and slab: kRows rows of 8 bytes.
+template <int kRows, int kThreads> struct Scales {
+    static constexpr int kBytes = kRows * kMxSlabScales;
+    static constexpr int kLoads = kBytes / 256, kWaves = kThreads / 64;    // loads of 64 words, over the waves
+    static constexpr int kOwn = (kLoads + kWaves - 1) / kWaves;
+    uint32_t offset[kOwn];
+    const uint8_t* base;     // uniform over the workgroup
+    int left;                // words from this lane's on to its row's end
+
+    static __device__ int wave() { return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64)); }
+
+    __device__ void begin(const uint8_t* data, int64_t pitch, int64_t first, int64_t limit) {
+        const int lane = static_cast<int>(threadIdx.x % 64), last = limit - first < kRows ? static_cast<int>(limit - first) - 1 : kRows - 1;
+        base = data + first * pitch;
+        left = static_cast<int>(pitch / 4) - lane % 2;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            const int r = ((wave() + i * kWaves) * 64 + lane) / 2;
+            offset[i] = static_cast<uint32_t>(r < last ? r : last) * static_cast<uint32_t>(pitch) + lane % 2 * 4;
+        }
+    }
+    __device__ void load(char* lds) {
+        const uint64_t address = reinterpret_cast<uint64_t>(base);
+        vec16 buffer{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address))),
+                     static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32))), kBufferLimit, kBufferWord3};
+        asm volatile("s_nop 4" : "+s"(buffer));   // wait states between its writing and the loads
+        const uint32_t to = __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>((lds_void)(lds))));
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            if (kLoads % kWaves == 0 || wave() + i * kWaves < kLoads)
+                queue4(to + (wave() + i * kWaves) * 256, left > 0 ? offset[i] : kNowhere, buffer);
+        base += kMxSlabScales;
+        left -= 2;
+    }
+    // The scales of blocks 4 (lane / 32) .. + 3 of row base + lane % 32, a byte each.
+    static __device__ uint32_t word(const char* lds, int base, int lane) {
+        return *reinterpret_cast<const uint32_t*>(lds + (base + lane % 32) * kMxSlabScales + lane / 32 * 4);
+    }
+    static __device__ uint32_t byte(const char* lds, int row, int block) {
+        return *reinterpret_cast<const uint8_t*>(lds + row * kMxSlabScales + block);
+    }
+};
+
+// Chunk c (16 bytes) of row r of an image of 128-byte rows.
+template <class I> __device__ inline vec16 chunk_at(const char* lds, int r, int c) {
+    return *reinterpret_cast<const vec16*>(lds + r * kSlabBytes + ((c ^ I::turn(r)) << 4));
+}
+
+// A tile of a product of codes with codes.
+template <int kBM, int kBN, int kWM, int kWN> struct MxTile : Sums<kBM, kBN, kWM, kWN> {
+    using Base = Sums<kBM, kBN, kWM, kWN>;
+    using Base::acc;
+    using Base::kMs;
+    using Base::kNs;
+    using Base::kThreads;
+    using A = Direct<uint8_t, true, kBM, kThreads>;
+    using B = Direct<uint8_t, true, kBN, kThreads>;
+    using SA = Scales<kBM, kThreads>;
+    using SB = Scales<kBN, kThreads>;
+    static constexpr int kCodes = A::kBytes + B::kBytes;
+    static constexpr int kBuffer = kCodes + SA::kBytes + SB::kBytes;
+    static constexpr int kLds = 2 * kBuffer > kThreads / 64 * Base::kRegion ? 2 * kBuffer : kThreads / 64 * Base::kRegion;
+
+    template <int kStep> __device__ void add_step(const char* here, const uint32_t (&sa)[kMs], const uint32_t (&sb)[kNs]) {
+        const int lane = static_cast<int>(threadIdx.x % 64), chunk = 4 * (lane / 32) + kStep;
+        vec16 fa[kMs], fb[kNs];
+#pragma unroll
+        for (int i = 0; i < kMs; ++i) fa[i] = chunk_at<A>(here, Base::wave_row() + 32 * i + lane % 32, chunk);
+#pragma unroll
+        for (int j = 0; j < kNs; ++j) fb[j] = chunk_at<B>(here + A::kBytes, Base::wave_column() + 32 * j + lane % 32, chunk);
+#pragma unroll
+        for (int i = 0; i < kMs; ++i)
+#pragma unroll
+            for (int j = 0; j < kNs; ++j) acc[i][j] = multiply_mx<kStep>(fb[j], fa[i], sb[j], sa[i], acc[i][j]);
+    }
+
+    __device__ void add_slab(const char* here) {
+        const int lane = static_cast<int>(threadIdx.x % 64);
+        uint32_t sa[kMs], sb[kNs];
+#pragma unroll
+        for (int i = 0; i < kMs; ++i) sa[i] = SA::word(here + kCodes, Base::wave_row() + 32 * i, lane);
+#pragma unroll
+        for (int j = 0; j < kNs; ++j) sb[j] = SB::word(here + kCodes + SA::kBytes, Base::wave_column() + 32 * j, lane);
+        add_step<0>(here, sa, sb);
+        add_step<1>(here, sa, sb);
+        add_step<2>(here, sa, sb);
+        add_step<3>(here, sa, sb);
+    }
+
+    // Sums `bytes` bytes of codes a row.  The operands have begun.
+    __device__ void sum(A& a, B& b, SA& sa, SB& sb, int64_t bytes, char* lds) {
+        Base::clear();
+        auto load = [&](int64_t left, char* to) {
+            a.load(left, to);
+            b.load(left, to + A::kBytes);
+            sa.load(to + kCodes);
+            sb.load(to + kCodes + SA::kBytes);
+        };
+        load(bytes, lds);
+        int now = 0;
+        for (int64_t left = bytes; left > 0; left -= kSlabBytes) {
+            arrived<0>();   // this slab; and no wave reads the other buffer any more
+            if (left > kSlabBytes) load(left - kSlabBytes, lds + (now ^ 1) * kBuffer);
+            add_slab(lds + now * kBuffer);
+            now ^= 1;
+        }
+        __syncthreads();
+    }
+};
+
+template <class T, int kBM, int kBN, int kWM, int kWN>
+__global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void mx_rows4_kernel(MxRowsArgs m, uint32_t first, uint32_t blocks) {
+    using Work = MxTile<kBM, kBN, kWM, kWN>;
+    __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
+    const RowsArgs& a = m.rows;
+    const uint32_t id = first + xcd_major(blockIdx.x, gridDim.x);
+    if (id >= blocks) return;
+    const TileAt t = tile_at(id, static_cast<uint32_t>(a.tiles), (a.columns + kBN - 1) / kBN);
+    const Piece p = find_piece(a.offsets, a.experts, a.experts + 1, a.rows, kBM, t.row);
+    if (p.begin >= p.end) return;
+    const int column0 = static_cast<int>(t.column) * kBN;
+    if (p.group >= a.experts) return rows_of_none<T, kBM, kBN, Work::kThreads>(a, p, column0);
+    const int64_t matrix = static_cast<int64_t>(p.group) * a.columns;
+    typename Work::A opa;
+    typename Work::B opb;
+    typename Work::SA sa;
+    typename Work::SB sb;
+    opa.begin(static_cast<const uint8_t*>(a.a), m.code_pitch, p.begin, p.end, m.code_pitch);
+    opb.begin(static_cast<const uint8_t*>(a.b) + matrix * m.code_pitch, m.code_pitch, column0, a.columns, m.code_pitch);
+    sa.begin(m.a_scales, m.scale_pitch, p.begin, p.end);
+    sb.begin(m.b_scales + matrix * m.scale_pitch, m.scale_pitch, column0, a.columns);
+    Work work;
+    work.sum(opa, opb, sa, sb, m.code_pitch, lds);
+    finish_tile<T, kBM == 256>(work, a, p, column0, lds);
+}
+
+// A tile of a product of rows of T with codes.  A slab of the weight's codes lasts for kRatio slabs of the rows.
+template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> struct MixedTile : Sums<kBM, kBN, kWM, kWN> {
+    using Base = Sums<kBM, kBN, kWM, kWN>;
+    using Base::acc;
+    using Base::kMs;
+    using Base::kNs;
+    using Base::kThreads;
+    using A = std::conditional_t<kWay == kDirect, Direct<T, true, kBM, kThreads>,
+                                 std::conditional_t<kWay == kStaged, Staged<T, true, kBM, kThreads>, Gathered<T, true, kBM, kThreads>>>;
+    using B = Direct<uint8_t, true, kBN, kThreads>;
+    using SB = Scales<kBN, kThreads>;
+    static constexpr int kRatio = kMxSlab / kSlab<T>;
+    static constexpr int kCodes = B::kBytes + SB::kBytes;
+    static constexpr int kBytes = 2 * (A::kBytes + kCodes);
+    static constexpr int kLds = kBytes > kThreads / 64 * Base::kRegion ? kBytes : kThreads / 64 * Base::kRegion;
+
+    // Slab `part` of the kRatio of these codes.  A lane of half h takes values 32 (2 part + h) .. + 31 of the codes' slab,
+    // a block (fp32: half a block, 32 part + 16 h .. + 15), eight (four) at a step.
+    __device__ void add_slab(const char* rows, const char* codes, int part) {
+        const int lane = static_cast<int>(threadIdx.x % 64), half = lane / 32;
+        constexpr bool kWide = sizeof(T) == 4;
+        vec16 held[kNs];
+        float scale[kNs];
+#pragma unroll
+        for (int j = 0; j < kNs; ++j) {
+            const int r = Base::wave_column() + 32 * j + lane % 32, block = kWide ? part : 2 * part + half;
+            held[j] = chunk_at<B>(codes, r, block);
+            scale[j] = mx_scale(SB::byte(codes + B::kBytes, r, block));
+        }
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+            vec16 fa[kMs], fb[kNs];
+#pragma unroll
+            for (int i = 0; i < kMs; ++i) fa[i] = chunk_at<A>(rows, Base::wave_row() + 32 * i + lane % 32, 4 * half + step);
+#pragma unroll
+            for (int j = 0; j < kNs; ++j) {
+                const uint32_t word = kWide ? (half ? held[j][2 + step / 2] : held[j][step / 2]) : held[j][step];
+                fb[j] = mx_values<T>(word, scale[j], step % 2 == 1);
+            }
+#pragma unroll
+            for (int i = 0; i < kMs; ++i)
+#pragma unroll
+                for (int j = 0; j < kNs; ++j) acc[i][j] = multiply(T{}, fb[j], fa[i], acc[i][j]);
+        }
+    }
+
+    // Sums `depth` values of k; `bytes` bytes of codes a row.  The operands have begun.
+    __device__ void sum(A& a, B& b, SB& sb, int64_t depth, int64_t bytes, char* lds) {
+        Base::clear();
+        char* const codes = lds + 2 * A::kBytes;
+        int64_t codes_left = bytes;
+        int next = 0;                // buffer of the codes' next slab
+        auto load_codes = [&] {
+            if (codes_left <= 0) return;
+            b.load(codes_left, codes + next * kCodes);
+            sb.load(codes + next * kCodes + B::kBytes);
+            codes_left -= kSlabBytes;
+            next ^= 1;
+        };
+        load_codes();
+        int now = 0, part = 0, at = 0;
+        if constexpr (kWay == kDirect) {
+            a.load(depth, lds);
+            for (int64_t left = depth; left > 0; left -= kSlab<T>) {
+                arrived<0>();   // this slab; and no wave reads the other buffers any more
+                if (left > kSlab<T>) a.load(left - kSlab<T>, lds + (now ^ 1) * A::kBytes);
+                if (part == 0) load_codes();
+                add_slab(lds + now * A::kBytes, codes + at * kCodes, part);
+                now ^= 1;
+                if (++part == kRatio) part = 0, at ^= 1;
+            }
+        } else {
+            typename A::Held held;
+            a.load(held);
+            for (int64_t left = depth; left > 0; left -= kSlab<T>) {
+                a.store(held, lds + now * A::kBytes, left);
+                arrived<0>();   // the slab is there; and no wave reads the buffer of the slab before
+                if (left > kSlab<T>) a.load(held);
+                if (part == 0) load_codes();
+                add_slab(lds + now * A::kBytes, codes + at * kCodes, part);
+                now ^= 1;
+                if (++part == kRatio) part = 0, at ^= 1;
+            }
+        }
+        __syncthreads();
+    }
+};
+
+template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN>
+__global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void mx_mixed_kernel(MxRowsArgs m, uint32_t first, uint32_t blocks) {
+    using Work = MixedTile<T, kWay, kBM, kBN, kWM, kWN>;
+    __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
+    const RowsArgs& a = m.rows;
+    const uint32_t id = first + xcd_major(blockIdx.x, gridDim.x);
+    if (id >= blocks) return;
+    const TileAt t = tile_at(id, static_cast<uint32_t>(a.tiles), (a.columns + kBN - 1) / kBN);
+    const Piece p = find_piece(a.offsets, a.experts, a.experts + 1, a.rows, kBM, t.row);
+    if (p.begin >= p.end) return;
+    const int column0 = static_cast<int>(t.column) * kBN;
+    if (p.group >= a.experts) return rows_of_none<T, kBM, kBN, Work::kThreads>(a, p, column0);
+    const int64_t matrix = static_cast<int64_t>(p.group) * a.columns;
+    typename Work::A opa;
+    typename Work::B opb;
+    typename Work::SB sb;
+    opa.begin(static_cast<const T*>(a.a), a.lda, p.begin, p.end, a.depth);
+    opb.begin(static_cast<const uint8_t*>(a.b) + matrix * m.code_pitch, m.code_pitch, column0, a.columns, m.code_pitch);
+    sb.begin(m.b_scales + matrix * m.scale_pitch, m.scale_pitch, column0, a.columns);
+    Work work;
+    work.sum(opa, opb, sb, a.depth, m.code_pitch, lds);
+    finish_tile<T, kBM == 256>(work, a, p, column0, lds);
+}
+
+// Few rows a group, as few_rows_kernel: the weight's codes go straight into registers, once for every 16 kRowTiles rows.
+// A step takes four blocks of k, one a lane quarter, and a wave one of kSplit shares of the blocks.
+template <class T, bool kRows4, int kRowTiles, int kSplit>
+__global__ __launch_bounds__(64 * kFewWaves) void mx_few_rows_kernel(MxRowsArgs m) {
+    constexpr int kColumns = 16 * kFewWaves / kSplit;   // of a workgroup
+    constexpr int kAhead = kRows4 ? 4 : 2;              // steps in flight
+    constexpr int kParts = kRows4 ? 1 : kMxBlock / kPerVec<T>;   // 16-byte parts of a block of a row
+    __shared__ accum4 part[kFewWaves][kRowTiles][64];
+    const RowsArgs& a = m.rows;
+    const uint32_t across = (a.columns + kColumns - 1) / kColumns;
+    const Piece p = find_piece(a.offsets, a.experts, a.experts + 1, a.rows, 16 * kRowTiles, blockIdx.x / across);
+    if (p.begin >= p.end) return;
+    const int column0 = static_cast<int>(blockIdx.x % across) * kColumns;
+    const int lane = static_cast<int>(threadIdx.x % 64);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64));
+    const bool owned = p.group < a.experts;        // else rows of no expert
+    if (owned && column0 + wave / kSplit * 16 < a.columns) {
+        const int own = lane % 16, quarter = lane / 16;
+        int column = column0 + wave / kSplit * 16 + own;
+        column = column < a.columns ? column : a.columns - 1;   // those past the last are not stored
+        const int64_t at = static_cast<int64_t>(p.group) * a.columns + column;
+        const uint8_t* w = static_cast<const uint8_t*>(a.b) + at * m.code_pitch;
+        const uint8_t* ws = m.b_scales + at * m.scale_pitch;
+        const T* x[kRowTiles];
+        const uint8_t* xc[kRowTiles];
+        const uint8_t* xs[kRowTiles];
+#pragma unroll
+        for (int t = 0; t < kRowTiles; ++t) {
+            int64_t row = p.begin + 16 * t + own;
+            row = row < p.end ? row : p.end - 1;
+            x[t] = static_cast<const T*>(a.a) + row * a.lda;
+            xc[t] = static_cast<const uint8_t*>(a.a) + row * m.code_pitch;
+            xs[t] = m.a_scales + row * m.scale_pitch;
+        }
+        accum4 acc[kRowTiles] = {};
+        const int total = static_cast<int>(m.code_pitch / kMxBytes), steps = (total + 3) / 4;
+        const int share = (steps + kSplit - 1) / kSplit * 4;
+        const int first = wave % kSplit * share, last = first + share < total ? first + share : total;
+        for (int b0 = first; b0 < last; b0 += 4 * kAhead) {
+            vec16 fw[kAhead], fx[kAhead][kRowTiles][kParts];
+            uint32_t sw[kAhead], sx[kAhead][kRowTiles];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int block = b0 + 4 * u + quarter;
+                const bool inside = block < last;
+                fw[u] = inside ? *reinterpret_cast<const vec16*>(w + block * kMxBytes) : vec16{};
+                sw[u] = inside ? ws[block] : 0u;
+#pragma unroll
+                for (int t = 0; t < kRowTiles; ++t) {
+                    if constexpr (kRows4) {
+                        fx[u][t][0] = inside ? *reinterpret_cast<const vec16*>(xc[t] + block * kMxBytes) : vec16{};
+                        sx[u][t] = inside ? xs[t][block] : 0u;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kParts; ++i) {
+                            const int k = block * kMxBlock + i * kPerVec<T>, count = inside ? a.depth - k : 0;
+                            fx[u][t][i] = count > 0 ? load_end(x[t] + k, count, k) : vec16{};
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if constexpr (kRows4) {
+#pragma unroll
+                    for (int t = 0; t < kRowTiles; ++t) acc[t] = multiply16_mx(fw[u], fx[u][t][0], sw[u], sx[u][t], acc[t]);
+                } else {
+                    const float scale = mx_scale(sw[u]);
+#pragma unroll
+                    for (int i = 0; i < kParts; ++i) {
+                        const vec16 values = mx_values<T>(fw[u][i * kPerVec<T> / 8], scale, sizeof(T) == 4 && i % 2 == 1);
+#pragma unroll
+                        for (int t = 0; t < kRowTiles; ++t) acc[t] = multiply16(T{}, values, fx[u][t][i], acc[t]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kRowTiles; ++t) part[wave][t][lane] = acc[t];
+    }
+    __syncthreads();
+    finish_few<T, kRowTiles, kSplit>(part, a, p, column0, owned);
+}
+
+template <int kBM, int kBN, int kWM, int kWN, class Launch> int in_tiles(MxRowsArgs m, Launch&& launch) {
+    const int64_t across = (m.rows.columns + kBN - 1) / kBN;
+    m.rows.tiles = piece_ids(m.rows.rows, kBM, m.rows.offsets != nullptr, m.rows.experts, true);
+    const int64_t blocks = m.rows.tiles * across;
+    if (blocks >= int64_t{1} << 31) return fail("linear: too many tiles for one launch");
+    constexpr int kThreads = 64 * (kBM / kWM) * (kBN / kWN);
+    in_launches(blocks, kThreads, [&](uint32_t first, uint32_t count) {
+        launch(m, whole_xcds(count), kThreads, first, static_cast<uint32_t>(blocks));
+    });
+    return check_launch("linear of 4-bit weights");
+}
+
+template <class T, int kBM, int kBN, int kWM, int kWN> int launch_rows4(const MxRowsArgs& m, hipStream_t stream) {
+    return in_tiles<kBM, kBN, kWM, kWN>(m, [&](const MxRowsArgs& a, uint32_t grid, int threads, uint32_t first, uint32_t blocks) {
+        mx_rows4_kernel<T, kBM, kBN, kWM, kWN><<<grid, threads, 0, stream>>>(a, first, blocks);
+    });
+}
+
+template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> int launch_mixed(const MxRowsArgs& m, hipStream_t stream) {
+    return in_tiles<kBM, kBN, kWM, kWN>(m, [&](const MxRowsArgs& a, uint32_t grid, int threads, uint32_t first, uint32_t blocks) {
+        mx_mixed_kernel<T, kWay, kBM, kBN, kWM, kWN><<<grid, threads, 0, stream>>>(a, first, blocks);
+    });
+}
+
+template <class T, bool kRows4, int kRowTiles, int kSplit> int launch_mx_few_as(const MxRowsArgs& m, hipStream_t stream) {
+    const RowsArgs& a = m.rows;
+    const int64_t across = (a.columns + 16 * kFewWaves / kSplit - 1) / (16 * kFewWaves / kSplit);
+    const int64_t blocks = piece_ids(a.rows, 16 * kRowTiles, a.offsets != nullptr, a.experts, true) * across;
+    if (blocks > most_blocks(64 * kFewWaves)) return fail("linear: too many tiles for one launch");
+    mx_few_rows_kernel<T, kRows4, kRowTiles, kSplit><<<static_cast<uint32_t>(blocks), 64 * kFewWaves, 0, stream>>>(m);
+    return check_launch("linear of 4-bit weights");
+}
+
+template <class T, bool kRows4, int kRowTiles> int launch_mx_few(const MxRowsArgs& m, hipStream_t stream) {
+    const int64_t steps = m.code_pitch / (4 * kMxBytes);
+    const int64_t busy = m.rows.rows < m.rows.experts ? m.rows.rows : m.rows.experts;
+    if (steps >= 16 || busy * m.rows.columns < 64 * kCus) return launch_mx_few_as<T, kRows4, kRowTiles, 8>(m, stream);
+    return launch_mx_few_as<T, kRows4, kRowTiles, 2>(m, stream);
+}
+
+template <class T, Way kWay> int launch_mixed_of(const MxRowsArgs& m, hipStream_t stream) {
+    const RowsArgs& a = m.rows;
+    const int64_t each = a.rows / a.experts;
+    const int64_t large = (a.rows + 255) / 256 * ((a.columns + 255) / 256);
+    const int64_t wide = (a.rows + 127) / 128 * ((a.columns + 127) / 128);
+    if constexpr (kWay == kDirect)
+        if (a.columns > 128 && even(large) && each >= 1024) return launch_mixed<T, kWay, 256, 256, 64, 128>(m, stream);
+    if constexpr (kWay != kGathered)
+        if (a.columns > 64 && wide >= kCus && each >= 128) return launch_mixed<T, kWay, 128, 128, 64, 64>(m, stream);
+    return launch_mixed<T, kWay, 64, 64, 32, 32>(m, stream);
+}
+
+template <class T, bool kRows4> int launch_mx_by_rows(const MxRowsArgs& m, hipStream_t stream) {
+    const RowsArgs& a = m.rows;
+    const int64_t each = (a.rows + a.experts - 1) / a.experts * (a.experts > 1 ? 2 : 1);   // room for twice the average
+    if (each <= 16) return launch_mx_few<T, kRows4, 1>(m, stream);
+    if (each <= 32) return launch_mx_few<T, kRows4, 2>(m, stream);
+    if constexpr (kRows4) {
+        const int64_t large = (a.rows + 255) / 256 * ((a.columns + 255) / 256);
+        const int64_t wide = (a.rows + 127) / 128 * ((a.columns + 127) / 128);
+        if (a.columns > 128 && even(large) && a.rows / a.experts >= 1024) return launch_rows4<T, 256, 256, 64, 128>(m, stream);
+        if (a.columns > 64 && wide >= kCus && a.rows / a.experts >= 128) return launch_rows4<T, 128, 128, 64, 64>(m, stream);
+        return launch_rows4<T, 64, 64, 32, 32>(m, stream);
+    } else {
+        switch (way_of<T>(a.a, a.lda, a.depth)) {
+            case kDirect: return launch_mixed_of<T, kDirect>(m, stream);
+            case kStaged: return launch_mixed_of<T, kStaged>(m, stream);
+            default: return launch_mixed_of<T, kGathered>(m, stream);
+        }
+    }
+}
+
+}  // namespace
+
+template <class T> int launch_mx(const MxRowsArgs& m, hipStream_t stream) {
+    return m.a_scales ? launch_mx_by_rows<T, true>(m, stream) : launch_mx_by_rows<T, false>(m, stream);
+}
+
+}  // namespace odie
+
+#define ODIE_MX_FOR(T)                                                        \
+    namespace odie {                                                          \
+    template int launch_mx<T>(const MxRowsArgs&, hipStream_t);                \
+    }
