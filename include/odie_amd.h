@@ -667,7 +667,7 @@ int odie_choose_backward(const float* upstream, const int32_t* expert, const flo
 /* loss = experts / (M R) * sum over rows and experts of counts[e] p[i][e]: counts int32 [experts] are the entries of
  * expert [n][choices] that name each expert, M their number (entries outside 0..experts-1 are none), R the rows with an
  * entry, p the softmax of their logits (0 where all are masked).  Other rows' logits are not used; without entries the
- * loss is 0.  stats fp32 [n][3] or null: for the backward.  norm: one value, experts / (M R).
+ * loss is 0.  stats fp32 [n][4] or null: for the backward (16-byte aligned).  norm: one value, experts / (M R).
  * At most 32768 experts, n * choices < 2^31.  workspace: odie_balance_workspace bytes, 8-byte aligned. */
 int64_t odie_balance_workspace(int64_t n, int choices, int experts);
 int odie_balance_forward(const void* logits, int64_t stride, const int32_t* expert, int64_t n, int choices, int experts,

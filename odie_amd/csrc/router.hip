@@ -260,140 +260,261 @@ __global__ __launch_bounds__(kBlock) void choose_backward_kernel(ChooseBackwardA
 
 // --- balance -------------------------------------------------------------------------------------------
 
-constexpr int kCountBlocks = 2 * kCus;
+constexpr int kCountBlock = 1024;
 constexpr int kSharedCounts = 8192;      // experts whose counts a workgroup keeps in LDS
+constexpr int64_t kFewEntries = 1 << 15; // counted by one workgroup, which needs nothing cleared before
 
 struct BalanceArgs {
     const void* logits;
     const int32_t* expert;    // [n][choices]
     int32_t* counts;          // [experts]
-    int32_t* rows;            // R
-    float* stats;             // [n][3]: m, 1 / s (0: the row takes no part), t
-    double* partial;          // [blocks]
+    uint32_t* done;           // workgroups that have left their sums
+    float* stats;             // [n][4]: m, 1 / s (0: the row takes no part), t, 0
+    double* partial;          // [blocks]: sum of t
+    uint32_t* parts;          // [blocks]: rows that take part
     float* norm;              // E / (M R)
     float* loss;
-    int64_t stride, n, blocks;
+    int64_t stride, n;
     int choices, experts;
 };
 
 __global__ __launch_bounds__(kBlock) void balance_clear_kernel(BalanceArgs a) {
     for (int e = blockIdx.x * kBlock + threadIdx.x; e < a.experts; e += gridDim.x * kBlock) a.counts[e] = 0;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.rows = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;
 }
 
-__global__ __launch_bounds__(kBlock) void balance_count_kernel(BalanceArgs a) {
+// Each workgroup counts its entries in LDS and adds what it found (whole numbers, in any order).  kAlone: one workgroup
+// of all entries.  Entries that lie 16-byte aligned are read four at a time.
+template <bool kAlone> __global__ __launch_bounds__(kCountBlock) void balance_count_kernel(BalanceArgs a) {
     extern __shared__ int32_t held[];
     const bool shared = a.experts <= kSharedCounts;
+    const int64_t entries = a.n * a.choices, step = static_cast<int64_t>(gridDim.x) * kCountBlock;
+    const int64_t self = static_cast<int64_t>(blockIdx.x) * kCountBlock + threadIdx.x;
     int32_t* to = shared ? held : a.counts;
-    if (shared) {
-        for (int e = threadIdx.x; e < a.experts; e += kBlock) held[e] = 0;
+    if (shared || kAlone) {
+        for (int e = threadIdx.x; e < a.experts; e += kCountBlock) to[e] = 0;
+        if (kAlone && threadIdx.x == 0) *a.done = 0;
         __syncthreads();
     }
-    int32_t rows = 0;
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; row < a.n; row += static_cast<int64_t>(gridDim.x) * kBlock) {
-        bool any = false;
-        for (int j = 0; j < a.choices; ++j) {
-            const int e = a.expert[row * a.choices + j];
-            if (e < 0 || e >= a.experts) continue;
-            any = true;
-            atomicAdd(to + e, 1);
-        }
-        rows += any;
+    auto add = [&](int e) {
+        if (e >= 0 && e < a.experts) atomicAdd(to + e, 1);
+    };
+    const int64_t fours = reinterpret_cast<uintptr_t>(a.expert) % 16 == 0 ? entries / 4 : 0;
+    const int4* four = reinterpret_cast<const int4*>(a.expert);
+#pragma unroll 2
+    for (int64_t i = self; i < fours; i += step) {
+        const int4 e = four[i];
+        add(e.x), add(e.y), add(e.z), add(e.w);
     }
-    for (int step = 32; step > 0; step /= 2) rows += __shfl_down(rows, step);
-    if (threadIdx.x % 64 == 0 && rows) atomicAdd(a.rows, rows);
+    for (int64_t i = 4 * fours + self; i < entries; i += step) add(a.expert[i]);
     if (!shared) return;
     __syncthreads();
-    for (int e = threadIdx.x; e < a.experts; e += kBlock)
-        if (held[e]) atomicAdd(a.counts + e, held[e]);
+    for (int e = threadIdx.x; e < a.experts; e += kCountBlock) {
+        if (kAlone) a.counts[e] = held[e];
+        else if (held[e]) atomicAdd(a.counts + e, held[e]);
+    }
 }
 
-template <class T, int kLanes> __global__ __launch_bounds__(kBlock) void balance_rows_kernel(BalanceArgs a) {
+// A row's 16-byte chunks, kVecs a lane, loaded ahead of their use: without conditions, which would make the compiler wait
+// for loads in flight, from addresses moved back into the row where they would leave it; get() puts that right.  The first half of
+// several chunks is always whole (with_row).  Rows shorter than a chunk are gathered.
+template <class T, int kLanes, int kVecs> struct RowHold {
+    static constexpr int kV = kPerVec<T>;
+    vec16 chunk[kVecs];
+
+    __device__ void load(const T* row, int lane, int width) {
+        if (width < kV) {
+            chunk[0] = gather16(row, lane == 0 ? width : 0);
+            return;
+        }
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+            const int column = (v * kLanes + lane) * kV;
+            chunk[v] = load16(row + (v < kVecs / 2 || column < width - kV ? column : width - kV));
+        }
+    }
+    __device__ void get(int v, int lane, int width, float value[kV]) const {
+        const int count = width - (v * kLanes + lane) * kV;
+        if (v < kVecs / 2 || count >= kV) {
+            widen<T>(chunk[v], value);
+            return;
+        }
+        widen<T>(count > 0 && width >= kV ? shift_down(chunk[v], (kV - count) * static_cast<int>(sizeof(T))) : chunk[v], value);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) value[i] = i < count ? value[i] : kNegInfinity;
+    }
+};
+
+// The counts of a lane's columns as fp32, 0 past the last.
+template <class T, int kLanes, int kVecs> __device__ inline void hold_counts(const int32_t* counts, int lane, int experts, float (&to)[kVecs][kPerVec<T>]) {
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v)
+#pragma unroll
+        for (int i = 0; i < kPerVec<T>; ++i) {
+            const int e = (v * kLanes + lane) * kPerVec<T> + i;
+            const int32_t count = counts[e < experts ? e : experts - 1];
+            to[v][i] = e < experts ? static_cast<float>(count) : 0.0f;
+        }
+}
+
+// Whether a row has an entry, for all of its lanes: asked for ahead (one entry a lane) and told later.
+template <int kLanes> struct Part {
+    int32_t id;
+
+    __device__ void load(const BalanceArgs& a, int64_t row, int lane) { id = a.expert[row * a.choices + (lane < a.choices ? lane : a.choices - 1)]; }
+    __device__ bool get(const BalanceArgs& a, int64_t row, int lane) const {
+        uint32_t any = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.experts);
+        for (int j = lane + kLanes; j < a.choices; j += kLanes) any |= static_cast<uint32_t>(a.expert[row * a.choices + j]) < static_cast<uint32_t>(a.experts);
+        return across<kLanes>(any, [](uint32_t x, uint32_t y) { return x | y; }) != 0;
+    }
+};
+
+__device__ inline void keep_row(const BalanceArgs& a, int64_t row, float m, float inverse, float t) {
+    if (a.stats) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(m, inverse, t, 0.0f);
+}
+
+// Adds the workgroups' sums; the last one to come makes the loss of them, in the order of the workgroups.
+__device__ inline void finish_balance(const BalanceArgs& a, double total, uint32_t rows) {
+    __shared__ double sums[kBlock / 64];
+    __shared__ uint32_t counts[2][kBlock / 64];
+    __shared__ bool last;
+    const int wave = static_cast<int>(threadIdx.x) / 64;
+    total = sum_across<64>(total);
+    rows = sum_across<64>(rows);
+    if (threadIdx.x % 64 == 0) sums[wave] = total, counts[0][wave] = rows;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kBlock / 64; ++w) total += sums[w], rows += counts[0][w];
+        __hip_atomic_store(a.partial + blockIdx.x, total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(a.parts + blockIdx.x, rows, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // Stores and loads of agent scope go past the XCD's own L2, so that their order is all it takes: a release would
+        // write that L2 back, in every workgroup.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        last = __hip_atomic_fetch_add(a.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    total = 0.0, rows = 0;
+    uint32_t entries = 0;
+    for (uint32_t b = threadIdx.x; b < gridDim.x; b += kBlock) {
+        total += __hip_atomic_load(a.partial + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        rows += __hip_atomic_load(a.parts + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    for (int e = threadIdx.x; e < a.experts; e += kBlock) entries += static_cast<uint32_t>(a.counts[e]);
+    total = sum_across<64>(total);
+    rows = sum_across<64>(rows);
+    entries = sum_across<64>(entries);
+    if (threadIdx.x % 64 == 0) sums[wave] = total, counts[0][wave] = rows, counts[1][wave] = entries;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < kBlock / 64; ++w) total += sums[w], rows += counts[0][w], entries += counts[1][w];
+    const double norm = entries > 0 ? a.experts / (static_cast<double>(entries) * static_cast<double>(rows)) : 0.0;
+    *a.norm = static_cast<float>(norm);
+    *a.loss = static_cast<float>(entries > 0 ? total * norm : 0.0);
+}
+
+// Rows of up to 64 kVecs chunks: kLanes lanes a row, a row in registers and the next one under way, the counts of the
+// lane's columns in registers for all of its rows.
+template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) void balance_rows_kernel(BalanceArgs a) {
+    constexpr bool kExact = sizeof(T) == 4;
+    constexpr int kV = kPerVec<T>, kRows = kBlock / kLanes;
+    const int lane = static_cast<int>(threadIdx.x) % kLanes;
+    float counts[kVecs][kV];
+    hold_counts<T, kLanes, kVecs>(a.counts, lane, a.experts, counts);
+    const T* logits = static_cast<const T*>(a.logits);
+    double total = 0.0;
+    uint32_t rows = 0;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    int64_t at = static_cast<int64_t>(blockIdx.x) * kRows + static_cast<int>(threadIdx.x) / kLanes;
+    RowHold<T, kLanes, kVecs> next;
+    Part<kLanes> part_next;
+    if (a.n > 0) {      // without rows there is none to load ahead
+        next.load(logits + (at < a.n ? at : a.n - 1) * a.stride, lane, a.experts);
+        part_next.load(a, at < a.n ? at : a.n - 1, lane);
+    }
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.n; base += step, at += step) {
+        const RowHold<T, kLanes, kVecs> row = next;
+        const Part<kLanes> part = part_next;
+        const int64_t now = at < a.n ? at : a.n - 1, then = at + step < a.n ? at + step : a.n - 1;
+        next.load(logits + then * a.stride, lane, a.experts);
+        part_next.load(a, then, lane);
+        const bool any = part.get(a, now, lane);
+        float value[kVecs][kV], top = kNegInfinity;
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+            row.get(v, lane, a.experts, value[v]);
+#pragma unroll
+            for (int i = 0; i < kV; ++i) top = larger(top, value[v][i]);
+        }
+        top = max_across<kLanes>(top);
+        const float from = base_of(top);
+        float s = 0.0f, t = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v)
+#pragma unroll
+            for (int i = 0; i < kV; ++i) {
+                const float e = exponential<kExact>(value[v][i] - from);
+                s += e;
+                t = fmaf(e, counts[v][i], t);
+            }
+        s = sum_across<kLanes>(s);
+        t = sum_across<kLanes>(t);
+        const float inverse = any && !(top == kNegInfinity) ? 1.0f / s : 0.0f;
+        t = inverse == 0.0f ? 0.0f : t * inverse;
+        if (at < a.n && lane == 0) {
+            total += static_cast<double>(t);
+            rows += any;
+            keep_row(a, at, top, inverse, t);
+        }
+    }
+    finish_balance(a, total, rows);
+}
+
+// Longer rows: a wave a row, with a running maximum.
+template <class T> __global__ __launch_bounds__(kBlock) void balance_long_kernel(BalanceArgs a) {
     constexpr bool kExact = sizeof(T) == 4;
     constexpr int kV = kPerVec<T>;
-    __shared__ double sums[kBlock / 64];
-    const int lane = static_cast<int>(threadIdx.x) % kLanes;
+    const int lane = static_cast<int>(threadIdx.x) % 64;
     double total = 0.0;
-    for (int64_t base_row = static_cast<int64_t>(blockIdx.x) * (kBlock / kLanes); base_row < a.n;
-         base_row += static_cast<int64_t>(gridDim.x) * (kBlock / kLanes)) {
-        const int64_t at = base_row + static_cast<int>(threadIdx.x) / kLanes, row = at < a.n ? at : a.n - 1;
-        uint32_t any = 0;
-        for (int j = lane; j < a.choices; j += kLanes) {
-            const int e = a.expert[row * a.choices + j];
-            any |= e >= 0 && e < a.experts;
-        }
-        any = across<kLanes>(any, [](uint32_t x, uint32_t y) { return x | y; });
+    uint32_t rows = 0;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * (kBlock / 64) + static_cast<int>(threadIdx.x) / 64; row < a.n;
+         row += static_cast<int64_t>(gridDim.x) * (kBlock / 64)) {
+        Part<64> part;
+        part.load(a, row, lane);
+        const bool any = part.get(a, row, lane);
         const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
-        Running<kExact> run;
-        float t = 0.0f;
-        for (int column = lane * kV; column < a.experts; column += kLanes * kV) {
-            float value[kV];
+        float m = kNegInfinity, s = 0.0f, t = 0.0f;
+        for (int column = lane * kV; column < a.experts; column += 64 * kV) {
+            float value[kV], counts[kV];
             load_logits(logits, column, a.experts, value);
-            float top = value[0];
 #pragma unroll
-            for (int i = 1; i < kV; ++i) top = larger(top, value[i]);
-            top = larger(run.m, top);
-            const float base = base_of(top);
-            float s = 0.0f, more = 0.0f;
+            for (int i = 0; i < kV; ++i) counts[i] = column + i < a.experts ? static_cast<float>(a.counts[column + i]) : 0.0f;
+            float top = m;
+#pragma unroll
+            for (int i = 0; i < kV; ++i) top = larger(top, value[i]);
+            const float base = base_of(top), old = exponential<kExact>(m - base);
+            s *= old;
+            t *= old;
 #pragma unroll
             for (int i = 0; i < kV; ++i) {
                 const float e = exponential<kExact>(value[i] - base);
                 s += e;
-                if (column + i < a.experts) more = fmaf(e, static_cast<float>(a.counts[column + i]), more);
+                t = fmaf(e, counts[i], t);
             }
-            const float old = exponential<kExact>(run.m - base);
-            run.s = fmaf(run.s, old, s);
-            t = fmaf(t, old, more);
-            run.m = top;
+            m = top;
         }
-        const float top = max_across<kLanes>(run.m), old = exponential<kExact>(run.m - base_of(top));
-        const float s = sum_across<kLanes>(run.s * old);
-        t = sum_across<kLanes>(t * old);
-        const bool part = any && !(top == kNegInfinity);
-        const float inverse = part ? 1.0f / s : 0.0f;
-        t = part ? t * inverse : 0.0f;
-        if (at < a.n && lane == 0) {
+        const float top = max_across<64>(m), old = exponential<kExact>(m - base_of(top));
+        s = sum_across<64>(s * old);
+        t = sum_across<64>(t * old);
+        const float inverse = any && !(top == kNegInfinity) ? 1.0f / s : 0.0f;
+        t = inverse == 0.0f ? 0.0f : t * inverse;
+        if (lane == 0) {
             total += static_cast<double>(t);
-            if (a.stats) {
-                a.stats[row * 3] = top;
-                a.stats[row * 3 + 1] = inverse;
-                a.stats[row * 3 + 2] = t;
-            }
+            rows += any;
+            keep_row(a, row, top, inverse, t);
         }
     }
-    for (int step = 32; step > 0; step /= 2) total += __shfl_down(total, step);
-    if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = total;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kBlock / 64; ++w) total += sums[w];
-        a.partial[blockIdx.x] = total;
-    }
-}
-
-__global__ __launch_bounds__(kBlock) void balance_finish_kernel(BalanceArgs a) {
-    __shared__ double sums[kBlock / 64];
-    __shared__ int64_t entries[kBlock / 64];
-    double total = 0.0;
-    int64_t count = 0;
-    for (int64_t b = threadIdx.x; b < a.blocks; b += kBlock) total += a.partial[b];
-    for (int e = threadIdx.x; e < a.experts; e += kBlock) count += a.counts[e];
-    for (int step = 32; step > 0; step /= 2) {
-        total += __shfl_down(total, step);
-        count += __shfl_down(count, step);
-    }
-    if (threadIdx.x % 64 == 0) {
-        sums[threadIdx.x / 64] = total;
-        entries[threadIdx.x / 64] = count;
-    }
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    for (int w = 1; w < kBlock / 64; ++w) {
-        total += sums[w];
-        count += entries[w];
-    }
-    const double norm = count > 0 ? a.experts / (static_cast<double>(count) * *a.rows) : 0.0;
-    *a.norm = static_cast<float>(norm);
-    *a.loss = static_cast<float>(count > 0 ? total * norm : 0.0);
+    finish_balance(a, total, rows);
 }
 
 struct BalanceBackwardArgs {
@@ -407,27 +528,64 @@ struct BalanceBackwardArgs {
     int experts;
 };
 
-template <class T, int kLanes, bool kStream>
-__global__ __launch_bounds__(kBlock) void balance_backward_kernel(BalanceBackwardArgs a, uint32_t first) {
-    constexpr int kV = kPerVec<T>;
+template <class T, int kLanes, int kVecs, bool kStream>
+__global__ __launch_bounds__(kBlock) void balance_backward_kernel(BalanceBackwardArgs a) {
+    constexpr int kV = kPerVec<T>, kRows = kBlock / kLanes;
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
-    const int64_t row = (static_cast<int64_t>(first) + blockIdx.x) * (kBlock / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
-    if (row >= a.n) return;
-    const float m = a.stats[row * 3], inverse = a.stats[row * 3 + 1], t = a.stats[row * 3 + 2];
-    const float scale = *a.upstream * *a.norm * inverse;
-    const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
-    T* out = static_cast<T*>(a.dlogits) + row * a.experts;
-    for (int column = lane * kV; column < a.experts; column += kLanes * kV) {
-        float value[kV] = {};
-        if (inverse != 0.0f) {
+    float counts[kVecs][kV];
+    hold_counts<T, kLanes, kVecs>(a.counts, lane, a.experts, counts);
+    const float scale = *a.upstream * *a.norm;
+    const T* logits = static_cast<const T*>(a.logits);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    int64_t at = static_cast<int64_t>(blockIdx.x) * kRows + static_cast<int>(threadIdx.x) / kLanes;
+    if (at >= a.n) return;
+    RowHold<T, kLanes, kVecs> next;
+    next.load(logits + at * a.stride, lane, a.experts);
+    float4 stats_next = *reinterpret_cast<const float4*>(a.stats + at * 4);
+    for (; at < a.n; at += step) {
+        const RowHold<T, kLanes, kVecs> row = next;
+        const float4 stats = stats_next;
+        const int64_t then = at + step < a.n ? at + step : a.n - 1;
+        next.load(logits + then * a.stride, lane, a.experts);
+        stats_next = *reinterpret_cast<const float4*>(a.stats + then * 4);
+        const float each = scale * stats.y;
+        T* out = static_cast<T*>(a.dlogits) + at * a.experts;
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+            const int column = (v * kLanes + lane) * kV;
+            float value[kV];
+            row.get(v, lane, a.experts, value);
+#pragma unroll
+            for (int i = 0; i < kV; ++i) {
+                const float d = each * exponential<sizeof(T) == 4>(value[i] - stats.x) * (counts[v][i] - stats.z);
+                value[i] = stats.y == 0.0f ? 0.0f : d;
+            }
+            if (column < a.experts) store_some<kStream>(out + column, narrow<T>(value), a.experts - column);
+        }
+    }
+}
+
+template <class T, bool kStream> __global__ __launch_bounds__(kBlock) void balance_long_backward_kernel(BalanceBackwardArgs a) {
+    constexpr int kV = kPerVec<T>;
+    const int lane = static_cast<int>(threadIdx.x) % 64;
+    const float scale = *a.upstream * *a.norm;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * (kBlock / 64) + static_cast<int>(threadIdx.x) / 64; row < a.n;
+         row += static_cast<int64_t>(gridDim.x) * (kBlock / 64)) {
+        const float4 stats = *reinterpret_cast<const float4*>(a.stats + row * 4);
+        const float each = scale * stats.y;
+        const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
+        T* out = static_cast<T*>(a.dlogits) + row * a.experts;
+        for (int column = lane * kV; column < a.experts; column += 64 * kV) {
+            float value[kV];
             load_logits(logits, column, a.experts, value);
 #pragma unroll
             for (int i = 0; i < kV; ++i) {
                 const float count = column + i < a.experts ? static_cast<float>(a.counts[column + i]) : 0.0f;
-                value[i] = scale * exponential<sizeof(T) == 4>(value[i] - m) * (count - t);
+                const float d = each * exponential<sizeof(T) == 4>(value[i] - stats.x) * (count - stats.z);
+                value[i] = stats.y == 0.0f ? 0.0f : d;
             }
+            store_some<kStream>(out + column, narrow<T>(value), a.experts - column);
         }
-        store_some<kStream>(out + column, narrow<T>(value), a.experts - column);
     }
 }
 
@@ -513,9 +671,21 @@ ODIE_API int odie_choose_backward(const float* upstream, const int32_t* expert, 
 namespace odie {
 namespace {
 
-int64_t balance_blocks(int64_t n) {
-    const int64_t most = 8 * kCus, blocks = (n + 3) / 4;
-    return blocks < 1 ? 1 : (blocks < most ? blocks : most);
+// Lanes and 16-byte chunks a lane that hold a row; 0 chunks: longer rows.
+template <class T, class F> void with_row(int width, F&& f) {
+    const int chunks = (width + kPerVec<T> - 1) / kPerVec<T>;
+    if (chunks <= 64) with_lanes<T>(width, 1, [&](auto lanes) { f(lanes, std::integral_constant<int, 1>{}); });
+    else if (chunks <= 128) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    else if (chunks <= 256) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+    else if (chunks <= 512) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
+    else f(std::integral_constant<int, 64>{}, std::integral_constant<int, 0>{});
+}
+
+// Workgroups of the passes over rows, `lanes` lanes a row: as many as the CUs hold together by their registers (four each,
+// two with 8 chunks a lane), so that all of them run to the end.
+uint32_t row_blocks(int64_t n, int lanes, int vecs) {
+    const int64_t blocks = (n + kBlock / lanes - 1) / (kBlock / lanes), most = (vecs < 8 ? 4 : 2) * kCus;
+    return static_cast<uint32_t>(blocks < 1 ? 1 : (blocks < most ? blocks : most));
 }
 
 }  // namespace
@@ -523,7 +693,7 @@ int64_t balance_blocks(int64_t n) {
 
 ODIE_API int64_t odie_balance_workspace(int64_t n, int choices, int experts) {
     if (check_rows_of("odie_balance_workspace", experts, n, choices, experts, ODIE_F32)) return -1;
-    return 8 * (balance_blocks(n) + 1);
+    return 12 * static_cast<int64_t>(row_blocks(n, 64, 1)) + 8;
 }
 
 ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int32_t* expert, int64_t n, int choices,
@@ -532,26 +702,43 @@ ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int3
     const std::string what = "odie_balance_forward";
     if (check_rows_of(what, stride, n, choices, experts, dtype)) return -1;
     if (!loss || !counts || !norm || (n > 0 && (!logits || !expert))) return fail(what + ": null pointer");
+    if (reinterpret_cast<uintptr_t>(stats) % 16) return fail(what + ": stats must be 16-byte aligned");
     const int64_t need = odie_balance_workspace(n, choices, experts);
     if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 8 != 0)
         return fail(what + ": needs an 8-byte aligned workspace of " + std::to_string(need) + " bytes");
-    BalanceArgs a{logits, expert, counts, nullptr, stats, nullptr, norm, loss, stride, n, balance_blocks(n), choices, experts};
+    const int64_t most = row_blocks(n, 64, 1);
+    BalanceArgs a{};
+    a.logits = logits;
+    a.expert = expert;
+    a.counts = counts;
+    a.stats = stats;
     a.partial = static_cast<double*>(workspace);
-    a.rows = reinterpret_cast<int32_t*>(a.partial + a.blocks);
+    a.parts = reinterpret_cast<uint32_t*>(a.partial + most);
+    a.done = a.parts + most;
+    a.norm = norm;
+    a.loss = loss;
+    a.stride = stride;
+    a.n = n;
+    a.choices = choices;
+    a.experts = experts;
     const hipStream_t s = as_stream(stream);
-    balance_clear_kernel<<<(experts + kBlock - 1) / kBlock, kBlock, 0, s>>>(a);
-    if (n > 0) {
-        const int64_t wanted = (n + kBlock - 1) / kBlock;
-        balance_count_kernel<<<static_cast<uint32_t>(wanted < kCountBlocks ? wanted : kCountBlocks), kBlock,
-                               experts <= kSharedCounts ? experts * 4 : 0, s>>>(a);
+    const int64_t entries = n * choices;
+    const int shared = experts <= kSharedCounts ? experts * 4 : 0;
+    if (entries <= kFewEntries) {
+        balance_count_kernel<true><<<1, kCountBlock, shared, s>>>(a);
+    } else {
+        // Sixteen entries a thread at least, and two for each count that a workgroup adds at its end.
+        const int64_t each = 16 * kCountBlock > 2 * experts ? 16 * kCountBlock : 2 * experts, blocks = (entries + each - 1) / each;
+        balance_clear_kernel<<<(experts + kBlock - 1) / kBlock, kBlock, 0, s>>>(a);
+        balance_count_kernel<false><<<static_cast<uint32_t>(blocks < kCus ? blocks : kCus), kCountBlock, shared, s>>>(a);
     }
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        with_lanes<T>(experts, 1, [&](auto lanes) {
-            balance_rows_kernel<T, lanes><<<static_cast<uint32_t>(a.blocks), kBlock, 0, s>>>(a);
+        with_row<T>(experts, [&](auto lanes, auto vecs) {
+            if constexpr (vecs > 0) balance_rows_kernel<T, lanes, vecs><<<row_blocks(n, lanes, vecs), kBlock, 0, s>>>(a);
+            else balance_long_kernel<T><<<row_blocks(n, 64, 1), kBlock, 0, s>>>(a);
         });
     });
-    balance_finish_kernel<<<1, kBlock, 0, s>>>(a);
     return check_launch("balance");
 }
 
@@ -562,15 +749,15 @@ ODIE_API int odie_balance_backward(const float* upstream, const void* logits, in
     if (check_rows_of(what, stride, n, 1, experts, dtype)) return -1;
     if (n == 0) return 0;
     if (!upstream || !logits || !counts || !stats || !norm || !dlogits) return fail(what + ": null pointer");
+    if (reinterpret_cast<uintptr_t>(stats) % 16) return fail(what + ": stats must be 16-byte aligned");
     BalanceBackwardArgs a{upstream, logits, counts, stats, norm, dlogits, stride, n, experts};
     const hipStream_t s = as_stream(stream);
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        with_lanes<T>(experts, 1, [&](auto lanes) {
-            with_flag(n * experts * dtype_bytes(dtype) >= kStreamBytes, [&](auto far) {
-                in_launches((n + kBlock / lanes - 1) / (kBlock / lanes), kBlock, [&](uint32_t first, uint32_t count) {
-                    balance_backward_kernel<T, lanes, far><<<count, kBlock, 0, s>>>(a, first);
-                });
+        with_flag(n * experts * dtype_bytes(dtype) >= kStreamBytes, [&](auto far) {
+            with_row<T>(experts, [&](auto lanes, auto vecs) {
+                if constexpr (vecs > 0) balance_backward_kernel<T, lanes, vecs, far><<<row_blocks(n, lanes, vecs), kBlock, 0, s>>>(a);
+                else balance_long_backward_kernel<T, far><<<row_blocks(n, 64, 1), kBlock, 0, s>>>(a);
             });
         });
         return check_launch("balance gradient");

@@ -40,7 +40,28 @@ template <int kLanes> __device__ inline float sum_across(float x) {
 }
 
 // The larger one; a NaN wins.
-__device__ inline float larger(float a, float b) { return a > b || a != a ? a : b; }
+__device__ inline float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+template <int kLanes> __device__ inline uint32_t sum_across(uint32_t x) {
+    return across<kLanes>(x, [](uint32_t a, uint32_t b) { return a + b; });
+}
+
+// The same for fp64, whose halves move alike.
+template <int kLanes> __device__ inline double sum_across(double x) {
+    const auto move = [&](uint32_t& low, uint32_t& high, auto&& by) {
+        const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+        low = by(static_cast<uint32_t>(bits)), high = by(static_cast<uint32_t>(bits >> 32));
+        x += __builtin_bit_cast(double, static_cast<uint64_t>(high) << 32 | low);
+    };
+    uint32_t low, high;
+    if constexpr (kLanes > 1) move(low, high, [](uint32_t v) { return dpp_move<0xB1>(v); });
+    if constexpr (kLanes > 2) move(low, high, [](uint32_t v) { return dpp_move<0x4E>(v); });
+    if constexpr (kLanes > 4) move(low, high, [](uint32_t v) { return dpp_move<0x141>(v); });
+    if constexpr (kLanes > 8) move(low, high, [](uint32_t v) { return dpp_move<0x140>(v); });
+    if constexpr (kLanes > 16) move(low, high, [](uint32_t v) { return static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 16)); });
+    if constexpr (kLanes > 32) move(low, high, [](uint32_t v) { return static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 32)); });
+    return x;
+}
 
 template <int kLanes> __device__ inline float max_across(float x) {
     return as_float(across<kLanes>(as_bits(x), [](uint32_t a, uint32_t b) { return as_bits(larger(as_float(a), as_float(b))); }));

@@ -138,7 +138,7 @@ class _Choose(torch.autograd.Function):
 class _Balance(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, expert):
-        stats, norm = _floats(logits, logits.shape[0], 3), _floats(logits)
+        stats, norm = _floats(logits, logits.shape[0], 4), _floats(logits)
         loss, counts = _balance(logits, expert, stats, norm)
         ctx.mark_non_differentiable(counts)
         ctx.save_for_backward(logits, counts, stats, norm)

@@ -44,7 +44,7 @@ def test_balance_refusals(native):
         return native.odie_balance_forward(logits, stride, expert, n, choices, experts, dtype, loss, counts, stats, norm,
                                            workspace, size, 0)
 
-    def b(upstream=8, logits=8, stride=64, counts=8, stats=8, norm=8, n=4, experts=64, dtype=0, out=8):
+    def b(upstream=8, logits=8, stride=64, counts=8, stats=16, norm=8, n=4, experts=64, dtype=0, out=8):
         return native.odie_balance_backward(upstream, logits, stride, counts, stats, norm, n, experts, dtype, out, 0)
 
     for call, what in ((f, 'odie_balance_forward'), (b, 'odie_balance_backward')):
@@ -64,6 +64,8 @@ def test_balance_refusals(native):
     _refused(native, f(size=need - 1), 'workspace', str(need))
     _refused(native, f(workspace=4), 'aligned')
     _refused(native, f(workspace=None), 'workspace')
+    _refused(native, f(stats=8), 'stats', 'aligned')
+    _refused(native, b(stats=8), 'stats', 'aligned')
     assert native.odie_balance_workspace(-1, 2, 64) == -1 and native.odie_balance_workspace(1 << 30, 4, 64) == -1
     assert native.odie_balance_workspace(1 << 28, 4, 64) < 1 << 20
     _refused(native, b(stats=None), 'null')
