@@ -85,10 +85,6 @@ template <int kRows, int kThreads> struct Scales {
         base += kMxSlabScales;
         left -= 2;
     }
-    // The scales of blocks 4 (lane / 32) .. + 3 of row base + lane % 32, a byte each.
-    static __device__ uint32_t word(const char* lds, int base, int lane) {
-        return *reinterpret_cast<const uint32_t*>(lds + (base + lane % 32) * kMxSlabScales + lane / 32 * 4);
-    }
     static __device__ uint32_t byte(const char* lds, int row, int block) {
         return *reinterpret_cast<const uint8_t*>(lds + row * kMxSlabScales + block);
     }
@@ -99,7 +95,62 @@ template <class I> __device__ inline vec16 chunk_at(const char* lds, int r, int 
     return *reinterpret_cast<const vec16*>(lds + r * kSlabBytes + ((c ^ I::turn(r)) << 4));
 }
 
-// A tile of a product of codes with codes.
+// The buffer descriptor of what lies from a uniform address on.
+__device__ inline vec16 buffer_of(const uint8_t* base) {
+    const uint64_t address = reinterpret_cast<uint64_t>(base);
+    vec16 buffer{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address))),
+                 static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32))), kBufferLimit, kBufferWord3};
+    asm volatile("s_nop 4" : "+s"(buffer));   // wait states between its writing and the loads
+    return buffer;
+}
+__device__ inline uint32_t lds_address(const char* lds, int more) {
+    return __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>((lds_void)(lds))) + more);
+}
+
+// Both operands' scales on their way to LDS, 16 bytes a row: those of two slabs, a group.  Four lanes take a row, so that a
+// load touches 16 lines (two lanes a row and slab: 32; all loads of a 256 x 256 tile alone then took a third longer).
+template <int kBM, int kBN, int kThreads> struct ScaleRows {
+    static constexpr int kRowBytes = 16, kBytes = (kBM + kBN) * kRowBytes, kWaves = kThreads / 64;
+    static constexpr int kLoads = kBytes / 256 / kWaves;       // a wave's loads of 16 rows
+    static_assert(kLoads * kWaves * 256 == kBytes && kBM % 16 == 0, "whole loads a wave");
+    uint32_t offset[kLoads];
+    const uint8_t *a, *b;    // uniform over the workgroup
+    int left;                // words from this lane's on to its row's end
+
+    static __device__ int part(int i) { return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64)) + i * kWaves; }
+
+    // Rows past the last read the last.
+    __device__ void begin(const uint8_t* rows, const uint8_t* columns, int64_t pitch, int64_t rows_left, int64_t columns_left) {
+        a = rows, b = columns;
+        const int lane = static_cast<int>(threadIdx.x % 64);
+        left = static_cast<int>(pitch / 4) - lane % 4;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int at = part(i) * 16 + lane / 4, r = at < kBM ? at : at - kBM;
+            const int64_t limit = (at < kBM ? rows_left : columns_left) - 1;
+            offset[i] = static_cast<uint32_t>(r < limit ? r : limit) * static_cast<uint32_t>(pitch) + lane % 4 * 4;
+        }
+    }
+    // Queues the next group's into lds.
+    __device__ void load(char* lds) {
+        const vec16 buffer_a = buffer_of(a), buffer_b = buffer_of(b);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t to = lds_address(lds, part(i) * 256), from = left > 0 ? offset[i] : kNowhere;
+            if (part(i) * 16 < kBM) queue4(to, from, buffer_a);
+            else queue4(to, from, buffer_b);
+        }
+        a += kRowBytes, b += kRowBytes;
+        left -= 4;
+    }
+    // The scales of the four blocks that a lane half takes of slab `slab % 2` of the group, a byte each.
+    static __device__ uint32_t word(const char* lds, int r, int slab, int half) {
+        return *reinterpret_cast<const uint32_t*>(lds + r * kRowBytes + slab % 2 * kMxSlabScales + half * 4);
+    }
+};
+
+// A tile of a product of codes with codes.  A slab is eight blocks of k, 128 bytes of codes: a lane of half h takes blocks
+// 4 h .. 4 h + 3, one at each of four steps.
 template <int kBM, int kBN, int kWM, int kWN> struct MxTile : Sums<kBM, kBN, kWM, kWN> {
     using Base = Sums<kBM, kBN, kWM, kWN>;
     using Base::acc;
@@ -108,11 +159,10 @@ template <int kBM, int kBN, int kWM, int kWN> struct MxTile : Sums<kBM, kBN, kWM
     using Base::kThreads;
     using A = Direct<uint8_t, true, kBM, kThreads>;
     using B = Direct<uint8_t, true, kBN, kThreads>;
-    using SA = Scales<kBM, kThreads>;
-    using SB = Scales<kBN, kThreads>;
-    static constexpr int kCodes = A::kBytes + B::kBytes;
-    static constexpr int kBuffer = kCodes + SA::kBytes + SB::kBytes;
-    static constexpr int kLds = 2 * kBuffer > kThreads / 64 * Base::kRegion ? 2 * kBuffer : kThreads / 64 * Base::kRegion;
+    using S = ScaleRows<kBM, kBN, kThreads>;
+    static constexpr int kBuffer = A::kBytes + B::kBytes;
+    static constexpr int kBytes = 2 * (kBuffer + S::kBytes);
+    static constexpr int kLds = kBytes > kThreads / 64 * Base::kRegion ? kBytes : kThreads / 64 * Base::kRegion;
 
     template <int kStep> __device__ void add_step(const char* here, const uint32_t (&sa)[kMs], const uint32_t (&sb)[kNs]) {
         const int lane = static_cast<int>(threadIdx.x % 64), chunk = 4 * (lane / 32) + kStep;
@@ -127,13 +177,13 @@ template <int kBM, int kBN, int kWM, int kWN> struct MxTile : Sums<kBM, kBN, kWM
             for (int j = 0; j < kNs; ++j) acc[i][j] = multiply_mx<kStep>(fb[j], fa[i], sb[j], sa[i], acc[i][j]);
     }
 
-    __device__ void add_slab(const char* here) {
+    __device__ void add_slab(const char* here, const char* scales, int slab) {
         const int lane = static_cast<int>(threadIdx.x % 64);
         uint32_t sa[kMs], sb[kNs];
 #pragma unroll
-        for (int i = 0; i < kMs; ++i) sa[i] = SA::word(here + kCodes, Base::wave_row() + 32 * i, lane);
+        for (int i = 0; i < kMs; ++i) sa[i] = S::word(scales, Base::wave_row() + 32 * i + lane % 32, slab, lane / 32);
 #pragma unroll
-        for (int j = 0; j < kNs; ++j) sb[j] = SB::word(here + kCodes + SA::kBytes, Base::wave_column() + 32 * j, lane);
+        for (int j = 0; j < kNs; ++j) sb[j] = S::word(scales, kBM + Base::wave_column() + 32 * j + lane % 32, slab, lane / 32);
         add_step<0>(here, sa, sb);
         add_step<1>(here, sa, sb);
         add_step<2>(here, sa, sb);
@@ -141,21 +191,23 @@ template <int kBM, int kBN, int kWM, int kWN> struct MxTile : Sums<kBM, kBN, kWM
     }
 
     // Sums `bytes` bytes of codes a row.  The operands have begun.
-    __device__ void sum(A& a, B& b, SA& sa, SB& sb, int64_t bytes, char* lds) {
+    __device__ void sum(A& a, B& b, S& s, int bytes, char* lds) {
         Base::clear();
-        auto load = [&](int64_t left, char* to) {
+        char* const scales = lds + 2 * kBuffer;
+        auto load = [&](int slab) {
+            const int left = bytes - slab * kSlabBytes;
+            if (left <= 0) return;
+            char* const to = lds + slab % 2 * kBuffer;
             a.load(left, to);
             b.load(left, to + A::kBytes);
-            sa.load(to + kCodes);
-            sb.load(to + kCodes + SA::kBytes);
+            if (slab % 2 == 0) s.load(scales + slab / 2 % 2 * S::kBytes);
         };
-        load(bytes, lds);
-        int now = 0;
-        for (int64_t left = bytes; left > 0; left -= kSlabBytes) {
+        load(0);
+        const int slabs = (bytes + kSlabBytes - 1) / kSlabBytes;
+        for (int i = 0; i < slabs; ++i) {
             arrived<0>();   // this slab; and no wave reads the other buffer any more
-            if (left > kSlabBytes) load(left - kSlabBytes, lds + (now ^ 1) * kBuffer);
-            add_slab(lds + now * kBuffer);
-            now ^= 1;
+            load(i + 1);
+            add_slab(lds + i % 2 * kBuffer, scales + i / 2 % 2 * S::kBytes, i);
         }
         __syncthreads();
     }
@@ -176,14 +228,13 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void mx_rows4_kerne
     const int64_t matrix = static_cast<int64_t>(p.group) * a.columns;
     typename Work::A opa;
     typename Work::B opb;
-    typename Work::SA sa;
-    typename Work::SB sb;
+    typename Work::S scales;
     opa.begin(static_cast<const uint8_t*>(a.a), m.code_pitch, p.begin, p.end, m.code_pitch);
     opb.begin(static_cast<const uint8_t*>(a.b) + matrix * m.code_pitch, m.code_pitch, column0, a.columns, m.code_pitch);
-    sa.begin(m.a_scales, m.scale_pitch, p.begin, p.end);
-    sb.begin(m.b_scales + matrix * m.scale_pitch, m.scale_pitch, column0, a.columns);
+    scales.begin(m.a_scales + p.begin * m.scale_pitch, m.b_scales + (matrix + column0) * m.scale_pitch, m.scale_pitch,
+                 p.end - p.begin, a.columns - column0);
     Work work;
-    work.sum(opa, opb, sa, sb, m.code_pitch, lds);
+    work.sum(opa, opb, scales, static_cast<int>(m.code_pitch), lds);
     finish_tile<T, kBM == 256>(work, a, p, column0, lds);
 }
 
