@@ -653,8 +653,8 @@ int odie_embed_backward(const void* upstream, int64_t upstream_stride, const voi
 
 /* The `choices` largest logits of each row, the lowest index first among equal ones (a NaN is the largest): expert int32
  * [n][choices], -1 where the row has fewer above -inf, and weights [n][choices], their softmax over the chosen
- * (normalize = 1) or over all experts (0), 0 with -1.  stats fp32 [n][2] or null: what the backward needs with
- * normalize = 0.  At most 32768 experts and 64 choices, n * choices < 2^31. */
+ * (normalize = 1) or over all experts (0), 0 with -1.  stats fp32 [n][2] (8-byte aligned) or null: what the backward needs
+ * with normalize = 0.  At most 32768 experts and 64 choices, n * choices < 2^31. */
 int odie_choose_forward(const void* logits, int64_t stride, int64_t n, int experts, int choices, int normalize, int dtype,
                         int32_t* expert, float* weights, float* stats, uint64_t stream);
 

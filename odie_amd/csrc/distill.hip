@@ -48,16 +48,37 @@ __device__ inline float entry_of(const DistillArgs& a, int64_t row, int j, int64
     return id >= 0 && id < a.classes ? teacher_of(a, row * a.top + j) * a.inverse : kNegInfinity;
 }
 
-// Adds the logits / T of columns [begin, end) to run, lane `lane` of `lanes`.
-template <class T, class R> __device__ inline void add_columns(const DistillArgs& a, const T* row, int begin, int end, int lane, int lanes, R& run) {
-    constexpr int kV = kPerVec<T>;
-    for (int column = begin + lane * kV; column < end; column += lanes * kV) {
+// Calls f(column, values) for the chunks of columns [begin, end) that lane `lane` of kLanes takes, kAhead whole ones at a
+// time, whose loads are in flight together.
+template <class T, int kLanes, int kAhead, class F> __device__ inline void for_chunks(const T* row, int begin, int end, int width, int lane, F&& f) {
+    constexpr int kV = kPerVec<T>, kStep = kLanes * kV;
+    int column = begin + lane * kV;
+    for (; column + (kAhead - 1) * kStep + kV <= end; column += kAhead * kStep) {
+        vec16 chunk[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) chunk[u] = load16(row + column + u * kStep);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            float value[kV];
+            widen<T>(chunk[u], value);
+            f(column + u * kStep, value);
+        }
+    }
+    for (; column < end; column += kStep) {
         float value[kV];
-        load_logits(row, column, a.classes, value);
+        load_logits(row, column, width, value);
+        f(column, value);
+    }
+}
+
+// Adds the logits / T of columns [begin, end) to run.
+template <class T, int kLanes, class R> __device__ inline void add_columns(const DistillArgs& a, const T* row, int begin, int end, int lane, R& run) {
+    constexpr int kV = kPerVec<T>;
+    for_chunks<T, kLanes, kLanes == kBlock ? 4 : 1>(row, begin, end, a.classes, lane, [&](int, float (&value)[kV]) {
 #pragma unroll
         for (int i = 0; i < kV; ++i) value[i] *= a.inverse;
         run.add(value);
-    }
+    });
 }
 
 // A row's loss from its softmax (m, s): kLanes lanes of one wave share the entries.
@@ -105,7 +126,7 @@ template <class T, int kLanes> __global__ __launch_bounds__(kBlock) void distill
     const int64_t at = (static_cast<int64_t>(first) + blockIdx.x) * (kBlock / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
     const int64_t row = at < a.n ? at : a.n - 1;
     Running<sizeof(T) == 4> run;
-    add_columns(a, static_cast<const T*>(a.logits) + row * a.stride, 0, a.classes, lane, kLanes, run);
+    add_columns<T, kLanes>(a, static_cast<const T*>(a.logits) + row * a.stride, 0, a.classes, lane, run);
     run.template join_lanes<kLanes>();
     finish_row<T, kLanes>(a, row, lane, at < a.n, run.m, run.s);
 }
@@ -117,7 +138,7 @@ template <class T> __global__ __launch_bounds__(kBlock) void distill_piece_kerne
     const int piece = static_cast<int>(id % a.pieces), begin = piece * a.piece;
     const int end = begin + a.piece < a.classes ? begin + a.piece : a.classes;
     Running<sizeof(T) == 4> run;
-    add_columns(a, static_cast<const T*>(a.logits) + row * a.stride, begin, end, static_cast<int>(threadIdx.x), kBlock, run);
+    add_columns<T, kBlock>(a, static_cast<const T*>(a.logits) + row * a.stride, begin, end, static_cast<int>(threadIdx.x), run);
     run.template join_lanes<64>();
     if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = make_float2(run.m, run.s);
     __syncthreads();
@@ -176,15 +197,14 @@ __global__ __launch_bounds__(kBlock) void distill_backward_kernel(DistillArgs a,
         for (int i = 0; i < 4; ++i) stats[i] = a.stats[row * 4 + i];
         scale = a.upstream[row] * a.inverse;
         const float each = scale * stats[1];
-        for (int column = begin + lane * kV; column < end; column += kLanes * kV) {
-            float value[kV] = {};
-            if (stats[3] != 0.0f) {
-                load_logits(logits, column, a.classes, value);
+        for_chunks<T, kLanes, kLanes == kBlock ? 4 : 1>(logits, begin, end, a.classes, lane, [&](int column, float (&value)[kV]) {
 #pragma unroll
-                for (int i = 0; i < kV; ++i) value[i] = each * exponential<sizeof(T) == 4>(fmaf(value[i], a.inverse, -stats[0]));
+            for (int i = 0; i < kV; ++i) {
+                const float p = each * exponential<sizeof(T) == 4>(fmaf(value[i], a.inverse, -stats[0]));
+                value[i] = stats[3] == 0.0f ? 0.0f : p;
             }
             store_some<kStream>(out + column, narrow<T>(value), a.classes - column);
-        }
+        });
     }
     // the entries' classes once more, after every lane's stores
     if constexpr (kLanes == kBlock) __syncthreads();

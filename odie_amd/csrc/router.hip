@@ -20,48 +20,121 @@ constexpr int kMaxExperts = 1 << 15;
 constexpr int kMaxChoices = 64;
 constexpr int64_t kMaxEntries = (int64_t{1} << 31) - 1;
 
-// Whole numbers in the order of the values, above 0 but for -inf: -0 and 0 alike, every NaN above +inf.
-__device__ inline uint32_t order_of(float x) {
-    if (x != x) return 0xffffffffu;
-    const uint32_t bits = as_bits(x + 0.0f);
-    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
-}
-__device__ inline float value_of(uint32_t order) {
-    if (order == 0xffffffffu) return as_float(0x7fc00000u);
-    return as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
-}
-template <class T> __device__ inline uint32_t order16(float x) {   // x a value of T
-    if (x != x) return 0xffffu;
-    const uint32_t bits = __builtin_bit_cast(uint16_t, static_cast<T>(x + 0.0f));
-    return bits & 0x8000u ? bits ^ 0xffffu : bits | 0x8000u;
-}
-template <class T> __device__ inline float value16(uint32_t order) {
-    if (order == 0xffffu) return as_float(0x7fc00000u);
-    return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(order & 0x8000u ? order & 0x7fffu : order ^ 0xffffu)));
-}
+template <class N> __device__ inline N most_of(N a, N b) { return a > b ? a : b; }
+template <class N> __device__ inline N least_of(N a, N b) { return a < b ? a : b; }
 
-// A logit above -inf with its index as one whole number above 0: the larger the logit and, among equal ones, the lower
-// the index, the larger the key.  A 16-bit logit and its index fit 32 bits.
+// Logits with their indices as whole numbers: the larger the logit and, among equal ones, the lower the index, the larger
+// the key.  A logit's bits become a signed number in the order of the values by negating the magnitude of
+// negative ones (which makes -0 and 0 alike); a NaN is the largest.  A 16-bit logit and its index fit 32 bits.
 template <class T> struct Keys {
-    using Key = uint32_t;
-    static __device__ Key of(float value, int index) { return order16<T>(value) << 16 | static_cast<uint32_t>(0xffff - index); }
-    static __device__ int index(Key key) { return 0xffff - static_cast<int>(key & 0xffffu); }
-    static __device__ float value(Key key) { return value16<T>(key >> 16); }
+    using Key = int32_t;
+    static constexpr Key kNone = INT32_MIN;
+    static constexpr uint32_t kInfinity = std::is_same_v<T, __bf16> ? 0x7f80u : 0x7c00u;
+    typedef int16_t two __attribute__((ext_vector_type(2)));
+
+    // The keys of a 16-byte chunk whose first index is `index` (a multiple of 8).  kChecked: with NaN in it.
+    template <bool kChecked> static __device__ void of(const vec16& chunk, int index, Key key[8]) {
+        const uint32_t rest = static_cast<uint32_t>(0xffff - index);      // its low three bits are ones
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t word = chunk[w];       // a bit cast of the element itself would take the vector's first
+            const two bits = __builtin_bit_cast(two, word), sign = bits >> static_cast<int16_t>(15);
+            const two size = bits & static_cast<int16_t>(0x7fff), order = (size ^ sign) - sign;
+            uint32_t pair = __builtin_bit_cast(uint32_t, order);
+            if constexpr (kChecked) {
+                const uint32_t sizes = __builtin_bit_cast(uint32_t, size);
+                if ((sizes & 0xffffu) > kInfinity) pair |= 0x7fffu, pair &= 0xffff7fffu;
+                if (sizes >> 16 > kInfinity) pair |= 0x7fff0000u, pair &= 0x7fffffffu;
+            }
+            key[2 * w] = static_cast<Key>(pair << 16 | (rest ^ (2 * w)));
+            key[2 * w + 1] = static_cast<Key>((pair & 0xffff0000u) | (rest ^ (2 * w + 1)));
+        }
+    }
+    static __device__ bool has_nan(const vec16& chunk) {
+        typedef uint16_t twos __attribute__((ext_vector_type(2)));
+        twos most{};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t sizes = chunk[w] & 0x7fff7fffu;
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(twos, sizes));
+        }
+        return most[0] > kInfinity || most[1] > kInfinity;
+    }
+    static __device__ int index(Key key) { return 0xffff - static_cast<int>(key & 0xffff); }
+    static __device__ float value(Key key) {
+        const int order = key >> 16;
+        return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(order < 0 ? 0x8000 | -order : order)));
+    }
+    static __device__ Key second(Key most, Key less, Key key) { return most_of(least_of(most, less), least_of(most_of(most, less), key)); }   // the middle one
     template <int kLanes> static __device__ Key best(Key key) {
-        return across<kLanes>(key, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+        return static_cast<Key>(across<kLanes>(static_cast<uint32_t>(key), [](uint32_t a, uint32_t b) {
+            return static_cast<uint32_t>(most_of(static_cast<int32_t>(a), static_cast<int32_t>(b)));
+        }));
     }
 };
 template <> struct Keys<float> {
-    using Key = uint64_t;
-    static __device__ Key of(float value, int index) { return static_cast<uint64_t>(order_of(value)) << 32 | static_cast<uint32_t>(~index); }
+    using Key = int64_t;
+    static constexpr Key kNone = INT64_MIN;
+
+    static __device__ Key of(float value, int index) {
+        const int32_t bits = __builtin_bit_cast(int32_t, value), sign = bits >> 31, size = bits & 0x7fffffff;
+        const int32_t order = size > 0x7f800000 ? 0x7fffffff : (size ^ sign) - sign;
+        return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(order)) << 32 | static_cast<uint32_t>(~index));
+    }
+    template <bool kChecked> static __device__ void of(const vec16& chunk, int index, Key key[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) key[i] = of(as_float(chunk[i]), index + i);
+    }
+    static __device__ bool has_nan(const vec16&) { return false; }      // of() tells
     static __device__ int index(Key key) { return static_cast<int>(~static_cast<uint32_t>(key)); }
-    static __device__ float value(Key key) { return value_of(static_cast<uint32_t>(key >> 32)); }
+    static __device__ float value(Key key) {
+        const int32_t order = static_cast<int32_t>(key >> 32);
+        return __builtin_bit_cast(float, order < 0 ? INT32_MIN | -order : order);
+    }
+    static __device__ Key second(Key most, Key less, Key key) { return most_of(less, least_of(most, key)); }
     template <int kLanes> static __device__ Key best(Key key) {
         // the largest order first, then the largest rest among the lanes that hold it
-        const auto most = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
-        const uint32_t order = static_cast<uint32_t>(key >> 32), top = across<kLanes>(order, most);
-        const uint32_t rest = across<kLanes>(order == top ? static_cast<uint32_t>(key) : 0u, most);
-        return static_cast<uint64_t>(top) << 32 | rest;
+        const int32_t order = static_cast<int32_t>(key >> 32);
+        const int32_t top = static_cast<int32_t>(across<kLanes>(static_cast<uint32_t>(order), [](uint32_t a, uint32_t b) {
+            return static_cast<uint32_t>(most_of(static_cast<int32_t>(a), static_cast<int32_t>(b)));
+        }));
+        const uint32_t rest = across<kLanes>(order == top ? static_cast<uint32_t>(key) : 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+        return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(top)) << 32 | rest);
+    }
+};
+
+// A row's 16-byte chunks, kVecs a lane, loaded ahead of their use: without conditions, which would make the compiler wait
+// for loads in flight, from addresses moved back into the row where they would leave it; settle() puts that right.  The first half of
+// several chunks is always whole (with_row).  Rows shorter than a chunk are gathered.
+template <class T, int kLanes, int kVecs> struct RowHold {
+    static constexpr int kV = kPerVec<T>;
+    vec16 chunk[kVecs];
+
+    __device__ void load(const T* row, int lane, int width) {
+        if (width < kV) {
+            chunk[0] = gather16(row, lane == 0 ? width : 0);
+            return;
+        }
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+            const int column = (v * kLanes + lane) * kV;
+            chunk[v] = load16(row + (v < kVecs / 2 || column < width - kV ? column : width - kV));
+        }
+    }
+    // Moves what lies across the row's end to its place, zeros past it; before get().
+    __device__ void settle(int lane, int width) {
+#pragma unroll
+        for (int v = kVecs / 2; v < kVecs; ++v) {
+            const int count = width - (v * kLanes + lane) * kV;
+            if (count < kV && width >= kV) chunk[v] = count > 0 ? shift_down(chunk[v], (kV - count) * static_cast<int>(sizeof(T))) : vec16{};
+        }
+    }
+    __device__ void get(int v, int lane, int width, float value[kV]) const {
+        const int count = width - (v * kLanes + lane) * kV;
+        widen<T>(chunk[v], value);
+        if (v >= kVecs / 2 && count < kV)
+#pragma unroll
+            for (int i = 0; i < kV; ++i) value[i] = i < count ? value[i] : kNegInfinity;
     }
 };
 
@@ -75,72 +148,97 @@ struct ChooseArgs {
     int normalize;
 };
 
-// Rows of up to 64 kVecs 16-byte chunks in registers, kLanes lanes and kVecs chunks a lane.
-template <class T, int kLanes, int kVecs>
-__global__ __launch_bounds__(kBlock) void choose_kernel(ChooseArgs a, uint32_t first_block) {
+// Rows of up to 64 kVecs chunks in registers, the next one under way.  Each lane keeps its two largest keys; a choice takes
+// the largest of all lanes, whose lane goes on to its second, and looks through its keys again once both are gone: at four
+// choices of 1024 about once in 500 rows.
+template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) void choose_kernel(ChooseArgs a) {
     using K = Keys<T>;
     using Key = typename K::Key;
-    constexpr int kV = kPerVec<T>, kValues = kVecs * kV;
+    constexpr int kV = kPerVec<T>, kValues = kVecs * kV, kRows = kBlock / kLanes;
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
-    const int64_t at = (static_cast<int64_t>(first_block) + blockIdx.x) * (kBlock / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
-    const int64_t row = at < a.n ? at : a.n - 1;
-    const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
-    float value[kVecs][kV];
-    Key key[kValues], local = 0;
+    const T* logits = static_cast<const T*>(a.logits);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    int64_t at = static_cast<int64_t>(blockIdx.x) * kRows + static_cast<int>(threadIdx.x) / kLanes;
+    RowHold<T, kLanes, kVecs> next;
+    next.load(logits + (at < a.n ? at : a.n - 1) * a.stride, lane, a.experts);
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.n; base += step, at += step) {
+        RowHold<T, kLanes, kVecs> row = next;
+        next.load(logits + (at + step < a.n ? at + step : a.n - 1) * a.stride, lane, a.experts);
+        row.settle(lane, a.experts);
+        Key key[kValues];
+        bool nan = false;
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v) load_logits(logits, (v * kLanes + lane) * kV, a.experts, value[v]);
-#pragma unroll
-    for (int v = 0; v < kVecs; ++v)
-#pragma unroll
-        for (int i = 0; i < kV; ++i) {
-            const int index = (v * kLanes + lane) * kV + i;
-            key[v * kV + i] = value[v][i] == kNegInfinity ? 0 : K::of(value[v][i], index);
-            local = key[v * kV + i] > local ? key[v * kV + i] : local;
+        for (int v = 0; v < kVecs; ++v) {
+            K::template of<false>(row.chunk[v], (v * kLanes + lane) * kV, key + v * kV);
+            nan |= K::has_nan(row.chunk[v]);
         }
-    Key mine = 0, first = 0;      // lane j: the j-th choice
-    for (int j = 0; j < a.choices; ++j) {
-        const Key best = K::template best<kLanes>(local);
-        if (j == 0) first = best;
-        if (lane == j) mine = best;
-        local = 0;
+        if (__any(nan)) {
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) K::template of<true>(row.chunk[v], (v * kLanes + lane) * kV, key + v * kV);
+        }
+#pragma unroll
+        for (int v = kVecs / 2; v < kVecs; ++v) {
+            const int count = a.experts - (v * kLanes + lane) * kV;
+            if (count < kV)
+#pragma unroll
+                for (int i = 0; i < kV; ++i) key[v * kV + i] = i < count ? key[v * kV + i] : K::kNone;
+        }
+        Key most = K::kNone, less = K::kNone;
 #pragma unroll
         for (int i = 0; i < kValues; ++i) {
-            key[i] = key[i] == best ? 0 : key[i];
-            local = key[i] > local ? key[i] : local;
+            less = K::second(most, less, key[i]);
+            most = most_of(most, key[i]);
         }
-    }
-    const float m = first ? K::value(first) : kNegInfinity, base = base_of(m);
-    const float own = mine ? expf(K::value(mine) - base) : 0.0f;
-    float s;
-    if (a.normalize) {
-        s = sum_across<kLanes>(own);
-    } else {
-        s = 0.0f;
+        Key mine = K::kNone, first = K::kNone;      // lane j: the j-th choice
+        bool left = most != K::kNone;
+        for (int j = 0; j < a.choices; ++j) {
+            const Key best = K::template best<kLanes>(most);
+            if (j == 0) first = best;
+            if (lane == j) mine = best;
+            if (most == best) most = less, less = K::kNone;
+            if (__any(left && most == K::kNone)) {
+                Key below = K::kNone;
 #pragma unroll
-        for (int v = 0; v < kVecs; ++v)
+                for (int i = 0; i < kValues; ++i) below = most_of(below, key[i] < best ? key[i] : K::kNone);
+                if (most == K::kNone) {
+                    most = below;
+                    left = below != K::kNone;
+                }
+            }
+        }
+        const float m = first == K::kNone ? kNegInfinity : K::value(first), base_value = base_of(m);
+        const float chosen = mine == K::kNone ? kNegInfinity : K::value(mine);
+        const bool held = !(chosen == kNegInfinity);
+        const float own = held ? expf(chosen - base_value) : 0.0f;
+        float s = own;
+        if (!a.normalize) {
+            s = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kV; ++i) s += exponential<sizeof(T) == 4>(value[v][i] - base);
+            for (int v = 0; v < kVecs; ++v) {
+                float value[kV];
+                row.get(v, lane, a.experts, value);
+#pragma unroll
+                for (int i = 0; i < kV; ++i) s += exponential<sizeof(T) == 4>(value[i] - base_value);
+            }
+        }
         s = sum_across<kLanes>(s);
-    }
-    const float inverse = first ? 1.0f / s : 0.0f;
-    if (at >= a.n) return;
-    if (lane < a.choices) {
-        a.expert[row * a.choices + lane] = mine ? K::index(mine) : -1;
-        a.weights[row * a.choices + lane] = mine ? own * inverse : 0.0f;
-    }
-    if (a.stats && lane == 0) {
-        a.stats[row * 2] = m;
-        a.stats[row * 2 + 1] = inverse;
+        const float inverse = m == kNegInfinity ? 0.0f : 1.0f / s;
+        if (at >= a.n) continue;
+        if (lane < a.choices) {
+            a.expert[at * a.choices + lane] = held ? K::index(mine) : -1;
+            a.weights[at * a.choices + lane] = held ? own * inverse : 0.0f;
+        }
+        if (a.stats && lane == 0) *reinterpret_cast<float2*>(a.stats + at * 2) = make_float2(m, inverse);
     }
 }
 
 // The largest key of the workgroup, for every thread; `part` holds a key a wave.
-__device__ inline uint64_t block_best(uint64_t key, uint64_t* part) {
+__device__ inline int64_t block_best(int64_t key, int64_t* part) {
     key = Keys<float>::best<64>(key);
     __syncthreads();
     if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = key;
     __syncthreads();
-    for (int w = 0; w < kBlock / 64; ++w) key = part[w] > key ? part[w] : key;
+    for (int w = 0; w < kBlock / 64; ++w) key = most_of(key, part[w]);
     return key;
 }
 
@@ -148,28 +246,29 @@ __device__ inline uint64_t block_best(uint64_t key, uint64_t* part) {
 template <class T> __global__ __launch_bounds__(kBlock) void choose_long_kernel(ChooseArgs a) {
     using K = Keys<float>;
     constexpr int kV = kPerVec<T>;
-    __shared__ uint64_t part[kBlock / 64];
+    __shared__ int64_t part[kBlock / 64];
     __shared__ float sums[kBlock / 64];
     for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
         const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
-        uint64_t mine = 0, first = 0, last = ~uint64_t{0};
+        int64_t mine = K::kNone, first = K::kNone, last = INT64_MAX;
         for (int j = 0; j < a.choices; ++j) {
-            uint64_t local = 0;
+            int64_t local = K::kNone;
             for (int column = static_cast<int>(threadIdx.x) * kV; column < a.experts; column += kBlock * kV) {
                 float value[kV];
                 load_logits(logits, column, a.experts, value);
 #pragma unroll
                 for (int i = 0; i < kV; ++i) {
-                    const uint64_t key = value[i] == kNegInfinity ? 0 : K::of(value[i], column + i);
-                    if (key < last && key > local) local = key;
+                    const int64_t key = column + i < a.experts ? K::of(value[i], column + i) : K::kNone;
+                    if (key < last) local = most_of(local, key);
                 }
             }
             last = block_best(local, part);
             if (j == 0) first = last;
             if (static_cast<int>(threadIdx.x) == j) mine = last;
         }
-        const float m = first ? K::value(first) : kNegInfinity, base = base_of(m);
-        const float own = mine ? expf(K::value(mine) - base) : 0.0f;
+        const float m = K::value(first), base = base_of(m), chosen = mine == K::kNone ? kNegInfinity : K::value(mine);
+        const bool held = !(chosen == kNegInfinity);
+        const float own = held ? expf(chosen - base) : 0.0f;
         float s = own;
         if (!a.normalize) {
             s = 0.0f;
@@ -186,10 +285,10 @@ template <class T> __global__ __launch_bounds__(kBlock) void choose_long_kernel(
         __syncthreads();
         s = 0.0f;
         for (int w = 0; w < kBlock / 64; ++w) s += sums[w];
-        const float inverse = first ? 1.0f / s : 0.0f;
+        const float inverse = m == kNegInfinity ? 0.0f : 1.0f / s;
         if (static_cast<int>(threadIdx.x) < a.choices) {
-            a.expert[row * a.choices + threadIdx.x] = mine ? K::index(mine) : -1;
-            a.weights[row * a.choices + threadIdx.x] = mine ? own * inverse : 0.0f;
+            a.expert[row * a.choices + threadIdx.x] = held ? K::index(mine) : -1;
+            a.weights[row * a.choices + threadIdx.x] = held ? own * inverse : 0.0f;
         }
         if (a.stats && threadIdx.x == 0) {
             a.stats[row * 2] = m;
@@ -315,36 +414,6 @@ template <bool kAlone> __global__ __launch_bounds__(kCountBlock) void balance_co
     }
 }
 
-// A row's 16-byte chunks, kVecs a lane, loaded ahead of their use: without conditions, which would make the compiler wait
-// for loads in flight, from addresses moved back into the row where they would leave it; get() puts that right.  The first half of
-// several chunks is always whole (with_row).  Rows shorter than a chunk are gathered.
-template <class T, int kLanes, int kVecs> struct RowHold {
-    static constexpr int kV = kPerVec<T>;
-    vec16 chunk[kVecs];
-
-    __device__ void load(const T* row, int lane, int width) {
-        if (width < kV) {
-            chunk[0] = gather16(row, lane == 0 ? width : 0);
-            return;
-        }
-#pragma unroll
-        for (int v = 0; v < kVecs; ++v) {
-            const int column = (v * kLanes + lane) * kV;
-            chunk[v] = load16(row + (v < kVecs / 2 || column < width - kV ? column : width - kV));
-        }
-    }
-    __device__ void get(int v, int lane, int width, float value[kV]) const {
-        const int count = width - (v * kLanes + lane) * kV;
-        if (v < kVecs / 2 || count >= kV) {
-            widen<T>(chunk[v], value);
-            return;
-        }
-        widen<T>(count > 0 && width >= kV ? shift_down(chunk[v], (kV - count) * static_cast<int>(sizeof(T))) : chunk[v], value);
-#pragma unroll
-        for (int i = 0; i < kV; ++i) value[i] = i < count ? value[i] : kNegInfinity;
-    }
-};
-
 // The counts of a lane's columns as fp32, 0 past the last.
 template <class T, int kLanes, int kVecs> __device__ inline void hold_counts(const int32_t* counts, int lane, int experts, float (&to)[kVecs][kPerVec<T>]) {
 #pragma unroll
@@ -433,12 +502,13 @@ template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) v
         part_next.load(a, at < a.n ? at : a.n - 1, lane);
     }
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.n; base += step, at += step) {
-        const RowHold<T, kLanes, kVecs> row = next;
+        RowHold<T, kLanes, kVecs> row = next;
         const Part<kLanes> part = part_next;
         const int64_t now = at < a.n ? at : a.n - 1, then = at + step < a.n ? at + step : a.n - 1;
         next.load(logits + then * a.stride, lane, a.experts);
         part_next.load(a, then, lane);
         const bool any = part.get(a, now, lane);
+        row.settle(lane, a.experts);
         float value[kVecs][kV], top = kNegInfinity;
 #pragma unroll
         for (int v = 0; v < kVecs; ++v) {
@@ -543,11 +613,12 @@ __global__ __launch_bounds__(kBlock) void balance_backward_kernel(BalanceBackwar
     next.load(logits + at * a.stride, lane, a.experts);
     float4 stats_next = *reinterpret_cast<const float4*>(a.stats + at * 4);
     for (; at < a.n; at += step) {
-        const RowHold<T, kLanes, kVecs> row = next;
+        RowHold<T, kLanes, kVecs> row = next;
         const float4 stats = stats_next;
         const int64_t then = at + step < a.n ? at + step : a.n - 1;
         next.load(logits + then * a.stride, lane, a.experts);
         stats_next = *reinterpret_cast<const float4*>(a.stats + then * 4);
+        row.settle(lane, a.experts);
         const float each = scale * stats.y;
         T* out = static_cast<T*>(a.dlogits) + at * a.experts;
 #pragma unroll
@@ -607,10 +678,24 @@ int check_rows_of(const std::string& what, int64_t stride, int64_t n, int choice
     return 0;
 }
 
-template <class T, int kLanes, int kVecs> void launch_choose(const ChooseArgs& a, hipStream_t stream) {
-    in_launches((a.n + kBlock / kLanes - 1) / (kBlock / kLanes), kBlock, [&](uint32_t first, uint32_t count) {
-        choose_kernel<T, kLanes, kVecs><<<count, kBlock, 0, stream>>>(a, first);
-    });
+// Lanes and 16-byte chunks a lane that hold a row; 0 chunks: longer rows.
+template <class T, class F> void with_row(int width, int least, F&& f) {
+    const int chunks = (width + kPerVec<T> - 1) / kPerVec<T>;
+    if (chunks <= 64) with_lanes<T>(width, least, [&](auto lanes) { f(lanes, std::integral_constant<int, 1>{}); });
+    else if (chunks <= 128) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    else if (chunks <= 256) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+    else if (chunks <= 512) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
+    else f(std::integral_constant<int, 64>{}, std::integral_constant<int, 0>{});
+}
+
+// Workgroups of the passes over rows, `lanes` lanes a row: as many as the CUs hold together by their registers, so that
+// all of them run to the end: two each with 8 chunks a lane, four with 4, six with fewer (65536 x 1024 fp16, choice: 52.5 us
+// with four, 50 with six, 49 with eight; 300007 x 1000 bf16, balance: 170, 160, 158).  Passes that also write a row lose by
+// more than four (its gradient: 243, 251, 262).
+uint32_t row_blocks(int64_t n, int lanes, int vecs, bool writes = false) {
+    const int64_t blocks = (n + kBlock / lanes - 1) / (kBlock / lanes);
+    const int64_t most = (vecs == 8 ? 2 : (vecs == 4 || writes ? 4 : 6)) * kCus;
+    return static_cast<uint32_t>(blocks < 1 ? 1 : (blocks < most ? blocks : most));
 }
 
 }  // namespace
@@ -625,20 +710,15 @@ ODIE_API int odie_choose_forward(const void* logits, int64_t stride, int64_t n, 
     if (choices > kMaxChoices || choices > experts) return fail(what + ": choices must be within 1..64 and the experts");
     if (n == 0) return 0;
     if (!logits || !expert || !weights) return fail(what + ": null pointer");
+    if (reinterpret_cast<uintptr_t>(stats) % 8) return fail(what + ": stats must be 8-byte aligned");
     ChooseArgs a{logits, stride, n, expert, weights, stats, experts, choices, normalize};
     const hipStream_t s = as_stream(stream);
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        const int chunks = (experts + kPerVec<T> - 1) / kPerVec<T>;
-        if (chunks > 64 * (sizeof(T) == 4 ? 16 : 8)) {
-            choose_long_kernel<T><<<static_cast<uint32_t>(n < 16 * kCus ? n : 16 * kCus), kBlock, 0, s>>>(a);
-            return check_launch("choose");
-        }
-        if (chunks <= 64) with_lanes<T>(experts, choices, [&](auto lanes) { launch_choose<T, lanes, 1>(a, s); });
-        else if (chunks <= 128) launch_choose<T, 64, 2>(a, s);
-        else if (chunks <= 256) launch_choose<T, 64, 4>(a, s);
-        else if (chunks <= 512) launch_choose<T, 64, 8>(a, s);
-        else if constexpr (sizeof(T) == 4) launch_choose<T, 64, 16>(a, s);
+        with_row<T>(experts, choices, [&](auto lanes, auto vecs) {
+            if constexpr (vecs > 0) choose_kernel<T, lanes, vecs><<<row_blocks(n, lanes, vecs), kBlock, 0, s>>>(a);
+            else choose_long_kernel<T><<<static_cast<uint32_t>(n < 16 * kCus ? n : 16 * kCus), kBlock, 0, s>>>(a);
+        });
         return check_launch("choose");
     });
 }
@@ -667,29 +747,6 @@ ODIE_API int odie_choose_backward(const float* upstream, const int32_t* expert, 
         return check_launch("choose gradient");
     });
 }
-
-namespace odie {
-namespace {
-
-// Lanes and 16-byte chunks a lane that hold a row; 0 chunks: longer rows.
-template <class T, class F> void with_row(int width, F&& f) {
-    const int chunks = (width + kPerVec<T> - 1) / kPerVec<T>;
-    if (chunks <= 64) with_lanes<T>(width, 1, [&](auto lanes) { f(lanes, std::integral_constant<int, 1>{}); });
-    else if (chunks <= 128) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-    else if (chunks <= 256) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
-    else if (chunks <= 512) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
-    else f(std::integral_constant<int, 64>{}, std::integral_constant<int, 0>{});
-}
-
-// Workgroups of the passes over rows, `lanes` lanes a row: as many as the CUs hold together by their registers (four each,
-// two with 8 chunks a lane), so that all of them run to the end.
-uint32_t row_blocks(int64_t n, int lanes, int vecs) {
-    const int64_t blocks = (n + kBlock / lanes - 1) / (kBlock / lanes), most = (vecs < 8 ? 4 : 2) * kCus;
-    return static_cast<uint32_t>(blocks < 1 ? 1 : (blocks < most ? blocks : most));
-}
-
-}  // namespace
-}  // namespace odie
 
 ODIE_API int64_t odie_balance_workspace(int64_t n, int choices, int experts) {
     if (check_rows_of("odie_balance_workspace", experts, n, choices, experts, ODIE_F32)) return -1;
@@ -734,7 +791,7 @@ ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int3
     }
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        with_row<T>(experts, [&](auto lanes, auto vecs) {
+        with_row<T>(experts, 1, [&](auto lanes, auto vecs) {
             if constexpr (vecs > 0) balance_rows_kernel<T, lanes, vecs><<<row_blocks(n, lanes, vecs), kBlock, 0, s>>>(a);
             else balance_long_kernel<T><<<row_blocks(n, 64, 1), kBlock, 0, s>>>(a);
         });
@@ -755,9 +812,9 @@ ODIE_API int odie_balance_backward(const float* upstream, const void* logits, in
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
         with_flag(n * experts * dtype_bytes(dtype) >= kStreamBytes, [&](auto far) {
-            with_row<T>(experts, [&](auto lanes, auto vecs) {
-                if constexpr (vecs > 0) balance_backward_kernel<T, lanes, vecs, far><<<row_blocks(n, lanes, vecs), kBlock, 0, s>>>(a);
-                else balance_long_backward_kernel<T, far><<<row_blocks(n, 64, 1), kBlock, 0, s>>>(a);
+            with_row<T>(experts, 1, [&](auto lanes, auto vecs) {
+                if constexpr (vecs > 0) balance_backward_kernel<T, lanes, vecs, far><<<row_blocks(n, lanes, vecs, true), kBlock, 0, s>>>(a);
+                else balance_long_backward_kernel<T, far><<<row_blocks(n, 64, 1, true), kBlock, 0, s>>>(a);
             });
         });
         return check_launch("balance gradient");

@@ -33,6 +33,7 @@ def test_choose_refusals(native):
         _refused(native, call(weights=None), what, 'null')
         assert call(n=0) == 0
     _refused(native, f(logits=None), 'null')
+    _refused(native, f(stats=4), 'stats', 'aligned')
     _refused(native, b(stats=None), 'null')
     _refused(native, b(upstream=None), 'null')
     _refused(native, b(out=None), 'null')
