@@ -179,7 +179,9 @@ template <class T> __device__ inline void patch_entry(const DistillArgs& a, int6
     out[id] = static_cast<T>(value);
 }
 
-// A piece of a row's gradient: kLanes threads (some of a wave's, or the workgroup).
+// A piece of a row's gradient: kLanes threads (some of a wave's, or the workgroup).  A workgroup's stores begin on lines
+// of 128 bytes, whatever the row does (8192 x 65032 bf16: 514 -> 465 us; rows that begin on lines themselves 455): the row's elements before
+// the first line go one by one, and its pieces are cut at lines.
 template <class T, int kLanes, bool kStream>
 __global__ __launch_bounds__(kBlock) void distill_backward_kernel(DistillArgs a, uint32_t first) {
     constexpr int kV = kPerVec<T>;
@@ -187,22 +189,32 @@ __global__ __launch_bounds__(kBlock) void distill_backward_kernel(DistillArgs a,
     const int64_t at = (static_cast<int64_t>(first) + blockIdx.x) * (kBlock / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
     const int64_t row = at / a.pieces;
     const bool inside = row < a.n;
-    const int begin = static_cast<int>(at % a.pieces) * a.piece;
-    const int end = begin + a.piece < a.classes ? begin + a.piece : a.classes;
+    const int piece = static_cast<int>(at % a.pieces);
     const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
     T* out = static_cast<T*>(a.dlogits) + row * a.classes;
+    constexpr int kLine = 128 / static_cast<int>(sizeof(T));
+    const int past = kLanes == kBlock ? static_cast<int>(reinterpret_cast<uintptr_t>(out) / sizeof(T) % kLine) : 0;   // the line before
+    const int begin = piece == 0 ? 0 : piece * a.piece - past;
+    const int end = piece == a.pieces - 1 ? a.classes : (piece + 1) * a.piece - past;
+    const int head = piece == 0 && past > 0 ? (kLine - past < end ? kLine - past : end) : 0;
     float stats[4] = {}, scale = 0.0f;
     if (inside) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) stats[i] = a.stats[row * 4 + i];
         scale = a.upstream[row] * a.inverse;
         const float each = scale * stats[1];
-        for_chunks<T, kLanes, kLanes == kBlock ? 4 : 1>(logits, begin, end, a.classes, lane, [&](int column, float (&value)[kV]) {
+        const auto gradient = [&](float logit) {
+            const float p = each * exponential<sizeof(T) == 4>(fmaf(logit, a.inverse, -stats[0]));
+            return stats[3] == 0.0f ? 0.0f : p;
+        };
+        for (int column = lane; column < head; column += kLanes) {
+            float value = gradient(static_cast<float>(logits[column]));
+            asm("" : "+v"(value));      // rounded to fp32, then to T, as its neighbours are
+            out[column] = static_cast<T>(value);
+        }
+        for_chunks<T, kLanes, kLanes == kBlock ? 4 : 1>(logits, begin + head, end, a.classes, lane, [&](int column, float (&value)[kV]) {
 #pragma unroll
-            for (int i = 0; i < kV; ++i) {
-                const float p = each * exponential<sizeof(T) == 4>(fmaf(value[i], a.inverse, -stats[0]));
-                value[i] = stats[3] == 0.0f ? 0.0f : p;
-            }
+            for (int i = 0; i < kV; ++i) value[i] = gradient(value[i]);
             store_some<kStream>(out + column, narrow<T>(value), a.classes - column);
         });
     }
