@@ -46,13 +46,13 @@ def linear(x, weight, bias=None, *, activation='none', residual=None, offsets=No
     n, inputs = x.shape
     lead = 1 if offsets is None else 2      # dimensions before the inputs
     four_bits = isinstance(weight, Microscaled)
-    if (not (four_bits or isinstance(weight, torch.Tensor)) or weight.ndim != lead + 1 or weight.shape[-1] != inputs
-            or not (four_bits or weight.dtype == x.dtype) or weight.device != x.device or weight.shape[0] == 0
-            or weight.shape[-2] == 0):
+    shape = weight.shape if four_bits or isinstance(weight, torch.Tensor) else ()
+    if (len(shape) != lead + 1 or shape[-1] != inputs or not (four_bits or weight.dtype == x.dtype)
+            or weight.device != x.device or shape[0] == 0 or shape[-2] == 0):
         raise ValueError('weight must be %s of x\'s dtype and device' %
                          ('[outputs, inputs]' if offsets is None else '[experts, outputs, inputs]'))
-    outputs, experts = weight.shape[-2], 1 if offsets is None else weight.shape[0]
-    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.shape != weight.shape[:-1]
+    outputs, experts = shape[-2], 1 if offsets is None else shape[0]
+    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.shape != shape[:-1]
                              or bias.dtype != x.dtype or bias.device != x.device):
         raise ValueError('bias must be %s of x\'s dtype and device' %
                          ('[outputs]' if offsets is None else '[experts, outputs]'))
@@ -130,16 +130,16 @@ class _Linear(torch.autograd.Function):
 
 
 def _forward4(x, weight, bias, residual, offsets, activation, pre):
-    n, outputs = x.shape[0], weight.shape[-2]
+    n, (*experts, outputs, inputs) = x.shape[0], weight.shape
     if isinstance(x, Microscaled):
         rows, rows_scales, stride = x.codes, x.scales, 0
     else:
         rows, rows_scales, stride = x, None, pitch(x)
-    out = torch.empty((n, outputs), dtype=x.dtype, device=x.device)
+    out = rows.new_empty((n, outputs), dtype=x.dtype)
     _lib.call('odie_mx_linear_forward', rows, rows.data_ptr(), _lib.ptr(rows_scales), stride, n, weight.codes.data_ptr(),
               weight.scales.data_ptr(), _lib.ptr(bias), _lib.ptr(residual), 0 if residual is None else pitch(residual),
-              _lib.ptr(offsets), 1 if offsets is None else weight.shape[0], weight.width, outputs, DTYPES[x.dtype],
-              activation, out.data_ptr(), outputs, _lib.ptr(pre))
+              _lib.ptr(offsets), experts[0] if experts else 1, inputs, outputs, DTYPES[x.dtype], activation,
+              out.data_ptr(), outputs, _lib.ptr(pre))
     return out
 
 

@@ -25,7 +25,7 @@ class Microscaled:
     first in the low half, each sign, two bits of exponent and one of fraction, 0 past the width; scales uint8 [...,
     blocks rounded up to a multiple of 4]: 2^(scale - 127), 255 for NaN, 0 past the last block.  dtype (fp32, fp16 or
     bf16): of the tensor it stands for, and of what is computed from it.  Both are taken as they are, or
-    copied where they are not contiguous and aligned."""
+    copied where they are not contiguous and aligned.  shape, ndim and device are the tensor's."""
 
     def __init__(self, codes, scales, width, dtype=torch.bfloat16):
         if (not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor) or codes.dtype != torch.uint8
@@ -38,27 +38,18 @@ class Microscaled:
                              'whole fours')
         if dtype not in DTYPES:
             raise ValueError('dtype must be fp32, fp16 or bf16')
-        self.codes, self.scales = _aligned(codes, 16), _aligned(scales, 4)
-        self.width, self.dtype = width, dtype
+        self._hold(_aligned(codes, 16), _aligned(scales, 4), width, dtype, (*codes.shape[:-1], width))
 
-    @property
-    def shape(self):
-        return torch.Size((*self.codes.shape[:-1], self.width))
-
-    @property
-    def ndim(self):
-        return self.codes.ndim
-
-    @property
-    def device(self):
-        return self.codes.device
+    def _hold(self, codes, scales, width, dtype, shape):
+        self.codes, self.scales, self.width, self.dtype = codes, scales, width, dtype
+        self.shape, self.ndim, self.device = torch.Size(shape), len(shape), codes.device
 
     def dequantize(self, dtype=None):
         """The tensor of dtype (its own if not given), rounded where that does not hold a value."""
         dtype = self.dtype if dtype is None else dtype
         if dtype not in DTYPES:
             raise ValueError('dtype must be fp32, fp16 or bf16')
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        out = self.codes.new_empty(self.shape, dtype=dtype)
         _lib.call('odie_mx_dequantize', self.codes, self.codes.data_ptr(), self.scales.data_ptr(),
                   math.prod(self.shape[:-1]), self.width, DTYPES[dtype], out.data_ptr(), self.width)
         return out
@@ -74,13 +65,15 @@ def quantize(x):
     an infinity becomes NaN.  The result is whole numbers: no gradient passes through them."""
     if not isinstance(x, torch.Tensor) or x.dtype not in DTYPES or x.ndim not in (2, 3) or not x.is_cuda:
         raise ValueError('x must be a CUDA fp32, fp16 or bf16 tensor of two or three dimensions')
-    if not 1 <= x.shape[-1] <= 1 << 20:
+    *lead, width = x.shape
+    if not 1 <= width <= 1 << 20:
         raise ValueError('x must have 1 to 2^20 columns')
-    x = x.detach()
-    rows = row_major(x if x.ndim == 2 else x.reshape(-1, x.shape[-1]))
-    n, width = rows.shape
-    codes = torch.empty((*x.shape[:-1], 16 * _blocks(width)), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], (_blocks(width) + 3) // 4 * 4), dtype=torch.uint8, device=x.device)
-    _lib.call('odie_mx_quantize', rows, rows.data_ptr(), pitch(rows), n, width, DTYPES[x.dtype], codes.data_ptr(),
-              scales.data_ptr())
-    return Microscaled(codes, scales, width, x.dtype)
+    rows = row_major(x if x.ndim == 2 else x.detach().reshape(-1, width))
+    blocks = _blocks(width)
+    codes = x.new_empty((*lead, 16 * blocks), dtype=torch.uint8)
+    scales = x.new_empty((*lead, (blocks + 3) // 4 * 4), dtype=torch.uint8)
+    _lib.call('odie_mx_quantize', rows, rows.data_ptr(), pitch(rows), rows.shape[0], width, DTYPES[x.dtype],
+              codes.data_ptr(), scales.data_ptr())
+    made = Microscaled.__new__(Microscaled)     # nothing to check
+    made._hold(codes, scales, width, x.dtype, (*lead, width))
+    return made

@@ -76,12 +76,12 @@ def distill(logits, ids, teacher, *, temperature=1.0):
 
 
 def _floats(logits, *shape):
-    return torch.empty(shape, dtype=torch.float32, device=logits.device)
+    return logits.new_empty(shape, dtype=torch.float32)
 
 
 def _choose(logits, choices, normalize, stats):
     n, experts = logits.shape
-    expert = torch.empty((n, choices), dtype=torch.int32, device=logits.device)
+    expert = logits.new_empty((n, choices), dtype=torch.int32)
     weights = _floats(logits, n, choices)
     _lib.call('odie_choose_forward', logits, logits.data_ptr(), pitch(logits), n, experts, choices, int(normalize),
               DTYPES[logits.dtype], expert.data_ptr(), weights.data_ptr(), _lib.ptr(stats))
@@ -91,7 +91,7 @@ def _choose(logits, choices, normalize, stats):
 def _balance(logits, expert, stats, norm):
     n, experts = logits.shape
     choices = expert.shape[1]
-    loss, counts = _floats(logits), torch.empty(experts, dtype=torch.int32, device=logits.device)
+    loss, counts = _floats(logits), logits.new_empty(experts, dtype=torch.int32)
     norm = _floats(logits) if norm is None else norm
     scratch = _lib.scratch('odie_balance_workspace', logits, n, choices, experts)
     _lib.call('odie_balance_forward', logits, logits.data_ptr(), pitch(logits), expert.data_ptr(), n, choices, experts,
@@ -150,7 +150,7 @@ class _Balance(torch.autograd.Function):
         logits, counts, stats, norm = ctx.saved_tensors
         n, experts = logits.shape
         upstream = upstream.contiguous()
-        dlogits = torch.empty((n, experts), dtype=logits.dtype, device=logits.device)
+        dlogits = logits.new_empty((n, experts))
         _lib.call('odie_balance_backward', logits, upstream.data_ptr(), logits.data_ptr(), pitch(logits),
                   counts.data_ptr(), stats.data_ptr(), norm.data_ptr(), n, experts, DTYPES[logits.dtype],
                   dlogits.data_ptr())
@@ -172,7 +172,7 @@ class _Distill(torch.autograd.Function):
         logits, ids, teacher, stats = ctx.saved_tensors
         n, classes = logits.shape
         upstream = upstream.contiguous()
-        dlogits = torch.empty((n, classes), dtype=logits.dtype, device=logits.device)
+        dlogits = logits.new_empty((n, classes))
         _lib.call('odie_distill_backward', logits, upstream.data_ptr(), logits.data_ptr(), pitch(logits), ids.data_ptr(),
                   ids.element_size(), teacher.data_ptr(), DTYPES[teacher.dtype], stats.data_ptr(), n, classes,
                   ids.shape[1], ctx.temperature, DTYPES[logits.dtype], dlogits.data_ptr())
