@@ -8,6 +8,9 @@ number of experts with a weight each: a blend over the borders of neighbouring t
   sent  = dispatch(x, order)                       [N * choices, width], sorted by expert
   ...   = linear(sent, W, b, offsets=order.offsets)
   y     = combine(rows, order, weights)            y[i] = sum_j weights[i, j] rows[slots[i, j]]
+
+RoutedMixture has the learned router (odie_amd.router), and MicroscaledMixture keeps a mixture's layers in 4 bits
+(odie_amd.microscale).
 """
 import math
 import numbers
@@ -19,6 +22,8 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .embedding import embed
 from .linear import ACTIVATIONS, linear
+from .microscale import Microscaled, quantize
+from .router import choose
 from .rows import DTYPES, check_rows, pitch, records, row_major
 
 
@@ -164,11 +169,74 @@ class ExpertMixture(nn.Module):
     def forward(self, x, expert, weights=None, ids=None):
         """x [N, inputs], expert [N, choices] (other values than 0..experts-1: none), weights [N, choices];
         ids [N] with codes.  Returns [N, outputs]."""
-        if (ids is None) != (self.table is None):
-            raise ValueError('give ids exactly where the mixture has codes')
-        if ids is not None:
-            x = torch.cat((x, embed(self.table, ids, self.scale)), dim=1)
-        order = expert_order(expert, self.experts)
-        hidden = linear(dispatch(x, order), self.weight1, self.bias1, activation=self.activation, offsets=order.offsets)
-        rows = linear(hidden, self.weight2, self.bias2, offsets=order.offsets)
-        return combine(rows, order, weights)
+        return _blend(self, self.weight1, self.weight2, x, expert, weights, ids)
+
+    def microscaled(self, *, rows=False):
+        """A MicroscaledMixture of the parameters as they are now."""
+        return MicroscaledMixture(self, rows=rows)
+
+
+def _blend(mixture, weight1, weight2, x, expert, weights, ids, rows4=False):
+    if (ids is None) != (mixture.table is None):
+        raise ValueError('give ids exactly where the mixture has codes')
+    if ids is not None:
+        x = torch.cat((x, embed(mixture.table, ids, mixture.scale)), dim=1)
+    order = expert_order(expert, mixture.experts)
+    bits = quantize if rows4 else (lambda value: value)
+    hidden = linear(bits(dispatch(x, order)), weight1, mixture.bias1, activation=mixture.activation, offsets=order.offsets)
+    rows = linear(bits(hidden), weight2, mixture.bias2, offsets=order.offsets)
+    return combine(rows, order, weights)
+
+
+class MicroscaledMixture(nn.Module):
+    """An ExpertMixture whose layers' weights are kept in 4 bits, 4.25 each with their scales: for serving it, or for
+    training what lies before it (x and the router's weights get their gradients; the mixture's own parameters,
+    copied here, are buffers).  With rows=True the rows that enter a layer are quantised to 4 bits too, and there is no
+    gradient of x."""
+
+    def __init__(self, mixture, *, rows=False):
+        super().__init__()
+        self.experts, self.activation, self.scale, self.rows = mixture.experts, mixture.activation, mixture.scale, bool(rows)
+        self.dtype, self.widths = mixture.weight1.dtype, (mixture.weight1.shape[2], mixture.weight2.shape[2])
+        for name in ('table', 'bias1', 'bias2'):
+            value = getattr(mixture, name)
+            self.register_buffer(name, None if value is None else value.detach().clone())
+        for layer in (1, 2):
+            weight = quantize(getattr(mixture, 'weight%d' % layer))
+            self.register_buffer('codes%d' % layer, weight.codes)
+            self.register_buffer('scales%d' % layer, weight.scales)
+
+    def forward(self, x, expert, weights=None, ids=None):
+        """As ExpertMixture.forward."""
+        weight1, weight2 = (Microscaled(getattr(self, 'codes%d' % layer), getattr(self, 'scales%d' % layer),
+                                        self.widths[layer - 1], self.dtype) for layer in (1, 2))
+        if self.rows:
+            if records(x):
+                raise ValueError('rows of 4 bits have no backward: detach x')
+        return _blend(self, weight1, weight2, x, expert, weights, ids, self.rows)
+
+
+class RoutedMixture(nn.Module):
+    """A mixture that chooses its experts itself: logits = x R^T, and each row's `choices` largest with their softmax
+    weights (over the chosen, or with normalize=False over all) blend the experts' decoders.  The arguments are
+    ExpertMixture's and choose's."""
+
+    def __init__(self, experts, choices, inputs, hidden, outputs, *, normalize=True, activation='relu', codes=0, vocab=0,
+                 dtype=torch.float16, device='cuda', seed=0):
+        super().__init__()
+        self.mixture = ExpertMixture(experts, inputs, hidden, outputs, activation=activation, codes=codes, vocab=vocab,
+                                     dtype=dtype, device=device, seed=seed)
+        self.choices, self.normalize = int(choices), bool(normalize)
+        generator = torch.Generator().manual_seed(seed + 1)
+        value = torch.randn(experts, inputs, generator=generator) * inputs ** -0.5
+        self.router = nn.Parameter(value.to(device=device, dtype=dtype))
+
+    def forward(self, x, ids=None, allowed=None):
+        """y [N, outputs], the router's logits [N, experts] (for balance and distill of odie_amd.router) and the chosen
+        expert int32 [N, choices].  allowed (bool, [N, experts] or [experts]): where False, the expert is not
+        chosen; a row without an allowed one gets zeros."""
+        logits = linear(x, self.router)
+        if allowed is not None:
+            logits = logits.masked_fill(~allowed, -math.inf)
+        expert, weights = choose(logits, self.choices, normalize=self.normalize)
+        return self.mixture(x, expert, weights, ids), logits, expert
