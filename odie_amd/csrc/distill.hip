@@ -17,6 +17,7 @@ constexpr int kBlock = 256;
 constexpr int kMaxClasses = 1 << 24;
 constexpr int kMaxTop = 1024;
 constexpr int kShort = 512;        // classes of a row that some lanes of a wave take
+constexpr int kMostPiece = 1 << 16; // classes of a longer row's piece in the backward
 
 struct DistillArgs {
     const void* logits;       // [n][classes], stride
@@ -161,18 +162,22 @@ template <class T> __global__ __launch_bounds__(64) void distill_join_kernel(Dis
     finish_row<T, 64>(a, row, static_cast<int>(threadIdx.x), true, run.m, run.s);
 }
 
-// The gradient at the row's entry j where it is the first of its class: p - Q.
-template <class T> __device__ inline void patch_entry(const DistillArgs& a, int64_t row, int j, int begin, int end, const T* logits, T* out, float scale,
-                                                      const float* stats) {
+// The gradient at the row's entry j, p - Q, from the piece [begin, end) of the row.  The first entry of a class that several
+// name (`twice`, a bit for each class of the piece) adds up the others'.
+template <class T>
+__device__ inline void patch_entry(const DistillArgs& a, int64_t row, int j, int begin, int end, const uint32_t* twice, const T* logits,
+                                   T* out, float scale, const float (&stats)[4]) {
     int64_t id, other;
     const float entry = entry_of(a, row, j, id);
     if (id < begin || id >= end) return;
     float share = expf(entry - stats[2]) * stats[3];
-    for (int i = 0; i < a.top; ++i) {
-        if (i == j || id_of(a, row * a.top + i) != id) continue;
-        if (i < j) return;
-        share += expf(entry_of(a, row, i, other) - stats[2]) * stats[3];
-    }
+    const int place = static_cast<int>(id) - begin;
+    if (twice[place / 32] >> place % 32 & 1)
+        for (int i = 0; i < a.top; ++i) {
+            if (i == j || id_of(a, row * a.top + i) != id) continue;
+            if (i < j) return;
+            share += expf(entry_of(a, row, i, other) - stats[2]) * stats[3];
+        }
     const float p = expf(static_cast<float>(logits[id]) * a.inverse - stats[0]) * stats[1];
     float value = scale * (p - share);
     asm("" : "+v"(value));      // rounded to fp32, then to T, as its neighbours are
@@ -181,11 +186,15 @@ template <class T> __device__ inline void patch_entry(const DistillArgs& a, int6
 
 // A piece of a row's gradient: kLanes threads (some of a wave's, or the workgroup).  A workgroup's stores begin on lines
 // of 128 bytes, whatever the row does (8192 x 65032 bf16: 514 -> 465 us; rows that begin on lines themselves 455): the row's elements before
-// the first line go one by one, and its pieces are cut at lines.
+// the first line go one by one, and its pieces are cut at lines.  Two bits for each class of the piece tell whether no, one or
+// several entries name it: those of a class that one names, as a teacher's largest logits do, need not look for others
+// (8192 x 1024 with 128 entries a row: 129 us where each looks at all, 18 so).
 template <class T, int kLanes, bool kStream>
 __global__ __launch_bounds__(kBlock) void distill_backward_kernel(DistillArgs a, uint32_t first) {
-    constexpr int kV = kPerVec<T>;
+    constexpr int kV = kPerVec<T>, kWords = kLanes == kBlock ? (kMostPiece + 64) / 32 : kShort / 32;
+    __shared__ uint32_t bits[kBlock / kLanes][2][kWords];
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
+    uint32_t *const once = bits[static_cast<int>(threadIdx.x) / kLanes][0], *const twice = bits[static_cast<int>(threadIdx.x) / kLanes][1];
     const int64_t at = (static_cast<int64_t>(first) + blockIdx.x) * (kBlock / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
     const int64_t row = at / a.pieces;
     const bool inside = row < a.n;
@@ -197,6 +206,17 @@ __global__ __launch_bounds__(kBlock) void distill_backward_kernel(DistillArgs a,
     const int begin = piece == 0 ? 0 : piece * a.piece - past;
     const int end = piece == a.pieces - 1 ? a.classes : (piece + 1) * a.piece - past;
     const int head = piece == 0 && past > 0 ? (kLine - past < end ? kLine - past : end) : 0;
+    for (int w = lane; w < (end - begin + 31) / 32; w += kLanes) once[w] = twice[w] = 0;
+    if constexpr (kLanes == kBlock) __syncthreads();
+    else wave_fence();
+    if (inside)
+        for (int j = lane; j < a.top; j += kLanes) {
+            const int64_t id = id_of(a, row * a.top + j);
+            if (id < begin || id >= end) continue;
+            const int place = static_cast<int>(id) - begin;
+            const uint32_t bit = 1u << place % 32;
+            if (atomicOr(once + place / 32, bit) & bit) atomicOr(twice + place / 32, bit);
+        }
     float stats[4] = {}, scale = 0.0f;
     if (inside) {
 #pragma unroll
@@ -222,7 +242,7 @@ __global__ __launch_bounds__(kBlock) void distill_backward_kernel(DistillArgs a,
     if constexpr (kLanes == kBlock) __syncthreads();
     else __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
     if (!inside || stats[3] == 0.0f) return;
-    for (int j = lane; j < a.top; j += kLanes) patch_entry(a, row, j, begin, end, logits, out, scale, stats);
+    for (int j = lane; j < a.top; j += kLanes) patch_entry(a, row, j, begin, end, twice, logits, out, scale, stats);
 }
 
 int check_distill(const std::string& what, int64_t n, int classes, int top, int dtype) {
@@ -233,10 +253,13 @@ int check_distill(const std::string& what, int64_t n, int classes, int top, int 
     return 0;
 }
 
-// Pieces that a long row is cut into, each of whole rounds of its workgroup: about four workgroups a CU at least.
-void cut(DistillArgs& a, int values) {
+// Pieces that a long row is cut into, each of whole rounds of its workgroup: about four workgroups a CU at least, and at most
+// `most` classes a piece.
+void cut(DistillArgs& a, int values, int64_t most) {
     const int64_t wanted = a.n < 4 * kCus ? (4 * kCus + a.n - 1) / a.n : 1, round = static_cast<int64_t>(kBlock) * values;
-    const int64_t rounds = (a.classes + round - 1) / round, pieces = wanted < rounds ? wanted : rounds;
+    const int64_t rounds = (a.classes + round - 1) / round, least = (a.classes + most - 1) / most;
+    int64_t pieces = wanted < rounds ? wanted : rounds;
+    pieces = pieces < least ? least : pieces;
     a.piece = static_cast<int>((rounds + pieces - 1) / pieces * round);
     a.pieces = (a.classes + a.piece - 1) / a.piece;
 }
@@ -260,7 +283,7 @@ ODIE_API int64_t odie_distill_workspace(int64_t n, int classes, int dtype) {
     DistillArgs a{};
     a.n = n;
     a.classes = classes;
-    cut(a, dtype == ODIE_F32 ? 4 : 8);
+    cut(a, dtype == ODIE_F32 ? 4 : 8, kMaxClasses);
     return a.pieces > 1 ? n * a.pieces * static_cast<int64_t>(sizeof(float2)) : 0;
 }
 
@@ -291,7 +314,7 @@ ODIE_API int odie_distill_forward(const void* logits, int64_t stride, const void
             });
             return check_launch("distill");
         }
-        cut(a, kPerVec<T>);
+        cut(a, kPerVec<T>, kMaxClasses);
         in_launches(n * a.pieces, kBlock, [&](uint32_t first, uint32_t count) {
             distill_piece_kernel<T><<<count, kBlock, 0, s>>>(a, first);
         });
@@ -324,7 +347,7 @@ ODIE_API int odie_distill_backward(const float* upstream, const void* logits, in
                     });
                 });
             } else {
-                cut(a, kPerVec<T>);
+                cut(a, kPerVec<T>, kMostPiece);
                 in_launches(n * a.pieces, kBlock, [&](uint32_t first, uint32_t count) {
                     distill_backward_kernel<T, kBlock, far><<<count, kBlock, 0, s>>>(a, first);
                 });
