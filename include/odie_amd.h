@@ -721,6 +721,16 @@ int odie_mx_linear_forward(const void* x, const uint8_t* x_scales, int64_t x_str
                            const int32_t* offsets, int experts, int inputs, int outputs, int dtype, int activation, void* out,
                            int64_t out_stride, void* pre, uint64_t stream);
 
+/* Gradients of odie_mx_linear_forward with rows of dtype: dx [rows][inputs] (0 in rows of no expert) and dbias (shaped as
+ * bias), each or null; as odie_linear_backward with the weight's values in dtype.  codes and scales may be null without dx.
+ * workspace: 256-byte aligned, odie_mx_linear_workspace bytes (the weight in dtype among them). */
+int64_t odie_mx_linear_workspace(int64_t rows, int experts, int grouped, int inputs, int outputs, int dtype,
+                                 int activation, int want_dx, int want_dbias);
+int odie_mx_linear_backward(const void* upstream, int64_t upstream_stride, const void* pre, int64_t rows,
+                            const uint8_t* codes, const uint8_t* scales, const int32_t* offsets, int experts, int inputs,
+                            int outputs, int dtype, int activation, void* dx, void* dbias, void* workspace,
+                            int64_t workspace_bytes, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -99,6 +99,8 @@ SIGNATURES = {
     'odie_mx_dequantize': ([_P, _P, _I64, _I64, _I, _P, _I64, _U64], _I),
     'odie_mx_linear_forward': ([_P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _P, _I, _I, _I, _I, _I, _P, _I64, _P, _U64],
                                _I),
+    'odie_mx_linear_workspace': ([_I64, _I, _I, _I, _I, _I, _I, _I, _I], _I64),
+    'odie_mx_linear_backward': ([_P, _I64, _P, _I64, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _I64, _U64], _I),
     'odie_create': ([C.c_char_p], _P),
     'odie_step': ([_P, _U64, _I, _I], _I),
     'odie_configure': ([_P, C.c_char_p], _I),

@@ -84,23 +84,6 @@ def _forward(x, weight, bias, residual, offsets, activation, pre):
     return out
 
 
-def _gradients(upstream, x, weight, pre, offsets, ctx, want_x, want_weight, want_bias):
-    rows = row_major(upstream)
-    n, inputs = rows.shape[0], ctx.inputs
-    outputs, experts = rows.shape[1], 1 if offsets is None else ctx.weights[0]
-    dtype = DTYPES[rows.dtype]
-    dx = rows.new_empty((n, inputs)) if want_x else None
-    dweight = rows.new_empty(ctx.weights) if want_weight else None
-    dbias = rows.new_empty(ctx.weights[:-1]) if want_bias else None
-    scratch = _lib.scratch('odie_linear_workspace', rows, n, experts, int(offsets is not None), inputs, outputs,
-                           dtype, ctx.activation, int(want_weight), int(want_bias))
-    _lib.call('odie_linear_backward', rows, rows.data_ptr(), pitch(rows), _lib.ptr(x), 0 if x is None else pitch(x),
-              _lib.ptr(pre), n, _lib.ptr(weight), _lib.ptr(offsets), experts, inputs, outputs, dtype,
-              ctx.activation, _lib.ptr(dx), _lib.ptr(dweight), _lib.ptr(dbias), _lib.ptr(scratch),
-              0 if scratch is None else scratch.numel())
-    return dx, dweight, dbias
-
-
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, offsets, activation):
@@ -125,7 +108,19 @@ class _Linear(torch.autograd.Function):
         want_x, want_weight, want_bias, want_residual = ctx.needs_input_grad[:4]
         dx = dweight = dbias = None
         if want_x or want_weight or want_bias:
-            dx, dweight, dbias = _gradients(upstream, x, weight, pre, offsets, ctx, want_x, want_weight, want_bias)
+            rows = row_major(upstream)
+            n, inputs = rows.shape[0], ctx.inputs
+            outputs, experts = rows.shape[1], 1 if offsets is None else ctx.weights[0]
+            dtype = DTYPES[rows.dtype]
+            dx = rows.new_empty((n, inputs)) if want_x else None
+            dweight = rows.new_empty(ctx.weights) if want_weight else None
+            dbias = rows.new_empty(ctx.weights[:-1]) if want_bias else None
+            scratch = _lib.scratch('odie_linear_workspace', rows, n, experts, int(offsets is not None), inputs, outputs,
+                                   dtype, ctx.activation, int(want_weight), int(want_bias))
+            _lib.call('odie_linear_backward', rows, rows.data_ptr(), pitch(rows), _lib.ptr(x),
+                      0 if x is None else pitch(x), _lib.ptr(pre), n, _lib.ptr(weight), _lib.ptr(offsets), experts, inputs, outputs, dtype,
+                      ctx.activation, _lib.ptr(dx), _lib.ptr(dweight), _lib.ptr(dbias), _lib.ptr(scratch),
+                      0 if scratch is None else scratch.numel())
         return dx, dweight, dbias, upstream if want_residual else None, None, None
 
 
@@ -144,7 +139,7 @@ def _forward4(x, weight, bias, residual, offsets, activation, pre):
 
 
 class _Linear4(torch.autograd.Function):
-    """A weight of 4 bits: gradients of x, bias and residual.  The backward widens the weight to x's dtype first."""
+    """A weight of 4 bits: gradients of x, bias and residual."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, offsets, activation):
@@ -156,7 +151,7 @@ class _Linear4(torch.autograd.Function):
         # what the wanted gradients read
         ctx.save_for_backward(weight.codes if want_x else None, weight.scales if want_x else None, pre,
                               offsets if computed else None)
-        ctx.activation, ctx.inputs, ctx.weights, ctx.dtype = activation, x.shape[1], weight.shape, x.dtype
+        ctx.activation, ctx.inputs, ctx.weights = activation, x.shape[1], weight.shape
         return out
 
     @staticmethod
@@ -166,6 +161,14 @@ class _Linear4(torch.autograd.Function):
         want_x, _, want_bias, want_residual = ctx.needs_input_grad[:4]
         dx = dbias = None
         if want_x or want_bias:
-            weight = Microscaled(codes, scales, ctx.inputs, ctx.dtype).dequantize() if want_x else None
-            dx, _, dbias = _gradients(upstream, None, weight, pre, offsets, ctx, want_x, False, want_bias)
+            rows = row_major(upstream)
+            n, inputs, (*experts, outputs) = rows.shape[0], ctx.inputs, ctx.weights[:-1]
+            experts, dtype = experts[0] if experts else 1, DTYPES[rows.dtype]
+            dx = rows.new_empty((n, inputs)) if want_x else None
+            dbias = rows.new_empty(ctx.weights[:-1]) if want_bias else None
+            scratch = _lib.scratch('odie_mx_linear_workspace', rows, n, experts, int(offsets is not None), inputs, outputs,
+                                   dtype, ctx.activation, int(want_x), int(want_bias))
+            _lib.call('odie_mx_linear_backward', rows, rows.data_ptr(), pitch(rows), _lib.ptr(pre), n, _lib.ptr(codes),
+                      _lib.ptr(scales), _lib.ptr(offsets), experts, inputs, outputs, dtype, ctx.activation, _lib.ptr(dx),
+                      _lib.ptr(dbias), _lib.ptr(scratch), 0 if scratch is None else scratch.numel())
         return dx, None, dbias, upstream if want_residual else None, None, None

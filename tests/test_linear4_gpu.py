@@ -105,6 +105,51 @@ def test_every_activation_bias_and_residual(activation, dtype):
             _check_rows_of_4_bits(x, quantize(w), b, r, activation, activation)
 
 
+# gradients that are formed in one pass: each tile's and slab's edges, rows that fill no tile
+ONE_PASS = [(65536, 1, 8), (65537, 64, 9), (65600, 65, 64), (65665, 128, 71), (65700, 129, 264), (66000, 256, 136),
+            (70000, 33, 12), (65999, 250, 520)]
+
+
+@pytest.mark.parametrize('dtype', (torch.float16, torch.bfloat16), ids=str)
+@pytest.mark.parametrize('shape', ONE_PASS, ids=str)
+def test_gradients_in_one_pass(shape, dtype):
+    n, inputs, outputs = shape
+    for activation in ACTIVATIONS[1:]:
+        print('gradients of 4 bits', shape, dtype, activation, flush=True)
+        x, w, b, r, dy = _case(inputs, n, inputs, outputs, dtype, whole=activation == 'relu')
+        _check_rows_of_t(x, quantize(w), b, r, dy, activation, str(shape) + activation)
+        # alone, and from rows of another stride and start
+        q = quantize(w)
+        leaf, shift = x.clone().requires_grad_(True), b.clone().requires_grad_(True)
+        whole = torch.autograd.grad(linear(leaf, q, shift, activation=activation), (leaf, shift), dy)
+        assert torch.equal(torch.autograd.grad(linear(leaf, q, b, activation=activation), leaf, dy)[0], whole[0])
+        wide = torch.zeros(n, outputs + 13, dtype=dtype, device='cuda')
+        wide[:, 5:5 + outputs] = dy
+        got = torch.autograd.grad(linear(leaf, q, shift, activation=activation), (leaf, shift), wide[:, 5:5 + outputs])
+        assert torch.equal(got[0], whole[0]) and torch.equal(got[1], whole[1])
+
+
+@pytest.mark.parametrize('dtype', (torch.float16, torch.bfloat16), ids=str)
+@pytest.mark.parametrize('inputs', (48, 100, 200))
+def test_experts_gradients_in_one_pass(inputs, dtype):
+    """Groups that end inside tiles, empty ones, and rows of no expert, whose upstream and sums may be anything."""
+    counts, rest, outputs = [30001, 1, 0, 20000, 127, 16384, 0], 77, 72
+    n, experts = sum(counts) + rest, len(counts)
+    x, w, b, r, dy = _case(inputs, n, inputs, outputs, dtype, lead=(experts,))
+    x[sum(counts):], dy[sum(counts):] = float('nan'), float('inf')
+    q, offsets = quantize(w), _offsets(counts)
+    leaves = [t.detach().requires_grad_(True) for t in (x, b)]
+    dx, db = torch.autograd.grad(linear(leaves[0], q, leaves[1], activation='gelu', offsets=offsets), leaves, dy)
+    at = 0
+    for e, count in enumerate(counts):
+        rows = slice(at, at + count)
+        layer = Layer64(x[rows], _weight64(q)[e].to(dtype), b[e], None, dy[rows], 'gelu')
+        check(dx[rows], layer.dx, layer.dx_error, 'expert %d' % e)
+        check(db[e], layer.db, layer.db_error, 'expert %d' % e)
+        at += count
+    assert not dx[at:].any()
+
+
 def _offsets(counts):
     return torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=torch.int32, device='cuda')
 

@@ -45,3 +45,28 @@ def test_linear_refusals(native, change, word):
     _refused(native, native.odie_mx_linear_forward(*a.values()), 'odie_mx_linear_forward', word)
     a.update(dict(x=16, x_scales=16, codes=16, scales=16, out=8, rows=0, dtype=1, activation=0, inputs=16, outputs=8, experts=1))
     assert native.odie_mx_linear_forward(*a.values()) == 0      # nothing to do
+
+
+@pytest.mark.parametrize('change,word', [
+    (dict(dtype=-1), 'dtype'), (dict(activation=9), 'activation'), (dict(rows=-3), 'rows'), (dict(experts=2), 'offsets'),
+    (dict(inputs=0), 'inputs'), (dict(outputs=1 << 21), 'outputs'), (dict(experts=1 << 15, outputs=1 << 20, offsets=8), 'below 2^31'),
+    (dict(upstream=None), 'null'), (dict(pre=None), 'null'), (dict(codes=None), 'null'), (dict(scales=None), 'null'),
+    (dict(upstream_stride=7), 'overlap'), (dict(codes=8), 'aligned'), (dict(scales=18), 'aligned'), (dict(workspace=None), 'workspace'),
+    (dict(workspace=128), 'aligned'), (dict(workspace_bytes=10), 'workspace')])
+def test_linear_backward_refusals(native, change, word):
+    for rows in (10, 100000):       # apart, and in one pass
+        a = dict(upstream=8, upstream_stride=8, pre=8, rows=rows, codes=16, scales=16, offsets=None, experts=1, inputs=16, outputs=8,
+                 dtype=1, activation=1, dx=8, dbias=8, workspace=256, workspace_bytes=1 << 40, stream=0)
+        a.update(change)
+        _refused(native, native.odie_mx_linear_backward(*a.values()), 'odie_mx_linear_backward', word)
+
+
+def test_linear_workspace(native):
+    size = native.odie_mx_linear_workspace
+    # the weight as fp16, in rows of whole 16 bytes
+    assert size(10, 1, 0, 64, 48, 1, 0, 1, 0) == 64 * 48 * 2
+    assert size(100000, 1, 0, 60, 48, 1, 4, 1, 0) == 64 * 48 * 2        # one pass
+    assert size(100000, 1, 0, 60, 48, 1, 4, 1, 1) > 64 * 48 * 2         # and sums of the bias' gradient
+    assert size(10, 1, 0, 64, 48, 1, 4, 1, 0) >= 64 * 48 * 2 + 10 * 48 * 2      # dz
+    assert size(10, 1, 0, 64, 48, 1, 0, 0, 0) == 0
+    assert size(-1, 1, 0, 64, 48, 1, 0, 1, 0) == -1 and size(10, 2, 0, 64, 48, 1, 0, 1, 0) == -1
