@@ -17,6 +17,7 @@ constexpr int kBlock = 256;
 constexpr int kMaxClasses = 1 << 24;
 constexpr int kMaxTop = 1024;
 constexpr int kShort = 512;        // classes of a row that some lanes of a wave take
+constexpr int kMedium = 4096;      // and where there are many rows
 constexpr int kMostPiece = 1 << 16; // classes of a longer row's piece in the backward
 
 struct DistillArgs {
@@ -121,7 +122,7 @@ template <class T, int kLanes> __device__ inline void finish_row(const DistillAr
     }
 }
 
-// Rows of up to kShort classes, kLanes lanes each.
+// Shorter rows, kLanes lanes each.
 template <class T, int kLanes> __global__ __launch_bounds__(kBlock) void distill_short_kernel(DistillArgs a, uint32_t first) {
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
     const int64_t at = (static_cast<int64_t>(first) + blockIdx.x) * (kBlock / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
@@ -191,7 +192,7 @@ __device__ inline void patch_entry(const DistillArgs& a, int64_t row, int j, int
 // (8192 x 1024 with 128 entries a row: 129 us where each looks at all, 18 so).
 template <class T, int kLanes, bool kStream>
 __global__ __launch_bounds__(kBlock) void distill_backward_kernel(DistillArgs a, uint32_t first) {
-    constexpr int kV = kPerVec<T>, kWords = kLanes == kBlock ? (kMostPiece + 64) / 32 : kShort / 32;
+    constexpr int kV = kPerVec<T>, kWords = kLanes == kBlock ? (kMostPiece + 64) / 32 : (kLanes == 64 ? kMedium / 32 : kLanes / 4);
     __shared__ uint32_t bits[kBlock / kLanes][2][kWords];
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
     uint32_t *const once = bits[static_cast<int>(threadIdx.x) / kLanes][0], *const twice = bits[static_cast<int>(threadIdx.x) / kLanes][1];
@@ -253,6 +254,10 @@ int check_distill(const std::string& what, int64_t n, int classes, int top, int 
     return 0;
 }
 
+// Whether a row takes some lanes or a wave, else a workgroup or several.  us forward and backward as a wave and as a workgroup,
+// bf16: 8192 x 1024 (forward) 7.8 and 12.2, 8192 x 2048 25 and 33, 8192 x 8192 73 and 68, 1024 x 4000 14.3 and 12.0.
+bool by_lanes(int64_t n, int classes) { return classes <= kShort || (classes <= kMedium && n >= 4096); }
+
 // Pieces that a long row is cut into, each of whole rounds of its workgroup: about four workgroups a CU at least, and at most
 // `most` classes a piece.
 void cut(DistillArgs& a, int values, int64_t most) {
@@ -279,7 +284,7 @@ using namespace odie;
 
 ODIE_API int64_t odie_distill_workspace(int64_t n, int classes, int dtype) {
     if (check_distill("odie_distill_workspace", n, classes, 1, dtype)) return -1;
-    if (n == 0 || classes <= kShort) return 0;
+    if (n == 0 || by_lanes(n, classes)) return 0;
     DistillArgs a{};
     a.n = n;
     a.classes = classes;
@@ -306,7 +311,7 @@ ODIE_API int odie_distill_forward(const void* logits, int64_t stride, const void
     const hipStream_t s = as_stream(stream);
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        if (classes <= kShort) {
+        if (by_lanes(n, classes)) {
             with_lanes<T>(classes, [&](auto lanes) {
                 in_launches((n + kBlock / lanes - 1) / (kBlock / lanes), kBlock, [&](uint32_t first, uint32_t count) {
                     distill_short_kernel<T, lanes><<<count, kBlock, 0, s>>>(a, first);
@@ -340,7 +345,7 @@ ODIE_API int odie_distill_backward(const float* upstream, const void* logits, in
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
         with_flag(n * classes * dtype_bytes(dtype) >= kStreamBytes, [&](auto far) {
-            if (classes <= kShort) {
+            if (by_lanes(n, classes)) {
                 with_lanes<T>(classes, [&](auto lanes) {
                     in_launches((n + kBlock / lanes - 1) / (kBlock / lanes), kBlock, [&](uint32_t first, uint32_t count) {
                         distill_backward_kernel<T, lanes, far><<<count, kBlock, 0, s>>>(a, first);

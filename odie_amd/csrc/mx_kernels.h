@@ -467,6 +467,9 @@ template <class T, bool kRows4, int kRowTiles, int kSplit> int launch_mx_few_as(
     return check_launch("linear of 4-bit weights");
 }
 
+// The depth over all eight waves where a share is still long or there are too few workgroups otherwise, else over two.  us
+// with eight and with two: 2048 -> 2048 bf16, one row 4.3 and 8.3, 16 rows 5.5 and 13.6; 512 -> 4096 3.4 and 4.0; 512 -> 16384
+// 5.3 and 4.2; 16 rows over 64 experts of 512 -> 1024 10.8 and 7.2; 4096 -> 16384 16.0 and 17.7.
 template <class T, bool kRows4, int kRowTiles> int launch_mx_few(const MxRowsArgs& m, hipStream_t stream) {
     const int64_t steps = m.code_pitch / (4 * kMxBytes);
     const int64_t busy = m.rows.rows < m.rows.experts ? m.rows.rows : m.rows.experts;
@@ -474,6 +477,9 @@ template <class T, bool kRows4, int kRowTiles> int launch_mx_few(const MxRowsArg
     return launch_mx_few_as<T, kRows4, kRowTiles, 2>(m, stream);
 }
 
+// Tiles as linear's, by the work there is.  us of bf16 products as 256 x 256, 128 x 128 and 64 x 64: rows of bf16, 65536 x
+// 1024 x 4096 522, 624 and 849, 16384 x 1024 x 1024 37, 45 and 57, 4096 x 2048 x 2048 (128 tiles of the largest) -, 42 and 58,
+// 131072 rows over 64 experts of 256 -> 512 88, 90 and 110; 4-bit rows 247, 308 and 382, 17, 22 and 28, -, 19 and 22, 61, 63 and 72.
 template <class T, Way kWay> int launch_mixed_of(const MxRowsArgs& m, hipStream_t stream) {
     const RowsArgs& a = m.rows;
     const int64_t each = a.rows / a.experts;
@@ -488,9 +494,14 @@ template <class T, Way kWay> int launch_mixed_of(const MxRowsArgs& m, hipStream_
 
 template <class T, bool kRows4> int launch_mx_by_rows(const MxRowsArgs& m, hipStream_t stream) {
     const RowsArgs& a = m.rows;
-    const int64_t each = (a.rows + a.experts - 1) / a.experts * (a.experts > 1 ? 2 : 1);   // room for twice the average
-    if (each <= 16) return launch_mx_few<T, kRows4, 1>(m, stream);
-    if (each <= 32) return launch_mx_few<T, kRows4, 2>(m, stream);
+    // Few rows: up to 64 for one matrix (4-bit rows 32), up to 256 (128) in all over several.  us of few rows and of tiles,
+    // bf16: 2048 -> 2048, 16 rows 5.5 and 15.0, 32 rows 7.4 and 15.2, 64 rows 11.6 and 15.3; 4-bit rows 4.5 and 7.1, 5.6 and
+    // 7.2, 8.0 and 7.4.  Over 64 experts of 512 -> 1024, 64 rows 8.0 and 12.8, 256 rows 13.0 and 13.4, 512 rows 15.8 and 13.6;
+    // 4-bit rows, 64 rows 7.2 and 8.2, 256 rows 8.7 and 8.5, 512 rows 11.5 and 8.6.
+    if (a.experts > 1 ? a.rows <= (kRows4 ? 128 : 256) : a.rows <= 16) return launch_mx_few<T, kRows4, 1>(m, stream);
+    if (a.experts == 1 && a.rows <= 32) return launch_mx_few<T, kRows4, 2>(m, stream);
+    if constexpr (!kRows4)
+        if (a.experts == 1 && a.rows <= 64) return launch_mx_few<T, kRows4, 4>(m, stream);
     if constexpr (kRows4) {
         const int64_t large = (a.rows + 255) / 256 * ((a.columns + 255) / 256);
         const int64_t wide = (a.rows + 127) / 128 * ((a.columns + 127) / 128);

@@ -361,13 +361,15 @@ __global__ __launch_bounds__(kBlock) void choose_backward_kernel(ChooseBackwardA
 
 constexpr int kCountBlock = 1024;
 constexpr int kSharedCounts = 8192;      // experts whose counts a workgroup keeps in LDS
-constexpr int64_t kFewEntries = 1 << 15; // counted by one workgroup, which needs nothing cleared before
+constexpr int64_t kFewEntries = 1 << 14; // counted by one workgroup, which needs nothing cleared before
+constexpr uint32_t kFewBlocks = 64;      // of which the last one makes the loss
 
 struct BalanceArgs {
     const void* logits;
     const int32_t* expert;    // [n][choices]
     int32_t* counts;          // [experts]
-    uint32_t* done;           // workgroups that have left their sums
+    uint32_t* done;           // workgroups that have left their sums, or null: a launch of its own makes the loss
+    uint32_t blocks;          // workgroups of the rows
     float* stats;             // [n][4]: m, 1 / s (0: the row takes no part), t, 0
     double* partial;          // [blocks]: sum of t
     uint32_t* parts;          // [blocks]: rows that take part
@@ -379,7 +381,7 @@ struct BalanceArgs {
 
 __global__ __launch_bounds__(kBlock) void balance_clear_kernel(BalanceArgs a) {
     for (int e = blockIdx.x * kBlock + threadIdx.x; e < a.experts; e += gridDim.x * kBlock) a.counts[e] = 0;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;
+    if (a.done && blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;
 }
 
 // Each workgroup counts its entries in LDS and adds what it found (whole numbers, in any order).  kAlone: one workgroup
@@ -392,7 +394,7 @@ template <bool kAlone> __global__ __launch_bounds__(kCountBlock) void balance_co
     int32_t* to = shared ? held : a.counts;
     if (shared || kAlone) {
         for (int e = threadIdx.x; e < a.experts; e += kCountBlock) to[e] = 0;
-        if (kAlone && threadIdx.x == 0) *a.done = 0;
+        if (kAlone && a.done && threadIdx.x == 0) *a.done = 0;
         __syncthreads();
     }
     auto add = [&](int e) {
@@ -442,45 +444,58 @@ __device__ inline void keep_row(const BalanceArgs& a, int64_t row, float m, floa
     if (a.stats) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(m, inverse, t, 0.0f);
 }
 
-// Adds the workgroups' sums; the last one to come makes the loss of them, in the order of the workgroups.
-__device__ inline void finish_balance(const BalanceArgs& a, double total, uint32_t rows) {
-    __shared__ double sums[kBlock / 64];
-    __shared__ uint32_t counts[2][kBlock / 64];
-    __shared__ bool last;
-    const int wave = static_cast<int>(threadIdx.x) / 64;
-    total = sum_across<64>(total);
-    rows = sum_across<64>(rows);
-    if (threadIdx.x % 64 == 0) sums[wave] = total, counts[0][wave] = rows;
+// The sums of the workgroup's threads, in thread 0.
+struct BalanceSums {
+    double total;
+    uint32_t rows, entries;
+};
+__device__ inline BalanceSums sum_block(BalanceSums x) {
+    __shared__ BalanceSums part[kBlock / 64];
+    x = BalanceSums{sum_across<64>(x.total), sum_across<64>(x.rows), sum_across<64>(x.entries)};
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kBlock / 64; ++w) total += sums[w], rows += counts[0][w];
-        __hip_atomic_store(a.partial + blockIdx.x, total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(a.parts + blockIdx.x, rows, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        // Stores and loads of agent scope go past the XCD's own L2, so that their order is all it takes: a release would
-        // write that L2 back, in every workgroup.
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        last = __hip_atomic_fetch_add(a.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-    }
+    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = x;
     __syncthreads();
-    if (!last) return;
-    total = 0.0, rows = 0;
-    uint32_t entries = 0;
-    for (uint32_t b = threadIdx.x; b < gridDim.x; b += kBlock) {
-        total += __hip_atomic_load(a.partial + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        rows += __hip_atomic_load(a.parts + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    for (int e = threadIdx.x; e < a.experts; e += kBlock) entries += static_cast<uint32_t>(a.counts[e]);
-    total = sum_across<64>(total);
-    rows = sum_across<64>(rows);
-    entries = sum_across<64>(entries);
-    if (threadIdx.x % 64 == 0) sums[wave] = total, counts[0][wave] = rows, counts[1][wave] = entries;
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    for (int w = 1; w < kBlock / 64; ++w) total += sums[w], rows += counts[0][w], entries += counts[1][w];
-    const double norm = entries > 0 ? a.experts / (static_cast<double>(entries) * static_cast<double>(rows)) : 0.0;
-    *a.norm = static_cast<float>(norm);
-    *a.loss = static_cast<float>(entries > 0 ? total * norm : 0.0);
+    if (threadIdx.x == 0)
+        for (int w = 1; w < kBlock / 64; ++w) x.total += part[w].total, x.rows += part[w].rows, x.entries += part[w].entries;
+    return x;
 }
+
+// The loss from the workgroups' sums, in their order.
+__device__ inline void make_loss(const BalanceArgs& a) {
+    BalanceSums x{};
+    for (uint32_t b = threadIdx.x; b < a.blocks; b += kBlock) {
+        x.total += __hip_atomic_load(a.partial + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        x.rows += __hip_atomic_load(a.parts + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    for (int e = threadIdx.x; e < a.experts; e += kBlock) x.entries += static_cast<uint32_t>(a.counts[e]);
+    x = sum_block(x);
+    if (threadIdx.x != 0) return;
+    const double norm = x.entries > 0 ? a.experts / (static_cast<double>(x.entries) * static_cast<double>(x.rows)) : 0.0;
+    *a.norm = static_cast<float>(norm);
+    *a.loss = static_cast<float>(x.entries > 0 ? x.total * norm : 0.0);
+}
+
+// Leaves the workgroup's sums.  Of few workgroups the last one to come goes on to the loss; each takes its turn at one
+// address, about 10 ns (65536 x 64: 1536 workgroups 25 us, 9 and 3 with a launch of its own).
+__device__ inline void finish_balance(const BalanceArgs& a, double total, uint32_t rows) {
+    __shared__ bool last;
+    const BalanceSums x = sum_block(BalanceSums{total, rows, 0});
+    if (threadIdx.x == 0) {
+        __hip_atomic_store(a.partial + blockIdx.x, x.total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(a.parts + blockIdx.x, x.rows, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = false;
+        if (a.done) {
+            // Stores and loads of agent scope go past the XCD's own L2, so that their order is all it takes: a release
+            // would write that L2 back, in every workgroup.
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            last = __hip_atomic_fetch_add(a.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.blocks - 1;
+        }
+    }
+    __syncthreads();
+    if (last) make_loss(a);
+}
+
+__global__ __launch_bounds__(kBlock) void balance_loss_kernel(BalanceArgs a) { make_loss(a); }
 
 // Rows of up to 64 kVecs chunks: kLanes lanes a row, a row in registers and the next one under way, the counts of the
 // lane's columns in registers for all of its rows.
@@ -771,7 +786,10 @@ ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int3
     a.stats = stats;
     a.partial = static_cast<double*>(workspace);
     a.parts = reinterpret_cast<uint32_t*>(a.partial + most);
-    a.done = a.parts + most;
+    with_dtype(dtype, [&](auto t) {
+        with_row<decltype(t)>(experts, 1, [&](auto lanes, auto vecs) { a.blocks = row_blocks(n, lanes, vecs); });
+    });
+    a.done = a.blocks <= kFewBlocks ? a.parts + most : nullptr;
     a.norm = norm;
     a.loss = loss;
     a.stride = stride;
@@ -792,10 +810,11 @@ ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int3
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         with_row<T>(experts, 1, [&](auto lanes, auto vecs) {
-            if constexpr (vecs > 0) balance_rows_kernel<T, lanes, vecs><<<row_blocks(n, lanes, vecs), kBlock, 0, s>>>(a);
-            else balance_long_kernel<T><<<row_blocks(n, 64, 1), kBlock, 0, s>>>(a);
+            if constexpr (vecs > 0) balance_rows_kernel<T, lanes, vecs><<<a.blocks, kBlock, 0, s>>>(a);
+            else balance_long_kernel<T><<<a.blocks, kBlock, 0, s>>>(a);
         });
     });
+    if (!a.done) balance_loss_kernel<<<1, kBlock, 0, s>>>(a);
     return check_launch("balance");
 }
 

@@ -185,7 +185,7 @@ def _check_balance(logits, expert, what):
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 @pytest.mark.parametrize('width', WIDTHS)
 def test_balance(width, dtype):
-    for n, choices in ((1, 1), (6, 3), (130, 2), (4099, 1)):
+    for n, choices in ((1, 1), (6, 3), (130, 2), (4099, 1), (9001, 3)):
         if n * width > 5_000_000:
             continue
         print('balance', n, width, choices, dtype, flush=True)
@@ -271,8 +271,8 @@ def _check_distill(logits, ids, teacher, temperature, what):
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 @pytest.mark.parametrize('width', WIDTHS + (70001,))
 def test_distill(width, dtype):
-    # 1100 rows of 513 classes on: a workgroup a row; fewer: several
-    for n, top, temperature in ((1, 1, 1.0), (5, 3, 2.0), (70, 33, 0.7), (1100, 8, 1.0), (3, 300, 4.0)):
+    # from 513 classes on: 1100 rows a workgroup a row, fewer several, 4100 rows a wave a row
+    for n, top, temperature in ((1, 1, 1.0), (5, 3, 2.0), (70, 33, 0.7), (1100, 8, 1.0), (3, 300, 4.0), (4100, 70, 2.0)):
         if n * width > 12_000_000:
             continue
         print('distill', n, width, top, dtype, flush=True)
