@@ -54,7 +54,8 @@ typedef struct odie_grid_level {
 /* dtype codes */
 #define ODIE_F32 0
 #define ODIE_F16 1
-#define ODIE_BF16 2   /* the row operators (odie_linear_*, odie_sort_*, odie_rows_*, odie_embed_*) alone */
+#define ODIE_BF16 2   /* the row operators (odie_linear_*, odie_sort_*, odie_rows_*, odie_embed_*), the router's (odie_choose_*,
+                       * odie_balance_*, odie_distill_*) and the 4-bit ones (odie_mx_*) alone */
 
 /* Forward encode of n coordinates in [0,1]^2 (coords fp32 [n,2]).
  * Experts: coordinates [offsets[e], offsets[e+1]) read the table at params + e*expert_params

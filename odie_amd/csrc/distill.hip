@@ -26,7 +26,8 @@ struct DistillArgs {
     const void* teacher;      // [n][top]
     const float* upstream;    // [n] (backward)
     float* loss;              // [n] (forward)
-    float* stats;             // [n][4]: m and 1 / s of logits / T (1 / s 0: all masked), and of teacher / T (0: no entries)
+    // [n][4]: m and 1 / s of logits / T (1 / s 0: all masked), and of teacher / T (0: no entries)
+    float* stats;
     void* dlogits;            // [n][classes] (backward)
     float2* partial;          // [n][pieces]: m and s of a piece of a row (forward)
     int64_t stride, n;
@@ -50,9 +51,10 @@ __device__ inline float entry_of(const DistillArgs& a, int64_t row, int j, int64
     return id >= 0 && id < a.classes ? teacher_of(a, row * a.top + j) * a.inverse : kNegInfinity;
 }
 
-// Calls f(column, values) for the chunks of columns [begin, end) that lane `lane` of kLanes takes, kAhead whole ones at a
-// time, whose loads are in flight together.
-template <class T, int kLanes, int kAhead, class F> __device__ inline void for_chunks(const T* row, int begin, int end, int width, int lane, F&& f) {
+// Calls f(column, values) for the chunks of columns [begin, end) that lane `lane` of kLanes takes, kAhead whole ones at
+// a time, whose loads are in flight together.
+template <class T, int kLanes, int kAhead, class F>
+__device__ inline void for_chunks(const T* row, int begin, int end, int width, int lane, F&& f) {
     constexpr int kV = kPerVec<T>, kStep = kLanes * kV;
     int column = begin + lane * kV;
     for (; column + (kAhead - 1) * kStep + kV <= end; column += kAhead * kStep) {
@@ -74,7 +76,8 @@ template <class T, int kLanes, int kAhead, class F> __device__ inline void for_c
 }
 
 // Adds the logits / T of columns [begin, end) to run.
-template <class T, int kLanes, class R> __device__ inline void add_columns(const DistillArgs& a, const T* row, int begin, int end, int lane, R& run) {
+template <class T, int kLanes, class R>
+__device__ inline void add_columns(const DistillArgs& a, const T* row, int begin, int end, int lane, R& run) {
     constexpr int kV = kPerVec<T>;
     for_chunks<T, kLanes, kLanes == kBlock ? 4 : 1>(row, begin, end, a.classes, lane, [&](int, float (&value)[kV]) {
 #pragma unroll
@@ -84,7 +87,8 @@ template <class T, int kLanes, class R> __device__ inline void add_columns(const
 }
 
 // A row's loss from its softmax (m, s): kLanes lanes of one wave share the entries.
-template <class T, int kLanes> __device__ inline void finish_row(const DistillArgs& a, int64_t row, int lane, bool store, float m, float s) {
+template <class T, int kLanes>
+__device__ inline void finish_row(const DistillArgs& a, int64_t row, int lane, bool store, float m, float s) {
     float top = kNegInfinity;
     for (int j = lane; j < a.top; j += kLanes) {
         int64_t id;
@@ -123,9 +127,11 @@ template <class T, int kLanes> __device__ inline void finish_row(const DistillAr
 }
 
 // Shorter rows, kLanes lanes each.
-template <class T, int kLanes> __global__ __launch_bounds__(kBlock) void distill_short_kernel(DistillArgs a, uint32_t first) {
+template <class T, int kLanes>
+__global__ __launch_bounds__(kBlock) void distill_short_kernel(DistillArgs a, uint32_t first) {
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
-    const int64_t at = (static_cast<int64_t>(first) + blockIdx.x) * (kBlock / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
+    const int64_t at =
+        (static_cast<int64_t>(first) + blockIdx.x) * (kBlock / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
     const int64_t row = at < a.n ? at : a.n - 1;
     Running<sizeof(T) == 4> run;
     add_columns<T, kLanes>(a, static_cast<const T*>(a.logits) + row * a.stride, 0, a.classes, lane, run);
@@ -133,14 +139,16 @@ template <class T, int kLanes> __global__ __launch_bounds__(kBlock) void distill
     finish_row<T, kLanes>(a, row, lane, at < a.n, run.m, run.s);
 }
 
-// Longer rows: a workgroup a piece.  Where a row is one piece, its loss too.
+// Longer rows: a workgroup a piece.  Where a row is one piece, its loss too.  8192 x 65032 bf16: 208 us, 1.07 GB at 5.1
+// TB/s: HBM (a chunk at a time 221).
 template <class T> __global__ __launch_bounds__(kBlock) void distill_piece_kernel(DistillArgs a, uint32_t first) {
     __shared__ float2 part[kBlock / 64];
     const int64_t id = static_cast<int64_t>(first) + blockIdx.x, row = id / a.pieces;
     const int piece = static_cast<int>(id % a.pieces), begin = piece * a.piece;
     const int end = begin + a.piece < a.classes ? begin + a.piece : a.classes;
     Running<sizeof(T) == 4> run;
-    add_columns<T, kBlock>(a, static_cast<const T*>(a.logits) + row * a.stride, begin, end, static_cast<int>(threadIdx.x), run);
+    add_columns<T, kBlock>(a, static_cast<const T*>(a.logits) + row * a.stride, begin, end,
+                           static_cast<int>(threadIdx.x), run);
     run.template join_lanes<64>();
     if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = make_float2(run.m, run.s);
     __syncthreads();
@@ -163,10 +171,11 @@ template <class T> __global__ __launch_bounds__(64) void distill_join_kernel(Dis
     finish_row<T, 64>(a, row, static_cast<int>(threadIdx.x), true, run.m, run.s);
 }
 
-// The gradient at the row's entry j, p - Q, from the piece [begin, end) of the row.  The first entry of a class that several
-// name (`twice`, a bit for each class of the piece) adds up the others'.
+// The gradient at the row's entry j, p - Q, from the piece [begin, end) of the row.  The first entry of a class that
+// several name (`twice`, a bit for each class of the piece) adds up the others'.
 template <class T>
-__device__ inline void patch_entry(const DistillArgs& a, int64_t row, int j, int begin, int end, const uint32_t* twice, const T* logits,
+__device__ inline void patch_entry(const DistillArgs& a, int64_t row, int j, int begin, int end, const uint32_t* twice,
+                                   const T* logits,
                                    T* out, float scale, const float (&stats)[4]) {
     int64_t id, other;
     const float entry = entry_of(a, row, j, id);
@@ -185,25 +194,30 @@ __device__ inline void patch_entry(const DistillArgs& a, int64_t row, int j, int
     out[id] = static_cast<T>(value);
 }
 
-// A piece of a row's gradient: kLanes threads (some of a wave's, or the workgroup).  A workgroup's stores begin on lines
-// of 128 bytes, whatever the row does (8192 x 65032 bf16: 514 -> 465 us; rows that begin on lines themselves 455): the row's elements before
-// the first line go one by one, and its pieces are cut at lines.  Two bits for each class of the piece tell whether no, one or
-// several entries name it: those of a class that one names, as a teacher's largest logits do, need not look for others
-// (8192 x 1024 with 128 entries a row: 129 us where each looks at all, 18 so).
+// A piece of a row's gradient: kLanes threads (some of a wave's, or the workgroup).  A workgroup's stores begin on
+// lines of 128 bytes, whatever the row does (8192 x 65032 bf16: 514 -> 465 us; rows that begin on lines themselves 455;
+// 452, 2.13 GB at 4.7 TB/s, in all): the row's elements before the first line go one by one, and its pieces are cut at
+// lines.  Two bits for each class of the piece tell whether no, one or several entries name it: those of a class that
+// one names, as a teacher's largest logits do, need not look for others (8192 x 1024 with 128 entries a row: 129 us
+// where each looks at all, 18 so).
 template <class T, int kLanes, bool kStream>
 __global__ __launch_bounds__(kBlock) void distill_backward_kernel(DistillArgs a, uint32_t first) {
-    constexpr int kV = kPerVec<T>, kWords = kLanes == kBlock ? (kMostPiece + 64) / 32 : (kLanes == 64 ? kMedium / 32 : kLanes / 4);
+    constexpr int kV = kPerVec<T>,
+        kWords = kLanes == kBlock ? (kMostPiece + 64) / 32 : (kLanes == 64 ? kMedium / 32 : kLanes / 4);
     __shared__ uint32_t bits[kBlock / kLanes][2][kWords];
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
-    uint32_t *const once = bits[static_cast<int>(threadIdx.x) / kLanes][0], *const twice = bits[static_cast<int>(threadIdx.x) / kLanes][1];
-    const int64_t at = (static_cast<int64_t>(first) + blockIdx.x) * (kBlock / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
+    uint32_t *const once = bits[static_cast<int>(threadIdx.x) / kLanes][0],
+        *const twice = bits[static_cast<int>(threadIdx.x) / kLanes][1];
+    const int64_t at =
+        (static_cast<int64_t>(first) + blockIdx.x) * (kBlock / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
     const int64_t row = at / a.pieces;
     const bool inside = row < a.n;
     const int piece = static_cast<int>(at % a.pieces);
     const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
     T* out = static_cast<T*>(a.dlogits) + row * a.classes;
     constexpr int kLine = 128 / static_cast<int>(sizeof(T));
-    const int past = kLanes == kBlock ? static_cast<int>(reinterpret_cast<uintptr_t>(out) / sizeof(T) % kLine) : 0;   // the line before
+    // the line before
+    const int past = kLanes == kBlock ? static_cast<int>(reinterpret_cast<uintptr_t>(out) / sizeof(T) % kLine) : 0;
     const int begin = piece == 0 ? 0 : piece * a.piece - past;
     const int end = piece == a.pieces - 1 ? a.classes : (piece + 1) * a.piece - past;
     const int head = piece == 0 && past > 0 ? (kLine - past < end ? kLine - past : end) : 0;
@@ -233,7 +247,8 @@ __global__ __launch_bounds__(kBlock) void distill_backward_kernel(DistillArgs a,
             asm("" : "+v"(value));      // rounded to fp32, then to T, as its neighbours are
             out[column] = static_cast<T>(value);
         }
-        for_chunks<T, kLanes, kLanes == kBlock ? 4 : 1>(logits, begin + head, end, a.classes, lane, [&](int column, float (&value)[kV]) {
+        for_chunks<T, kLanes, kLanes == kBlock ? 4 : 1>(logits, begin + head, end, a.classes, lane,
+                                                        [&](int column, float (&value)[kV]) {
 #pragma unroll
             for (int i = 0; i < kV; ++i) value[i] = gradient(value[i]);
             store_some<kStream>(out + column, narrow<T>(value), a.classes - column);
@@ -254,14 +269,16 @@ int check_distill(const std::string& what, int64_t n, int classes, int top, int 
     return 0;
 }
 
-// Whether a row takes some lanes or a wave, else a workgroup or several.  us forward and backward as a wave and as a workgroup,
-// bf16: 8192 x 1024 (forward) 7.8 and 12.2, 8192 x 2048 25 and 33, 8192 x 8192 73 and 68, 1024 x 4000 14.3 and 12.0.
+// Whether a row takes some lanes or a wave, else a workgroup or several.  us forward and backward as a wave and as a
+// workgroup, bf16: 8192 x 1024 (forward) 7.8 and 12.2, 8192 x 2048 25 and 33, 8192 x 8192 73 and 68, 1024 x 4000 14.3
+// and 12.0.
 bool by_lanes(int64_t n, int classes) { return classes <= kShort || (classes <= kMedium && n >= 4096); }
 
-// Pieces that a long row is cut into, each of whole rounds of its workgroup: about four workgroups a CU at least, and at most
-// `most` classes a piece.
+// Pieces that a long row is cut into, each of whole rounds of its workgroup: about four workgroups a CU at least, and
+// at most `most` classes a piece.
 void cut(DistillArgs& a, int values, int64_t most) {
-    const int64_t wanted = a.n < 4 * kCus ? (4 * kCus + a.n - 1) / a.n : 1, round = static_cast<int64_t>(kBlock) * values;
+    const int64_t wanted = a.n < 4 * kCus ? (4 * kCus + a.n - 1) / a.n : 1,
+        round = static_cast<int64_t>(kBlock) * values;
     const int64_t rounds = (a.classes + round - 1) / round, least = (a.classes + most - 1) / most;
     int64_t pieces = wanted < rounds ? wanted : rounds;
     pieces = pieces < least ? least : pieces;
@@ -292,28 +309,33 @@ ODIE_API int64_t odie_distill_workspace(int64_t n, int classes, int dtype) {
     return a.pieces > 1 ? n * a.pieces * static_cast<int64_t>(sizeof(float2)) : 0;
 }
 
-ODIE_API int odie_distill_forward(const void* logits, int64_t stride, const void* ids, int id_bytes, const void* teacher,
+ODIE_API int odie_distill_forward(const void* logits, int64_t stride, const void* ids, int id_bytes,
+                                  const void* teacher,
                                   int teacher_dtype, int64_t n, int classes, int top, float temperature, int dtype,
-                                  float* loss, float* stats, void* workspace, int64_t workspace_bytes, uint64_t stream) {
+                                  float* loss, float* stats, void* workspace, int64_t workspace_bytes,
+                                      uint64_t stream) {
     const std::string what = "odie_distill_forward";
     if (check_distill(what, n, classes, top, dtype)) return -1;
     if (!known_dtype(teacher_dtype)) return fail(what + ": teacher_dtype must be 0 (fp32), 1 (fp16) or 2 (bf16)");
     if (id_bytes != 4 && id_bytes != 8) return fail(what + ": id_bytes must be 4 or 8");
-    if (!(temperature > 0.0f) || !(1.0f / temperature > 0.0f) || std::isinf(1.0f / temperature)) return fail(what + ": temperature must be above 0 and finite");
+    if (!(temperature > 0.0f) || !(1.0f / temperature > 0.0f) || std::isinf(1.0f / temperature))
+        return fail(what + ": temperature must be above 0 and finite");
     if (n == 0) return 0;
     if (!logits || !ids || !teacher || !loss) return fail(what + ": null pointer");
     if (stride < classes) return fail(what + ": rows overlap (a stride below the row's width)");
     const int64_t need = odie_distill_workspace(n, classes, dtype);
     if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 8 != 0))
         return fail(what + ": needs an 8-byte aligned workspace of " + std::to_string(need) + " bytes");
-    DistillArgs a{logits, ids, teacher, nullptr, loss, stats, nullptr, static_cast<float2*>(workspace), stride, n, classes,
+    DistillArgs a{logits, ids, teacher, nullptr, loss, stats, nullptr, static_cast<float2*>(workspace), stride, n,
+        classes,
                   top, id_bytes, teacher_dtype, 1, classes, 1.0f / temperature};
     const hipStream_t s = as_stream(stream);
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
         if (by_lanes(n, classes)) {
             with_lanes<T>(classes, [&](auto lanes) {
-                in_launches((n + kBlock / lanes - 1) / (kBlock / lanes), kBlock, [&](uint32_t first, uint32_t count) {
+                in_launches((n + kBlock / lanes - 1) / (kBlock / lanes), kBlock,
+                                [&](uint32_t first, uint32_t count) {
                     distill_short_kernel<T, lanes><<<count, kBlock, 0, s>>>(a, first);
                 });
             });
@@ -335,11 +357,13 @@ ODIE_API int odie_distill_backward(const float* upstream, const void* logits, in
     if (check_distill(what, n, classes, top, dtype)) return -1;
     if (!known_dtype(teacher_dtype)) return fail(what + ": teacher_dtype must be 0 (fp32), 1 (fp16) or 2 (bf16)");
     if (id_bytes != 4 && id_bytes != 8) return fail(what + ": id_bytes must be 4 or 8");
-    if (!(temperature > 0.0f) || !(1.0f / temperature > 0.0f) || std::isinf(1.0f / temperature)) return fail(what + ": temperature must be above 0 and finite");
+    if (!(temperature > 0.0f) || !(1.0f / temperature > 0.0f) || std::isinf(1.0f / temperature))
+        return fail(what + ": temperature must be above 0 and finite");
     if (n == 0) return 0;
     if (!upstream || !logits || !ids || !teacher || !stats || !dlogits) return fail(what + ": null pointer");
     if (stride < classes) return fail(what + ": rows overlap (a stride below the row's width)");
-    DistillArgs a{logits, ids, teacher, upstream, nullptr, const_cast<float*>(stats), dlogits, nullptr, stride, n, classes,
+    DistillArgs a{logits, ids, teacher, upstream, nullptr, const_cast<float*>(stats), dlogits, nullptr, stride, n,
+        classes,
                   top, id_bytes, teacher_dtype, 1, classes, 1.0f / temperature};
     const hipStream_t s = as_stream(stream);
     return with_dtype(dtype, [&](auto t) -> int {
@@ -347,7 +371,8 @@ ODIE_API int odie_distill_backward(const float* upstream, const void* logits, in
         with_flag(n * classes * dtype_bytes(dtype) >= kStreamBytes, [&](auto far) {
             if (by_lanes(n, classes)) {
                 with_lanes<T>(classes, [&](auto lanes) {
-                    in_launches((n + kBlock / lanes - 1) / (kBlock / lanes), kBlock, [&](uint32_t first, uint32_t count) {
+                    in_launches((n + kBlock / lanes - 1) / (kBlock / lanes), kBlock,
+                                [&](uint32_t first, uint32_t count) {
                         distill_backward_kernel<T, lanes, far><<<count, kBlock, 0, s>>>(a, first);
                     });
                 });

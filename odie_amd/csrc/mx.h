@@ -24,10 +24,12 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // The two values of byte kByte of `codes`.
 template <int kByte> __device__ inline uint32_t mx_pair(_Float16, uint32_t codes, float scale) {
-    return __builtin_bit_cast(uint32_t, static_cast<f16x2>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, kByte)));
+    return __builtin_bit_cast(
+        uint32_t, static_cast<f16x2>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, kByte)));
 }
 template <int kByte> __device__ inline uint32_t mx_pair(__bf16, uint32_t codes, float scale) {
-    return __builtin_bit_cast(uint32_t, static_cast<bf16x2>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, kByte)));
+    return __builtin_bit_cast(
+        uint32_t, static_cast<bf16x2>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, kByte)));
 }
 template <int kByte> __device__ inline f32x2 mx_pair(float, uint32_t codes, float scale) {
     return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, kByte);

@@ -7,7 +7,8 @@
 namespace odie {
 
 struct MxInputArgs {
-    RowsArgs rows;        // a: dy; b: the weight [experts][outputs], stride `pitch`; out: dx; depth: outputs; columns: inputs
+    // a: dy; b: the weight [experts][outputs], stride `pitch`; out: dx; depth: outputs; columns: inputs
+    RowsArgs rows;
     const void* pre;      // z [rows][outputs]
     float* sums;          // [piece ids][outputs], or null
     int64_t pitch;
@@ -17,7 +18,9 @@ struct MxInputArgs {
 struct MxInputTile {
     int rows, inputs;
 };
-inline MxInputTile mx_input_tile(int inputs) { return MxInputTile{128, inputs <= 64 ? 64 : (inputs <= 128 ? 128 : 256)}; }
+inline MxInputTile mx_input_tile(int inputs) {
+    return MxInputTile{128, inputs <= 64 ? 64 : (inputs <= 128 ? 128 : 256)};
+}
 
 template <class T> int launch_mx_input(const MxInputArgs& a, hipStream_t stream);
 
@@ -52,11 +55,13 @@ template <class T, int kRows, int kThreads> struct SlopeRows : Image<T, true, kR
     __device__ void load(Held& held) {
         const int k = next + lead < depth - I::kVec ? next + lead : depth - I::kVec;
 #pragma unroll
-        for (int i = 0; i < I::kChunks; ++i) held.dy[i] = load16(dy[i] + k), held.z[i] = load16(tile + (z[i] + static_cast<uint32_t>(k)));
+        for (int i = 0; i < I::kChunks; ++i)
+            held.dy[i] = load16(dy[i] + k), held.z[i] = load16(tile + (z[i] + static_cast<uint32_t>(k)));
         next += kSlab<T>;
     }
     // `left` columns of this slab exist; the rest become 0.  sum: this thread's rows' sums, before the rounding.
-    template <int kActivation> __device__ void store(const Held& held, char* lds, int left, float (&sum)[I::kVec]) const {
+    template <int kActivation> __device__ void store(const Held& held, char* lds, int left,
+                                                     float (&sum)[I::kVec]) const {
         const int count = left < kSlab<T> ? left - lead : kSlab<T>;
         const int moved = count < I::kVec ? (I::kVec - count) * static_cast<int>(sizeof(T)) : 0;
 #pragma unroll
@@ -93,8 +98,10 @@ template <class T, int kRows, int kThreads> struct SlopeRows : Image<T, true, kR
 #pragma unroll
         for (int e = 0; e < I::kVec; ++e) {
             float s = sum[e];
-            s += __builtin_bit_cast(float, dpp_move<0x128>(__builtin_bit_cast(uint32_t, s)));     // the next row: lane ^ 8
-            s += __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, s), 0x441F));   // two on: lane ^ 17
+            // the next row: lane ^ 8
+            s += __builtin_bit_cast(float, dpp_move<0x128>(__builtin_bit_cast(uint32_t, s)));
+            // two on: lane ^ 17
+            s += __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, s), 0x441F));
             s += __shfl_xor(s, 34);                                                               // four on
             sum[e] = s;
         }
@@ -104,10 +111,10 @@ template <class T, int kRows, int kThreads> struct SlopeRows : Image<T, true, kR
 // Waits for this wave's LDS reads, then for the other waves; loads under way stay so.
 __device__ inline void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// A tile.  A slab's slope takes a workgroup three times as long as its products do, and all of its waves are at the one or
-// the other: one buffer an operand, so that a CU has two workgroups, one at each.  131072 rows over 64 experts, 256 <- 512
-// fp16, silu: 110 to 118 us, 335 MB at 2.9 TB/s, bound by the slope's arithmetic (256 x 256 tiles with two buffers, one workgroup a
-// CU: 142).
+// A tile.  A slab's slope takes a workgroup three times as long as its products do, and all of its waves are at the one
+// or the other: one buffer an operand, so that a CU has two workgroups, one at each.  131072 rows over 64 experts, 256
+// <- 512 fp16, silu: 110 to 118 us, 335 MB at 2.9 TB/s, bound by the slope's arithmetic (256 x 256 tiles with two
+// buffers, one workgroup a CU: 142).
 template <class T, int kBM, int kBN, int kWM, int kWN> struct InputTile : Sums<kBM, kBN, kWM, kWN> {
     using Base = Sums<kBM, kBN, kWM, kWN>;
     using Base::acc;
@@ -170,7 +177,8 @@ template <class T, int kBM, int kBN, int kWM, int kWN> struct InputTile : Sums<k
 };
 
 template <class T, int kBM, int kBN, int kWM, int kWN>
-__global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN), 2) void mx_input_kernel(MxInputArgs m, uint32_t first, uint32_t blocks) {
+__global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN), 2) void mx_input_kernel(
+    MxInputArgs m, uint32_t first, uint32_t blocks) {
     using Work = InputTile<T, kBM, kBN, kWM, kWN>;
     __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
     const RowsArgs& a = m.rows;
@@ -182,10 +190,12 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN), 2) void mx_input_ke
     typename Work::A opa;
     typename Work::B opb;
     opa.begin(static_cast<const T*>(a.a), a.lda, static_cast<const T*>(m.pre), p.begin, p.end, a.depth);
-    opb.begin(static_cast<const T*>(a.b) + static_cast<int64_t>(p.group) * a.depth * m.pitch, m.pitch, 0, a.columns, a.depth);
+    opb.begin(static_cast<const T*>(a.b) + static_cast<int64_t>(p.group) * a.depth * m.pitch, m.pitch, 0, a.columns,
+              a.depth);
     Work work;
     with_activation(a.activation, [&](auto activation) {
-        work.template sum<activation>(opa, opb, a.depth, m.sums ? m.sums + static_cast<int64_t>(id) * a.depth : nullptr, lds);
+        work.template sum<activation>(opa, opb, a.depth,
+                                     m.sums ? m.sums + static_cast<int64_t>(id) * a.depth : nullptr, lds);
     });
     RowsArgs plain = a;      // dx as it is
     plain.activation = kNone;
@@ -197,7 +207,8 @@ template <class T, int kBM, int kBN, int kWM, int kWN> int launch_mx_input_as(Mx
     constexpr int kThreads = 64 * (kBM / kWM) * (kBN / kWN);
     if (blocks >= int64_t{1} << 31) return fail("linear: too many tiles for one launch");
     in_launches(blocks, kThreads, [&](uint32_t first, uint32_t count) {
-        mx_input_kernel<T, kBM, kBN, kWM, kWN><<<whole_xcds(count), kThreads, 0, stream>>>(m, first, static_cast<uint32_t>(blocks));
+        mx_input_kernel<T, kBM, kBN, kWM, kWN>
+            <<<whole_xcds(count), kThreads, 0, stream>>>(m, first, static_cast<uint32_t>(blocks));
     });
     return check_launch("linear of 4-bit weights, gradient");
 }

@@ -33,21 +33,27 @@ constexpr int kMxSlab = 256;          // values of k in a 128-byte row of codes:
 constexpr int kMxSlabScales = 8;
 
 __device__ inline i32x8 mx_operand(const vec16& v) {
-    return i32x8{static_cast<int>(v[0]), static_cast<int>(v[1]), static_cast<int>(v[2]), static_cast<int>(v[3]), 0, 0, 0, 0};
+    return i32x8{static_cast<int>(v[0]), static_cast<int>(v[1]), static_cast<int>(v[2]), static_cast<int>(v[3]),
+                 0, 0, 0, 0};
 }
 
-// acc[n][m] += the 64 values of k of two blocks, one a lane half; kByte of the scale words is theirs.  4: 4-bit operands.
-template <int kByte> __device__ inline accum16 multiply_mx(const vec16& b, const vec16& a, uint32_t sb, uint32_t sa, accum16 c) {
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(b), mx_operand(a), c, 4, 4, kByte, static_cast<int>(sb), kByte, static_cast<int>(sa));
+// acc[n][m] += the 64 values of k of two blocks, one a lane half; kByte of the scale words is theirs.  4: 4-bit
+// operands.
+template <int kByte>
+__device__ inline accum16 multiply_mx(const vec16& b, const vec16& a, uint32_t sb, uint32_t sa, accum16 c) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(b), mx_operand(a), c, 4, 4, kByte,
+                                                           static_cast<int>(sb), kByte, static_cast<int>(sa));
 }
 // The same for 16 x 16 tiles and 128 values, a block a lane quarter.
 __device__ inline accum4 multiply16_mx(const vec16& b, const vec16& a, uint32_t sb, uint32_t sa, accum4 c) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(b), mx_operand(a), c, 4, 4, 0, static_cast<int>(sb), 0, static_cast<int>(sa));
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(b), mx_operand(a), c, 4, 4, 0,
+                                                            static_cast<int>(sb), 0, static_cast<int>(sa));
 }
 
 // Queues 4 bytes a lane from buffer + offset to LDS address `to` + 4 * lane, as queue16 does 16.
 __device__ inline void queue4(uint32_t to, uint32_t offset, const vec16& buffer) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(buffer)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(offset),
+                 "s"(buffer)
                  : "memory", "m0");
 }
 
@@ -63,7 +69,8 @@ template <int kRows, int kThreads> struct Scales {
     static __device__ int wave() { return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64)); }
 
     __device__ void begin(const uint8_t* data, int64_t pitch, int64_t first, int64_t limit) {
-        const int lane = static_cast<int>(threadIdx.x % 64), last = limit - first < kRows ? static_cast<int>(limit - first) - 1 : kRows - 1;
+        const int lane = static_cast<int>(threadIdx.x % 64),
+            last = limit - first < kRows ? static_cast<int>(limit - first) - 1 : kRows - 1;
         base = data + first * pitch;
         left = static_cast<int>(pitch / 4) - lane % 2;
 #pragma unroll
@@ -75,9 +82,11 @@ template <int kRows, int kThreads> struct Scales {
     __device__ void load(char* lds) {
         const uint64_t address = reinterpret_cast<uint64_t>(base);
         vec16 buffer{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address))),
-                     static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32))), kBufferLimit, kBufferWord3};
+                     static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32))),
+                         kBufferLimit, kBufferWord3};
         asm volatile("s_nop 4" : "+s"(buffer));   // wait states between its writing and the loads
-        const uint32_t to = __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>((lds_void)(lds))));
+        const uint32_t to =
+            __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>((lds_void)(lds))));
 #pragma unroll
         for (int i = 0; i < kOwn; ++i)
             if (kLoads % kWaves == 0 || wave() + i * kWaves < kLoads)
@@ -99,7 +108,8 @@ template <class I> __device__ inline vec16 chunk_at(const char* lds, int r, int 
 __device__ inline vec16 buffer_of(const uint8_t* base) {
     const uint64_t address = reinterpret_cast<uint64_t>(base);
     vec16 buffer{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address))),
-                 static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32))), kBufferLimit, kBufferWord3};
+                 static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32))), kBufferLimit,
+                     kBufferWord3};
     asm volatile("s_nop 4" : "+s"(buffer));   // wait states between its writing and the loads
     return buffer;
 }
@@ -107,8 +117,9 @@ __device__ inline uint32_t lds_address(const char* lds, int more) {
     return __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>((lds_void)(lds))) + more);
 }
 
-// Both operands' scales on their way to LDS, 16 bytes a row: those of two slabs, a group.  Four lanes take a row, so that a
-// load touches 16 lines (two lanes a row and slab: 32; all loads of a 256 x 256 tile alone then took a third longer).
+// Both operands' scales on their way to LDS, 16 bytes a row: those of two slabs, a group.  Four lanes take a row, so
+// that a load touches 16 lines (two lanes a row and slab: 32; all loads of a 256 x 256 tile alone then took a third
+// longer).
 template <int kBM, int kBN, int kThreads> struct ScaleRows {
     static constexpr int kRowBytes = 16, kBytes = (kBM + kBN) * kRowBytes, kWaves = kThreads / 64;
     static constexpr int kLoads = kBytes / 256 / kWaves;       // a wave's loads of 16 rows
@@ -117,10 +128,13 @@ template <int kBM, int kBN, int kThreads> struct ScaleRows {
     const uint8_t *a, *b;    // uniform over the workgroup
     int left;                // words from this lane's on to its row's end
 
-    static __device__ int part(int i) { return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64)) + i * kWaves; }
+    static __device__ int part(int i) {
+        return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64)) + i * kWaves;
+    }
 
     // Rows past the last read the last.
-    __device__ void begin(const uint8_t* rows, const uint8_t* columns, int64_t pitch, int64_t rows_left, int64_t columns_left) {
+    __device__ void begin(const uint8_t* rows, const uint8_t* columns, int64_t pitch, int64_t rows_left,
+                          int64_t columns_left) {
         a = rows, b = columns;
         const int lane = static_cast<int>(threadIdx.x % 64);
         left = static_cast<int>(pitch / 4) - lane % 4;
@@ -149,8 +163,16 @@ template <int kBM, int kBN, int kThreads> struct ScaleRows {
     }
 };
 
-// A tile of a product of codes with codes.  A slab is eight blocks of k, 128 bytes of codes: a lane of half h takes blocks
-// 4 h .. 4 h + 3, one at each of four steps.
+// A tile of a product of codes with codes.  A slab is eight blocks of k, 128 bytes of codes: a lane of half h takes
+// blocks 4 h .. 4 h + 3, one at each of four steps.
+//
+// 16384 x 4096 x 4096, bf16 out: 162 to 185 us, 3.0 to 3.4 PFLOP/s, with bias and gelu 197 to 230; 4096 more of k take
+// 124 to 158 us (the clock falls by a tenth and more under this load).  Parts of it timed alone: the products from
+// registers 85 us, with their LDS reads 98 to 120, the loads 95.  Loads of the next slab take most of a slab's
+// products' time, and neither covers the other wholly.  Slower, with the epilogue's arithmetic: 128 x 128 tiles 234 to
+// 280 us (twice the loads); 256 x 128, two workgroups a CU, slabs of half the depth in three buffers 246 to 285 (half
+// lines), or one buffer each 229 to 256; fragments read a step ahead, eight waves 259 to 275, four waves of 128 x 128
+// 239 to 254.
 template <int kBM, int kBN, int kWM, int kWN> struct MxTile : Sums<kBM, kBN, kWM, kWN> {
     using Base = Sums<kBM, kBN, kWM, kWN>;
     using Base::acc;
@@ -164,13 +186,15 @@ template <int kBM, int kBN, int kWM, int kWN> struct MxTile : Sums<kBM, kBN, kWM
     static constexpr int kBytes = 2 * (kBuffer + S::kBytes);
     static constexpr int kLds = kBytes > kThreads / 64 * Base::kRegion ? kBytes : kThreads / 64 * Base::kRegion;
 
-    template <int kStep> __device__ void add_step(const char* here, const uint32_t (&sa)[kMs], const uint32_t (&sb)[kNs]) {
+    template <int kStep> __device__ void add_step(const char* here, const uint32_t (&sa)[kMs],
+                                                  const uint32_t (&sb)[kNs]) {
         const int lane = static_cast<int>(threadIdx.x % 64), chunk = 4 * (lane / 32) + kStep;
         vec16 fa[kMs], fb[kNs];
 #pragma unroll
         for (int i = 0; i < kMs; ++i) fa[i] = chunk_at<A>(here, Base::wave_row() + 32 * i + lane % 32, chunk);
 #pragma unroll
-        for (int j = 0; j < kNs; ++j) fb[j] = chunk_at<B>(here + A::kBytes, Base::wave_column() + 32 * j + lane % 32, chunk);
+        for (int j = 0; j < kNs; ++j)
+            fb[j] = chunk_at<B>(here + A::kBytes, Base::wave_column() + 32 * j + lane % 32, chunk);
 #pragma unroll
         for (int i = 0; i < kMs; ++i)
 #pragma unroll
@@ -183,7 +207,8 @@ template <int kBM, int kBN, int kWM, int kWN> struct MxTile : Sums<kBM, kBN, kWM
 #pragma unroll
         for (int i = 0; i < kMs; ++i) sa[i] = S::word(scales, Base::wave_row() + 32 * i + lane % 32, slab, lane / 32);
 #pragma unroll
-        for (int j = 0; j < kNs; ++j) sb[j] = S::word(scales, kBM + Base::wave_column() + 32 * j + lane % 32, slab, lane / 32);
+        for (int j = 0; j < kNs; ++j)
+            sb[j] = S::word(scales, kBM + Base::wave_column() + 32 * j + lane % 32, slab, lane / 32);
         add_step<0>(here, sa, sb);
         add_step<1>(here, sa, sb);
         add_step<2>(here, sa, sb);
@@ -214,7 +239,8 @@ template <int kBM, int kBN, int kWM, int kWN> struct MxTile : Sums<kBM, kBN, kWM
 };
 
 template <class T, int kBM, int kBN, int kWM, int kWN>
-__global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void mx_rows4_kernel(MxRowsArgs m, uint32_t first, uint32_t blocks) {
+__global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void mx_rows4_kernel(
+    MxRowsArgs m, uint32_t first, uint32_t blocks) {
     using Work = MxTile<kBM, kBN, kWM, kWN>;
     __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
     const RowsArgs& a = m.rows;
@@ -238,7 +264,9 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void mx_rows4_kerne
     finish_tile<T, kBM == 256>(work, a, p, column0, lds);
 }
 
-// A tile of a product of rows of T with codes.  A slab of the weight's codes lasts for kRatio slabs of the rows.
+// A tile of a product of rows of T with codes.  A slab of the weight's codes lasts for kRatio slabs of the rows. 16384
+// x 4096 x 4096 bf16 450 to 500 us, 1100 to 1220 TFLOP/s, with bias and gelu 490 to 530; 131072 rows over 64 experts,
+// 256 -> 512 fp16 with silu and the sums kept 100 to 110 us, 340 MB at 3.1 to 3.4 TB/s.
 template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> struct MixedTile : Sums<kBM, kBN, kWM, kWN> {
     using Base = Sums<kBM, kBN, kWM, kWN>;
     using Base::acc;
@@ -246,7 +274,8 @@ template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> struct MixedTil
     using Base::kNs;
     using Base::kThreads;
     using A = std::conditional_t<kWay == kDirect, Direct<T, true, kBM, kThreads>,
-                                 std::conditional_t<kWay == kStaged, Staged<T, true, kBM, kThreads>, Gathered<T, true, kBM, kThreads>>>;
+                                 std::conditional_t<kWay == kStaged, Staged<T, true, kBM, kThreads>,
+                                                    Gathered<T, true, kBM, kThreads>>>;
     using B = Direct<uint8_t, true, kBN, kThreads>;
     using SB = Scales<kBN, kThreads>;
     static constexpr int kRatio = kMxSlab / kSlab<T>;
@@ -254,8 +283,8 @@ template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> struct MixedTil
     static constexpr int kBytes = 2 * (A::kBytes + kCodes);
     static constexpr int kLds = kBytes > kThreads / 64 * Base::kRegion ? kBytes : kThreads / 64 * Base::kRegion;
 
-    // Slab `part` of the kRatio of these codes.  A lane of half h takes values 32 (2 part + h) .. + 31 of the codes' slab,
-    // a block (fp32: half a block, 32 part + 16 h .. + 15), eight (four) at a step.
+    // Slab `part` of the kRatio of these codes.  A lane of half h takes values 32 (2 part + h) .. + 31 of the codes'
+    // slab, a block (fp32: half a block, 32 part + 16 h .. + 15), eight (four) at a step.
     __device__ void add_slab(const char* rows, const char* codes, int part) {
         const int lane = static_cast<int>(threadIdx.x % 64), half = lane / 32;
         constexpr bool kWide = sizeof(T) == 4;
@@ -271,7 +300,8 @@ template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> struct MixedTil
         for (int step = 0; step < 4; ++step) {
             vec16 fa[kMs], fb[kNs];
 #pragma unroll
-            for (int i = 0; i < kMs; ++i) fa[i] = chunk_at<A>(rows, Base::wave_row() + 32 * i + lane % 32, 4 * half + step);
+            for (int i = 0; i < kMs; ++i)
+                fa[i] = chunk_at<A>(rows, Base::wave_row() + 32 * i + lane % 32, 4 * half + step);
 #pragma unroll
             for (int j = 0; j < kNs; ++j) {
                 const uint32_t word = kWide ? (half ? held[j][2 + step / 2] : held[j][step / 2]) : held[j][step];
@@ -327,7 +357,8 @@ template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> struct MixedTil
 };
 
 template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN>
-__global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void mx_mixed_kernel(MxRowsArgs m, uint32_t first, uint32_t blocks) {
+__global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void mx_mixed_kernel(
+    MxRowsArgs m, uint32_t first, uint32_t blocks) {
     using Work = MixedTile<T, kWay, kBM, kBN, kWM, kWN>;
     __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
     const RowsArgs& a = m.rows;
@@ -350,8 +381,10 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void mx_mixed_kerne
     finish_tile<T, kBM == 256>(work, a, p, column0, lds);
 }
 
-// Few rows a group, as few_rows_kernel: the weight's codes go straight into registers, once for every 16 kRowTiles rows.
-// A step takes four blocks of k, one a lane quarter, and a wave one of kSplit shares of the blocks.
+// Few rows a group, as few_rows_kernel: the weight's codes go straight into registers, once for every 16 kRowTiles
+// rows. A step takes four blocks of k, one a lane quarter, and a wave one of kSplit shares of the blocks.  Bound by the
+// latency of a chain of loads: one bf16 row through 2048 -> 2048 (2.2 MB) 4.3 us, 16 rows over 64 experts of 512 ->
+// 1024 7.2 us.  Twice the steps in flight: 4.7 and 7.4.
 template <class T, bool kRows4, int kRowTiles, int kSplit>
 __global__ __launch_bounds__(64 * kFewWaves) void mx_few_rows_kernel(MxRowsArgs m) {
     constexpr int kColumns = 16 * kFewWaves / kSplit;   // of a workgroup
@@ -415,12 +448,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx_few_rows_kernel(MxRowsArgs 
             for (int u = 0; u < kAhead; ++u) {
                 if constexpr (kRows4) {
 #pragma unroll
-                    for (int t = 0; t < kRowTiles; ++t) acc[t] = multiply16_mx(fw[u], fx[u][t][0], sw[u], sx[u][t], acc[t]);
+                    for (int t = 0; t < kRowTiles; ++t)
+                        acc[t] = multiply16_mx(fw[u], fx[u][t][0], sw[u], sx[u][t], acc[t]);
                 } else {
                     const float scale = mx_scale(sw[u]);
 #pragma unroll
                     for (int i = 0; i < kParts; ++i) {
-                        const vec16 values = mx_values<T>(fw[u][i * kPerVec<T> / 8], scale, sizeof(T) == 4 && i % 2 == 1);
+                        const vec16 values =
+                            mx_values<T>(fw[u][i * kPerVec<T> / 8], scale, sizeof(T) == 4 && i % 2 == 1);
 #pragma unroll
                         for (int t = 0; t < kRowTiles; ++t) acc[t] = multiply16(T{}, values, fx[u][t][i], acc[t]);
                     }
@@ -447,18 +482,22 @@ template <int kBM, int kBN, int kWM, int kWN, class Launch> int in_tiles(MxRowsA
 }
 
 template <class T, int kBM, int kBN, int kWM, int kWN> int launch_rows4(const MxRowsArgs& m, hipStream_t stream) {
-    return in_tiles<kBM, kBN, kWM, kWN>(m, [&](const MxRowsArgs& a, uint32_t grid, int threads, uint32_t first, uint32_t blocks) {
+    return in_tiles<kBM, kBN, kWM, kWN>(m, [&](const MxRowsArgs& a, uint32_t grid, int threads,
+                                               uint32_t first, uint32_t blocks) {
         mx_rows4_kernel<T, kBM, kBN, kWM, kWN><<<grid, threads, 0, stream>>>(a, first, blocks);
     });
 }
 
-template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> int launch_mixed(const MxRowsArgs& m, hipStream_t stream) {
-    return in_tiles<kBM, kBN, kWM, kWN>(m, [&](const MxRowsArgs& a, uint32_t grid, int threads, uint32_t first, uint32_t blocks) {
+template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN>
+int launch_mixed(const MxRowsArgs& m, hipStream_t stream) {
+    return in_tiles<kBM, kBN, kWM, kWN>(m, [&](const MxRowsArgs& a, uint32_t grid, int threads,
+                                               uint32_t first, uint32_t blocks) {
         mx_mixed_kernel<T, kWay, kBM, kBN, kWM, kWN><<<grid, threads, 0, stream>>>(a, first, blocks);
     });
 }
 
-template <class T, bool kRows4, int kRowTiles, int kSplit> int launch_mx_few_as(const MxRowsArgs& m, hipStream_t stream) {
+template <class T, bool kRows4, int kRowTiles, int kSplit>
+int launch_mx_few_as(const MxRowsArgs& m, hipStream_t stream) {
     const RowsArgs& a = m.rows;
     const int64_t across = (a.columns + 16 * kFewWaves / kSplit - 1) / (16 * kFewWaves / kSplit);
     const int64_t blocks = piece_ids(a.rows, 16 * kRowTiles, a.offsets != nullptr, a.experts, true) * across;
@@ -467,9 +506,9 @@ template <class T, bool kRows4, int kRowTiles, int kSplit> int launch_mx_few_as(
     return check_launch("linear of 4-bit weights");
 }
 
-// The depth over all eight waves where a share is still long or there are too few workgroups otherwise, else over two.  us
-// with eight and with two: 2048 -> 2048 bf16, one row 4.3 and 8.3, 16 rows 5.5 and 13.6; 512 -> 4096 3.4 and 4.0; 512 -> 16384
-// 5.3 and 4.2; 16 rows over 64 experts of 512 -> 1024 10.8 and 7.2; 4096 -> 16384 16.0 and 17.7.
+// The depth over all eight waves where a share is still long or there are too few workgroups otherwise, else over two.
+// us with eight and with two: 2048 -> 2048 bf16, one row 4.3 and 8.3, 16 rows 5.5 and 13.6; 512 -> 4096 3.4 and 4.0;
+// 512 -> 16384 5.3 and 4.2; 16 rows over 64 experts of 512 -> 1024 10.8 and 7.2; 4096 -> 16384 16.0 and 17.7.
 template <class T, bool kRows4, int kRowTiles> int launch_mx_few(const MxRowsArgs& m, hipStream_t stream) {
     const int64_t steps = m.code_pitch / (4 * kMxBytes);
     const int64_t busy = m.rows.rows < m.rows.experts ? m.rows.rows : m.rows.experts;
@@ -477,9 +516,10 @@ template <class T, bool kRows4, int kRowTiles> int launch_mx_few(const MxRowsArg
     return launch_mx_few_as<T, kRows4, kRowTiles, 2>(m, stream);
 }
 
-// Tiles as linear's, by the work there is.  us of bf16 products as 256 x 256, 128 x 128 and 64 x 64: rows of bf16, 65536 x
-// 1024 x 4096 522, 624 and 849, 16384 x 1024 x 1024 37, 45 and 57, 4096 x 2048 x 2048 (128 tiles of the largest) -, 42 and 58,
-// 131072 rows over 64 experts of 256 -> 512 88, 90 and 110; 4-bit rows 247, 308 and 382, 17, 22 and 28, -, 19 and 22, 61, 63 and 72.
+// Tiles as linear's, by the work there is.  us of bf16 products as 256 x 256, 128 x 128 and 64 x 64: rows of bf16,
+// 65536 x 1024 x 4096 522, 624 and 849, 16384 x 1024 x 1024 37, 45 and 57, 4096 x 2048 x 2048 (128 tiles of the
+// largest) -, 42 and 58, 131072 rows over 64 experts of 256 -> 512 88, 90 and 110; 4-bit rows 247, 308 and 382, 17, 22
+// and 28, -, 19 and 22, 61, 63 and 72.
 template <class T, Way kWay> int launch_mixed_of(const MxRowsArgs& m, hipStream_t stream) {
     const RowsArgs& a = m.rows;
     const int64_t each = a.rows / a.experts;
@@ -494,10 +534,10 @@ template <class T, Way kWay> int launch_mixed_of(const MxRowsArgs& m, hipStream_
 
 template <class T, bool kRows4> int launch_mx_by_rows(const MxRowsArgs& m, hipStream_t stream) {
     const RowsArgs& a = m.rows;
-    // Few rows: up to 64 for one matrix (4-bit rows 32), up to 256 (128) in all over several.  us of few rows and of tiles,
-    // bf16: 2048 -> 2048, 16 rows 5.5 and 15.0, 32 rows 7.4 and 15.2, 64 rows 11.6 and 15.3; 4-bit rows 4.5 and 7.1, 5.6 and
-    // 7.2, 8.0 and 7.4.  Over 64 experts of 512 -> 1024, 64 rows 8.0 and 12.8, 256 rows 13.0 and 13.4, 512 rows 15.8 and 13.6;
-    // 4-bit rows, 64 rows 7.2 and 8.2, 256 rows 8.7 and 8.5, 512 rows 11.5 and 8.6.
+    // Few rows: up to 64 for one matrix (4-bit rows 32), up to 256 (128) in all over several.  us of few rows and of
+    // tiles, bf16: 2048 -> 2048, 16 rows 5.5 and 15.0, 32 rows 7.4 and 15.2, 64 rows 11.6 and 15.3; 4-bit rows 4.5 and
+    // 7.1, 5.6 and 7.2, 8.0 and 7.4.  Over 64 experts of 512 -> 1024, 64 rows 8.0 and 12.8, 256 rows 13.0 and 13.4, 512
+    // rows 15.8 and 13.6; 4-bit rows, 64 rows 7.2 and 8.2, 256 rows 8.7 and 8.5, 512 rows 11.5 and 8.6.
     if (a.experts > 1 ? a.rows <= (kRows4 ? 128 : 256) : a.rows <= 16) return launch_mx_few<T, kRows4, 1>(m, stream);
     if (a.experts == 1 && a.rows <= 32) return launch_mx_few<T, kRows4, 2>(m, stream);
     if constexpr (!kRows4)
@@ -505,8 +545,10 @@ template <class T, bool kRows4> int launch_mx_by_rows(const MxRowsArgs& m, hipSt
     if constexpr (kRows4) {
         const int64_t large = (a.rows + 255) / 256 * ((a.columns + 255) / 256);
         const int64_t wide = (a.rows + 127) / 128 * ((a.columns + 127) / 128);
-        if (a.columns > 128 && even(large) && a.rows / a.experts >= 1024) return launch_rows4<T, 256, 256, 64, 128>(m, stream);
-        if (a.columns > 64 && wide >= kCus && a.rows / a.experts >= 128) return launch_rows4<T, 128, 128, 64, 64>(m, stream);
+        if (a.columns > 128 && even(large) && a.rows / a.experts >= 1024)
+            return launch_rows4<T, 256, 256, 64, 128>(m, stream);
+        if (a.columns > 64 && wide >= kCus && a.rows / a.experts >= 128)
+            return launch_rows4<T, 128, 128, 64, 64>(m, stream);
         return launch_rows4<T, 64, 64, 32, 32>(m, stream);
     } else {
         switch (way_of<T>(a.a, a.lda, a.depth)) {

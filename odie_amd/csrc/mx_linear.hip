@@ -6,7 +6,8 @@
 namespace odie {
 namespace {
 
-int check_sizes(const std::string& what, int64_t rows, int experts, bool grouped, int inputs, int outputs, int dtype, int activation) {
+int check_sizes(const std::string& what, int64_t rows, int experts, bool grouped, int inputs, int outputs, int dtype,
+                int activation) {
     constexpr int kMost = 1 << 20;
     if (!known_dtype(dtype)) return fail(what + ": dtype must be 0 (fp32), 1 (fp16) or 2 (bf16)");
     if (activation < 0 || activation >= kActivations) return fail(what + ": activation must be within 0..5");
@@ -15,7 +16,8 @@ int check_sizes(const std::string& what, int64_t rows, int experts, bool grouped
         return fail(what + ": inputs and outputs must be within 1..2^20");
     if (experts < 1 || experts > 1 << 15) return fail(what + ": experts must be within 1..32768");
     if (!grouped && experts != 1) return fail(what + ": several experts need offsets");
-    if (static_cast<int64_t>(experts) * outputs > (int64_t{1} << 31) - 1) return fail(what + ": experts times outputs must be below 2^31");
+    if (static_cast<int64_t>(experts) * outputs > (int64_t{1} << 31) - 1)
+        return fail(what + ": experts times outputs must be below 2^31");
     return 0;
 }
 
@@ -27,18 +29,25 @@ struct GradientPlan {
     int64_t weight_bytes, sums_bytes, rest_bytes;   // the weight, its fused sums, or what odie_linear_backward takes
 };
 
-// Fused where dz is formed once for all of dx: the inputs fit a tile, in 16 bits, and the rows make two tiles a CU; fewer
-// leave each CU one long chain of slabs.  us apart and fused, with the weight and the bias: 131072 rows over 64 fp16 experts,
-// silu, 64 -> 64 36 and 24, 128 -> 256 79 and 60, 256 -> 512 173 and 130; 65536 rows, 256 -> 512, gelu, 77 and 66; 300007 rows,
-// 192 -> 40, 77 and 70; but 16384 rows over 64, 256 -> 1024, 63 and 74, 2048 over 4 20 and 37.
+// Fused where dz is formed once for all of dx: the inputs fit a tile, in 16 bits, and the rows make two tiles a CU;
+// fewer leave each CU one long chain of slabs.  us apart and fused, with the weight and the bias: 131072 rows over 64
+// fp16 experts, silu, 64 -> 64 36 and 24, 128 -> 256 79 and 60, 256 -> 512 173 and 130; 65536 rows, 256 -> 512, gelu,
+// 77 and 66; 300007 rows, 192 -> 40, 77 and 70; but 16384 rows over 64, 256 -> 1024, 63 and 74, 2048 over 4 20 and 37.
 GradientPlan gradient_plan(int64_t rows, int experts, bool grouped, int inputs, int outputs, int dtype, int activation,
                            bool want_dx, bool want_dbias) {
     GradientPlan p{};
-    p.fused = want_dx && activation != kNone && dtype != ODIE_F32 && inputs <= 256 && outputs >= 8 && rows >= 2 * kCus * mx_input_tile(inputs).rows && rows / experts >= 128;
+    p.fused = want_dx && activation != kNone && dtype != ODIE_F32 && inputs <= 256 && outputs >= 8 &&
+        rows >= 2 * kCus * mx_input_tile(inputs).rows && rows / experts >= 128;
     p.pitch = p.fused ? (inputs + 7) / 8 * 8 : inputs;
     p.weight_bytes = want_dx ? padded(static_cast<int64_t>(experts) * outputs * p.pitch * dtype_bytes(dtype)) : 0;
-    if (p.fused) p.sums_bytes = want_dbias ? padded(piece_ids(rows, mx_input_tile(inputs).rows, grouped, experts, false) * outputs * 4) : 0;
-    else p.rest_bytes = odie_linear_workspace(rows, experts, grouped, inputs, outputs, dtype, activation, 0, want_dbias);
+    if (p.fused) {
+        if (want_dbias)
+            p.sums_bytes =
+                padded(piece_ids(rows, mx_input_tile(inputs).rows, grouped, experts, false) * outputs * 4);
+    } else {
+        p.rest_bytes = odie_linear_workspace(rows, experts, grouped, inputs, outputs, dtype, activation, 0,
+                                             want_dbias);
+    }
     return p;
 }
 
@@ -49,8 +58,9 @@ using namespace odie;
 
 ODIE_API int odie_mx_linear_forward(const void* x, const uint8_t* x_scales, int64_t x_stride, int64_t rows,
                                     const uint8_t* codes, const uint8_t* scales, const void* bias, const void* residual,
-                                    int64_t residual_stride, const int32_t* offsets, int experts, int inputs, int outputs,
-                                    int dtype, int activation, void* out, int64_t out_stride, void* pre, uint64_t stream) {
+                                    int64_t residual_stride, const int32_t* offsets, int experts, int inputs,
+                                    int outputs, int dtype, int activation, void* out, int64_t out_stride, void* pre,
+                                    uint64_t stream) {
     const std::string what = "odie_mx_linear_forward";
     if (check_sizes(what, rows, experts, offsets != nullptr, inputs, outputs, dtype, activation)) return -1;
     if (rows == 0) return 0;
@@ -85,8 +95,10 @@ ODIE_API int odie_mx_linear_forward(const void* x, const uint8_t* x_scales, int6
 
 ODIE_API int64_t odie_mx_linear_workspace(int64_t rows, int experts, int grouped, int inputs, int outputs, int dtype,
                                           int activation, int want_dx, int want_dbias) {
-    if (check_sizes("odie_mx_linear_workspace", rows, experts, grouped != 0, inputs, outputs, dtype, activation)) return -1;
-    const GradientPlan p = gradient_plan(rows, experts, grouped != 0, inputs, outputs, dtype, activation, want_dx != 0, want_dbias != 0);
+    if (check_sizes("odie_mx_linear_workspace", rows, experts, grouped != 0, inputs, outputs, dtype, activation))
+        return -1;
+    const GradientPlan p = gradient_plan(rows, experts, grouped != 0, inputs, outputs, dtype, activation, want_dx != 0,
+                                         want_dbias != 0);
     return p.weight_bytes + p.sums_bytes + p.rest_bytes;
 }
 
@@ -96,20 +108,24 @@ ODIE_API int odie_mx_linear_backward(const void* upstream, int64_t upstream_stri
                                      void* workspace, int64_t workspace_bytes, uint64_t stream) {
     const std::string what = "odie_mx_linear_backward";
     if (check_sizes(what, rows, experts, offsets != nullptr, inputs, outputs, dtype, activation)) return -1;
-    if (rows > 0 && (!upstream || (dx && (!codes || !scales)) || (activation != kNone && !pre))) return fail(what + ": null pointer");
+    if (rows > 0 && (!upstream || (dx && (!codes || !scales)) || (activation != kNone && !pre)))
+        return fail(what + ": null pointer");
     if (rows > 0 && upstream_stride < outputs) return fail(what + ": rows overlap (a stride below the row's width)");
     if (dx && (reinterpret_cast<uintptr_t>(codes) % 16 || reinterpret_cast<uintptr_t>(scales) % 4))
         return fail(what + ": codes must be 16-byte and scales 4-byte aligned");
-    const GradientPlan p = gradient_plan(rows, experts, offsets != nullptr, inputs, outputs, dtype, activation, dx != nullptr, dbias != nullptr);
+    const GradientPlan p = gradient_plan(rows, experts, offsets != nullptr, inputs, outputs, dtype, activation,
+                                         dx != nullptr, dbias != nullptr);
     const int64_t need = p.weight_bytes + p.sums_bytes + p.rest_bytes;
     if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0))
         return fail(what + ": needs a 256-byte aligned workspace of " + std::to_string(need) + " bytes");
     char* const weight = static_cast<char*>(workspace);
-    if (dx && rows > 0 && odie_mx_dequantize(codes, scales, static_cast<int64_t>(experts) * outputs, inputs, dtype, weight, p.pitch, stream)) return -1;
+    if (dx && rows > 0 && odie_mx_dequantize(codes, scales, static_cast<int64_t>(experts) * outputs, inputs, dtype,
+                                             weight, p.pitch, stream))
+        return -1;
     if (!p.fused)
-        return odie_linear_backward(upstream, upstream_stride, nullptr, 0, pre, rows, dx ? weight : nullptr, offsets, experts,
-                                    inputs, outputs, dtype, activation, dx, nullptr, dbias, weight + p.weight_bytes,
-                                    p.rest_bytes, stream);
+        return odie_linear_backward(upstream, upstream_stride, nullptr, 0, pre, rows, dx ? weight : nullptr, offsets,
+                                    experts, inputs, outputs, dtype, activation, dx, nullptr, dbias,
+                                    weight + p.weight_bytes, p.rest_bytes, stream);
     const hipStream_t s = as_stream(stream);
     MxInputArgs m{};
     m.rows.a = upstream;

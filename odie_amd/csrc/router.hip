@@ -1,8 +1,8 @@
 // A learned router over experts: the choice of each row's experts with their softmax weights, and the loss that
 // keeps their load even, with their gradients.
 //
-//   choose   e_1 .. e_k: the row's largest logits, the lowest index first among equal ones; w_j = exp(l_ej - m) / s, s over
-//            the chosen (normalised) or over all experts
+//   choose   e_1 .. e_k: the row's largest logits, the lowest index first among equal ones; w_j = exp(l_ej - m) / s, s
+//            over the chosen (normalised) or over all experts
 //            dl_e = [e = e_j] w_j g_j - q_e sum_i w_i g_i, q the softmax over the chosen or over all
 //   balance  c_e entries of expert e, M in all; R rows that have an entry; t_i = sum_e c_e p_ie over row i's softmax
 //            loss = E / (M R) sum_i t_i,  dl_ie = g E / (M R) p_ie (c_e - t_i)
@@ -23,8 +23,8 @@ constexpr int64_t kMaxEntries = (int64_t{1} << 31) - 1;
 template <class N> __device__ inline N most_of(N a, N b) { return a > b ? a : b; }
 template <class N> __device__ inline N least_of(N a, N b) { return a < b ? a : b; }
 
-// Logits with their indices as whole numbers: the larger the logit and, among equal ones, the lower the index, the larger
-// the key.  A logit's bits become a signed number in the order of the values by negating the magnitude of
+// Logits with their indices as whole numbers: the larger the logit and, among equal ones, the lower the index, the
+// larger the key.  A logit's bits become a signed number in the order of the values by negating the magnitude of
 // negative ones (which makes -0 and 0 alike); a NaN is the largest.  A 16-bit logit and its index fit 32 bits.
 template <class T> struct Keys {
     using Key = int32_t;
@@ -65,7 +65,10 @@ template <class T> struct Keys {
         const int order = key >> 16;
         return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(order < 0 ? 0x8000 | -order : order)));
     }
-    static __device__ Key second(Key most, Key less, Key key) { return most_of(least_of(most, less), least_of(most_of(most, less), key)); }   // the middle one
+    // the middle one
+    static __device__ Key second(Key most, Key less, Key key) {
+        return most_of(least_of(most, less), least_of(most_of(most, less), key));
+    }
     template <int kLanes> static __device__ Key best(Key key) {
         return static_cast<Key>(across<kLanes>(static_cast<uint32_t>(key), [](uint32_t a, uint32_t b) {
             return static_cast<uint32_t>(most_of(static_cast<int32_t>(a), static_cast<int32_t>(b)));
@@ -79,7 +82,8 @@ template <> struct Keys<float> {
     static __device__ Key of(float value, int index) {
         const int32_t bits = __builtin_bit_cast(int32_t, value), sign = bits >> 31, size = bits & 0x7fffffff;
         const int32_t order = size > 0x7f800000 ? 0x7fffffff : (size ^ sign) - sign;
-        return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(order)) << 32 | static_cast<uint32_t>(~index));
+        return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(order)) << 32 |
+                                    static_cast<uint32_t>(~index));
     }
     template <bool kChecked> static __device__ void of(const vec16& chunk, int index, Key key[4]) {
 #pragma unroll
@@ -95,17 +99,19 @@ template <> struct Keys<float> {
     template <int kLanes> static __device__ Key best(Key key) {
         // the largest order first, then the largest rest among the lanes that hold it
         const int32_t order = static_cast<int32_t>(key >> 32);
-        const int32_t top = static_cast<int32_t>(across<kLanes>(static_cast<uint32_t>(order), [](uint32_t a, uint32_t b) {
+        const int32_t top =
+            static_cast<int32_t>(across<kLanes>(static_cast<uint32_t>(order), [](uint32_t a, uint32_t b) {
             return static_cast<uint32_t>(most_of(static_cast<int32_t>(a), static_cast<int32_t>(b)));
         }));
-        const uint32_t rest = across<kLanes>(order == top ? static_cast<uint32_t>(key) : 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+        const uint32_t rest = across<kLanes>(order == top ? static_cast<uint32_t>(key) : 0u,
+                                             [](uint32_t a, uint32_t b) { return a > b ? a : b; });
         return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(top)) << 32 | rest);
     }
 };
 
-// A row's 16-byte chunks, kVecs a lane, loaded ahead of their use: without conditions, which would make the compiler wait
-// for loads in flight, from addresses moved back into the row where they would leave it; settle() puts that right.  The first half of
-// several chunks is always whole (with_row).  Rows shorter than a chunk are gathered.
+// A row's 16-byte chunks, kVecs a lane, loaded ahead of their use: without conditions, which would make the compiler
+// wait for loads in flight, from addresses moved back into the row where they would leave it; settle() puts that right.
+// The first half of several chunks is always whole (with_row).  Rows shorter than a chunk are gathered.
 template <class T, int kLanes, int kVecs> struct RowHold {
     static constexpr int kV = kPerVec<T>;
     vec16 chunk[kVecs];
@@ -126,7 +132,8 @@ template <class T, int kLanes, int kVecs> struct RowHold {
 #pragma unroll
         for (int v = kVecs / 2; v < kVecs; ++v) {
             const int count = width - (v * kLanes + lane) * kV;
-            if (count < kV && width >= kV) chunk[v] = count > 0 ? shift_down(chunk[v], (kV - count) * static_cast<int>(sizeof(T))) : vec16{};
+            if (count < kV && width >= kV)
+                chunk[v] = count > 0 ? shift_down(chunk[v], (kV - count) * static_cast<int>(sizeof(T))) : vec16{};
         }
     }
     __device__ void get(int v, int lane, int width, float value[kV]) const {
@@ -148,9 +155,11 @@ struct ChooseArgs {
     int normalize;
 };
 
-// Rows of up to 64 kVecs chunks in registers, the next one under way.  Each lane keeps its two largest keys; a choice takes
-// the largest of all lanes, whose lane goes on to its second, and looks through its keys again once both are gone: at four
-// choices of 1024 about once in 500 rows.
+// Rows of up to 64 kVecs chunks in registers, the next one under way.  Each lane keeps its two largest keys; a choice
+// takes the largest of all lanes, whose lane goes on to its second, and looks through its keys again once both are
+// gone: at four choices of 1024 about once in 500 rows.  65536 x 1024 fp16, four choices with weights among all: 50 us,
+// 134 MB at 2.7 TB/s, bound by the arithmetic (about 450 instructions a row; with a search of all keys for each choice
+// 61 us); one row 2 us.
 template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) void choose_kernel(ChooseArgs a) {
     using K = Keys<T>;
     using Key = typename K::Key;
@@ -242,7 +251,8 @@ __device__ inline int64_t block_best(int64_t key, int64_t* part) {
     return key;
 }
 
-// Longer rows: a workgroup a row, which it reads once for each choice, the one below the last.
+// Longer rows: a workgroup a row, which it reads once for each choice, the one below the last.  8192 x 8000 fp16, four
+// choices: 149 us (as such, 8192 x 4096 75 us, in registers 31).
 template <class T> __global__ __launch_bounds__(kBlock) void choose_long_kernel(ChooseArgs a) {
     using K = Keys<float>;
     constexpr int kV = kPerVec<T>;
@@ -308,12 +318,14 @@ struct ChooseBackwardArgs {
     int experts, choices;
 };
 
-// kLanes lanes a row write its gradient chunk by chunk; each lane holds one of the row's entries.
+// kLanes lanes a row write its gradient chunk by chunk; each lane holds one of the row's entries.  65536 x 1024 fp16,
+// weights among all: 46 us, 268 MB at 5.8 TB/s (the logits partly from the last-level cache); over the chosen 32 us.
 template <class T, int kLanes, bool kAll, bool kStream>
 __global__ __launch_bounds__(kBlock) void choose_backward_kernel(ChooseBackwardArgs a, uint32_t first) {
     constexpr int kV = kPerVec<T>;
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
-    const int64_t at = (static_cast<int64_t>(first) + blockIdx.x) * (kBlock / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
+    const int64_t at =
+        (static_cast<int64_t>(first) + blockIdx.x) * (kBlock / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
     const int64_t row = at < a.n ? at : a.n - 1;
     int own = -1;
     float weighted = 0.0f, weight = 0.0f;      // w_j g_j, w_j
@@ -362,7 +374,7 @@ __global__ __launch_bounds__(kBlock) void choose_backward_kernel(ChooseBackwardA
 constexpr int kCountBlock = 1024;
 constexpr int kSharedCounts = 8192;      // experts whose counts a workgroup keeps in LDS
 constexpr int64_t kFewEntries = 1 << 14; // counted by one workgroup, which needs nothing cleared before
-constexpr uint32_t kFewBlocks = 64;      // of which the last one makes the loss
+constexpr uint32_t kFewBlocks = 256;     // of which the last one makes the loss
 
 struct BalanceArgs {
     const void* logits;
@@ -385,7 +397,9 @@ __global__ __launch_bounds__(kBlock) void balance_clear_kernel(BalanceArgs a) {
 }
 
 // Each workgroup counts its entries in LDS and adds what it found (whole numbers, in any order).  kAlone: one workgroup
-// of all entries.  Entries that lie 16-byte aligned are read four at a time.
+// of all entries (16384 in 2.6 us, as several with their clearing 5.5).  Entries that lie 16-byte aligned are read four
+// at a time. 1.2 million entries of 1000 experts: 6 us (with 512 workgroups, whose counts are half a million additions,
+// 27).
 template <bool kAlone> __global__ __launch_bounds__(kCountBlock) void balance_count_kernel(BalanceArgs a) {
     extern __shared__ int32_t held[];
     const bool shared = a.experts <= kSharedCounts;
@@ -417,7 +431,8 @@ template <bool kAlone> __global__ __launch_bounds__(kCountBlock) void balance_co
 }
 
 // The counts of a lane's columns as fp32, 0 past the last.
-template <class T, int kLanes, int kVecs> __device__ inline void hold_counts(const int32_t* counts, int lane, int experts, float (&to)[kVecs][kPerVec<T>]) {
+template <class T, int kLanes, int kVecs>
+__device__ inline void hold_counts(const int32_t* counts, int lane, int experts, float (&to)[kVecs][kPerVec<T>]) {
 #pragma unroll
     for (int v = 0; v < kVecs; ++v)
 #pragma unroll
@@ -432,10 +447,13 @@ template <class T, int kLanes, int kVecs> __device__ inline void hold_counts(con
 template <int kLanes> struct Part {
     int32_t id;
 
-    __device__ void load(const BalanceArgs& a, int64_t row, int lane) { id = a.expert[row * a.choices + (lane < a.choices ? lane : a.choices - 1)]; }
+    __device__ void load(const BalanceArgs& a, int64_t row, int lane) {
+        id = a.expert[row * a.choices + (lane < a.choices ? lane : a.choices - 1)];
+    }
     __device__ bool get(const BalanceArgs& a, int64_t row, int lane) const {
         uint32_t any = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.experts);
-        for (int j = lane + kLanes; j < a.choices; j += kLanes) any |= static_cast<uint32_t>(a.expert[row * a.choices + j]) < static_cast<uint32_t>(a.experts);
+        for (int j = lane + kLanes; j < a.choices; j += kLanes)
+            any |= static_cast<uint32_t>(a.expert[row * a.choices + j]) < static_cast<uint32_t>(a.experts);
         return across<kLanes>(any, [](uint32_t x, uint32_t y) { return x | y; }) != 0;
     }
 };
@@ -456,7 +474,8 @@ __device__ inline BalanceSums sum_block(BalanceSums x) {
     if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = x;
     __syncthreads();
     if (threadIdx.x == 0)
-        for (int w = 1; w < kBlock / 64; ++w) x.total += part[w].total, x.rows += part[w].rows, x.entries += part[w].entries;
+        for (int w = 1; w < kBlock / 64; ++w)
+            x.total += part[w].total, x.rows += part[w].rows, x.entries += part[w].entries;
     return x;
 }
 
@@ -470,13 +489,15 @@ __device__ inline void make_loss(const BalanceArgs& a) {
     for (int e = threadIdx.x; e < a.experts; e += kBlock) x.entries += static_cast<uint32_t>(a.counts[e]);
     x = sum_block(x);
     if (threadIdx.x != 0) return;
-    const double norm = x.entries > 0 ? a.experts / (static_cast<double>(x.entries) * static_cast<double>(x.rows)) : 0.0;
+    const double norm =
+        x.entries > 0 ? a.experts / (static_cast<double>(x.entries) * static_cast<double>(x.rows)) : 0.0;
     *a.norm = static_cast<float>(norm);
     *a.loss = static_cast<float>(x.entries > 0 ? x.total * norm : 0.0);
 }
 
-// Leaves the workgroup's sums.  Of few workgroups the last one to come goes on to the loss; each takes its turn at one
-// address, about 10 ns (65536 x 64: 1536 workgroups 25 us, 9 and 3 with a launch of its own).
+// Leaves the workgroup's sums.  Of few workgroups the last one to come goes on to the loss, which saves a launch (3 us
+// of host time); each of them takes its turn at one address, about 10 ns (65536 x 64: 1536 workgroups 25 us, with a
+// launch of its own 8.4 and 3.4; 4096 x 64: 256 workgroups 7.0, and 3.8 and 1.8).
 __device__ inline void finish_balance(const BalanceArgs& a, double total, uint32_t rows) {
     __shared__ bool last;
     const BalanceSums x = sum_block(BalanceSums{total, rows, 0});
@@ -498,7 +519,8 @@ __device__ inline void finish_balance(const BalanceArgs& a, double total, uint32
 __global__ __launch_bounds__(kBlock) void balance_loss_kernel(BalanceArgs a) { make_loss(a); }
 
 // Rows of up to 64 kVecs chunks: kLanes lanes a row, a row in registers and the next one under way, the counts of the
-// lane's columns in registers for all of its rows.
+// lane's columns in registers for all of its rows.  300007 x 1000 bf16: 140 to 170 us, 600 MB at 3.6 to 4.3 TB/s (with
+// the counts read for each row 524 us; with loads under conditions, which the compiler waits for, 214).
 template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) void balance_rows_kernel(BalanceArgs a) {
     constexpr bool kExact = sizeof(T) == 4;
     constexpr int kV = kPerVec<T>, kRows = kBlock / kLanes;
@@ -573,7 +595,8 @@ template <class T> __global__ __launch_bounds__(kBlock) void balance_long_kernel
             float value[kV], counts[kV];
             load_logits(logits, column, a.experts, value);
 #pragma unroll
-            for (int i = 0; i < kV; ++i) counts[i] = column + i < a.experts ? static_cast<float>(a.counts[column + i]) : 0.0f;
+            for (int i = 0; i < kV; ++i)
+                counts[i] = column + i < a.experts ? static_cast<float>(a.counts[column + i]) : 0.0f;
             float top = m;
 #pragma unroll
             for (int i = 0; i < kV; ++i) top = larger(top, value[i]);
@@ -613,6 +636,7 @@ struct BalanceBackwardArgs {
     int experts;
 };
 
+// The same way.  300007 x 1000 bf16: 243 us, 1.2 GB at 4.9 TB/s: HBM.
 template <class T, int kLanes, int kVecs, bool kStream>
 __global__ __launch_bounds__(kBlock) void balance_backward_kernel(BalanceBackwardArgs a) {
     constexpr int kV = kPerVec<T>, kRows = kBlock / kLanes;
@@ -651,7 +675,8 @@ __global__ __launch_bounds__(kBlock) void balance_backward_kernel(BalanceBackwar
     }
 }
 
-template <class T, bool kStream> __global__ __launch_bounds__(kBlock) void balance_long_backward_kernel(BalanceBackwardArgs a) {
+template <class T, bool kStream>
+__global__ __launch_bounds__(kBlock) void balance_long_backward_kernel(BalanceBackwardArgs a) {
     constexpr int kV = kPerVec<T>;
     const int lane = static_cast<int>(threadIdx.x) % 64;
     const float scale = *a.upstream * *a.norm;
@@ -704,9 +729,9 @@ template <class T, class F> void with_row(int width, int least, F&& f) {
 }
 
 // Workgroups of the passes over rows, `lanes` lanes a row: as many as the CUs hold together by their registers, so that
-// all of them run to the end: two each with 8 chunks a lane, four with 4, six with fewer (65536 x 1024 fp16, choice: 52.5 us
-// with four, 50 with six, 49 with eight; 300007 x 1000 bf16, balance: 170, 160, 158).  Passes that also write a row lose by
-// more than four (its gradient: 243, 251, 262).
+// all of them run to the end: two each with 8 chunks a lane, four with 4, six with fewer (65536 x 1024 fp16, choice:
+// 52.5 us with four, 50 with six, 49 with eight; 300007 x 1000 bf16, balance: 170, 160, 158).  Passes that also write a
+// row lose by more than four (its gradient: 243, 251, 262).
 uint32_t row_blocks(int64_t n, int lanes, int vecs, bool writes = false) {
     const int64_t blocks = (n + kBlock / lanes - 1) / (kBlock / lanes);
     const int64_t most = (vecs == 8 ? 2 : (vecs == 4 || writes ? 4 : 6)) * kCus;
@@ -722,7 +747,8 @@ ODIE_API int odie_choose_forward(const void* logits, int64_t stride, int64_t n, 
                                  int dtype, int32_t* expert, float* weights, float* stats, uint64_t stream) {
     const std::string what = "odie_choose_forward";
     if (check_rows_of(what, stride, n, choices, experts, dtype)) return -1;
-    if (choices > kMaxChoices || choices > experts) return fail(what + ": choices must be within 1..64 and the experts");
+    if (choices > kMaxChoices || choices > experts)
+        return fail(what + ": choices must be within 1..64 and the experts");
     if (n == 0) return 0;
     if (!logits || !expert || !weights) return fail(what + ": null pointer");
     if (reinterpret_cast<uintptr_t>(stats) % 8) return fail(what + ": stats must be 8-byte aligned");
@@ -738,12 +764,14 @@ ODIE_API int odie_choose_forward(const void* logits, int64_t stride, int64_t n, 
     });
 }
 
-ODIE_API int odie_choose_backward(const float* upstream, const int32_t* expert, const float* weights, const void* logits,
+ODIE_API int odie_choose_backward(const float* upstream, const int32_t* expert, const float* weights,
+                                  const void* logits,
                                   int64_t stride, const float* stats, int64_t n, int experts, int choices, int dtype,
                                   void* dlogits, uint64_t stream) {
     const std::string what = "odie_choose_backward";
     if (check_rows_of(what, logits ? stride : experts, n, choices, experts, dtype)) return -1;
-    if (choices > kMaxChoices || choices > experts) return fail(what + ": choices must be within 1..64 and the experts");
+    if (choices > kMaxChoices || choices > experts)
+        return fail(what + ": choices must be within 1..64 and the experts");
     if (n == 0) return 0;
     if (!upstream || !expert || !weights || !dlogits || (logits && !stats)) return fail(what + ": null pointer");
     ChooseBackwardArgs a{upstream, expert, weights, logits, stats, dlogits, stride, n, experts, choices};
@@ -753,7 +781,8 @@ ODIE_API int odie_choose_backward(const float* upstream, const int32_t* expert, 
         with_lanes<T>(experts, choices, [&](auto lanes) {
             with_flag(logits != nullptr, [&](auto all) {
                 with_flag(n * experts * dtype_bytes(dtype) >= kStreamBytes, [&](auto far) {
-                    in_launches((n + kBlock / lanes - 1) / (kBlock / lanes), kBlock, [&](uint32_t first, uint32_t count) {
+                    in_launches((n + kBlock / lanes - 1) / (kBlock / lanes), kBlock,
+                                [&](uint32_t first, uint32_t count) {
                         choose_backward_kernel<T, lanes, all, far><<<count, kBlock, 0, s>>>(a, first);
                     });
                 });
@@ -803,9 +832,11 @@ ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int3
         balance_count_kernel<true><<<1, kCountBlock, shared, s>>>(a);
     } else {
         // Sixteen entries a thread at least, and two for each count that a workgroup adds at its end.
-        const int64_t each = 16 * kCountBlock > 2 * experts ? 16 * kCountBlock : 2 * experts, blocks = (entries + each - 1) / each;
+        const int64_t each = 16 * kCountBlock > 2 * experts ? 16 * kCountBlock : 2 * experts,
+            blocks = (entries + each - 1) / each;
         balance_clear_kernel<<<(experts + kBlock - 1) / kBlock, kBlock, 0, s>>>(a);
-        balance_count_kernel<false><<<static_cast<uint32_t>(blocks < kCus ? blocks : kCus), kCountBlock, shared, s>>>(a);
+        balance_count_kernel<false>
+            <<<static_cast<uint32_t>(blocks < kCus ? blocks : kCus), kCountBlock, shared, s>>>(a);
     }
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
@@ -819,8 +850,8 @@ ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int3
 }
 
 ODIE_API int odie_balance_backward(const float* upstream, const void* logits, int64_t stride, const int32_t* counts,
-                                   const float* stats, const float* norm, int64_t n, int experts, int dtype, void* dlogits,
-                                   uint64_t stream) {
+                                   const float* stats, const float* norm, int64_t n, int experts, int dtype,
+                                   void* dlogits, uint64_t stream) {
     const std::string what = "odie_balance_backward";
     if (check_rows_of(what, stride, n, 1, experts, dtype)) return -1;
     if (n == 0) return 0;
@@ -832,7 +863,9 @@ ODIE_API int odie_balance_backward(const float* upstream, const void* logits, in
         using T = decltype(t);
         with_flag(n * experts * dtype_bytes(dtype) >= kStreamBytes, [&](auto far) {
             with_row<T>(experts, 1, [&](auto lanes, auto vecs) {
-                if constexpr (vecs > 0) balance_backward_kernel<T, lanes, vecs, far><<<row_blocks(n, lanes, vecs, true), kBlock, 0, s>>>(a);
+                if constexpr (vecs > 0)
+                    balance_backward_kernel<T, lanes, vecs, far>
+                        <<<row_blocks(n, lanes, vecs, true), kBlock, 0, s>>>(a);
                 else balance_long_backward_kernel<T, far><<<row_blocks(n, 64, 1, true), kBlock, 0, s>>>(a);
             });
         });

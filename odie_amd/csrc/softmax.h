@@ -36,7 +36,8 @@ __device__ inline uint32_t as_bits(float x) { return __builtin_bit_cast(uint32_t
 __device__ inline float as_float(uint32_t x) { return __builtin_bit_cast(float, x); }
 
 template <int kLanes> __device__ inline float sum_across(float x) {
-    return as_float(across<kLanes>(as_bits(x), [](uint32_t a, uint32_t b) { return as_bits(as_float(a) + as_float(b)); }));
+    return as_float(across<kLanes>(
+        as_bits(x), [](uint32_t a, uint32_t b) { return as_bits(as_float(a) + as_float(b)); }));
 }
 
 // The larger one; a NaN wins.
@@ -58,13 +59,16 @@ template <int kLanes> __device__ inline double sum_across(double x) {
     if constexpr (kLanes > 2) move(low, high, [](uint32_t v) { return dpp_move<0x4E>(v); });
     if constexpr (kLanes > 4) move(low, high, [](uint32_t v) { return dpp_move<0x141>(v); });
     if constexpr (kLanes > 8) move(low, high, [](uint32_t v) { return dpp_move<0x140>(v); });
-    if constexpr (kLanes > 16) move(low, high, [](uint32_t v) { return static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 16)); });
-    if constexpr (kLanes > 32) move(low, high, [](uint32_t v) { return static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 32)); });
+    if constexpr (kLanes > 16)
+        move(low, high, [](uint32_t v) { return static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 16)); });
+    if constexpr (kLanes > 32)
+        move(low, high, [](uint32_t v) { return static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 32)); });
     return x;
 }
 
 template <int kLanes> __device__ inline float max_across(float x) {
-    return as_float(across<kLanes>(as_bits(x), [](uint32_t a, uint32_t b) { return as_bits(larger(as_float(a), as_float(b))); }));
+    return as_float(across<kLanes>(
+        as_bits(x), [](uint32_t a, uint32_t b) { return as_bits(larger(as_float(a), as_float(b))); }));
 }
 
 // exp(x).  kExact: the library's; else the hardware's exp2, off by 2^-23 (1 + |x|) relative, for sums and for results

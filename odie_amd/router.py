@@ -46,7 +46,7 @@ def balance(logits, expert):
     expert = expert.contiguous()
     if records(logits):
         return _Balance.apply(logits, expert)
-    return _balance(logits, expert, None, None)
+    return _balance(logits, expert, False)[:2]
 
 
 def distill(logits, ids, teacher, *, temperature=1.0):
@@ -88,16 +88,19 @@ def _choose(logits, choices, normalize, stats):
     return expert, weights
 
 
-def _balance(logits, expert, stats, norm):
+def _balance(logits, expert, keep):
+    """loss, counts, and one buffer of: the norm, padding up to four, with `keep` the rows' statistics, the workspace."""
     n, experts = logits.shape
     choices = expert.shape[1]
     loss, counts = _floats(logits), logits.new_empty(experts, dtype=torch.int32)
-    norm = _floats(logits) if norm is None else norm
-    scratch = _lib.scratch('odie_balance_workspace', logits, n, choices, experts)
+    need = _lib.library().odie_balance_workspace(n, choices, experts)
+    stats = 4 * n if keep else 0
+    kept = _floats(logits, 4 + stats + max(need, 0) // 4)
+    at = kept.data_ptr()
     _lib.call('odie_balance_forward', logits, logits.data_ptr(), pitch(logits), expert.data_ptr(), n, choices, experts,
-              DTYPES[logits.dtype], loss.data_ptr(), counts.data_ptr(), _lib.ptr(stats), norm.data_ptr(),
-              _lib.ptr(scratch), 0 if scratch is None else scratch.numel())
-    return loss, counts
+              DTYPES[logits.dtype], loss.data_ptr(), counts.data_ptr(), at + 16 if keep else None, at,
+              at + 16 + 4 * stats, need)
+    return loss, counts, kept
 
 
 def _distill(logits, ids, teacher, temperature, stats):
@@ -138,21 +141,20 @@ class _Choose(torch.autograd.Function):
 class _Balance(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, expert):
-        stats, norm = _floats(logits, logits.shape[0], 4), _floats(logits)
-        loss, counts = _balance(logits, expert, stats, norm)
+        loss, counts, kept = _balance(logits, expert, True)
         ctx.mark_non_differentiable(counts)
-        ctx.save_for_backward(logits, counts, stats, norm)
+        ctx.save_for_backward(logits, counts, kept)
         return loss, counts
 
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream, _):
-        logits, counts, stats, norm = ctx.saved_tensors
+        logits, counts, kept = ctx.saved_tensors
         n, experts = logits.shape
         upstream = upstream.contiguous()
         dlogits = logits.new_empty((n, experts))
         _lib.call('odie_balance_backward', logits, upstream.data_ptr(), logits.data_ptr(), pitch(logits),
-                  counts.data_ptr(), stats.data_ptr(), norm.data_ptr(), n, experts, DTYPES[logits.dtype],
+                  counts.data_ptr(), kept.data_ptr() + 16, kept.data_ptr(), n, experts, DTYPES[logits.dtype],
                   dlogits.data_ptr())
         return dlogits, None
 
