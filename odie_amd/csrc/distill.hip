@@ -175,8 +175,7 @@ template <class T> __global__ __launch_bounds__(64) void distill_join_kernel(Dis
 // several name (`twice`, a bit for each class of the piece) adds up the others'.
 template <class T>
 __device__ inline void patch_entry(const DistillArgs& a, int64_t row, int j, int begin, int end, const uint32_t* twice,
-                                   const T* logits,
-                                   T* out, float scale, const float (&stats)[4]) {
+                                   const T* logits, T* out, float scale, const float (&stats)[4]) {
     int64_t id, other;
     const float entry = entry_of(a, row, j, id);
     if (id < begin || id >= end) return;
@@ -202,12 +201,12 @@ __device__ inline void patch_entry(const DistillArgs& a, int64_t row, int j, int
 // where each looks at all, 18 so).
 template <class T, int kLanes, bool kStream>
 __global__ __launch_bounds__(kBlock) void distill_backward_kernel(DistillArgs a, uint32_t first) {
-    constexpr int kV = kPerVec<T>,
-        kWords = kLanes == kBlock ? (kMostPiece + 64) / 32 : (kLanes == 64 ? kMedium / 32 : kLanes / 4);
+    constexpr int kV = kPerVec<T>;
+    constexpr int kWords = kLanes == kBlock ? (kMostPiece + 64) / 32 : (kLanes == 64 ? kMedium / 32 : kLanes / 4);
     __shared__ uint32_t bits[kBlock / kLanes][2][kWords];
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
     uint32_t *const once = bits[static_cast<int>(threadIdx.x) / kLanes][0],
-        *const twice = bits[static_cast<int>(threadIdx.x) / kLanes][1];
+                   *const twice = bits[static_cast<int>(threadIdx.x) / kLanes][1];
     const int64_t at =
         (static_cast<int64_t>(first) + blockIdx.x) * (kBlock / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
     const int64_t row = at / a.pieces;
@@ -216,7 +215,7 @@ __global__ __launch_bounds__(kBlock) void distill_backward_kernel(DistillArgs a,
     const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
     T* out = static_cast<T*>(a.dlogits) + row * a.classes;
     constexpr int kLine = 128 / static_cast<int>(sizeof(T));
-    // the line before
+    // elements of the line before
     const int past = kLanes == kBlock ? static_cast<int>(reinterpret_cast<uintptr_t>(out) / sizeof(T) % kLine) : 0;
     const int begin = piece == 0 ? 0 : piece * a.piece - past;
     const int end = piece == a.pieces - 1 ? a.classes : (piece + 1) * a.piece - past;
@@ -277,8 +276,8 @@ bool by_lanes(int64_t n, int classes) { return classes <= kShort || (classes <= 
 // Pieces that a long row is cut into, each of whole rounds of its workgroup: about four workgroups a CU at least, and
 // at most `most` classes a piece.
 void cut(DistillArgs& a, int values, int64_t most) {
-    const int64_t wanted = a.n < 4 * kCus ? (4 * kCus + a.n - 1) / a.n : 1,
-        round = static_cast<int64_t>(kBlock) * values;
+    const int64_t wanted = a.n < 4 * kCus ? (4 * kCus + a.n - 1) / a.n : 1;
+    const int64_t round = static_cast<int64_t>(kBlock) * values;
     const int64_t rounds = (a.classes + round - 1) / round, least = (a.classes + most - 1) / most;
     int64_t pieces = wanted < rounds ? wanted : rounds;
     pieces = pieces < least ? least : pieces;
@@ -310,10 +309,9 @@ ODIE_API int64_t odie_distill_workspace(int64_t n, int classes, int dtype) {
 }
 
 ODIE_API int odie_distill_forward(const void* logits, int64_t stride, const void* ids, int id_bytes,
-                                  const void* teacher,
-                                  int teacher_dtype, int64_t n, int classes, int top, float temperature, int dtype,
-                                  float* loss, float* stats, void* workspace, int64_t workspace_bytes,
-                                      uint64_t stream) {
+                                  const void* teacher, int teacher_dtype, int64_t n, int classes, int top,
+                                  float temperature, int dtype, float* loss, float* stats, void* workspace,
+                                  int64_t workspace_bytes, uint64_t stream) {
     const std::string what = "odie_distill_forward";
     if (check_distill(what, n, classes, top, dtype)) return -1;
     if (!known_dtype(teacher_dtype)) return fail(what + ": teacher_dtype must be 0 (fp32), 1 (fp16) or 2 (bf16)");
@@ -327,8 +325,7 @@ ODIE_API int odie_distill_forward(const void* logits, int64_t stride, const void
     if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 8 != 0))
         return fail(what + ": needs an 8-byte aligned workspace of " + std::to_string(need) + " bytes");
     DistillArgs a{logits, ids, teacher, nullptr, loss, stats, nullptr, static_cast<float2*>(workspace), stride, n,
-        classes,
-                  top, id_bytes, teacher_dtype, 1, classes, 1.0f / temperature};
+                  classes, top, id_bytes, teacher_dtype, 1, classes, 1.0f / temperature};
     const hipStream_t s = as_stream(stream);
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
@@ -363,8 +360,7 @@ ODIE_API int odie_distill_backward(const float* upstream, const void* logits, in
     if (!upstream || !logits || !ids || !teacher || !stats || !dlogits) return fail(what + ": null pointer");
     if (stride < classes) return fail(what + ": rows overlap (a stride below the row's width)");
     DistillArgs a{logits, ids, teacher, upstream, nullptr, const_cast<float*>(stats), dlogits, nullptr, stride, n,
-        classes,
-                  top, id_bytes, teacher_dtype, 1, classes, 1.0f / temperature};
+                  classes, top, id_bytes, teacher_dtype, 1, classes, 1.0f / temperature};
     const hipStream_t s = as_stream(stream);
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);

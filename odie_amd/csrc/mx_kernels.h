@@ -69,8 +69,8 @@ template <int kRows, int kThreads> struct Scales {
     static __device__ int wave() { return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64)); }
 
     __device__ void begin(const uint8_t* data, int64_t pitch, int64_t first, int64_t limit) {
-        const int lane = static_cast<int>(threadIdx.x % 64),
-            last = limit - first < kRows ? static_cast<int>(limit - first) - 1 : kRows - 1;
+        const int lane = static_cast<int>(threadIdx.x % 64);
+        const int last = limit - first < kRows ? static_cast<int>(limit - first) - 1 : kRows - 1;
         base = data + first * pitch;
         left = static_cast<int>(pitch / 4) - lane % 2;
 #pragma unroll
@@ -83,7 +83,7 @@ template <int kRows, int kThreads> struct Scales {
         const uint64_t address = reinterpret_cast<uint64_t>(base);
         vec16 buffer{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address))),
                      static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32))),
-                         kBufferLimit, kBufferWord3};
+                     kBufferLimit, kBufferWord3};
         asm volatile("s_nop 4" : "+s"(buffer));   // wait states between its writing and the loads
         const uint32_t to =
             __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>((lds_void)(lds))));
@@ -108,8 +108,8 @@ template <class I> __device__ inline vec16 chunk_at(const char* lds, int r, int 
 __device__ inline vec16 buffer_of(const uint8_t* base) {
     const uint64_t address = reinterpret_cast<uint64_t>(base);
     vec16 buffer{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address))),
-                 static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32))), kBufferLimit,
-                     kBufferWord3};
+                 static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32))),
+                 kBufferLimit, kBufferWord3};
     asm volatile("s_nop 4" : "+s"(buffer));   // wait states between its writing and the loads
     return buffer;
 }

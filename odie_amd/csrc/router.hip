@@ -99,10 +99,10 @@ template <> struct Keys<float> {
     template <int kLanes> static __device__ Key best(Key key) {
         // the largest order first, then the largest rest among the lanes that hold it
         const int32_t order = static_cast<int32_t>(key >> 32);
-        const int32_t top =
-            static_cast<int32_t>(across<kLanes>(static_cast<uint32_t>(order), [](uint32_t a, uint32_t b) {
+        const auto larger_order = [](uint32_t a, uint32_t b) {
             return static_cast<uint32_t>(most_of(static_cast<int32_t>(a), static_cast<int32_t>(b)));
-        }));
+        };
+        const int32_t top = static_cast<int32_t>(across<kLanes>(static_cast<uint32_t>(order), larger_order));
         const uint32_t rest = across<kLanes>(order == top ? static_cast<uint32_t>(key) : 0u,
                                              [](uint32_t a, uint32_t b) { return a > b ? a : b; });
         return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(top)) << 32 | rest);
@@ -765,9 +765,8 @@ ODIE_API int odie_choose_forward(const void* logits, int64_t stride, int64_t n, 
 }
 
 ODIE_API int odie_choose_backward(const float* upstream, const int32_t* expert, const float* weights,
-                                  const void* logits,
-                                  int64_t stride, const float* stats, int64_t n, int experts, int choices, int dtype,
-                                  void* dlogits, uint64_t stream) {
+                                  const void* logits, int64_t stride, const float* stats, int64_t n, int experts,
+                                  int choices, int dtype, void* dlogits, uint64_t stream) {
     const std::string what = "odie_choose_backward";
     if (check_rows_of(what, logits ? stride : experts, n, choices, experts, dtype)) return -1;
     if (choices > kMaxChoices || choices > experts)
@@ -832,8 +831,8 @@ ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int3
         balance_count_kernel<true><<<1, kCountBlock, shared, s>>>(a);
     } else {
         // Sixteen entries a thread at least, and two for each count that a workgroup adds at its end.
-        const int64_t each = 16 * kCountBlock > 2 * experts ? 16 * kCountBlock : 2 * experts,
-            blocks = (entries + each - 1) / each;
+        const int64_t each = 16 * kCountBlock > 2 * experts ? 16 * kCountBlock : 2 * experts;
+        const int64_t blocks = (entries + each - 1) / each;
         balance_clear_kernel<<<(experts + kBlock - 1) / kBlock, kBlock, 0, s>>>(a);
         balance_count_kernel<false>
             <<<static_cast<uint32_t>(blocks < kCus ? blocks : kCus), kCountBlock, shared, s>>>(a);

@@ -55,7 +55,7 @@ def distill(logits, ids, teacher, *, temperature=1.0):
     and q the softmax of teacher / temperature ([N, top], any floating dtype of the three) over them alone.
 
     An id outside 0..classes-1 or a teacher's -inf is no entry; a row without any has loss 0 and no gradient.
-    Entries of one class count each.  One entry a row is the cross entropy of that class.  A row whose logits are all
+    The temperature is within 2^-100..2^100.  Entries of one class count each.  One entry a row is the cross entropy of that class.  A row whose logits are all
     -inf has p = 0 and, with an entry, an infinite loss.  The teacher is fixed: it takes no gradient."""
     logits = check_rows('logits', logits)
     n, device = logits.shape[0], logits.device
@@ -68,7 +68,7 @@ def distill(logits, ids, teacher, *, temperature=1.0):
     if records(teacher):
         raise ValueError('teacher takes no gradient: detach it')
     if not isinstance(temperature, numbers.Real) or not 2.0 ** -100 <= temperature <= 2.0 ** 100:
-        raise ValueError('temperature must be a number above 0')
+        raise ValueError('temperature must be a number within 2^-100..2^100')
     ids, teacher = ids.contiguous(), teacher.contiguous()
     if records(logits):
         return _Distill.apply(logits, ids, teacher, float(temperature))
