@@ -70,7 +70,7 @@ def test_a_training_step_of_all_parameters():
     q = torch.log_softmax(teacher.double() / 2, 1)
     total64 = (y64 - target.double()).square().mean() + 0.1 * loss64 + 0.05 * (q.exp() * (q - own)).sum(1).mean()
     grads64 = torch.autograd.grad(total64, [x64] + [p[name] for name in names])
-    assert abs(float(total) - float(total64)) < 2.0 ** -13
+    assert abs(float(total.detach()) - float(total64.detach())) < 2.0 ** -13
     for name, got, expected in zip(['x'] + names, grads, grads64):
         assert (got.double() - expected).abs().max() <= 2.0 ** -13 * max(1.0, float(expected.abs().max())), name
 
@@ -222,3 +222,63 @@ def test_combine_takes_what_choose_gives():
     rows = dispatch(torch.tensor([[1.0], [10.0]], device='cuda'), order)
     y = combine(rows, order, weights)
     assert torch.allclose(y, torch.tensor([[1.0], [10.0]], device='cuda'))
+
+
+def test_no_rows():
+    model = RoutedMixture(4, 2, 16, 32, 3, codes=4, vocab=5, seed=1)
+    x = torch.zeros(0, 16, device='cuda', dtype=torch.float16, requires_grad=True)
+    ids = torch.zeros(0, device='cuda', dtype=torch.int64)
+    y, logits, expert = model(x, ids)
+    assert y.shape == (0, 3) and logits.shape == (0, 4) and expert.shape == (0, 2)
+    loss = y.float().sum() + balance(logits, expert)[0] + distill(logits, expert, logits.detach()[:, :2]).sum()
+    grads = torch.autograd.grad(loss, [x] + list(model.parameters()))
+    assert float(loss) == 0 and not any(g.any() for g in grads)
+    for rows in (False, True):
+        assert model.mixture.microscaled(rows=rows)(x.detach(), expert, None, ids).shape == (0, 3)
+
+
+def _passes(x, q, bias, ids, teacher):
+    """A layer whose gradients come in one pass, and a distillation of few rows, cut in pieces."""
+    leaf, own = x.detach().requires_grad_(True), bias.detach().requires_grad_(True)
+    y = linear(leaf, q, own, activation='silu')
+    logits = y.view(-1, 64 * 4096)[:1]
+    loss = distill(logits, ids, teacher)
+    return [t.detach() for t in (y, loss, *torch.autograd.grad(y.float().square().sum() / 64 + loss.sum(), (leaf, own)))]
+
+
+def test_two_graphs_at_once():
+    """Two captured passes with workspaces, replayed on two streams together, each on inputs of its own."""
+    generator = torch.Generator(device='cuda').manual_seed(3)
+    made, graphs = [], []
+    for seed in range(2):
+        x = torch.empty(70000 // 4096 * 4096, 48, device='cuda', dtype=torch.float16)
+        q = quantize(torch.randn(64, 48, generator=generator, device='cuda', dtype=torch.float16))
+        bias = torch.randn(64, generator=generator, device='cuda', dtype=torch.float16)
+        ids = torch.randint(0, 64 * 4096, (1, 9), generator=generator, device='cuda')
+        teacher = torch.randn(1, 9, generator=generator, device='cuda')
+        made.append((x, q, bias, ids, teacher))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for inputs in made:
+        inputs[0].normal_(generator=generator)
+        with torch.cuda.stream(side):
+            _passes(*inputs)
+    torch.cuda.synchronize()
+    for inputs in made:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outputs = _passes(*inputs)
+        graphs.append((graph, outputs))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for replay in range(3):
+        for inputs in made:
+            inputs[0].normal_(generator=generator)
+        torch.cuda.synchronize()
+        for (graph, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for inputs, (_, outputs) in zip(made, graphs):
+            kept = [t.clone() for t in outputs]
+            for index, (a, b) in enumerate(zip(kept, _passes(*inputs))):
+                assert torch.equal(a, b), (replay, index)

@@ -220,6 +220,59 @@ def test_balance_of_padding_and_masks(dtype):
         assert not torch.autograd.grad(loss, leaf)[0].any()
 
 
+@pytest.mark.parametrize('n, width, choices', ((300, 40, 100), (5, 10, 1000), (400, 10000, 64), (130, 32768, 130), (700, 5000, 30)))
+def test_balance_of_many_entries_a_row(n, width, choices):
+    """More entries than lanes of a row; counts of many experts, from many entries; long rows with padding."""
+    generator = _generator(n)
+    logits = _logits(generator, torch.float16, n, width)
+    expert = torch.randint(-width // 4, width, (n, choices), generator=generator, device='cuda', dtype=torch.int32)
+    expert[1::3] = -1
+    expert[0, :-1] = -1
+    expert[0, -1] = width - 1       # the only entry of its row is the last
+    _check_balance(logits, expert, '%dx%d, %d entries' % (n, width, choices))
+
+
+def test_entries_of_any_layout():
+    """Entries that do not lie on 16 bytes, or not together; a teacher of another type, in columns of a wider one."""
+    generator = _generator(21)
+    logits = _logits(generator, torch.float32, 9000, 50)
+    wide = torch.randint(-1, 50, (9002, 6), generator=generator, device='cuda', dtype=torch.int32)
+    for expert in (wide.flatten()[1:1 + 9000 * 3].view(9000, 3), wide[2:, 1:5], wide[1:9001, ::2], wide[:9000, :1].expand(9000, 4)):
+        _check_balance(logits, expert, 'entries')
+        teacher = _logits(generator, torch.bfloat16, expert.shape[1], 9000).t()
+        ids, copy = expert.long(), (expert.long().contiguous(), teacher.contiguous())
+        ids = ids.t().contiguous().t()
+        leaf = logits.clone().requires_grad_(True)
+        got = distill(leaf, ids, teacher)
+        expected = distill(logits, *copy)
+        assert torch.equal(got, expected) and torch.equal(distill(logits, expert, teacher), expected)
+        twin = logits.clone().requires_grad_(True)
+        assert torch.equal(torch.autograd.grad(got.sum(), leaf)[0], torch.autograd.grad(distill(twin, *copy).sum(), twin)[0])
+
+
+def test_no_rows():
+    for width in (1, 40, 9000):
+        x = torch.zeros(0, width, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+        ids, teacher = torch.zeros(0, 2, device='cuda', dtype=torch.int64), torch.zeros(0, 2, device='cuda')
+        for normalize in (True, False):
+            expert, weights = choose(x, 1, normalize=normalize)
+            assert expert.shape == weights.shape == (0, 1)
+            assert torch.autograd.grad(weights.sum(), x)[0].shape == (0, width)
+        loss = distill(x, ids, teacher)
+        assert loss.shape == (0,) and torch.autograd.grad(loss.sum(), x)[0].shape == (0, width)
+        loss, counts = balance(x, expert)
+        assert loss == 0 and counts.shape == (width,) and not counts.any()
+
+
+def test_inference_mode():
+    x = torch.randn(5, 12, device='cuda')
+    ids = torch.zeros(5, 1, device='cuda', dtype=torch.int64)
+    expected = [*choose(x, 3), *balance(x, choose(x, 3)[0]), distill(x, ids, x[:, :1])]
+    with torch.inference_mode():
+        got = [*choose(x, 3), *balance(x, choose(x, 3)[0]), distill(x, ids, x[:, :1])]
+    assert all(torch.equal(a, b) for a, b in zip(got, expected))
+
+
 def test_even_load_has_a_loss_of_one():
     logits = torch.zeros(64, 16, device='cuda')
     expert = torch.arange(64, device='cuda', dtype=torch.int32).view(64, 1) % 16
