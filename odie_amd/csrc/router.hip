@@ -155,24 +155,57 @@ struct ChooseArgs {
     int normalize;
 };
 
-// Rows of up to 64 kVecs chunks in registers, the next one under way.  Each lane keeps its two largest keys; a choice
-// takes the largest of all lanes, whose lane goes on to its second, and looks through its keys again once both are
-// gone: at four choices of 1024 about once in 500 rows.  65536 x 1024 fp16, four choices with weights among all: 50 us,
-// 134 MB at 2.7 TB/s, bound by the arithmetic (about 450 instructions a row; with a search of all keys for each choice
-// 61 us); one row 2 us.
-template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) void choose_kernel(ChooseArgs a) {
+// The largest key, and the sum, over the kLanes threads of a row, for each of them.  More than a wave: by LDS, where
+// every other call (`turn`) takes the same place, so that one barrier a call is enough.
+template <class K, int kLanes, int kWaves>
+__device__ inline typename K::Key best_of(typename K::Key key, typename K::Key (&part)[2][kWaves], int& turn) {
+    if constexpr (kLanes <= 64) return K::template best<kLanes>(key);
+    key = K::template best<64>(key);
+    turn ^= 1;
+    if (threadIdx.x % 64 == 0) part[turn][threadIdx.x / 64] = key;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) key = most_of(key, part[turn][w]);
+    return key;
+}
+template <int kLanes, int kWaves> __device__ inline float sum_of(float x, float (&part)[2][kWaves], int& turn) {
+    if constexpr (kLanes <= 64) return sum_across<kLanes>(x);
+    x = sum_across<64>(x);
+    turn ^= 1;
+    if (threadIdx.x % 64 == 0) part[turn][threadIdx.x / 64] = x;
+    __syncthreads();
+    x = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) x += part[turn][w];
+    return x;
+}
+
+// Rows of up to kLanes kVecs chunks in registers, the next one under way.  Each lane keeps its two largest keys; a
+// choice takes the largest of all lanes, whose lane goes on to its second, and looks through its keys again once both
+// are gone: at four choices of 1024 about once in 500 rows.  65536 x 1024 fp16, four choices with weights among all: 50
+// us, 134 MB at 2.7 TB/s, bound by the arithmetic (about 450 instructions a row; with a search of all keys for each
+// choice 61 us); one row 2 us.  8192 rows of 4096, 8000, 16000 and 32000 bf16: 24, 39, 92 and 172 us (a row read for
+// each choice -, 124, 235 and 454).
+template <class T, int kLanes, int kVecs>
+__global__ __launch_bounds__(kLanes > kBlock ? kLanes : kBlock) void choose_kernel(ChooseArgs a) {
     using K = Keys<T>;
     using Key = typename K::Key;
-    constexpr int kV = kPerVec<T>, kValues = kVecs * kV, kRows = kBlock / kLanes;
+    constexpr int kV = kPerVec<T>, kValues = kVecs * kV;
+    constexpr int kThreads = kLanes > kBlock ? kLanes : kBlock, kRows = kThreads / kLanes, kWaves = kThreads / 64;
+    __shared__ Key part[2][kWaves];
+    __shared__ float sums[2][kWaves];
+    int turn = 0, sums_turn = 0;
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
     const T* logits = static_cast<const T*>(a.logits);
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
     int64_t at = static_cast<int64_t>(blockIdx.x) * kRows + static_cast<int>(threadIdx.x) / kLanes;
+    constexpr bool kAhead = kLanes < 1024;      // whose registers do not hold two rows
     RowHold<T, kLanes, kVecs> next;
-    next.load(logits + (at < a.n ? at : a.n - 1) * a.stride, lane, a.experts);
+    if constexpr (kAhead) next.load(logits + (at < a.n ? at : a.n - 1) * a.stride, lane, a.experts);
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.n; base += step, at += step) {
+        if constexpr (!kAhead) next.load(logits + at * a.stride, lane, a.experts);
         RowHold<T, kLanes, kVecs> row = next;
-        next.load(logits + (at + step < a.n ? at + step : a.n - 1) * a.stride, lane, a.experts);
+        if constexpr (kAhead) next.load(logits + (at + step < a.n ? at + step : a.n - 1) * a.stride, lane, a.experts);
         row.settle(lane, a.experts);
         Key key[kValues];
         bool nan = false;
@@ -201,7 +234,7 @@ template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) v
         Key mine = K::kNone, first = K::kNone;      // lane j: the j-th choice
         bool left = most != K::kNone;
         for (int j = 0; j < a.choices; ++j) {
-            const Key best = K::template best<kLanes>(most);
+            const Key best = best_of<K, kLanes>(most, part, turn);
             if (j == 0) first = best;
             if (lane == j) mine = best;
             if (most == best) most = less, less = K::kNone;
@@ -230,7 +263,7 @@ template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) v
                 for (int i = 0; i < kV; ++i) s += exponential<sizeof(T) == 4>(value[i] - base_value);
             }
         }
-        s = sum_across<kLanes>(s);
+        s = sum_of<kLanes>(s, sums, sums_turn);
         const float inverse = m == kNegInfinity ? 0.0f : 1.0f / s;
         if (at >= a.n) continue;
         if (lane < a.choices) {
@@ -251,8 +284,8 @@ __device__ inline int64_t block_best(int64_t key, int64_t* part) {
     return key;
 }
 
-// Longer rows: a workgroup a row, which it reads once for each choice, the one below the last.  8192 x 8000 fp16, four
-// choices: 149 us (as such, 8192 x 4096 75 us, in registers 31).
+// A workgroup a row, which it reads once for each choice, the one below the last: for rows that do not fit its
+// registers, and where long rows of fp32, whose keys take 64 bits, have few choices (by_turns).
 template <class T> __global__ __launch_bounds__(kBlock) void choose_long_kernel(ChooseArgs a) {
     using K = Keys<float>;
     constexpr int kV = kPerVec<T>;
@@ -700,6 +733,8 @@ __global__ __launch_bounds__(kBlock) void balance_long_backward_kernel(BalanceBa
     }
 }
 
+template <int kNumber> using Number = std::integral_constant<int, kNumber>;
+
 // Calls f with the lanes a row of `width` values takes: 8 to 64, and at least `least`.
 template <class T, class F> void with_lanes(int width, int least, F&& f) {
     const int chunks = (width + kPerVec<T> - 1) / kPerVec<T>, wanted = chunks > least ? chunks : least;
@@ -733,9 +768,18 @@ template <class T, class F> void with_row(int width, int least, F&& f) {
 // 52.5 us with four, 50 with six, 49 with eight; 300007 x 1000 bf16, balance: 170, 160, 158).  Passes that also write a
 // row lose by more than four (its gradient: 243, 251, 262).
 uint32_t row_blocks(int64_t n, int lanes, int vecs, bool writes = false) {
-    const int64_t blocks = (n + kBlock / lanes - 1) / (kBlock / lanes);
+    const int rows = lanes > kBlock ? 1 : kBlock / lanes;
+    const int64_t blocks = (n + rows - 1) / rows;
     const int64_t most = (vecs == 8 ? 2 : (vecs == 4 || writes ? 4 : 6)) * kCus;
     return static_cast<uint32_t>(blocks < 1 ? 1 : (blocks < most ? blocks : most));
+}
+
+// Whether a choice reads its rows once for each of the choices, instead of once in all.  us in registers and by turns,
+// fp32: 8192 x 4000, one choice 37 and 25, two 43 and 41, four 52 and 73; 8192 x 8000, four 165 and 143; 8192 x 16000,
+// one 173 and 100, four 304 and 294, eight 476 and 580; 1000 x 8000, four 24 and 26; one row of 8000 6.5 and 16.  16
+// bits, 8192 rows, one choice: 8000 31 and 37, 16000 70 and 64, 32000 144 and 133.
+bool by_turns(int64_t n, int chunks, int choices, bool wide) {
+    return chunks > 4096 || (wide && n >= 4 * kCus && chunks > 512 && choices <= (chunks > 1024 ? 4 : 1));
 }
 
 }  // namespace
@@ -756,10 +800,22 @@ ODIE_API int odie_choose_forward(const void* logits, int64_t stride, int64_t n, 
     const hipStream_t s = as_stream(stream);
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        with_row<T>(experts, choices, [&](auto lanes, auto vecs) {
-            if constexpr (vecs > 0) choose_kernel<T, lanes, vecs><<<row_blocks(n, lanes, vecs), kBlock, 0, s>>>(a);
-            else choose_long_kernel<T><<<static_cast<uint32_t>(n < 16 * kCus ? n : 16 * kCus), kBlock, 0, s>>>(a);
-        });
+        const int chunks = (experts + kPerVec<T> - 1) / kPerVec<T>;
+        if (by_turns(n, chunks, choices, sizeof(T) == 4)) {
+            choose_long_kernel<T><<<static_cast<uint32_t>(n < 16 * kCus ? n : 16 * kCus), kBlock, 0, s>>>(a);
+            return check_launch("choose");
+        }
+        const auto launch = [&](auto lanes, auto vecs) {
+            constexpr int kThreads = lanes > kBlock ? lanes : kBlock;
+            choose_kernel<T, lanes, vecs><<<row_blocks(n, lanes, vecs), kThreads, 0, s>>>(a);
+        };
+        if (chunks <= 64) with_lanes<T>(experts, choices, [&](auto lanes) { launch(lanes, Number<1>{}); });
+        else if (chunks <= 128) launch(Number<64>{}, Number<2>{});
+        else if (chunks <= 256) launch(Number<64>{}, Number<4>{});
+        else if (chunks <= 512) launch(Number<256>{}, Number<2>{});
+        else if (chunks <= 1024) launch(Number<256>{}, Number<4>{});
+        else if (chunks <= 2048) launch(Number<512>{}, Number<4>{});
+        else launch(Number<1024>{}, Number<4>{});
         return check_launch("choose");
     });
 }

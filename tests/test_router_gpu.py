@@ -92,7 +92,19 @@ def test_choose(width, dtype, normalize):
 
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
-@pytest.mark.parametrize('width', (8, 64, 1000, 5000))
+@pytest.mark.parametrize('width', (2051, 4099, 8192, 8193, 16384, 16391, 32768))
+def test_choose_of_long_rows(width, dtype):
+    """Rows of several waves, by the number of rows and choices; all choices of some lie in one lane's part."""
+    for n, choices, normalize in ((1, 4, False), (1030, 1, True), (1030, 4, False), (1030, 5, True), (3, 64, False)):
+        print('choose', n, width, choices, dtype, normalize, flush=True)
+        logits = _logits(_generator(width + n), dtype, n, width, blocked=0.1)
+        logits[n // 2, :16] = logits[n // 2].abs().amax().clamp(max=100) + torch.arange(16, device='cuda').to(dtype)
+        logits[n // 3, -1] = 300.0
+        _check_choose(logits, choices, normalize, width, '%dx%d, %d of them' % (n, width, choices))
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('width', (8, 64, 1000, 2100, 5000, 12000, 20000))
 def test_choose_ties_and_masks(width, dtype):
     """Equal logits go by index, -0 and 0 are equal, and rows may have fewer allowed experts than choices, or none."""
     logits = torch.zeros(6, width, device='cuda', dtype=dtype)
@@ -113,7 +125,7 @@ def test_choose_ties_and_masks(width, dtype):
 
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
-@pytest.mark.parametrize('width', (16, 300, 5000))
+@pytest.mark.parametrize('width', (16, 300, 2100, 5000, 12000, 20000))
 def test_choose_infinities_and_nan(width, dtype):
     """A NaN or +inf is the largest and makes its own row's weights NaN, and no other row's."""
     logits = _logits(_generator(3), dtype, 4, width)
