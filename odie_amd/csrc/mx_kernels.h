@@ -79,6 +79,10 @@ template <int kRows, int kThreads> struct Scales {
             offset[i] = static_cast<uint32_t>(r < last ? r : last) * static_cast<uint32_t>(pitch) + lane % 2 * 4;
         }
     }
+    __device__ void skip(int slabs) {
+        base += slabs * kMxSlabScales;
+        left -= 2 * slabs;
+    }
     __device__ void load(char* lds) {
         const uint64_t address = reinterpret_cast<uint64_t>(base);
         vec16 buffer{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address))),
@@ -145,6 +149,10 @@ template <int kBM, int kBN, int kThreads> struct ScaleRows {
             offset[i] = static_cast<uint32_t>(r < limit ? r : limit) * static_cast<uint32_t>(pitch) + lane % 4 * 4;
         }
     }
+    __device__ void skip(int groups) {
+        a += groups * kRowBytes, b += groups * kRowBytes;
+        left -= groups * 4;
+    }
     // Queues the next group's into lds.
     __device__ void load(char* lds) {
         const vec16 buffer_a = buffer_of(a), buffer_b = buffer_of(b);
@@ -173,7 +181,7 @@ template <int kBM, int kBN, int kThreads> struct ScaleRows {
 // 280 us (twice the loads); 256 x 128, two workgroups a CU, slabs of half the depth in three buffers 246 to 285 (half
 // lines), or one buffer each 229 to 256; fragments read a step ahead, eight waves 259 to 275, four waves of 128 x 128
 // 239 to 254.
-template <int kBM, int kBN, int kWM, int kWN> struct MxTile : Sums<kBM, kBN, kWM, kWN> {
+template <int kBM, int kBN, int kWM, int kWN, bool kShared> struct MxTile : Sums<kBM, kBN, kWM, kWN> {
     using Base = Sums<kBM, kBN, kWM, kWN>;
     using Base::acc;
     using Base::kMs;
@@ -215,8 +223,9 @@ template <int kBM, int kBN, int kWM, int kWN> struct MxTile : Sums<kBM, kBN, kWM
         add_step<3>(here, sa, sb);
     }
 
-    // Sums `bytes` bytes of codes a row.  The operands have begun.
-    __device__ void sum(A& a, B& b, S& s, int bytes, char* lds) {
+    // Sums `bytes` bytes of codes a row, in `slabs` slabs: those past the bytes add nothing, but wait as the others do.
+    // The operands have begun.
+    __device__ void sum(A& a, B& b, S& s, int bytes, int slabs, char* lds) {
         Base::clear();
         char* const scales = lds + 2 * kBuffer;
         auto load = [&](int slab) {
@@ -228,21 +237,52 @@ template <int kBM, int kBN, int kWM, int kWN> struct MxTile : Sums<kBM, kBN, kWM
             if (slab % 2 == 0) s.load(scales + slab / 2 % 2 * S::kBytes);
         };
         load(0);
-        const int slabs = (bytes + kSlabBytes - 1) / kSlabBytes;
         for (int i = 0; i < slabs; ++i) {
             arrived<0>();   // this slab; and no wave reads the other buffer any more
             load(i + 1);
-            add_slab(lds + i % 2 * kBuffer, scales + i / 2 % 2 * S::kBytes, i);
+            if (!kShared || i * kSlabBytes < bytes) add_slab(lds + i % 2 * kBuffer, scales + i / 2 % 2 * S::kBytes, i);
         }
         __syncthreads();
     }
 };
 
-template <class T, int kBM, int kBN, int kWM, int kWN>
-__global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void mx_rows4_kernel(
+// The depth of a product over kSplit groups of a tile's threads (threadIdx.y), whole slabs of codes each: a tile of few
+// rows is a long chain of slabs that wait for their loads, and one of four waves leaves a CU idle at each (shares_of).
+struct Share {
+    int64_t first, count;    // slabs of codes: the group's first, and each group's number of them
+};
+template <int kSplit> __device__ inline Share share_of(int64_t slabs) {
+    const int64_t count = (slabs + kSplit - 1) / kSplit;
+    return Share{count * __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.y)), count};
+}
+
+// Adds the groups' sums up in the first one's, in their order.  `lds` holds them behind its epilogue's.
+template <int kSplit, class Work> __device__ inline void join_groups(Work& work, char* lds) {
+    constexpr int kValues = Work::kMs * Work::kNs * 16, kWaves = Work::kThreads / 64;
+    float* const own = reinterpret_cast<float*>(lds + kWaves * Work::kRegion);
+    float* const held = own + Work::wave() * kValues * 64 + threadIdx.x % 64;
+    auto& acc = work.acc;
+    if (threadIdx.y > 0)
+#pragma unroll
+        for (int v = 0; v < kValues; ++v)
+            held[((threadIdx.y - 1) * kWaves * kValues + v) * 64] = acc[v / 16 / Work::kNs][v / 16 % Work::kNs][v % 16];
+    __syncthreads();
+    if (threadIdx.y > 0) return;
+    for (int g = 0; g < kSplit - 1; ++g)
+#pragma unroll
+        for (int v = 0; v < kValues; ++v)
+            acc[v / 16 / Work::kNs][v / 16 % Work::kNs][v % 16] += held[(g * kWaves * kValues + v) * 64];
+}
+template <int kSplit, class Work> constexpr int shared_bytes() {
+    constexpr int kJoin = Work::kThreads / 64 * (Work::kRegion + (kSplit - 1) * Work::kMs * Work::kNs * 16 * 256);
+    return kSplit == 1 ? Work::kLds : (kSplit * Work::kBytes > kJoin ? kSplit * Work::kBytes : kJoin);
+}
+
+template <class T, int kBM, int kBN, int kWM, int kWN, int kSplit>
+__global__ __launch_bounds__(kSplit * 64 * (kBM / kWM) * (kBN / kWN)) void mx_rows4_kernel(
     MxRowsArgs m, uint32_t first, uint32_t blocks) {
-    using Work = MxTile<kBM, kBN, kWM, kWN>;
-    __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
+    using Work = MxTile<kBM, kBN, kWM, kWN, (kSplit > 1)>;
+    __shared__ __attribute__((aligned(16))) char lds[shared_bytes<kSplit, Work>()];
     const RowsArgs& a = m.rows;
     const uint32_t id = first + xcd_major(blockIdx.x, gridDim.x);
     if (id >= blocks) return;
@@ -250,24 +290,45 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void mx_rows4_kerne
     const Piece p = find_piece(a.offsets, a.experts, a.experts + 1, a.rows, kBM, t.row);
     if (p.begin >= p.end) return;
     const int column0 = static_cast<int>(t.column) * kBN;
-    if (p.group >= a.experts) return rows_of_none<T, kBM, kBN, Work::kThreads>(a, p, column0);
+    if (p.group >= a.experts) {
+        if (threadIdx.y == 0) rows_of_none<T, kBM, kBN, Work::kThreads>(a, p, column0);
+        return;
+    }
     const int64_t matrix = static_cast<int64_t>(p.group) * a.columns;
+    const int64_t slabs = (m.code_pitch + kSlabBytes - 1) / kSlabBytes;
+    Share share{0, slabs};
+    if constexpr (kSplit > 1) {
+        share = share_of<kSplit>((slabs + 1) / 2);      // in pairs, which share their scales' loads
+        share.first *= 2, share.count *= 2;
+    }
+    const int64_t skip = share.first * kSlabBytes;
+    char* const own = lds + (kSplit > 1 ? share.first / share.count * Work::kBytes : 0);
     typename Work::A opa;
     typename Work::B opb;
     typename Work::S scales;
-    opa.begin(static_cast<const uint8_t*>(a.a), m.code_pitch, p.begin, p.end, m.code_pitch);
-    opb.begin(static_cast<const uint8_t*>(a.b) + matrix * m.code_pitch, m.code_pitch, column0, a.columns, m.code_pitch);
+    opa.begin(static_cast<const uint8_t*>(a.a) + skip, m.code_pitch, p.begin, p.end, m.code_pitch);
+    opb.begin(static_cast<const uint8_t*>(a.b) + matrix * m.code_pitch + skip, m.code_pitch, column0, a.columns,
+              m.code_pitch);
     scales.begin(m.a_scales + p.begin * m.scale_pitch, m.b_scales + (matrix + column0) * m.scale_pitch, m.scale_pitch,
                  p.end - p.begin, a.columns - column0);
+    scales.skip(static_cast<int>(share.first / 2));
     Work work;
-    work.sum(opa, opb, scales, static_cast<int>(m.code_pitch), lds);
+    const int64_t bytes = m.code_pitch - skip;
+    work.sum(opa, opb, scales, static_cast<int>(kSplit > 1 && bytes > share.count * kSlabBytes
+                                                ? share.count * kSlabBytes : bytes),
+             static_cast<int>(share.count), own);
+    if constexpr (kSplit > 1) {
+        join_groups<kSplit>(work, lds);
+        if (threadIdx.y > 0) return;
+    }
     finish_tile<T, kBM == 256>(work, a, p, column0, lds);
 }
 
 // A tile of a product of rows of T with codes.  A slab of the weight's codes lasts for kRatio slabs of the rows. 16384
 // x 4096 x 4096 bf16 450 to 500 us, 1100 to 1220 TFLOP/s, with bias and gelu 490 to 530; 131072 rows over 64 experts,
 // 256 -> 512 fp16 with silu and the sums kept 100 to 110 us, 340 MB at 3.1 to 3.4 TB/s.
-template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> struct MixedTile : Sums<kBM, kBN, kWM, kWN> {
+template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN, bool kShared>
+struct MixedTile : Sums<kBM, kBN, kWM, kWN> {
     using Base = Sums<kBM, kBN, kWM, kWN>;
     using Base::acc;
     using Base::kMs;
@@ -314,8 +375,9 @@ template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> struct MixedTil
         }
     }
 
-    // Sums `depth` values of k; `bytes` bytes of codes a row.  The operands have begun.
-    __device__ void sum(A& a, B& b, SB& sb, int64_t depth, int64_t bytes, char* lds) {
+    // Sums `depth` values of k; `bytes` bytes of codes a row.  kShared: in `slabs` slabs of the rows, of which those
+    // past the depth add nothing, but wait as the others do.  The operands have begun.
+    __device__ void sum(A& a, B& b, SB& sb, int64_t depth, int64_t bytes, int slabs, char* lds) {
         Base::clear();
         char* const codes = lds + 2 * A::kBytes;
         int64_t codes_left = bytes;
@@ -331,11 +393,11 @@ template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> struct MixedTil
         int now = 0, part = 0, at = 0;
         if constexpr (kWay == kDirect) {
             a.load(depth, lds);
-            for (int64_t left = depth; left > 0; left -= kSlab<T>) {
+            for (int64_t left = depth; kShared ? slabs-- > 0 : left > 0; left -= kSlab<T>) {
                 arrived<0>();   // this slab; and no wave reads the other buffers any more
                 if (left > kSlab<T>) a.load(left - kSlab<T>, lds + (now ^ 1) * A::kBytes);
                 if (part == 0) load_codes();
-                add_slab(lds + now * A::kBytes, codes + at * kCodes, part);
+                if (!kShared || left > 0) add_slab(lds + now * A::kBytes, codes + at * kCodes, part);
                 now ^= 1;
                 if (++part == kRatio) part = 0, at ^= 1;
             }
@@ -356,11 +418,12 @@ template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN> struct MixedTil
     }
 };
 
-template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN>
-__global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void mx_mixed_kernel(
+template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN, int kSplit>
+__global__ __launch_bounds__(kSplit * 64 * (kBM / kWM) * (kBN / kWN)) void mx_mixed_kernel(
     MxRowsArgs m, uint32_t first, uint32_t blocks) {
-    using Work = MixedTile<T, kWay, kBM, kBN, kWM, kWN>;
-    __shared__ __attribute__((aligned(16))) char lds[Work::kLds];
+    static_assert(kSplit == 1 || kWay == kDirect, "shares are of rows that go straight to LDS");
+    using Work = MixedTile<T, kWay, kBM, kBN, kWM, kWN, (kSplit > 1)>;
+    __shared__ __attribute__((aligned(16))) char lds[shared_bytes<kSplit, Work>()];
     const RowsArgs& a = m.rows;
     const uint32_t id = first + xcd_major(blockIdx.x, gridDim.x);
     if (id >= blocks) return;
@@ -368,16 +431,34 @@ __global__ __launch_bounds__(64 * (kBM / kWM) * (kBN / kWN)) void mx_mixed_kerne
     const Piece p = find_piece(a.offsets, a.experts, a.experts + 1, a.rows, kBM, t.row);
     if (p.begin >= p.end) return;
     const int column0 = static_cast<int>(t.column) * kBN;
-    if (p.group >= a.experts) return rows_of_none<T, kBM, kBN, Work::kThreads>(a, p, column0);
+    if (p.group >= a.experts) {
+        if (threadIdx.y == 0) rows_of_none<T, kBM, kBN, Work::kThreads>(a, p, column0);
+        return;
+    }
     const int64_t matrix = static_cast<int64_t>(p.group) * a.columns;
+    Share share{0, 0};
+    if constexpr (kSplit > 1) share = share_of<kSplit>((m.code_pitch + kSlabBytes - 1) / kSlabBytes);
+    const int64_t skip = share.first * kMxSlab, most = share.count * kMxSlab;     // values of k
+    char* const own = lds + (kSplit > 1 ? share.first / share.count * Work::kBytes : 0);
     typename Work::A opa;
     typename Work::B opb;
     typename Work::SB sb;
-    opa.begin(static_cast<const T*>(a.a), a.lda, p.begin, p.end, a.depth);
-    opb.begin(static_cast<const uint8_t*>(a.b) + matrix * m.code_pitch, m.code_pitch, column0, a.columns, m.code_pitch);
+    opa.begin(static_cast<const T*>(a.a) + skip, a.lda, p.begin, p.end, a.depth);
+    opb.begin(static_cast<const uint8_t*>(a.b) + matrix * m.code_pitch + skip / 2, m.code_pitch, column0, a.columns,
+              m.code_pitch);
     sb.begin(m.b_scales + matrix * m.scale_pitch, m.scale_pitch, column0, a.columns);
+    int64_t depth = a.depth - skip, bytes = m.code_pitch - skip / 2;
+    if constexpr (kSplit > 1) {
+        sb.skip(static_cast<int>(share.first));
+        depth = depth < most ? depth : most;
+        bytes = bytes < most / 2 ? bytes : most / 2;
+    }
     Work work;
-    work.sum(opa, opb, sb, a.depth, m.code_pitch, lds);
+    work.sum(opa, opb, sb, depth, bytes, static_cast<int>(share.count) * Work::kRatio, own);
+    if constexpr (kSplit > 1) {
+        join_groups<kSplit>(work, lds);
+        if (threadIdx.y > 0) return;
+    }
     finish_tile<T, kBM == 256>(work, a, p, column0, lds);
 }
 
@@ -469,30 +550,31 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx_few_rows_kernel(MxRowsArgs 
     finish_few<T, kRowTiles, kSplit>(part, a, p, column0, owned);
 }
 
-template <int kBM, int kBN, int kWM, int kWN, class Launch> int in_tiles(MxRowsArgs m, Launch&& launch) {
+template <int kBM, int kBN, int kWM, int kWN, int kSplit, class Launch> int in_tiles(MxRowsArgs m, Launch&& launch) {
     const int64_t across = (m.rows.columns + kBN - 1) / kBN;
     m.rows.tiles = piece_ids(m.rows.rows, kBM, m.rows.offsets != nullptr, m.rows.experts, true);
     const int64_t blocks = m.rows.tiles * across;
     if (blocks >= int64_t{1} << 31) return fail("linear: too many tiles for one launch");
     constexpr int kThreads = 64 * (kBM / kWM) * (kBN / kWN);
-    in_launches(blocks, kThreads, [&](uint32_t first, uint32_t count) {
-        launch(m, whole_xcds(count), kThreads, first, static_cast<uint32_t>(blocks));
+    in_launches(blocks, kSplit * kThreads, [&](uint32_t first, uint32_t count) {
+        launch(m, whole_xcds(count), dim3(kThreads, kSplit), first, static_cast<uint32_t>(blocks));
     });
     return check_launch("linear of 4-bit weights");
 }
 
-template <class T, int kBM, int kBN, int kWM, int kWN> int launch_rows4(const MxRowsArgs& m, hipStream_t stream) {
-    return in_tiles<kBM, kBN, kWM, kWN>(m, [&](const MxRowsArgs& a, uint32_t grid, int threads,
-                                               uint32_t first, uint32_t blocks) {
-        mx_rows4_kernel<T, kBM, kBN, kWM, kWN><<<grid, threads, 0, stream>>>(a, first, blocks);
+template <class T, int kBM, int kBN, int kWM, int kWN, int kSplit = 1>
+int launch_rows4(const MxRowsArgs& m, hipStream_t stream) {
+    return in_tiles<kBM, kBN, kWM, kWN, kSplit>(m, [&](const MxRowsArgs& a, uint32_t grid, dim3 threads,
+                                                       uint32_t first, uint32_t blocks) {
+        mx_rows4_kernel<T, kBM, kBN, kWM, kWN, kSplit><<<grid, threads, 0, stream>>>(a, first, blocks);
     });
 }
 
-template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN>
+template <class T, Way kWay, int kBM, int kBN, int kWM, int kWN, int kSplit = 1>
 int launch_mixed(const MxRowsArgs& m, hipStream_t stream) {
-    return in_tiles<kBM, kBN, kWM, kWN>(m, [&](const MxRowsArgs& a, uint32_t grid, int threads,
-                                               uint32_t first, uint32_t blocks) {
-        mx_mixed_kernel<T, kWay, kBM, kBN, kWM, kWN><<<grid, threads, 0, stream>>>(a, first, blocks);
+    return in_tiles<kBM, kBN, kWM, kWN, kSplit>(m, [&](const MxRowsArgs& a, uint32_t grid, dim3 threads,
+                                                       uint32_t first, uint32_t blocks) {
+        mx_mixed_kernel<T, kWay, kBM, kBN, kWM, kWN, kSplit><<<grid, threads, 0, stream>>>(a, first, blocks);
     });
 }
 
@@ -516,6 +598,21 @@ template <class T, bool kRows4, int kRowTiles> int launch_mx_few(const MxRowsArg
     return launch_mx_few_as<T, kRows4, kRowTiles, 2>(m, stream);
 }
 
+// Shares that the depth of a tile of 64 x 64 is cut into, where there are few tiles.  us of bf16 rows as one, two and
+// four: 100 x 4096 x 4096 27.7, 20.0 and 17.0, 300 35.3, 29.0 and 33.8, 512 36.9, 32.9 and 34.9; 256 x 2048 x 2048
+// 15.8, 12.2 and 11.1, 1000 20.3, 18.6 and 21.6; 100 x 1024 x 1024 9.5, 8.1 and 7.9; 100 x 512 x 512 6.5, 6.2 and 7.0;
+// 1000 rows over 64 experts of 512 -> 1024 14.0, 17.5 and 31.1.  Rows of 4 bits, whose slabs take less time: 100 x 4096
+// x 4096 11.4, 9.5 and 9.3, 300 15.1, 14.1 and 19.3; 100 x 2048 x 2048 7.6, 6.9 and 7.4, 1000 10.0, 10.2 and 14.5; 100
+// x 1024 x 1024 5.7, 5.8 and 6.6.
+inline int shares_of(const MxRowsArgs& m) {
+    const RowsArgs& a = m.rows;
+    const int64_t tiles = piece_ids(a.rows, 64, a.offsets != nullptr, a.experts, true) * ((a.columns + 63) / 64);
+    const int64_t slabs = (m.code_pitch + kSlabBytes - 1) / kSlabBytes;
+    if (m.a_scales) return slabs >= (tiles <= kCus ? 8 : 16) && tiles <= 2 * kCus ? 2 : 1;
+    if (tiles > 2 * kCus || slabs < 2) return 1;
+    return tiles <= kCus && slabs >= 4 ? 4 : 2;
+}
+
 // Tiles as linear's, by the work there is.  us of bf16 products as 256 x 256, 128 x 128 and 64 x 64: rows of bf16,
 // 65536 x 1024 x 4096 522, 624 and 849, 16384 x 1024 x 1024 37, 45 and 57, 4096 x 2048 x 2048 (128 tiles of the
 // largest) -, 42 and 58, 131072 rows over 64 experts of 256 -> 512 88, 90 and 110; 4-bit rows 247, 308 and 382, 17, 22
@@ -529,19 +626,31 @@ template <class T, Way kWay> int launch_mixed_of(const MxRowsArgs& m, hipStream_
         if (a.columns > 128 && even(large) && each >= 1024) return launch_mixed<T, kWay, 256, 256, 64, 128>(m, stream);
     if constexpr (kWay != kGathered)
         if (a.columns > 64 && wide >= kCus && each >= 128) return launch_mixed<T, kWay, 128, 128, 64, 64>(m, stream);
+    if constexpr (kWay == kDirect)
+        switch (shares_of(m)) {
+            case 4: return launch_mixed<T, kWay, 64, 64, 32, 32, 4>(m, stream);
+            case 2: return launch_mixed<T, kWay, 64, 64, 32, 32, 2>(m, stream);
+        }
     return launch_mixed<T, kWay, 64, 64, 32, 32>(m, stream);
 }
 
 template <class T, bool kRows4> int launch_mx_by_rows(const MxRowsArgs& m, hipStream_t stream) {
     const RowsArgs& a = m.rows;
-    // Few rows: up to 64 for one matrix (4-bit rows 32), up to 256 (128) in all over several.  us of few rows and of
-    // tiles, bf16: 2048 -> 2048, 16 rows 5.5 and 15.0, 32 rows 7.4 and 15.2, 64 rows 11.6 and 15.3; 4-bit rows 4.5 and
-    // 7.1, 5.6 and 7.2, 8.0 and 7.4.  Over 64 experts of 512 -> 1024, 64 rows 8.0 and 12.8, 256 rows 13.0 and 13.4, 512
-    // rows 15.8 and 13.6; 4-bit rows, 64 rows 7.2 and 8.2, 256 rows 8.7 and 8.5, 512 rows 11.5 and 8.6.
-    if (a.experts > 1 ? a.rows <= (kRows4 ? 128 : 256) : a.rows <= 16) return launch_mx_few<T, kRows4, 1>(m, stream);
-    if (a.experts == 1 && a.rows <= 32) return launch_mx_few<T, kRows4, 2>(m, stream);
-    if constexpr (!kRows4)
-        if (a.experts == 1 && a.rows <= 64) return launch_mx_few<T, kRows4, 4>(m, stream);
+    // Few rows: up to 64 for one matrix (4-bit rows 32), up to 256 (128) in all over several.  Each 16 columns read all
+    // the rows, so that rows times columns tell how long that takes.  us of few rows and of tiles, bf16: 4096 -> 4096,
+    // 16 rows 8.2 and 16.0, 32 rows 11.8 and 16.1, 48 rows 17.5 and 16.4, 64 rows 20.1 and 16.4; 1024 -> 4096, 64 rows
+    // 8.1 and 8.1; 2048 -> 2048, 48 rows 10.3 and 10.6, 64 rows 11.6 and 10.8; 2048 -> 16384, one row 9.0 and 11.1, 8
+    // rows 11.9 and 11.2, 16 rows 13.8 and 11.4, 64 rows 44.8 and 12.1; 4-bit rows, 4096 -> 4096, 32 rows 8.1 and 9.2,
+    // 4096 -> 16384, 16 rows 17.9 and 11.1.  Over 64 experts of 512 -> 1024, 64 rows 8.0 and 12.8, 256 rows 13.0 and
+    // 13.4, 512 rows 15.8 and 13.6; 4-bit rows, 64 rows 7.2 and 8.2, 256 rows 8.7 and 8.5, 512 rows 11.5 and 8.6.
+    if (a.experts > 1) {
+        if (a.rows <= (kRows4 ? 128 : 256)) return launch_mx_few<T, kRows4, 1>(m, stream);
+    } else if (a.rows * a.columns < 1 << 18 && (a.rows <= 48 || a.depth < 2048)) {
+        if (a.rows <= 16) return launch_mx_few<T, kRows4, 1>(m, stream);
+        if (a.rows <= 32) return launch_mx_few<T, kRows4, 2>(m, stream);
+        if constexpr (!kRows4)
+            if (a.rows <= 64) return launch_mx_few<T, kRows4, 4>(m, stream);
+    }
     if constexpr (kRows4) {
         const int64_t large = (a.rows + 255) / 256 * ((a.columns + 255) / 256);
         const int64_t wide = (a.rows + 127) / 128 * ((a.columns + 127) / 128);
@@ -549,6 +658,7 @@ template <class T, bool kRows4> int launch_mx_by_rows(const MxRowsArgs& m, hipSt
             return launch_rows4<T, 256, 256, 64, 128>(m, stream);
         if (a.columns > 64 && wide >= kCus && a.rows / a.experts >= 128)
             return launch_rows4<T, 128, 128, 64, 64>(m, stream);
+        if (shares_of(m) == 2) return launch_rows4<T, 64, 64, 32, 32, 2>(m, stream);
         return launch_rows4<T, 64, 64, 32, 32>(m, stream);
     } else {
         switch (way_of<T>(a.a, a.lda, a.depth)) {

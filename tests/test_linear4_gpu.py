@@ -105,6 +105,48 @@ def test_every_activation_bias_and_residual(activation, dtype):
             _check_rows_of_4_bits(x, quantize(w), b, r, activation, activation)
 
 
+# few tiles, whose depth is cut into shares: shares that end inside slabs, uneven and empty ones, one and two a CU
+SHARES = [(65, 264, 70), (100, 512, 64), (70, 520, 130), (66, 1032, 65), (65, 1288, 96), (100, 2048, 200), (129, 2312, 64),
+          (100, 4104, 72), (300, 1024, 4096), (20, 520, 13200), (33, 4096, 8000), (64, 2304, 40)]
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('shape', SHARES, ids=str)
+def test_shares_of_the_depth(shape, dtype):
+    n, inputs, outputs = shape
+    for activation in ('none', 'silu'):
+        print('shares', shape, dtype, activation, flush=True)
+        x, w, b, r, dy = _case(n + inputs, n, inputs, outputs, dtype)
+        _check_rows_of_t(x, quantize(w), b, r, dy, activation, str(shape))
+        _check_rows_of_4_bits(x, quantize(w), b, r, activation, str(shape))
+    # every sum exact: each share takes its own part, once
+    x, w, b, r, dy = _case(n + inputs, n, inputs, outputs, dtype, whole=True)
+    _check_rows_of_t(x, quantize(w), b, r, dy, 'relu', str(shape))
+    _check_rows_of_4_bits(x, quantize(w), b, r, 'relu', str(shape))
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_shares_of_experts(dtype):
+    """Groups that end inside tiles, an empty one, and rows of no expert."""
+    counts, inputs, outputs = [70, 0, 200, 1], 2312, 100
+    n = sum(counts) + 40
+    x, w, b, r, _ = _case(11, n, inputs, outputs, dtype, lead=(len(counts),))
+    x[n - 40:] = float('nan')
+    q, offsets = quantize(w), _offsets(counts)
+    y = linear(x, q, b, activation='gelu', residual=r, offsets=offsets)
+    y4 = linear(quantize(x), q, b, activation='gelu', residual=r, offsets=offsets)
+    wide, wide_x = _weight64(q), _weight64(quantize(x))
+    at = 0
+    for e, count in enumerate(counts):
+        rows = slice(at, at + count)
+        layer = Layer64(x[rows], wide[e].to(dtype), b[e], r[rows], None, 'gelu')
+        check(y[rows], layer.y, layer.y_error, 'group %d' % e)
+        layer = Layer64(_Typed(wide_x[rows], dtype), wide[e], b[e], r[rows], None, 'gelu')
+        check(y4[rows], layer.y, layer.y_error, 'group %d, 4-bit rows' % e)
+        at += count
+    assert torch.equal(y[at:], r[at:]) and torch.equal(y4[at:], r[at:])
+
+
 # gradients that are formed in one pass: each tile's and slab's edges, rows that fill no tile
 ONE_PASS = [(65536, 1, 8), (65537, 64, 9), (65600, 65, 64), (65665, 128, 71), (65700, 129, 264), (66000, 256, 136),
             (70000, 33, 12), (65999, 250, 520)]
