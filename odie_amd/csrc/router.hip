@@ -405,7 +405,7 @@ __global__ __launch_bounds__(kBlock) void choose_backward_kernel(ChooseBackwardA
 // --- balance -------------------------------------------------------------------------------------------
 
 constexpr int kCountBlock = 1024;
-constexpr int kSharedCounts = 8192;      // experts whose counts a workgroup keeps in LDS
+constexpr int kSharedCounts = 1 << 14;   // experts whose counts a workgroup keeps in LDS
 constexpr int64_t kFewEntries = 1 << 14; // counted by one workgroup, which needs nothing cleared before
 constexpr uint32_t kFewBlocks = 256;     // of which the last one makes the loss
 
@@ -439,7 +439,7 @@ template <bool kAlone> __global__ __launch_bounds__(kCountBlock) void balance_co
     const int64_t entries = a.n * a.choices, step = static_cast<int64_t>(gridDim.x) * kCountBlock;
     const int64_t self = static_cast<int64_t>(blockIdx.x) * kCountBlock + threadIdx.x;
     int32_t* to = shared ? held : a.counts;
-    if (shared || kAlone) {
+    if (shared) {
         for (int e = threadIdx.x; e < a.experts; e += kCountBlock) to[e] = 0;
         if (kAlone && a.done && threadIdx.x == 0) *a.done = 0;
         __syncthreads();
@@ -476,7 +476,8 @@ __device__ inline void hold_counts(const int32_t* counts, int lane, int experts,
         }
 }
 
-// Whether a row has an entry, for all of its lanes: asked for ahead (one entry a lane) and told later.
+// Whether a row has an entry among those of its lanes (of a wave's, where there are more): asked for ahead, one entry a
+// lane, and told later.
 template <int kLanes> struct Part {
     int32_t id;
 
@@ -487,7 +488,7 @@ template <int kLanes> struct Part {
         uint32_t any = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.experts);
         for (int j = lane + kLanes; j < a.choices; j += kLanes)
             any |= static_cast<uint32_t>(a.expert[row * a.choices + j]) < static_cast<uint32_t>(a.experts);
-        return across<kLanes>(any, [](uint32_t x, uint32_t y) { return x | y; }) != 0;
+        return across<(kLanes < 64 ? kLanes : 64)>(any, [](uint32_t x, uint32_t y) { return x | y; }) != 0;
     }
 };
 
@@ -515,10 +516,12 @@ __device__ inline BalanceSums sum_block(BalanceSums x) {
 // The loss from the workgroups' sums, in their order.
 __device__ inline void make_loss(const BalanceArgs& a) {
     BalanceSums x{};
+#pragma unroll 8
     for (uint32_t b = threadIdx.x; b < a.blocks; b += kBlock) {
         x.total += __hip_atomic_load(a.partial + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         x.rows += __hip_atomic_load(a.parts + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
+#pragma unroll 8
     for (int e = threadIdx.x; e < a.experts; e += kBlock) x.entries += static_cast<uint32_t>(a.counts[e]);
     x = sum_block(x);
     if (threadIdx.x != 0) return;
@@ -551,9 +554,20 @@ __device__ inline void finish_balance(const BalanceArgs& a, double total, uint32
 
 __global__ __launch_bounds__(kBlock) void balance_loss_kernel(BalanceArgs a) { make_loss(a); }
 
-// Rows of up to 64 kVecs chunks: kLanes lanes a row, a row in registers and the next one under way, the counts of the
-// lane's columns in registers for all of its rows.  300007 x 1000 bf16: 140 to 170 us, 600 MB at 3.6 to 4.3 TB/s (with
-// the counts read for each row 524 us; with loads under conditions, which the compiler waits for, 214).
+// Two numbers of each wave of a workgroup, to all of its threads by LDS; `turn` as for best_of.
+template <class F>
+__device__ inline void over_waves(float2 own, float2 (&part)[2][kBlock / 64], int& turn, F&& f) {
+    turn ^= 1;
+    if (threadIdx.x % 64 == 0) part[turn][threadIdx.x / 64] = own;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kBlock / 64; ++w) f(part[turn][w]);
+}
+
+// Rows of up to kLanes kVecs chunks: kLanes lanes a row, a row in registers and the next one under way, the counts of
+// the lane's columns in registers for all of its rows.  300007 x 1000 bf16: 140 to 170 us, 600 MB at 3.6 to 4.3 TB/s
+// (with the counts read for each row 524 us; with loads under conditions, which the compiler waits for, 214); 8192 x
+// 8000 39 us (a wave a row 122).
 template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) void balance_rows_kernel(BalanceArgs a) {
     constexpr bool kExact = sizeof(T) == 4;
     constexpr int kV = kPerVec<T>, kRows = kBlock / kLanes;
@@ -563,6 +577,9 @@ template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) v
     const T* logits = static_cast<const T*>(a.logits);
     double total = 0.0;
     uint32_t rows = 0;
+    constexpr int kTogether = kLanes < 64 ? kLanes : 64;
+    __shared__ float2 held[2][kBlock / 64];
+    int turn = 0;
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
     int64_t at = static_cast<int64_t>(blockIdx.x) * kRows + static_cast<int>(threadIdx.x) / kLanes;
     RowHold<T, kLanes, kVecs> next;
@@ -577,7 +594,7 @@ template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) v
         const int64_t now = at < a.n ? at : a.n - 1, then = at + step < a.n ? at + step : a.n - 1;
         next.load(logits + then * a.stride, lane, a.experts);
         part_next.load(a, then, lane);
-        const bool any = part.get(a, now, lane);
+        bool any = part.get(a, now, lane);
         row.settle(lane, a.experts);
         float value[kVecs][kV], top = kNegInfinity;
 #pragma unroll
@@ -586,7 +603,12 @@ template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) v
 #pragma unroll
             for (int i = 0; i < kV; ++i) top = larger(top, value[v][i]);
         }
-        top = max_across<kLanes>(top);
+        top = max_across<kTogether>(top);
+        if constexpr (kLanes > 64)
+            over_waves(make_float2(top, any ? 1.0f : 0.0f), held, turn, [&](const float2& x) {
+                top = larger(top, x.x);
+                any |= x.y != 0.0f;
+            });
         const float from = base_of(top);
         float s = 0.0f, t = 0.0f;
 #pragma unroll
@@ -597,8 +619,13 @@ template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) v
                 s += e;
                 t = fmaf(e, counts[v][i], t);
             }
-        s = sum_across<kLanes>(s);
-        t = sum_across<kLanes>(t);
+        s = sum_across<kTogether>(s);
+        t = sum_across<kTogether>(t);
+        if constexpr (kLanes > 64) {
+            const float2 own = make_float2(s, t);
+            s = t = 0.0f;
+            over_waves(own, held, turn, [&](const float2& x) { s += x.x, t += x.y; });
+        }
         const float inverse = any && !(top == kNegInfinity) ? 1.0f / s : 0.0f;
         t = inverse == 0.0f ? 0.0f : t * inverse;
         if (at < a.n && lane == 0) {
@@ -610,7 +637,22 @@ template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) v
     finish_balance(a, total, rows);
 }
 
-// Longer rows: a wave a row, with a running maximum.
+// The counts of a chunk's columns as fp32, 0 past the last.
+template <int kV> __device__ inline void load_counts(const int32_t* counts, int column, int experts, float (&to)[kV]) {
+    if (column + kV <= experts) {
+#pragma unroll
+        for (int w = 0; w < kV / 4; ++w) {
+            const vec16 four = load16(counts + column + 4 * w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[4 * w + i] = static_cast<float>(static_cast<int32_t>(four[i]));
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kV; ++i) to[i] = column + i < experts ? static_cast<float>(counts[column + i]) : 0.0f;
+}
+
+// Longer rows: a wave a row, with a running maximum.  8192 x 32000 bf16: 149 us forward and 230 backward.
 template <class T> __global__ __launch_bounds__(kBlock) void balance_long_kernel(BalanceArgs a) {
     constexpr bool kExact = sizeof(T) == 4;
     constexpr int kV = kPerVec<T>;
@@ -627,9 +669,7 @@ template <class T> __global__ __launch_bounds__(kBlock) void balance_long_kernel
         for (int column = lane * kV; column < a.experts; column += 64 * kV) {
             float value[kV], counts[kV];
             load_logits(logits, column, a.experts, value);
-#pragma unroll
-            for (int i = 0; i < kV; ++i)
-                counts[i] = column + i < a.experts ? static_cast<float>(a.counts[column + i]) : 0.0f;
+            load_counts(a.counts, column, a.experts, counts);
             float top = m;
 #pragma unroll
             for (int i = 0; i < kV; ++i) top = larger(top, value[i]);
@@ -720,12 +760,12 @@ __global__ __launch_bounds__(kBlock) void balance_long_backward_kernel(BalanceBa
         const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
         T* out = static_cast<T*>(a.dlogits) + row * a.experts;
         for (int column = lane * kV; column < a.experts; column += 64 * kV) {
-            float value[kV];
+            float value[kV], counts[kV];
             load_logits(logits, column, a.experts, value);
+            load_counts(a.counts, column, a.experts, counts);
 #pragma unroll
             for (int i = 0; i < kV; ++i) {
-                const float count = column + i < a.experts ? static_cast<float>(a.counts[column + i]) : 0.0f;
-                const float d = each * exponential<sizeof(T) == 4>(value[i] - stats.x) * (count - stats.z);
+                const float d = each * exponential<sizeof(T) == 4>(value[i] - stats.x) * (counts[i] - stats.z);
                 value[i] = stats.y == 0.0f ? 0.0f : d;
             }
             store_some<kStream>(out + column, narrow<T>(value), a.experts - column);
@@ -760,6 +800,8 @@ template <class T, class F> void with_row(int width, int least, F&& f) {
     else if (chunks <= 128) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
     else if (chunks <= 256) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
     else if (chunks <= 512) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
+    else if (chunks <= 1024) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+    else if (chunks <= 2048) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 8>{});
     else f(std::integral_constant<int, 64>{}, std::integral_constant<int, 0>{});
 }
 
@@ -773,6 +815,9 @@ uint32_t row_blocks(int64_t n, int lanes, int vecs, bool writes = false) {
     const int64_t most = (vecs == 8 ? 2 : (vecs == 4 || writes ? 4 : 6)) * kCus;
     return static_cast<uint32_t>(blocks < 1 ? 1 : (blocks < most ? blocks : most));
 }
+
+// The most workgroups that any width takes: a row each, six a CU.
+int64_t most_row_blocks(int64_t n) { return row_blocks(n, kBlock, 1); }
 
 // Whether a choice reads its rows once for each of the choices, instead of once in all.  us in registers and by turns,
 // fp32: 8192 x 4000, one choice 37 and 25, two 43 and 41, four 52 and 73; 8192 x 8000, four 165 and 143; 8192 x 16000,
@@ -849,7 +894,7 @@ ODIE_API int odie_choose_backward(const float* upstream, const int32_t* expert, 
 
 ODIE_API int64_t odie_balance_workspace(int64_t n, int choices, int experts) {
     if (check_rows_of("odie_balance_workspace", experts, n, choices, experts, ODIE_F32)) return -1;
-    return 12 * static_cast<int64_t>(row_blocks(n, 64, 1)) + 8;
+    return 12 * most_row_blocks(n) + 8;
 }
 
 ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int32_t* expert, int64_t n, int choices,
@@ -862,7 +907,7 @@ ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int3
     const int64_t need = odie_balance_workspace(n, choices, experts);
     if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 8 != 0)
         return fail(what + ": needs an 8-byte aligned workspace of " + std::to_string(need) + " bytes");
-    const int64_t most = row_blocks(n, 64, 1);
+    const int64_t most = most_row_blocks(n);
     BalanceArgs a{};
     a.logits = logits;
     a.expert = expert;
@@ -883,7 +928,7 @@ ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int3
     const hipStream_t s = as_stream(stream);
     const int64_t entries = n * choices;
     const int shared = experts <= kSharedCounts ? experts * 4 : 0;
-    if (entries <= kFewEntries) {
+    if (entries <= kFewEntries && experts <= kSharedCounts) {
         balance_count_kernel<true><<<1, kCountBlock, shared, s>>>(a);
     } else {
         // Sixteen entries a thread at least, and two for each count that a workgroup adds at its end.

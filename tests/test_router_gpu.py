@@ -232,11 +232,13 @@ def test_balance_of_padding_and_masks(dtype):
         assert not torch.autograd.grad(loss, leaf)[0].any()
 
 
-@pytest.mark.parametrize('n, width, choices', ((300, 40, 100), (5, 10, 1000), (400, 10000, 64), (130, 32768, 130), (700, 5000, 30)))
-def test_balance_of_many_entries_a_row(n, width, choices):
+@pytest.mark.parametrize('dtype', (torch.float16, torch.float32), ids=str)
+@pytest.mark.parametrize('n, width, choices', ((300, 40, 100), (5, 10, 1000), (400, 10000, 64), (130, 32768, 130), (700, 5000, 30), (1030, 8200, 2),
+                                                 (50, 16384, 3), (40, 16392, 3)))
+def test_balance_of_many_entries_a_row(n, width, choices, dtype):
     """More entries than lanes of a row; counts of many experts, from many entries; long rows with padding."""
     generator = _generator(n)
-    logits = _logits(generator, torch.float16, n, width)
+    logits = _logits(generator, dtype, n, width)
     expert = torch.randint(-width // 4, width, (n, choices), generator=generator, device='cuda', dtype=torch.int32)
     expert[1::3] = -1
     expert[0, :-1] = -1
