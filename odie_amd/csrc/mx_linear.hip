@@ -4,6 +4,14 @@
 #include "mx_kernels.h"
 
 namespace odie {
+
+// in mx_<type>.hip and mx_input_<type>.hip
+extern template int launch_mx<float>(const MxRowsArgs&, hipStream_t);
+extern template int launch_mx<_Float16>(const MxRowsArgs&, hipStream_t);
+extern template int launch_mx<__bf16>(const MxRowsArgs&, hipStream_t);
+extern template int launch_mx_input<_Float16>(const MxInputArgs&, hipStream_t);
+extern template int launch_mx_input<__bf16>(const MxInputArgs&, hipStream_t);
+
 namespace {
 
 int check_sizes(const std::string& what, int64_t rows, int experts, bool grouped, int inputs, int outputs, int dtype,

@@ -263,6 +263,18 @@ def test_rows_of_any_stride_and_start(n, dtype):
     assert torch.equal(linear(quantize(wide[:, 5:155]), q), linear(quantize(wide[:, 5:155].contiguous()), q))
 
 
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('shape', ((3, 2047, 8192), (3, 2045, 8192), (3, 2046, 8192), (20, 1023, 8192), (40, 1027, 8192)), ids=str)
+def test_few_rows_that_end_inside_16_bytes(shape, dtype):
+    """Every lane's last loads move down in registers, with the CUs full of other waves."""
+    n, inputs, outputs = shape
+    x, w, b, _, _ = _case(inputs, n, inputs, outputs, dtype)
+    q = quantize(w)
+    for _ in range(3):
+        layer = Layer64(x, _weight64(q).to(dtype), b, None, None, 'none')
+        check(linear(x, q, b), layer.y, layer.y_error, str(shape))
+
+
 def test_blocks_of_nan_and_infinite_rows():
     """A NaN block makes its output column NaN and no other; a NaN or infinite row its own outputs."""
     for n, outputs in ((3, 40), (50, 70), (3000, 300)):

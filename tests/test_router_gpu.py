@@ -104,6 +104,13 @@ def test_choose_of_long_rows(width, dtype):
 
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('width', (15, 62, 131, 515, 2051))
+def test_choose_of_many_rows_that_end_inside_16_bytes(width, dtype):
+    for choices, normalize in ((2, False), (8, False), (8, True)):
+        _check_choose(_logits(_generator(width), dtype, 20000, width), choices, normalize, width, '20000x%d' % width)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
 @pytest.mark.parametrize('width', (8, 64, 1000, 2100, 5000, 12000, 20000))
 def test_choose_ties_and_masks(width, dtype):
     """Equal logits go by index, -0 and 0 are equal, and rows may have fewer allowed experts than choices, or none."""
