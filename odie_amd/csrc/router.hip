@@ -351,9 +351,12 @@ struct ChooseBackwardArgs {
     int experts, choices;
 };
 
-// kLanes lanes a row write its gradient chunk by chunk; each lane holds one of the row's entries.  65536 x 1024 fp16,
-// weights among all: 46 us, 268 MB at 5.8 TB/s (the logits partly from the last-level cache); over the chosen 32 us.
-template <class T, int kLanes, bool kAll, bool kStream>
+// kLanes lanes a row write its gradient chunk by chunk; each lane holds one of the row's entries, and writes it once
+// more afterwards (kPatched) or hands it to the lane whose chunk it falls in.  Handing out costs about 26 instructions
+// an entry and round of chunks; writing again moves lines a second time (us handed out and patched, fp16: 65536 x 1024,
+// four of all 45 and 44, eight 61 and 45, 64 309 and 61; 10^6 x 64, two among themselves 28 and 39, eight of all 72 and
+// 64).  65536 x 1024, four of all: 268 MB at 6.1 TB/s (the logits partly from the last-level cache).
+template <class T, int kLanes, bool kAll, bool kStream, bool kPatched>
 __global__ __launch_bounds__(kBlock) void choose_backward_kernel(ChooseBackwardArgs a, uint32_t first) {
     constexpr int kV = kPerVec<T>;
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
@@ -372,12 +375,11 @@ __global__ __launch_bounds__(kBlock) void choose_backward_kernel(ChooseBackwardA
         }
     }
     const float total = sum_across<kLanes>(weighted);
+    const float result = fmaf(-weight, total, weighted);       // w_j is the entry's share in both kinds of weights
     float m = 0.0f, share = 0.0f;
     if constexpr (kAll) {
         m = base_of(a.stats[row * 2]);
         share = -total * a.stats[row * 2 + 1];
-    } else {
-        weighted = fmaf(-weight, total, weighted);
     }
     const bool empty = kAll && a.stats[row * 2 + 1] == 0.0f;   // a row of none; else 1 / s > 0 or NaN
     const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
@@ -391,14 +393,21 @@ __global__ __launch_bounds__(kBlock) void choose_backward_kernel(ChooseBackwardA
 #pragma unroll
             for (int i = 0; i < kV; ++i) value[i] = share * exponential<sizeof(T) == 4>(value[i] - m);
         }
-        for (int j = 0; j < a.choices; ++j) {
-            const int e = __shfl(own, j, kLanes);
-            const float add = __shfl(weighted, j, kLanes);
-            const int place = e < 0 ? -1 : e - column;
+        if constexpr (!kPatched)
+            for (int j = 0; j < a.choices; ++j) {
+                const int e = __shfl(own, j, kLanes);
+                const float whole = __shfl(result, j, kLanes);
+                const int place = e < 0 ? -1 : e - column;
 #pragma unroll
-            for (int i = 0; i < kV; ++i) value[i] += place == i ? add : 0.0f;
-        }
+                for (int i = 0; i < kV; ++i) value[i] = place == i ? whole : value[i];
+            }
         if (at < a.n && column < a.experts) store_some<kStream>(out + column, narrow<T>(value), a.experts - column);
+    }
+    if constexpr (kPatched) {
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");      // after the other lanes' stores
+        float value = result;
+        asm("" : "+v"(value));      // rounded to fp32, then to T, as its neighbours are
+        if (at < a.n && own >= 0) out[own] = static_cast<T>(value);
     }
 }
 
@@ -881,9 +890,11 @@ ODIE_API int odie_choose_backward(const float* upstream, const int32_t* expert, 
         with_lanes<T>(experts, choices, [&](auto lanes) {
             with_flag(logits != nullptr, [&](auto all) {
                 with_flag(n * experts * dtype_bytes(dtype) >= kStreamBytes, [&](auto far) {
-                    in_launches((n + kBlock / lanes - 1) / (kBlock / lanes), kBlock,
-                                [&](uint32_t first, uint32_t count) {
-                        choose_backward_kernel<T, lanes, all, far><<<count, kBlock, 0, s>>>(a, first);
+                    with_flag(choices > 4 || experts > lanes * kPerVec<T>, [&](auto patched) {
+                        in_launches((n + kBlock / lanes - 1) / (kBlock / lanes), kBlock,
+                                    [&](uint32_t first, uint32_t count) {
+                            choose_backward_kernel<T, lanes, all, far, patched><<<count, kBlock, 0, s>>>(a, first);
+                        });
                     });
                 });
             });
