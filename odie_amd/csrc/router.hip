@@ -351,11 +351,12 @@ struct ChooseBackwardArgs {
     int experts, choices;
 };
 
-// kLanes lanes a row write its gradient chunk by chunk; each lane holds one of the row's entries, and writes it once
-// more afterwards (kPatched) or hands it to the lane whose chunk it falls in.  Handing out costs about 26 instructions
-// an entry and round of chunks; writing again moves lines a second time (us handed out and patched, fp16: 65536 x 1024,
-// four of all 45 and 44, eight 61 and 45, 64 309 and 61; 10^6 x 64, two among themselves 28 and 39, eight of all 72 and
-// 64).  65536 x 1024, four of all: 268 MB at 6.1 TB/s (the logits partly from the last-level cache).
+// kLanes lanes a row write its gradient chunk by chunk; each lane holds one of the row's entries, and writes it once more
+// afterwards (kPatched) or hands it to the lane whose chunk it falls in.  Handing out costs about 26 instructions an
+// entry and round of chunks; writing again moves lines a second time (us handed out and patched, fp16: 65536 x 1024,
+// four of all 45 and 44, in turn with the choice itself 99 and 104, eight 61 and 45, 64 309 and 61; 10^6 x 64, two among
+// themselves 28 and 39, eight of all 72 and 64).  65536 x 1024, four of all: 268 MB at 6 TB/s (the logits partly from
+// the last-level cache).
 template <class T, int kLanes, bool kAll, bool kStream, bool kPatched>
 __global__ __launch_bounds__(kBlock) void choose_backward_kernel(ChooseBackwardArgs a, uint32_t first) {
     constexpr int kV = kPerVec<T>;
@@ -890,7 +891,7 @@ ODIE_API int odie_choose_backward(const float* upstream, const int32_t* expert, 
         with_lanes<T>(experts, choices, [&](auto lanes) {
             with_flag(logits != nullptr, [&](auto all) {
                 with_flag(n * experts * dtype_bytes(dtype) >= kStreamBytes, [&](auto far) {
-                    with_flag(choices > 4 || experts > lanes * kPerVec<T>, [&](auto patched) {
+                    with_flag(choices > 4 || experts > 2 * lanes * kPerVec<T>, [&](auto patched) {
                         in_launches((n + kBlock / lanes - 1) / (kBlock / lanes), kBlock,
                                     [&](uint32_t first, uint32_t count) {
                             choose_backward_kernel<T, lanes, all, far, patched><<<count, kBlock, 0, s>>>(a, first);
