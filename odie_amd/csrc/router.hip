@@ -25,7 +25,8 @@ template <class N> __device__ inline N least_of(N a, N b) { return a < b ? a : b
 
 // Logits with their indices as whole numbers: the larger the logit and, among equal ones, the lower the index, the
 // larger the key.  A logit's bits become a signed number in the order of the values by negating the magnitude of
-// negative ones (which makes -0 and 0 alike); a NaN is the largest.  A 16-bit logit and its index fit 32 bits.
+// negative ones (which makes -0 and 0 alike); a NaN is the largest.  A 16-bit logit and its index fit 32 bits.  No fp32
+// key is INT64_MAX, below which choose_long_kernel's search for the first choice begins.
 template <class T> struct Keys {
     using Key = int32_t;
     static constexpr Key kNone = INT32_MIN;
@@ -81,7 +82,7 @@ template <> struct Keys<float> {
 
     static __device__ Key of(float value, int index) {
         const int32_t bits = __builtin_bit_cast(int32_t, value), sign = bits >> 31, size = bits & 0x7fffffff;
-        const int32_t order = size > 0x7f800000 ? 0x7fffffff : (size ^ sign) - sign;
+        const int32_t order = size > 0x7f800000 ? 0x7fc00000 : (size ^ sign) - sign;
         return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(order)) << 32 |
                                     static_cast<uint32_t>(~index));
     }
