@@ -948,8 +948,9 @@ ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int3
         const int64_t each = 16 * kCountBlock > 2 * experts ? 16 * kCountBlock : 2 * experts;
         const int64_t blocks = (entries + each - 1) / each;
         balance_clear_kernel<<<(experts + kBlock - 1) / kBlock, kBlock, 0, s>>>(a);
-        balance_count_kernel<false>
-            <<<static_cast<uint32_t>(blocks < kCus ? blocks : kCus), kCountBlock, shared, s>>>(a);
+        if (entries > 0)      // none: the counts are cleared, and a launch of no workgroups is an error
+            balance_count_kernel<false>
+                <<<static_cast<uint32_t>(blocks < kCus ? blocks : kCus), kCountBlock, shared, s>>>(a);
     }
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
