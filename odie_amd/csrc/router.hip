@@ -9,7 +9,9 @@
 //
 // The loss is E sum_e (c_e / M) (mean over rows of p_ie) with its sums exchanged: each row needs its own
 // logits and the counts alone, and no sums down the columns exist.  Counts are whole numbers, and everything else
-// is added in a fixed order: the same call gives the same bits.
+// is added in a fixed order: the same call gives the same bits.  Where the load is even, c_e and t_i are both near M / E
+// and their difference near its root: the whole number next to M / E is taken off every count before it becomes fp32, and
+// t_i is the mean of what is left, so that nothing is rounded relative to M / E.
 #include "softmax.h"
 
 namespace odie {
@@ -424,9 +426,10 @@ struct BalanceArgs {
     const void* logits;
     const int32_t* expert;    // [n][choices]
     int32_t* counts;          // [experts]
+    uint32_t* entries;        // M
     uint32_t* done;           // workgroups that have left their sums, or null: a launch of its own makes the loss
     uint32_t blocks;          // workgroups of the rows
-    float* stats;             // [n][4]: m, 1 / s (0: the row takes no part), t, 0
+    float* stats;             // [n][4]: m, 1 / s (0: the row takes no part), t less even_count, even_count's bits
     double* partial;          // [blocks]: sum of t
     uint32_t* parts;          // [blocks]: rows that take part
     float* norm;              // E / (M R)
@@ -437,7 +440,10 @@ struct BalanceArgs {
 
 __global__ __launch_bounds__(kBlock) void balance_clear_kernel(BalanceArgs a) {
     for (int e = blockIdx.x * kBlock + threadIdx.x; e < a.experts; e += gridDim.x * kBlock) a.counts[e] = 0;
-    if (a.done && blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        *a.entries = 0;
+        if (a.done) *a.done = 0;
+    }
 }
 
 // Each workgroup counts its entries in LDS and adds what it found (whole numbers, in any order).  kAlone: one workgroup
@@ -446,17 +452,20 @@ __global__ __launch_bounds__(kBlock) void balance_clear_kernel(BalanceArgs a) {
 // 27).
 template <bool kAlone> __global__ __launch_bounds__(kCountBlock) void balance_count_kernel(BalanceArgs a) {
     extern __shared__ int32_t held[];
+    __shared__ uint32_t all;
     const bool shared = a.experts <= kSharedCounts;
     const int64_t entries = a.n * a.choices, step = static_cast<int64_t>(gridDim.x) * kCountBlock;
     const int64_t self = static_cast<int64_t>(blockIdx.x) * kCountBlock + threadIdx.x;
     int32_t* to = shared ? held : a.counts;
+    if (threadIdx.x == 0) all = 0;
     if (shared) {
         for (int e = threadIdx.x; e < a.experts; e += kCountBlock) to[e] = 0;
         if (kAlone && a.done && threadIdx.x == 0) *a.done = 0;
-        __syncthreads();
     }
+    __syncthreads();
+    uint32_t found = 0;
     auto add = [&](int e) {
-        if (e >= 0 && e < a.experts) atomicAdd(to + e, 1);
+        if (e >= 0 && e < a.experts) atomicAdd(to + e, 1), ++found;
     };
     const int64_t fours = reinterpret_cast<uintptr_t>(a.expert) % 16 == 0 ? entries / 4 : 0;
     const int4* four = reinterpret_cast<const int4*>(a.expert);
@@ -466,24 +475,37 @@ template <bool kAlone> __global__ __launch_bounds__(kCountBlock) void balance_co
         add(e.x), add(e.y), add(e.z), add(e.w);
     }
     for (int64_t i = 4 * fours + self; i < entries; i += step) add(a.expert[i]);
-    if (!shared) return;
+    found = sum_across<64>(found);
+    if (threadIdx.x % 64 == 0) atomicAdd(&all, found);
     __syncthreads();
+    if (threadIdx.x == 0) {
+        if (kAlone) *a.entries = all;
+        else atomicAdd(a.entries, all);
+    }
+    if (!shared) return;
     for (int e = threadIdx.x; e < a.experts; e += kCountBlock) {
         if (kAlone) a.counts[e] = held[e];
         else if (held[e]) atomicAdd(a.counts + e, held[e]);
     }
 }
 
-// The counts of a lane's columns as fp32, 0 past the last.
+// The whole number next to M / E.
+__device__ inline int32_t even_count(const BalanceArgs& a) {
+    const uint32_t experts = static_cast<uint32_t>(a.experts);
+    return static_cast<int32_t>((*a.entries + experts / 2) / experts);
+}
+
+// The counts of a lane's columns less `even`, as fp32; 0 past the last.
 template <class T, int kLanes, int kVecs>
-__device__ inline void hold_counts(const int32_t* counts, int lane, int experts, float (&to)[kVecs][kPerVec<T>]) {
+__device__ inline void hold_counts(const int32_t* counts, int32_t even, int lane, int experts,
+                                   float (&to)[kVecs][kPerVec<T>]) {
 #pragma unroll
     for (int v = 0; v < kVecs; ++v)
 #pragma unroll
         for (int i = 0; i < kPerVec<T>; ++i) {
             const int e = (v * kLanes + lane) * kPerVec<T> + i;
             const int32_t count = counts[e < experts ? e : experts - 1];
-            to[v][i] = e < experts ? static_cast<float>(count) : 0.0f;
+            to[v][i] = e < experts ? static_cast<float>(count - even) : 0.0f;
         }
 }
 
@@ -503,24 +525,26 @@ template <int kLanes> struct Part {
     }
 };
 
-__device__ inline void keep_row(const BalanceArgs& a, int64_t row, float m, float inverse, float t) {
-    if (a.stats) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(m, inverse, t, 0.0f);
+__device__ inline void keep_row(const BalanceArgs& a, int64_t row, float m, float inverse, float t, int32_t even) {
+    if (a.stats)
+        *reinterpret_cast<float4*>(a.stats + row * 4) =
+            make_float4(m, inverse, t, __builtin_bit_cast(float, even));
 }
 
 // The sums of the workgroup's threads, in thread 0.
 struct BalanceSums {
     double total;
-    uint32_t rows, entries;
+    uint32_t rows;
 };
 __device__ inline BalanceSums sum_block(BalanceSums x) {
     __shared__ BalanceSums part[kBlock / 64];
-    x = BalanceSums{sum_across<64>(x.total), sum_across<64>(x.rows), sum_across<64>(x.entries)};
+    x = BalanceSums{sum_across<64>(x.total), sum_across<64>(x.rows)};
     __syncthreads();
     if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = x;
     __syncthreads();
     if (threadIdx.x == 0)
         for (int w = 1; w < kBlock / 64; ++w)
-            x.total += part[w].total, x.rows += part[w].rows, x.entries += part[w].entries;
+            x.total += part[w].total, x.rows += part[w].rows;
     return x;
 }
 
@@ -532,14 +556,12 @@ __device__ inline void make_loss(const BalanceArgs& a) {
         x.total += __hip_atomic_load(a.partial + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         x.rows += __hip_atomic_load(a.parts + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-#pragma unroll 8
-    for (int e = threadIdx.x; e < a.experts; e += kBlock) x.entries += static_cast<uint32_t>(a.counts[e]);
     x = sum_block(x);
     if (threadIdx.x != 0) return;
-    const double norm =
-        x.entries > 0 ? a.experts / (static_cast<double>(x.entries) * static_cast<double>(x.rows)) : 0.0;
+    const uint32_t entries = *a.entries;
+    const double norm = entries > 0 ? a.experts / (static_cast<double>(entries) * static_cast<double>(x.rows)) : 0.0;
     *a.norm = static_cast<float>(norm);
-    *a.loss = static_cast<float>(x.entries > 0 ? x.total * norm : 0.0);
+    *a.loss = static_cast<float>(entries > 0 ? x.total * norm : 0.0);
 }
 
 // Leaves the workgroup's sums.  Of few workgroups the last one to come goes on to the loss, which saves a launch (3 us
@@ -547,7 +569,7 @@ __device__ inline void make_loss(const BalanceArgs& a) {
 // launch of its own 8.4 and 3.4; 4096 x 64: 256 workgroups 7.0, and 3.8 and 1.8).
 __device__ inline void finish_balance(const BalanceArgs& a, double total, uint32_t rows) {
     __shared__ bool last;
-    const BalanceSums x = sum_block(BalanceSums{total, rows, 0});
+    const BalanceSums x = sum_block(BalanceSums{total, rows});
     if (threadIdx.x == 0) {
         __hip_atomic_store(a.partial + blockIdx.x, x.total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __hip_atomic_store(a.parts + blockIdx.x, x.rows, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -583,8 +605,9 @@ template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) v
     constexpr bool kExact = sizeof(T) == 4;
     constexpr int kV = kPerVec<T>, kRows = kBlock / kLanes;
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
+    const int32_t even = even_count(a);
     float counts[kVecs][kV];
-    hold_counts<T, kLanes, kVecs>(a.counts, lane, a.experts, counts);
+    hold_counts<T, kLanes, kVecs>(a.counts, even, lane, a.experts, counts);
     const T* logits = static_cast<const T*>(a.logits);
     double total = 0.0;
     uint32_t rows = 0;
@@ -640,27 +663,28 @@ template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) v
         const float inverse = any && !(top == kNegInfinity) ? 1.0f / s : 0.0f;
         t = inverse == 0.0f ? 0.0f : t * inverse;
         if (at < a.n && lane == 0) {
-            total += static_cast<double>(t);
+            total += inverse == 0.0f ? 0.0 : static_cast<double>(even) + t;
             rows += any;
-            keep_row(a, at, top, inverse, t);
+            keep_row(a, at, top, inverse, t, even);
         }
     }
     finish_balance(a, total, rows);
 }
 
-// The counts of a chunk's columns as fp32, 0 past the last.
-template <int kV> __device__ inline void load_counts(const int32_t* counts, int column, int experts, float (&to)[kV]) {
+// The counts of a chunk's columns less `even`, as fp32; 0 past the last.
+template <int kV>
+__device__ inline void load_counts(const int32_t* counts, int32_t even, int column, int experts, float (&to)[kV]) {
     if (column + kV <= experts) {
 #pragma unroll
         for (int w = 0; w < kV / 4; ++w) {
             const vec16 four = load16(counts + column + 4 * w);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) to[4 * w + i] = static_cast<float>(static_cast<int32_t>(four[i]));
+            for (int i = 0; i < 4; ++i) to[4 * w + i] = static_cast<float>(static_cast<int32_t>(four[i]) - even);
         }
         return;
     }
 #pragma unroll
-    for (int i = 0; i < kV; ++i) to[i] = column + i < experts ? static_cast<float>(counts[column + i]) : 0.0f;
+    for (int i = 0; i < kV; ++i) to[i] = column + i < experts ? static_cast<float>(counts[column + i] - even) : 0.0f;
 }
 
 // Longer rows: a wave a row, with a running maximum.  8192 x 32000 bf16: 149 us forward and 230 backward.
@@ -668,6 +692,7 @@ template <class T> __global__ __launch_bounds__(kBlock) void balance_long_kernel
     constexpr bool kExact = sizeof(T) == 4;
     constexpr int kV = kPerVec<T>;
     const int lane = static_cast<int>(threadIdx.x) % 64;
+    const int32_t even = even_count(a);
     double total = 0.0;
     uint32_t rows = 0;
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * (kBlock / 64) + static_cast<int>(threadIdx.x) / 64; row < a.n;
@@ -680,7 +705,7 @@ template <class T> __global__ __launch_bounds__(kBlock) void balance_long_kernel
         for (int column = lane * kV; column < a.experts; column += 64 * kV) {
             float value[kV], counts[kV];
             load_logits(logits, column, a.experts, value);
-            load_counts(a.counts, column, a.experts, counts);
+            load_counts(a.counts, even, column, a.experts, counts);
             float top = m;
 #pragma unroll
             for (int i = 0; i < kV; ++i) top = larger(top, value[i]);
@@ -701,9 +726,9 @@ template <class T> __global__ __launch_bounds__(kBlock) void balance_long_kernel
         const float inverse = any && !(top == kNegInfinity) ? 1.0f / s : 0.0f;
         t = inverse == 0.0f ? 0.0f : t * inverse;
         if (lane == 0) {
-            total += static_cast<double>(t);
+            total += inverse == 0.0f ? 0.0 : static_cast<double>(even) + t;
             rows += any;
-            keep_row(a, row, top, inverse, t);
+            keep_row(a, row, top, inverse, t, even);
         }
     }
     finish_balance(a, total, rows);
@@ -720,13 +745,16 @@ struct BalanceBackwardArgs {
     int experts;
 };
 
+// What the forward took off every count: the same in each row's statistics.
+__device__ inline int32_t even_count(const BalanceBackwardArgs& a) { return __builtin_bit_cast(int32_t, a.stats[3]); }
+
 // The same way.  300007 x 1000 bf16: 243 us, 1.2 GB at 4.9 TB/s: HBM.
 template <class T, int kLanes, int kVecs, bool kStream>
 __global__ __launch_bounds__(kBlock) void balance_backward_kernel(BalanceBackwardArgs a) {
     constexpr int kV = kPerVec<T>, kRows = kBlock / kLanes;
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
     float counts[kVecs][kV];
-    hold_counts<T, kLanes, kVecs>(a.counts, lane, a.experts, counts);
+    hold_counts<T, kLanes, kVecs>(a.counts, even_count(a), lane, a.experts, counts);
     const float scale = *a.upstream * *a.norm;
     const T* logits = static_cast<const T*>(a.logits);
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
@@ -763,6 +791,7 @@ template <class T, bool kStream>
 __global__ __launch_bounds__(kBlock) void balance_long_backward_kernel(BalanceBackwardArgs a) {
     constexpr int kV = kPerVec<T>;
     const int lane = static_cast<int>(threadIdx.x) % 64;
+    const int32_t even = even_count(a);
     const float scale = *a.upstream * *a.norm;
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * (kBlock / 64) + static_cast<int>(threadIdx.x) / 64; row < a.n;
          row += static_cast<int64_t>(gridDim.x) * (kBlock / 64)) {
@@ -773,7 +802,7 @@ __global__ __launch_bounds__(kBlock) void balance_long_backward_kernel(BalanceBa
         for (int column = lane * kV; column < a.experts; column += 64 * kV) {
             float value[kV], counts[kV];
             load_logits(logits, column, a.experts, value);
-            load_counts(a.counts, column, a.experts, counts);
+            load_counts(a.counts, even, column, a.experts, counts);
 #pragma unroll
             for (int i = 0; i < kV; ++i) {
                 const float d = each * exponential<sizeof(T) == 4>(value[i] - stats.x) * (counts[i] - stats.z);
@@ -907,7 +936,7 @@ ODIE_API int odie_choose_backward(const float* upstream, const int32_t* expert, 
 
 ODIE_API int64_t odie_balance_workspace(int64_t n, int choices, int experts) {
     if (check_rows_of("odie_balance_workspace", experts, n, choices, experts, ODIE_F32)) return -1;
-    return 12 * most_row_blocks(n) + 8;
+    return 12 * most_row_blocks(n) + 8;      // sums of t, rows, entries, workgroups that are done
 }
 
 ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int32_t* expert, int64_t n, int choices,
@@ -931,7 +960,8 @@ ODIE_API int odie_balance_forward(const void* logits, int64_t stride, const int3
     with_dtype(dtype, [&](auto t) {
         with_row<decltype(t)>(experts, 1, [&](auto lanes, auto vecs) { a.blocks = row_blocks(n, lanes, vecs); });
     });
-    a.done = a.blocks <= kFewBlocks ? a.parts + most : nullptr;
+    a.entries = a.parts + most;
+    a.done = a.blocks <= kFewBlocks ? a.entries + 1 : nullptr;
     a.norm = norm;
     a.loss = loss;
     a.stride = stride;
