@@ -287,10 +287,11 @@ __device__ inline int64_t block_best(int64_t key, int64_t* part) {
     return key;
 }
 
-// A workgroup a row, which it reads once for each choice, the one below the last: for rows that do not fit its
-// registers, and where long rows of fp32, whose keys take 64 bits, have few choices (by_turns).
-template <class T> __global__ __launch_bounds__(kBlock) void choose_long_kernel(ChooseArgs a) {
-    using K = Keys<float>;
+// A workgroup a row of fp32, whose keys take 64 bits: it reads the row once for each choice, the one below the last.  For
+// rows that do not fit its registers, and long rows of few choices (by_turns).
+__global__ __launch_bounds__(kBlock) void choose_long_kernel(ChooseArgs a) {
+    using T = float;
+    using K = Keys<T>;
     constexpr int kV = kPerVec<T>;
     __shared__ int64_t part[kBlock / 64];
     __shared__ float sums[kBlock / 64];
@@ -322,7 +323,7 @@ template <class T> __global__ __launch_bounds__(kBlock) void choose_long_kernel(
                 float value[kV];
                 load_logits(logits, column, a.experts, value);
 #pragma unroll
-                for (int i = 0; i < kV; ++i) s += exponential<sizeof(T) == 4>(value[i] - base);
+                for (int i = 0; i < kV; ++i) s += exponential<true>(value[i] - base);
             }
         }
         s = sum_across<64>(s);
@@ -859,13 +860,13 @@ uint32_t row_blocks(int64_t n, int lanes, int vecs, bool writes = false) {
 // The most workgroups that any width takes: a row each, six a CU.
 int64_t most_row_blocks(int64_t n) { return row_blocks(n, kBlock, 1); }
 
-// Whether a choice reads its rows once for each of the choices, instead of once in all.  us in registers and by turns,
-// fp32: 8192 x 4000, one choice 37 and 25, two 43 and 41, four 52 and 73; 8192 x 8000, four 165 and 143; 8192 x 16000,
-// one 173 and 100, four 304 and 294, eight 476 and 580; 1000 x 8000, four 24 and 26; one row of 8000 6.5 and 16.  16
-// bits, 8192 rows, one choice: 8000 31 and 37, 16000 70 and 64, 32000 144 and 133.
-bool by_turns(int64_t n, int chunks, int choices, bool wide) {
-    return chunks > 4096 || (wide && n >= 4 * kCus && chunks > 512 && choices <= (chunks > 1024 ? 4 : 1));
+// Whether a choice reads its fp32 rows once for each of the choices, instead of once in all.  us in registers and by
+// turns: 8192 x 4000, one choice 37 and 25, two 43 and 41, four 52 and 73; 8192 x 8000, four 165 and 143; 8192 x 16000,
+// one 173 and 100, four 304 and 294, eight 476 and 580; 1000 x 8000, four 24 and 26; one row of 8000 6.5 and 16.
+bool by_turns(int64_t n, int chunks, int choices) {
+    return chunks > 4096 || (n >= 4 * kCus && chunks > 512 && choices <= (chunks > 1024 ? 4 : 1));
 }
+static_assert(kMaxExperts <= 4096 * kPerVec<_Float16>, "16-bit rows stay in registers");
 
 }  // namespace
 }  // namespace odie
@@ -886,10 +887,11 @@ ODIE_API int odie_choose_forward(const void* logits, int64_t stride, int64_t n, 
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
         const int chunks = (experts + kPerVec<T> - 1) / kPerVec<T>;
-        if (by_turns(n, chunks, choices, sizeof(T) == 4)) {
-            choose_long_kernel<T><<<static_cast<uint32_t>(n < 16 * kCus ? n : 16 * kCus), kBlock, 0, s>>>(a);
-            return check_launch("choose");
-        }
+        if constexpr (sizeof(T) == 4)
+            if (by_turns(n, chunks, choices)) {
+                choose_long_kernel<<<static_cast<uint32_t>(n < 16 * kCus ? n : 16 * kCus), kBlock, 0, s>>>(a);
+                return check_launch("choose");
+            }
         const auto launch = [&](auto lanes, auto vecs) {
             constexpr int kThreads = lanes > kBlock ? lanes : kBlock;
             choose_kernel<T, lanes, vecs><<<row_blocks(n, lanes, vecs), kThreads, 0, s>>>(a);
