@@ -11,7 +11,7 @@ import math
 import torch
 
 from . import _lib
-from .rows import DTYPES, pitch, row_major
+from .rows import DTYPES, pitch, row_major, tangents
 
 BLOCK = 32
 
@@ -62,12 +62,14 @@ def _aligned(value, bytes):
 
 def quantize(x):
     """x (CUDA fp32, fp16 or bf16, [N, width] or [experts, outputs, width]) as Microscaled.  A block that holds a NaN or
-    an infinity becomes NaN.  The result is whole numbers: no gradient passes through them."""
+    an infinity becomes NaN.  The result is whole numbers: no gradient passes through them, and x may not carry a tangent."""
     if not isinstance(x, torch.Tensor) or x.dtype not in DTYPES or x.ndim not in (2, 3) or not x.is_cuda:
         raise ValueError('x must be a CUDA fp32, fp16 or bf16 tensor of two or three dimensions')
     *lead, width = x.shape
     if not 1 <= width <= 1 << 20:
         raise ValueError('x must have 1 to 2^20 columns')
+    if tangents(x):
+        raise NotImplementedError('quantize has no forward-mode derivative')
     rows = row_major(x if x.ndim == 2 else x.detach().reshape(-1, width))
     blocks = _blocks(width)
     codes = x.new_empty((*lead, 16 * blocks), dtype=torch.uint8)

@@ -39,10 +39,14 @@ def pitch(rows):
     return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
 
 
+def tangents(*tensors):
+    """Whether one of the tensors carries a tangent (forward mode, also without gradients)."""
+    if forward_ad._current_level < 0:       # no level is open; asking each tensor costs more
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def records(*tensors):
     """Whether autograd has to see the call: it will ask for a gradient of one of the tensors, or one of them carries a
-    tangent (forward mode, also without gradients), which autograd refuses for these operators."""
-    if forward_ad._current_level >= 0:      # a level is open; asking each tensor costs more
-        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
-            return True
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    tangent, which autograd refuses for these operators."""
+    return tangents(*tensors) or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
