@@ -39,8 +39,6 @@ def linear(x, weight, bias=None, *, activation='none', residual=None, offsets=No
     if isinstance(x, Microscaled):
         if not isinstance(weight, Microscaled) or x.ndim != 2:
             raise ValueError('x of 4 bits must be [N, inputs], beside a weight of 4 bits')
-        if records(bias, residual):
-            raise ValueError('a layer of x of 4 bits has no backward: detach bias and residual')
     else:
         x = check_rows('x', x)
     n, inputs = x.shape
@@ -65,7 +63,10 @@ def linear(x, weight, bias=None, *, activation='none', residual=None, offsets=No
         offsets = offsets.contiguous()
     if four_bits:
         bias = None if bias is None else bias.contiguous()
-        if records(None if isinstance(x, Microscaled) else x, bias, residual):
+        fixed = isinstance(x, Microscaled)
+        if records(None if fixed else x, bias, residual):
+            if fixed:
+                raise ValueError('a layer of x of 4 bits has no backward: detach bias and residual')
             return _Linear4.apply(x, weight, bias, residual, offsets, _CODES[activation])
         return _forward4(x, weight, bias, residual, offsets, _CODES[activation], None)
     if records(x, weight, bias, residual):
