@@ -4,7 +4,8 @@ There is no CPU path.
 
 A value is +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} times its block's scale, a power of two: 4.25 bits a value.  The
 largest magnitude of a block is scaled into [4, 8) and clamped at 6; values are rounded to nearest even: off by at most a
-quarter of themselves from 1/6 of the largest on, and below that by a quarter of the scale.
+quarter of themselves from 1/4 of the largest on, which is one scale at least, and below one scale by a quarter of the
+scale.
 """
 import math
 
