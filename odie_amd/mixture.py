@@ -219,7 +219,8 @@ class MicroscaledMixture(nn.Module):
 class RoutedMixture(nn.Module):
     """A mixture that chooses its experts itself: logits = x R^T, and each row's `choices` largest with their softmax
     weights (over the chosen, or with normalize=False over all) blend the experts' decoders.  The arguments are
-    ExpertMixture's and choose's."""
+    ExpertMixture's and choose's.  The logits are of x's type, fp32 sums rounded once; for a choice by fp32 ones beside
+    16-bit layers: expert, weights = choose(linear(x.float(), m.router.float()), m.choices), m.mixture(x, expert, weights)."""
 
     def __init__(self, experts, choices, inputs, hidden, outputs, *, normalize=True, activation='relu', codes=0, vocab=0,
                  dtype=torch.float16, device='cuda', seed=0):
