@@ -65,7 +65,7 @@ __device__ inline void finish_tile(Work& work, const RowsArgs& a, const Piece& p
             for (int u = 0; u < kGroup; ++u)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) value[u][i] += shift[i];
-            if (pre && count > 0)
+            if (pre && count > 0)      // in T: linear.hip and mx_linear.hip say what that costs the gradients
 #pragma unroll
                 for (int u = 0; u < kGroup; ++u) {
                     const int64_t row = p.begin + r + u * kHeight;

@@ -26,8 +26,9 @@ template <class T> int launch_mx_input(const MxInputArgs& a, hipStream_t stream)
 
 namespace {
 
-// dy and z on their way to LDS as dz = dy act'(z), rounded to T.  Loads as Staged's; a thread's chunks are of the same
-// columns of a slab.
+// dy and z on their way to LDS as dz = dy act'(z).  Loads as Staged's; a thread's chunks are of the same columns of a
+// slab.  dz is rounded to T because the matrix instruction takes T, and so it is wherever a 16-bit layer's gradient is
+// formed: that is most of what dx is off by beside its own rounding (mx_linear.hip).
 template <class T, int kRows, int kThreads> struct SlopeRows : Image<T, true, kRows, kThreads> {
     using I = Image<T, true, kRows, kThreads>;
     struct Held {
@@ -113,8 +114,10 @@ __device__ inline void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_ba
 
 // A tile.  A slab's slope takes a workgroup three times as long as its products do, and all of its waves are at the one
 // or the other: one buffer an operand, so that a CU has two workgroups, one at each.  131072 rows over 64 experts, 256
-// <- 512 fp16, silu: 110 to 118 us, 335 MB at 2.9 TB/s, bound by the slope's arithmetic (256 x 256 tiles with two
-// buffers, one workgroup a CU: 142).
+// <- 512 fp16, silu: 107 to 120 us, 335 MB at 2.8 to 3.1 TB/s (71 us at a large copy's rate).  With relu, whose slope is
+// a comparison, 105, with gelu 142, without the sums 112: silu's arithmetic is 15 us of it.  Most is that a workgroup's
+// loads, slopes, products and epilogue follow one another, and two workgroups a CU cover them only in part (256 x 256
+// tiles with two buffers, one workgroup a CU: 142).
 template <class T, int kBM, int kBN, int kWM, int kWN> struct InputTile : Sums<kBM, kBN, kWM, kWN> {
     using Base = Sums<kBM, kBN, kWM, kWN>;
     using Base::acc;

@@ -185,9 +185,9 @@ template <int kLanes, int kWaves> __device__ inline float sum_of(float x, float 
 
 // Rows of up to kLanes kVecs chunks in registers, the next one under way.  Each lane keeps its two largest keys; a
 // choice takes the largest of all lanes, whose lane goes on to its second, and looks through its keys again once both
-// are gone: at four choices of 1024 about once in 500 rows.  65536 x 1024 fp16, four choices with weights among all: 50
-// us, 134 MB at 2.7 TB/s, bound by the arithmetic (about 450 instructions a row; with a search of all keys for each
-// choice 61 us); one row 2 us.  8192 rows of 4096, 8000, 16000 and 32000 bf16: 24, 39, 92 and 172 us (a row read for
+// are gone: at four choices of 1024 about once in 500 rows.  65536 x 1024 fp16, four choices with weights among all: 47
+// to 50 us, 134 MB at 2.7 to 2.9 TB/s, bound by the arithmetic (about 450 instructions a row, of which each choice's
+// reduction over a whole wave serves one row; with a search of all keys for each choice 61 us); one row 2 us.  8192 rows of 4096, 8000, 16000 and 32000 bf16: 24, 39, 92 and 172 us (a row read for
 // each choice -, 124, 235 and 454).
 template <class T, int kLanes, int kVecs>
 __global__ __launch_bounds__(kLanes > kBlock ? kLanes : kBlock) void choose_kernel(ChooseArgs a) {
@@ -357,10 +357,20 @@ struct ChooseBackwardArgs {
 
 // kLanes lanes a row write its gradient chunk by chunk; each lane holds one of the row's entries, and writes it once more
 // afterwards (kPatched) or hands it to the lane whose chunk it falls in.  Handing out costs about 26 instructions an
-// entry and round of chunks; writing again moves lines a second time (us handed out and patched, fp16: 65536 x 1024,
-// four of all 45 and 44, in turn with the choice itself 99 and 104, eight 61 and 45, 64 309 and 61; 10^6 x 64, two among
-// themselves 28 and 39, eight of all 72 and 64).  65536 x 1024, four of all: 268 MB at 6 TB/s (the logits partly from
-// the last-level cache).
+// entry and round of chunks; writing again moves lines a second time.  us handed out and patched, rows of 2^26 values in
+// all, choices among themselves and with weights of all:
+//   fp16 x 64    two 28, 48 and 41, 54    four 35, 54 and 40, 56    five 37, 56 and 42, 57    eight 47, 66 and 48, 61
+//        x 512   two 23, 48 and 26, 47    four 30, 52 and 29, 48    five 35, 55 and 30, 49    eight 45, 62 and 32, 49
+//        x 1024  two 23, 41 and 27, 43    four 27, 44 and 29, 44    five 30, 47 and 30, 45    eight 42, 57 and 34, 46
+//        x 1032  two 39, 49 and 38, 47    four 36, 56 and 40, 49    five 42, 62 and 42, 49    eight 60, 77 and 45, 51
+//        x 2048  two 24, 42 and 25, 43    four 26, 43 and 28, 43    five 30, 45 and 29, 44    eight 41, 55 and 31, 45
+//   fp32 x 512   two 46, 93 and 52, 107   four 45, 98 and 59, 106   five 43, 100 and 62, 105  eight 52, 114 and 69, 104
+//        x 520   two 64, 99 and 65, 114   four 68, 111 and 71, 117  five 67, 116 and 73, 119  eight 72, 135 and 80, 126
+//        x 1024  two 48, 84 and 52, 95    four 47, 90 and 56, 93    five 47, 92 and 58, 93    eight 50, 100 and 63, 94
+// and 64 of 1024 in fp16 309 and 61.  More than four choices are patched, which fp32 would do without up to eight among
+// themselves, and rows of more than two rounds, whose entries would be handed out as often: there the two are level but
+// for a few sizes, 13 % for one and up to 25 % (fp16 x 1280, two among themselves: 21 and 27) for the other.  65536 x 1024
+// fp16, four of all: 268 MB at 6 TB/s (the logits partly from the last-level cache).
 template <class T, int kLanes, bool kAll, bool kStream, bool kPatched>
 __global__ __launch_bounds__(kBlock) void choose_backward_kernel(ChooseBackwardArgs a, uint32_t first) {
     constexpr int kV = kPerVec<T>;
@@ -448,9 +458,9 @@ __global__ __launch_bounds__(kBlock) void balance_clear_kernel(BalanceArgs a) {
 }
 
 // Each workgroup counts its entries in LDS and adds what it found (whole numbers, in any order).  kAlone: one workgroup
-// of all entries (16384 in 2.6 us, as several with their clearing 5.5).  Entries that lie 16-byte aligned are read four
-// at a time. 1.2 million entries of 1000 experts: 6 us (with 512 workgroups, whose counts are half a million additions,
-// 27).
+// of all entries, which needs no launch that clears (16384 entries 4.1 us; 131072 by several 5.0, and 1.5 to clear).
+// Entries that lie 16-byte aligned are read four at a time. 1.2 million entries of 1000 experts: 6 us (with 512
+// workgroups, whose counts are half a million additions, 27).
 template <bool kAlone> __global__ __launch_bounds__(kCountBlock) void balance_count_kernel(BalanceArgs a) {
     extern __shared__ int32_t held[];
     __shared__ uint32_t all;

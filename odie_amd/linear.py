@@ -10,6 +10,7 @@ are then about 1.4 times as far from exact ones as a single rounding leaves them
 
 A weight may be microscaled 4-bit floating point (odie_amd.microscale), and so may x beside such a weight
 (odie_mx_linear_forward): layers that are served, or that stay as they are while what lies before them is trained.
+Their gradients of x round as above, by x's type.
 """
 import torch
 from torch.autograd.function import once_differentiable

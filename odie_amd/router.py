@@ -55,8 +55,9 @@ def distill(logits, ids, teacher, *, temperature=1.0):
     and q the softmax of teacher / temperature ([N, top], any floating dtype of the three) over them alone.
 
     An id outside 0..classes-1 or a teacher's -inf is no entry; a row without any has loss 0 and no gradient.
-    The temperature is within 2^-100..2^100.  Entries of one class count each.  One entry a row is the cross entropy of that class.  A row whose logits are all
-    -inf has p = 0 and, with an entry, an infinite loss.  The teacher is fixed: it takes no gradient."""
+    The temperature is within 2^-100..2^100.  Entries of one class count each.  One entry a row is the cross entropy
+    of that class.  A row whose logits are all -inf has p = 0 and, with an entry, an infinite loss.  The teacher is
+    fixed: it takes no gradient."""
     logits = check_rows('logits', logits)
     n, device = logits.shape[0], logits.device
     if (not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int32, torch.int64) or ids.ndim != 2
