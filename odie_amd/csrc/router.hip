@@ -9,9 +9,10 @@
 //
 // The loss is E sum_e (c_e / M) (mean over rows of p_ie) with its sums exchanged: each row needs its own
 // logits and the counts alone, and no sums down the columns exist.  Counts are whole numbers, and everything else
-// is added in a fixed order: the same call gives the same bits.  Where the load is even, c_e and t_i are both near M / E
-// and their difference near its root: the whole number next to M / E is taken off every count before it becomes fp32, and
-// t_i is the mean of what is left, so that nothing is rounded relative to M / E.
+// is added in a fixed order: the same call gives the same bits.  c_e - t_i may be far smaller than either: in an even
+// load both are near M / E, and in a row that is sure of one expert both are near that one's count.  So a row takes a
+// whole number near its t_i off the counts, which is exact, and t_i is that number and the mean of what is left; nothing
+// is rounded relative to a count.
 #include "softmax.h"
 
 namespace odie {
@@ -187,7 +188,8 @@ template <int kLanes, int kWaves> __device__ inline float sum_of(float x, float 
 // choice takes the largest of all lanes, whose lane goes on to its second, and looks through its keys again once both
 // are gone: at four choices of 1024 about once in 500 rows.  65536 x 1024 fp16, four choices with weights among all: 47
 // to 50 us, 134 MB at 2.7 to 2.9 TB/s, bound by the arithmetic (about 450 instructions a row, of which each choice's
-// reduction over a whole wave serves one row; with a search of all keys for each choice 61 us); one row 2 us.  8192 rows of 4096, 8000, 16000 and 32000 bf16: 24, 39, 92 and 172 us (a row read for
+// reduction over a whole wave serves one row; with a search of all keys for each choice 61 us); one row 2 us.  8192
+// rows of 4096, 8000, 16000 and 32000 bf16: 24, 39, 92 and 172 us (a row read for
 // each choice -, 124, 235 and 454).
 template <class T, int kLanes, int kVecs>
 __global__ __launch_bounds__(kLanes > kBlock ? kLanes : kBlock) void choose_kernel(ChooseArgs a) {
@@ -440,7 +442,7 @@ struct BalanceArgs {
     uint32_t* entries;        // M
     uint32_t* done;           // workgroups that have left their sums, or null: a launch of its own makes the loss
     uint32_t blocks;          // workgroups of the rows
-    float* stats;             // [n][4]: m, 1 / s (0: the row takes no part), t less even_count, even_count's bits
+    float* stats;             // [n][4]: m, 1 / s (0: the row takes no part), t less `whole`, the whole number's bits
     double* partial;          // [blocks]: sum of t
     uint32_t* parts;          // [blocks]: rows that take part
     float* norm;              // E / (M R)
@@ -506,17 +508,15 @@ __device__ inline int32_t even_count(const BalanceArgs& a) {
     return static_cast<int32_t>((*a.entries + experts / 2) / experts);
 }
 
-// The counts of a lane's columns less `even`, as fp32; 0 past the last.
+// The counts of a lane's columns; past the last, the last.
 template <class T, int kLanes, int kVecs>
-__device__ inline void hold_counts(const int32_t* counts, int32_t even, int lane, int experts,
-                                   float (&to)[kVecs][kPerVec<T>]) {
+__device__ inline void hold_counts(const int32_t* counts, int lane, int experts, int32_t (&to)[kVecs][kPerVec<T>]) {
 #pragma unroll
     for (int v = 0; v < kVecs; ++v)
 #pragma unroll
         for (int i = 0; i < kPerVec<T>; ++i) {
             const int e = (v * kLanes + lane) * kPerVec<T> + i;
-            const int32_t count = counts[e < experts ? e : experts - 1];
-            to[v][i] = e < experts ? static_cast<float>(count - even) : 0.0f;
+            to[v][i] = counts[e < experts ? e : experts - 1];
         }
 }
 
@@ -536,10 +536,10 @@ template <int kLanes> struct Part {
     }
 };
 
-__device__ inline void keep_row(const BalanceArgs& a, int64_t row, float m, float inverse, float t, int32_t even) {
+__device__ inline void keep_row(const BalanceArgs& a, int64_t row, float m, float inverse, float t, uint32_t whole) {
     if (a.stats)
         *reinterpret_cast<float4*>(a.stats + row * 4) =
-            make_float4(m, inverse, t, __builtin_bit_cast(float, even));
+            make_float4(m, inverse, t, as_float(whole));
 }
 
 // The sums of the workgroup's threads, in thread 0.
@@ -609,16 +609,22 @@ __device__ inline void over_waves(float2 own, float2 (&part)[2][kBlock / 64], in
 }
 
 // Rows of up to kLanes kVecs chunks: kLanes lanes a row, a row in registers and the next one under way, the counts of
-// the lane's columns in registers for all of its rows.  300007 x 1000 bf16: 140 to 170 us, 600 MB at 3.6 to 4.3 TB/s
-// (with the counts read for each row 524 us; with loads under conditions, which the compiler waits for, 214); 8192 x
-// 8000 39 us (a wave a row 122).
+// the lane's columns, less M / E, in registers for all of its rows.  A first sum gives a row's t and with it the whole
+// number that comes off for a second one, which costs 4 to 11 % (300007 x 1000 bf16: 136 to 154 us).  300007 x 1000 bf16:
+// 150 to 164 us, 600 MB at 3.7 to 4 TB/s (with the counts read for each row and one sum 524 us; with loads under
+// conditions, which the compiler waits for, 214); 8192 x 8000 43 us (a wave a row and one sum 122).
 template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) void balance_rows_kernel(BalanceArgs a) {
     constexpr bool kExact = sizeof(T) == 4;
     constexpr int kV = kPerVec<T>, kRows = kBlock / kLanes;
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
     const int32_t even = even_count(a);
+    int32_t held_counts[kVecs][kV];
+    hold_counts<T, kLanes, kVecs>(a.counts, lane, a.experts, held_counts);
     float counts[kVecs][kV];
-    hold_counts<T, kLanes, kVecs>(a.counts, even, lane, a.experts, counts);
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v)
+#pragma unroll
+        for (int i = 0; i < kV; ++i) counts[v][i] = static_cast<float>(held_counts[v][i] - even);
     const T* logits = static_cast<const T*>(a.logits);
     double total = 0.0;
     uint32_t rows = 0;
@@ -661,6 +667,7 @@ template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) v
 #pragma unroll
             for (int i = 0; i < kV; ++i) {
                 const float e = exponential<kExact>(value[v][i] - from);
+                value[v][i] = e;
                 s += e;
                 t = fmaf(e, counts[v][i], t);
             }
@@ -672,33 +679,48 @@ template <class T, int kLanes, int kVecs> __global__ __launch_bounds__(kBlock) v
             over_waves(own, held, turn, [&](const float2& x) { s += x.x, t += x.y; });
         }
         const float inverse = any && !(top == kNegInfinity) ? 1.0f / s : 0.0f;
+        const float near = inverse == 0.0f || !(inverse < INFINITY) ? 0.0f : rintf(t * inverse);    // NaN: 0
+        t = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v)
+#pragma unroll
+            for (int i = 0; i < kV; ++i) t = fmaf(value[v][i], counts[v][i] - near, t);
+        t = sum_across<kTogether>(t);
+        if constexpr (kLanes > 64) {
+            const float2 own = make_float2(t, 0.0f);
+            t = 0.0f;
+            over_waves(own, held, turn, [&](const float2& x) { t += x.x; });
+        }
         t = inverse == 0.0f ? 0.0f : t * inverse;
         if (at < a.n && lane == 0) {
-            total += inverse == 0.0f ? 0.0 : static_cast<double>(even) + t;
+            total += inverse == 0.0f ? 0.0 : static_cast<double>(even) + near + t;
             rows += any;
-            keep_row(a, at, top, inverse, t, even);
+            keep_row(a, at, top, inverse, t,
+                     static_cast<uint32_t>(even) + static_cast<uint32_t>(static_cast<int32_t>(near)));
         }
     }
     finish_balance(a, total, rows);
 }
 
-// The counts of a chunk's columns less `even`, as fp32; 0 past the last.
+// The counts of a chunk's columns; 0 past the last.
 template <int kV>
-__device__ inline void load_counts(const int32_t* counts, int32_t even, int column, int experts, float (&to)[kV]) {
+__device__ inline void load_counts(const int32_t* counts, int column, int experts, int32_t (&to)[kV]) {
     if (column + kV <= experts) {
 #pragma unroll
         for (int w = 0; w < kV / 4; ++w) {
             const vec16 four = load16(counts + column + 4 * w);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) to[4 * w + i] = static_cast<float>(static_cast<int32_t>(four[i]) - even);
+            for (int i = 0; i < 4; ++i) to[4 * w + i] = static_cast<int32_t>(four[i]);
         }
         return;
     }
 #pragma unroll
-    for (int i = 0; i < kV; ++i) to[i] = column + i < experts ? static_cast<float>(counts[column + i] - even) : 0.0f;
+    for (int i = 0; i < kV; ++i) to[i] = column + i < experts ? counts[column + i] : 0;
 }
 
-// Longer rows: a wave a row, with a running maximum.  8192 x 32000 bf16: 149 us forward and 230 backward.
+// Longer rows: a wave a row, with a running maximum.  They are not held for a second sum: one takes M / E off, another
+// nothing, and the row keeps the one that is off by less, the second where t is below half of M / E.  8192 x 32000 bf16:
+// 145 us forward and 228 backward.
 template <class T> __global__ __launch_bounds__(kBlock) void balance_long_kernel(BalanceArgs a) {
     constexpr bool kExact = sizeof(T) == 4;
     constexpr int kV = kPerVec<T>;
@@ -712,34 +734,40 @@ template <class T> __global__ __launch_bounds__(kBlock) void balance_long_kernel
         part.load(a, row, lane);
         const bool any = part.get(a, row, lane);
         const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
-        float m = kNegInfinity, s = 0.0f, t = 0.0f;
+        float m = kNegInfinity, s = 0.0f, t = 0.0f, all = 0.0f;
         for (int column = lane * kV; column < a.experts; column += 64 * kV) {
-            float value[kV], counts[kV];
+            float value[kV];
+            int32_t counts[kV];
             load_logits(logits, column, a.experts, value);
-            load_counts(a.counts, even, column, a.experts, counts);
+            load_counts(a.counts, column, a.experts, counts);
             float top = m;
 #pragma unroll
             for (int i = 0; i < kV; ++i) top = larger(top, value[i]);
             const float base = base_of(top), old = exponential<kExact>(m - base);
             s *= old;
             t *= old;
+            all *= old;
 #pragma unroll
             for (int i = 0; i < kV; ++i) {
                 const float e = exponential<kExact>(value[i] - base);
                 s += e;
-                t = fmaf(e, counts[i], t);
+                t = fmaf(e, static_cast<float>(counts[i] - even), t);
+                all = fmaf(e, static_cast<float>(counts[i]), all);
             }
             m = top;
         }
         const float top = max_across<64>(m), old = exponential<kExact>(m - base_of(top));
         s = sum_across<64>(s * old);
         t = sum_across<64>(t * old);
+        all = sum_across<64>(all * old);
         const float inverse = any && !(top == kNegInfinity) ? 1.0f / s : 0.0f;
-        t = inverse == 0.0f ? 0.0f : t * inverse;
+        const bool few = all * inverse < 0.5f * static_cast<float>(even);
+        t = inverse == 0.0f ? 0.0f : (few ? all : t) * inverse;
         if (lane == 0) {
-            total += inverse == 0.0f ? 0.0 : static_cast<double>(even) + t;
+            const int32_t whole = few ? 0 : even;
+            total += inverse == 0.0f ? 0.0 : static_cast<double>(whole) + t;
             rows += any;
-            keep_row(a, row, top, inverse, t, even);
+            keep_row(a, row, top, inverse, t, static_cast<uint32_t>(whole));
         }
     }
     finish_balance(a, total, rows);
@@ -756,16 +784,18 @@ struct BalanceBackwardArgs {
     int experts;
 };
 
-// What the forward took off every count: the same in each row's statistics.
-__device__ inline int32_t even_count(const BalanceBackwardArgs& a) { return __builtin_bit_cast(int32_t, a.stats[3]); }
+// c_e - t of a row: its whole number comes off first, exactly.
+__device__ inline float count_less_mean(int32_t count, const float4& stats) {
+    return static_cast<float>(static_cast<int32_t>(static_cast<uint32_t>(count) - as_bits(stats.w))) - stats.z;
+}
 
-// The same way.  300007 x 1000 bf16: 243 us, 1.2 GB at 4.9 TB/s: HBM.
+// The same way.  300007 x 1000 bf16: 255 us, 1.2 GB at 4.7 TB/s: HBM.
 template <class T, int kLanes, int kVecs, bool kStream>
 __global__ __launch_bounds__(kBlock) void balance_backward_kernel(BalanceBackwardArgs a) {
     constexpr int kV = kPerVec<T>, kRows = kBlock / kLanes;
     const int lane = static_cast<int>(threadIdx.x) % kLanes;
-    float counts[kVecs][kV];
-    hold_counts<T, kLanes, kVecs>(a.counts, even_count(a), lane, a.experts, counts);
+    int32_t counts[kVecs][kV];
+    hold_counts<T, kLanes, kVecs>(a.counts, lane, a.experts, counts);
     const float scale = *a.upstream * *a.norm;
     const T* logits = static_cast<const T*>(a.logits);
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
@@ -790,7 +820,8 @@ __global__ __launch_bounds__(kBlock) void balance_backward_kernel(BalanceBackwar
             row.get(v, lane, a.experts, value);
 #pragma unroll
             for (int i = 0; i < kV; ++i) {
-                const float d = each * exponential<sizeof(T) == 4>(value[i] - stats.x) * (counts[v][i] - stats.z);
+                const float d =
+                    each * exponential<sizeof(T) == 4>(value[i] - stats.x) * count_less_mean(counts[v][i], stats);
                 value[i] = stats.y == 0.0f ? 0.0f : d;
             }
             if (column < a.experts) store_some<kStream>(out + column, narrow<T>(value), a.experts - column);
@@ -802,7 +833,6 @@ template <class T, bool kStream>
 __global__ __launch_bounds__(kBlock) void balance_long_backward_kernel(BalanceBackwardArgs a) {
     constexpr int kV = kPerVec<T>;
     const int lane = static_cast<int>(threadIdx.x) % 64;
-    const int32_t even = even_count(a);
     const float scale = *a.upstream * *a.norm;
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * (kBlock / 64) + static_cast<int>(threadIdx.x) / 64; row < a.n;
          row += static_cast<int64_t>(gridDim.x) * (kBlock / 64)) {
@@ -811,12 +841,14 @@ __global__ __launch_bounds__(kBlock) void balance_long_backward_kernel(BalanceBa
         const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
         T* out = static_cast<T*>(a.dlogits) + row * a.experts;
         for (int column = lane * kV; column < a.experts; column += 64 * kV) {
-            float value[kV], counts[kV];
+            float value[kV];
+            int32_t counts[kV];
             load_logits(logits, column, a.experts, value);
-            load_counts(a.counts, even, column, a.experts, counts);
+            load_counts(a.counts, column, a.experts, counts);
 #pragma unroll
             for (int i = 0; i < kV; ++i) {
-                const float d = each * exponential<sizeof(T) == 4>(value[i] - stats.x) * (counts[i] - stats.z);
+                const float d =
+                    each * exponential<sizeof(T) == 4>(value[i] - stats.x) * count_less_mean(counts[i], stats);
                 value[i] = stats.y == 0.0f ? 0.0f : d;
             }
             store_some<kStream>(out + column, narrow<T>(value), a.experts - column);
